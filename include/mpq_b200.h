@@ -439,6 +439,50 @@ int mpq_cd_accept(float* x, int64_t ldx, const float* cand, int64_t ldc, const f
 int mpq_pack_bits(const uint8_t* src, int64_t sp, int64_t so, int n_pack, int n_other, int bits, int offset,
                   int32_t* out, int64_t ld_out, void* stream);
 
+/* ---- microscaled 4-bit floating point (MX4: E2M1 elements, one E8M0 scale for 32 of them) ----
+ * No counterpart in the reference (its grids are integer or E8P12); a 4-bit format of the tensor cores themselves.
+ * dtype: 0 float32, 1 bfloat16, 2 float16.  Stored form of a rows x cols matrix, with nb = ceil(cols / 32) blocks a
+ * row: codes rows x 16 nb bytes (column 2j in the low half of byte j; sign, two exponent bits, one mantissa bit);
+ * scales [ceil(rows / 128)][ceil(nb / 4)][512] bytes, (row, block) at byte (row % 32) 16 + (row % 128 / 32) 4 +
+ * block % 4 of its tile.  Both 16-byte aligned.  A block stands for code 2^(scale - 127); scale 255 is NaN. */
+
+/* Block scale max(E - 2, 0) with E the biased exponent of the largest magnitude (255 where the block is not finite),
+ * elements to nearest even, saturating at 6 scales.  Every byte of codes and scales is written. */
+int mpq_mx4_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols, uint8_t* codes, uint8_t* scales,
+                     void* stream);
+/* out[r, c] = code * 2^(scale - 127), rounded to dtype. */
+int mpq_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int rows, int cols, void* out, int dtype,
+                       int64_t ldo, void* stream);
+/* out (M x N, dtype) = A B^T + bias: A M x K and B N x K in the stored form, bias N values of dtype or NULL, FP32
+ * accumulation on the block-scaled tensor cores, one rounding.  `status`: as mpq_gemm_tc. */
+int mpq_mx4_gemm(int M, int N, int K, const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
+                 const uint8_t* b_scales, const void* bias, void* out, int dtype, int64_t ldo, int* status,
+                 void* stream);
+
+/* ---- softmax cross entropy over a vocabulary, from hidden states (T x H) and the output head (V x H) ----
+ * No counterpart in the reference (its perplexity scripts call a library's loss on whole logits).  The logits are
+ * never stored.  dtype: 1 bfloat16, 2 float16 (hidden, weight and their gradients); operands 16-byte aligned with
+ * leading dimensions that are multiples of 8.  Labels equal to `ignore` do not count; labels outside [0, V) give NaN.
+ * `status`: as mpq_gemm_tc. */
+
+/* Columns of `part` below. */
+int mpq_xent_tiles(int V);
+/* lse[t] = log sum_v exp(h_t . w_v), nll[t] = lse[t] - h_t . w_y (0 where ignored).  Workspaces: part, T x
+ * mpq_xent_tiles(V) pairs of floats (part_floats: floats it holds); tgt, T floats. */
+int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+                     const int64_t* labels, int64_t ignore, float* part, int64_t part_floats, float* tgt, float* lse,
+                     float* nll, int* status, void* stream);
+/* loss = sum of nll, divided by the number of counted labels where mean != 0 (NaN for none); count = that number. */
+int mpq_xent_reduce(int T, const float* nll, const int64_t* labels, int64_t ignore, int mean, float* loss, float* count,
+                    void* stream);
+/* dhidden (T x H) and dweight (V x H), either may be NULL, from lse and the upstream gradient gout[t * gstride] of
+ * each nll (divided by *count where count is given).  Workspaces: gmax, one float; d, T x piece 16-bit values (piece: a
+ * multiple of 256 columns); acc, T x H floats, needed for dhidden where V > piece. */
+int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+                      const int64_t* labels, int64_t ignore, const float* lse, const float* gout, int gstride,
+                      const float* count, float* gmax, void* d, int piece, float* acc, void* dhidden, int64_t lddh,
+                      void* dweight, int64_t lddw, int* status, void* stream);
+
 /* ---- rotation ----
  * Block Walsh-Hadamard of the last dim, blocks of `had` (power of two <= 16384), normalized by sqrt(had);
  * mode 0: y = H(x * signs) (right rotation), mode 1: y = H(x) * signs (inverse).  signs may be NULL.

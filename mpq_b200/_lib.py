@@ -102,6 +102,13 @@ SIGNATURES: Dict[str, Tuple[Any, ...]] = {
     "mpq_vamp_r1_parts_ctl": (P, I, P, P, P, P, P, I, I, L, F, P, P, P),
     "mpq_gemm_f16x3_parts": (I, I, I, P, P, L, P, P, P, L, P, I, P, L, P, P),
     "mpq_gram_chunk_topk": (P, L, P, L, P, P, P, I, I, P, P, I, I, P, P, L, P, P, P, I, F, P),
+    "mpq_mx4_quantize": (P, I, L, I, I, P, P, P),
+    "mpq_mx4_dequantize": (P, P, I, I, P, I, L, P),
+    "mpq_mx4_gemm": (I, I, I, P, P, P, P, P, P, I, L, P, P),
+    "mpq_xent_tiles": (I,),
+    "mpq_xent_forward": (I, I, I, I, P, L, P, L, P, L, P, L, P, P, P, P, P),
+    "mpq_xent_reduce": (I, P, P, L, I, P, P, P),
+    "mpq_xent_backward": (I, I, I, I, P, L, P, L, P, L, P, P, I, P, P, P, I, P, P, L, P, L, P, P),
 }
 
 _lib = None

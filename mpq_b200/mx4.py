@@ -1,0 +1,179 @@
+"""Microscaled 4-bit floating point (MX4): quantisation, reading back, and linear layers on it.
+
+A row is cut into blocks of 32 elements; a block holds 4-bit E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+negatives) and one power-of-two scale.  It is the 4-bit format that the tensor cores multiply directly, so it serves
+next to the solved formats of this package as the round-to-nearest baseline at 4.25 bits a weight:
+
+    w4 = quantize_mx4(layer.weight)         # once
+    y = mx4_linear(x, w4, layer.bias)       # x is quantised within the call, token by token
+    convert_linears_mx4(model.model)        # every nn.Linear below, in place
+
+The operators run forward only; tensors must be on the GPU (there is no CPU path).
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import ops
+from ._lib import call, ptr
+
+BLOCK = 32
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _dtype_code(dtype: torch.dtype) -> int:
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"MX4 operators take float32, bfloat16 or float16 tensors, not {dtype}")
+    return code
+
+
+def stored_shapes(rows: int, cols: int) -> Tuple[Tuple[int, int], Tuple[int, int, int]]:
+    """Shapes of the codes and the scales (uint8) of a rows x cols matrix: two codes to a byte, rows padded to whole
+    blocks; scales in tiles of 128 rows x 4 blocks, (row, block) at byte (row % 32) * 16 + (row % 128 // 32) * 4 +
+    block % 4 of its tile (the layout in which the tensor cores take them)."""
+    blocks = -(-cols // BLOCK)
+    return (rows, 16 * blocks), (-(-rows // 128), -(-blocks // 4), 512)
+
+
+class Mx4Tensor:
+    """A quantised matrix: ``codes`` and ``scales`` in the stored form (see ``stored_shapes``) and its ``shape``."""
+
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Tuple[int, int]):
+        rows, cols = int(shape[0]), int(shape[1])
+        want_codes, want_scales = stored_shapes(rows, cols)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise ValueError("MX4 codes and scales are uint8 tensors")
+        if codes.shape != want_codes or scales.shape != want_scales:
+            raise ValueError(f"a {rows} x {cols} MX4 matrix has codes {want_codes} and scales {want_scales}, got "
+                             f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+        if codes.device != scales.device:
+            raise ValueError("MX4 codes and scales are on different devices")
+        if not codes.is_contiguous() or codes.data_ptr() % 16:
+            codes = codes.clone(memory_format=torch.contiguous_format)
+        if not scales.is_contiguous() or scales.data_ptr() % 16:
+            scales = scales.clone(memory_format=torch.contiguous_format)
+        self.codes, self.scales, self.shape = codes, scales, (rows, cols)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def to(self, device) -> "Mx4Tensor":
+        return Mx4Tensor(self.codes.to(device), self.scales.to(device), self.shape)
+
+    def __repr__(self) -> str:
+        return f"Mx4Tensor({self.shape[0]} x {self.shape[1]}, {self.codes.device})"
+
+
+def _rows_of(x: torch.Tensor, what: str) -> torch.Tensor:
+    """x as a matrix of rows with unit column stride (a copy only where the strides ask for one)."""
+    if not x.is_cuda:
+        raise ValueError("mpq_b200 kernels require CUDA tensors (there is no CPU path)")
+    if x.dim() < 1:
+        raise ValueError(f"{what} needs at least one dimension")
+    x = x.detach()
+    if x.dim() != 2:
+        x = x.reshape(x.numel() // x.shape[-1] if x.shape[-1] else 0, x.shape[-1])
+    if x.numel() and (x.stride(1) != 1 and x.shape[1] != 1 or x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x
+
+
+def quantize_mx4(x: torch.Tensor) -> Mx4Tensor:
+    """Quantise the rows of x (..., cols): block scale 2^(floor(log2 max|x|) - 2), elements to the nearest E2M1 value
+    (ties to even), values beyond 6 scales saturate.  A block with an infinity or a NaN reads back as NaN."""
+    x = _rows_of(x, "quantize_mx4")
+    code = _dtype_code(x.dtype)
+    rows, cols = x.shape
+    shape_codes, shape_scales = stored_shapes(rows, cols)
+    codes = torch.empty(shape_codes, device=x.device, dtype=torch.uint8)
+    scales = torch.empty(shape_scales, device=x.device, dtype=torch.uint8)
+    with torch.cuda.device(x.device):
+        call("mpq_mx4_quantize", ptr(x), code, max(x.stride(0), cols), rows, cols, ptr(codes), ptr(scales))
+    return Mx4Tensor(codes, scales, (rows, cols))
+
+
+def dequantize_mx4(q: Mx4Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values a quantised matrix stands for (exact in float32 and bfloat16; float16 rounds or overflows where the
+    scale leaves its range)."""
+    code = _dtype_code(dtype)
+    if not q.codes.is_cuda:
+        raise ValueError("mpq_b200 kernels require CUDA tensors (there is no CPU path)")
+    rows, cols = q.shape
+    out = torch.empty(rows, cols, device=q.device, dtype=dtype)
+    with torch.cuda.device(q.device):
+        call("mpq_mx4_dequantize", ptr(q.codes), ptr(q.scales), rows, cols, ptr(out), code, max(cols, 1))
+    return out
+
+
+def mx4_linear(x: torch.Tensor, weight: Mx4Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y = Q(x) W^T + b for x (..., K) and a quantised W (N x K): x is quantised row by row, the products accumulate in
+    FP32, and y (x's dtype) is rounded once."""
+    rows = _rows_of(x, "mx4_linear")
+    code = _dtype_code(x.dtype)
+    n, k = weight.shape
+    if rows.shape[1] != k:
+        raise ValueError(f"mx4_linear: x has {rows.shape[1]} columns, the weight {k}")
+    if weight.device != x.device:
+        raise ValueError("mx4_linear: x and the weight are on different devices")
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype != x.dtype or bias.device != x.device:
+            raise ValueError(f"mx4_linear: the bias must be {n} values of x's dtype on x's device")
+        bias = bias.detach().contiguous()
+    m = rows.shape[0]
+    out = torch.empty(m, n, device=x.device, dtype=x.dtype)
+    if m and n:
+        if k == 0:
+            out.zero_() if bias is None else out.copy_(bias.expand(m, n))
+        else:
+            q = quantize_mx4(rows)
+            with torch.cuda.device(x.device):
+                call("mpq_mx4_gemm", m, n, k, ptr(q.codes), ptr(q.scales), ptr(weight.codes), ptr(weight.scales),
+                     ptr(bias), ptr(out), code, n, ptr(ops.status_word(x.device)))
+    return out.view(*x.shape[:-1], n)
+
+
+class Mx4Linear(torch.nn.Module):
+    """A linear layer with its weight in MX4 (forward only)."""
+
+    def __init__(self, weight: Mx4Tensor, bias: Optional[torch.Tensor] = None):
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        self.register_buffer("codes", weight.codes)
+        self.register_buffer("scales", weight.scales)
+        self.register_buffer("bias", None if bias is None else bias.detach().clone())
+
+    @classmethod
+    def from_linear(cls, linear: torch.nn.Linear) -> "Mx4Linear":
+        return cls(quantize_mx4(linear.weight), linear.bias)
+
+    @property
+    def mx4_weight(self) -> Mx4Tensor:
+        return Mx4Tensor(self.codes, self.scales, (self.out_features, self.in_features))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return mx4_linear(x, self.mx4_weight, self.bias)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+def convert_linears_mx4(module: torch.nn.Module) -> int:
+    """Replace every ``nn.Linear`` below ``module`` by an ``Mx4Linear`` of its weight; returns how many."""
+    done = 0
+    for name, child in module.named_children():
+        if isinstance(child, torch.nn.Linear):
+            setattr(module, name, Mx4Linear.from_linear(child))
+            done += 1
+        else:
+            done += convert_linears_mx4(child)
+    return done
+
+
+__all__ = ["Mx4Tensor", "Mx4Linear", "convert_linears_mx4", "dequantize_mx4", "mx4_linear", "quantize_mx4",
+           "stored_shapes"]

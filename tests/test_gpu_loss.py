@@ -1,0 +1,284 @@
+"""The vocabulary loss and its gradients against the formulas in 64 bits.
+
+Bounds, before any run: a logit off the tensor cores is within 1e-5 of sum |h| |w| (the bound that this package's other
+tensor-core products are held to) = delta_t at most for token t; a score is then within 2 delta_t, plus 1e-5 for the
+FP32 exponentials and logarithm.  The logits' gradient d is off by 2 delta_t + 1e-5 of p, and by one rounding u (2^-8
+for bf16, 2^-11 for f16) of itself; a product with it adds 1e-5 of the sum of magnitudes and the output's rounding u.
+"""
+import pytest
+import torch
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def inputs(t, v, h, dtype, dev, seed=0, ignored=0.2, lean=8.0):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(v, h, generator=g) * (1.5 / h ** 0.5)
+    y = torch.randint(0, v, (t,), generator=g)
+    x = torch.randn(t, h, generator=g) + lean * torch.rand(t, 1, generator=g) * w[y] / w[y].square().sum(1, keepdim=True)
+    y = torch.where(torch.rand(t, generator=g) < ignored, -100, y)
+    return x.to(dtype).to(dev), w.to(dtype).to(dev), y.to(dev)
+
+
+def formulas(x, w, y, gout=None, reduction="mean", ignore=-100):
+    """Scores and gradients in 64 bits, with the bounds above."""
+    u = U[x.dtype]
+    x, w, y = x.double().cpu(), w.double().cpu(), y.cpu()
+    keep = y != ignore
+    logits = x @ w.T
+    delta = 1e-5 * (x.abs() @ w.abs().T).amax(1)
+    lse = torch.logsumexp(logits, 1)
+    at = torch.where(keep, y, 0)[:, None]
+    nll = torch.where(keep, lse - logits.gather(1, at)[:, 0], 0.0)
+    share = keep.double() / (keep.sum() if reduction == "mean" else 1)
+    gout = torch.ones(()) if gout is None else gout.double().cpu()
+    g = share * gout
+    p = torch.exp(logits - lse[:, None])
+    d = p.scatter_add(1, at, -torch.ones_like(p[:, :1])) * g[:, None]
+    off = (p * (2 * delta + 1e-5)[:, None]) * g.abs()[:, None] + u * d.abs()
+    if x.shape[0] and u == 2.0 ** -11:  # f16 holds multiples of 2^-24 in units of 2^-15 of the largest g
+        off = off + 2.0 ** -40 * g.abs().max()
+    dh, dw = d @ w, d.T @ x
+    tol_h = off @ w.abs() + 1e-5 * (d.abs() @ w.abs()) + u * dh.abs() + (2.0 ** -24 if u == 2.0 ** -11 else 0)
+    tol_w = off.T @ x.abs() + 1e-5 * (d.abs().T @ x.abs()) + u * dw.abs() + (2.0 ** -24 if u == 2.0 ** -11 else 0)
+    return {"nll": nll, "tol": torch.where(keep, 2 * delta + 1e-5, 0.0), "share": share, "dh": dh, "dw": dw, "tol_h": tol_h,
+            "tol_w": tol_w}
+
+
+def within(got, want, tol):
+    err = (got.detach().cpu().double() - want).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+SHAPES = [(1, 1, 8), (1, 1000, 64), (2, 7, 24), (5, 257, 128), (31, 300, 8), (127, 511, 200), (128, 512, 64),
+          (129, 2049, 136), (200, 1000, 256), (300, 777, 1024), (513, 4100, 72)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+@pytest.mark.parametrize("t,v,h", SHAPES)
+def test_scores(cuda_dev, t, v, h, dtype):
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(t, v, h, dtype, cuda_dev)
+    ref = formulas(x, w, y)
+    nll = vocab_cross_entropy(x, w, y, reduction="none")
+    assert nll.dtype == torch.float32
+    within(nll, ref["nll"], ref["tol"])
+    total = vocab_cross_entropy(x, w, y, reduction="sum")
+    within(total, ref["nll"].sum(), ref["tol"].sum() + 1e-6 * ref["nll"].sum())
+    mean = vocab_cross_entropy(x, w, y)
+    if bool((y != -100).any()):
+        within(mean, (ref["nll"] * ref["share"]).sum(), (ref["tol"] * ref["share"]).sum() + 1e-6 * ref["nll"].max())
+    else:
+        assert bool(mean.isnan())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("piece", [None, 256, 600])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+@pytest.mark.parametrize("t,v,h", SHAPES)
+def test_gradients(cuda_dev, t, v, h, dtype, piece):
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(t, v, h, dtype, cuda_dev, 1)
+    y[0] = v - 1
+    x.requires_grad_(), w.requires_grad_()
+    ref = formulas(x.detach(), w.detach(), y)
+    dh, dw = torch.autograd.grad(vocab_cross_entropy(x, w, y, piece=piece), (x, w))
+    assert dh.dtype == dtype and dw.dtype == dtype
+    within(dh, ref["dh"], ref["tol_h"])
+    within(dw, ref["dw"], ref["tol_w"])
+    gout = torch.randn(t, generator=torch.Generator().manual_seed(3)).to(cuda_dev)
+    ref = formulas(x.detach(), w.detach(), y, gout, "none")
+    nll = vocab_cross_entropy(x, w, y, reduction="none", piece=piece)
+    dh, dw = torch.autograd.grad(nll, (x, w), gout)
+    within(dh, ref["dh"], ref["tol_h"])
+    within(dw, ref["dw"], ref["tol_w"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+def test_gradients_against_differences(cuda_dev, dtype):
+    """Central differences of the 64-bit loss along a direction: eps = 1e-5 leaves 1e-9 of curvature and rounding, so the
+    bound is the gradients' own summed along the direction."""
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(70, 900, 96, dtype, cuda_dev, 2)
+    x.requires_grad_(), w.requires_grad_()
+    dh, dw = torch.autograd.grad(vocab_cross_entropy(x, w, y), (x, w))
+    ref = formulas(x.detach(), w.detach(), y)
+    xd, wd, yd = x.detach().double().cpu(), w.detach().double().cpu(), y.cpu()
+    g = torch.Generator().manual_seed(0)
+    for _ in range(4):
+        a, b = torch.randn(xd.shape, generator=g).double(), torch.randn(wd.shape, generator=g).double()
+        loss = lambda e: torch.nn.functional.cross_entropy((xd + e * a) @ (wd + e * b).T, yd)  # noqa: E731
+        slope = (loss(1e-5) - loss(-1e-5)) / 2e-5
+        got = (dh.cpu().double() * a).sum() + (dw.cpu().double() * b).sum()
+        tol = (ref["tol_h"] * a.abs()).sum() + (ref["tol_w"] * b.abs()).sum() + 1e-7
+        assert abs(float(got - slope)) <= float(tol)
+
+
+@pytest.mark.gpu
+def test_one_gradient_at_a_time_and_scaled_loss(cuda_dev):
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(60, 700, 64, torch.bfloat16, cuda_dev, 4)
+    both = torch.autograd.grad(vocab_cross_entropy(x.requires_grad_(), w.requires_grad_(), y), (x, w))
+    only_h = torch.autograd.grad(vocab_cross_entropy(x, w.detach(), y), x)[0]
+    only_w = torch.autograd.grad(vocab_cross_entropy(x.detach(), w, y), w)[0]
+    assert torch.equal(both[0], only_h) and torch.equal(both[1], only_w)
+    scaled = torch.autograd.grad(64.0 * vocab_cross_entropy(x, w, y), (x, w))
+    assert torch.equal(scaled[0], 64 * both[0]) and torch.equal(scaled[1], 64 * both[1])
+
+
+@pytest.mark.gpu
+def test_small_upstream_gradients_in_f16(cuda_dev):
+    """A mean over many tokens: every entry of d is far below f16's normal range, its gradients are not lost."""
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(400, 3000, 64, torch.float16, cuda_dev, 5, ignored=0.0, lean=0.0)
+    x.requires_grad_()
+    ref = formulas(x.detach(), w, y)
+    scale = 2.0 ** 12
+    dh = torch.autograd.grad(scale * vocab_cross_entropy(x, w, y), x)[0]
+    within(dh / scale, ref["dh"], ref["tol_h"])
+    off = (dh.cpu().double() / scale - ref["dh"]).norm() / ref["dh"].norm()
+    assert float(off) <= 2 * U[torch.float16]
+
+
+@pytest.mark.gpu
+def test_rows_that_do_not_count(cuda_dev):
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(40, 500, 64, torch.bfloat16, cuda_dev, 6, ignored=0.0)
+    x[3] = float("nan")  # a padded position may hold anything
+    x[5] = float("inf")
+    y[3] = y[5] = y[7] = -100
+    x.requires_grad_()
+    loss = vocab_cross_entropy(x, w, y)
+    dh = torch.autograd.grad(loss, x)[0]
+    assert bool(loss.isfinite()) and bool(dh.isfinite().all())
+    assert not dh[[3, 5, 7]].any()
+    other = vocab_cross_entropy(x, w, torch.where(y == -100, 2 ** 40, y), ignore_index=2 ** 40)
+    assert torch.equal(other, loss)
+    seven = torch.where(y == -100, 7, y)
+    assert torch.equal(vocab_cross_entropy(x, w, seven, ignore_index=7, reduction="none") == 0, seven == 7)
+    none = torch.full_like(y, -100)
+    total = vocab_cross_entropy(x, w, none, reduction="sum")
+    assert float(total) == 0 and not torch.autograd.grad(total, x)[0].any()
+    mean = vocab_cross_entropy(x, w, none)
+    assert bool(mean.isnan()) and not torch.autograd.grad(mean, x)[0].any()
+
+
+@pytest.mark.gpu
+def test_labels_outside_the_vocabulary_give_nan(cuda_dev):
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(20, 300, 64, torch.bfloat16, cuda_dev, 7, ignored=0.0)
+    good = vocab_cross_entropy(x, w, y, reduction="none")
+    y[4], y[9] = 300, -1
+    x.requires_grad_()
+    nll = vocab_cross_entropy(x, w, y, reduction="none")
+    bad = torch.zeros(20, dtype=torch.bool, device=cuda_dev)
+    bad[[4, 9]] = True
+    assert torch.equal(nll.isnan(), bad) and torch.equal(nll[~bad], good[~bad])
+    dh = torch.autograd.grad(nll.sum(), x)[0]
+    assert torch.equal(dh.isnan().any(1), bad)
+
+
+@pytest.mark.gpu
+def test_large_logits_and_infinities(cuda_dev):
+    """Logits of +-3000: the running maximum keeps every exponential finite; a row with an infinity scores NaN alone."""
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(33, 600, 64, torch.bfloat16, cuda_dev, 8, ignored=0.0)
+    x = x * 400
+    ref = formulas(x, w, y)
+    nll = vocab_cross_entropy(x, w, y, reduction="none")
+    within(nll, ref["nll"], ref["tol"] + 1e-6 * ref["nll"])
+    x[2, 3] = float("inf")
+    again = vocab_cross_entropy(x, w, y, reduction="none")
+    keep = torch.arange(33, device=cuda_dev) != 2
+    assert torch.equal(again[keep], nll[keep]) and not bool(again[2].isfinite())
+
+
+@pytest.mark.gpu
+def test_shapes_strides_and_types_of_labels(cuda_dev):
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(60, 400, 128, torch.bfloat16, cuda_dev, 9)
+    want = vocab_cross_entropy(x, w, y, reduction="none")
+    assert torch.equal(vocab_cross_entropy(x.view(3, 20, 128), w, y.view(3, 20), reduction="none"), want.view(3, 20))
+    assert torch.equal(vocab_cross_entropy(x, w, y.int(), reduction="none"), want)
+    wide = torch.zeros(60, 300, device=cuda_dev, dtype=x.dtype)
+    wide[:, 5:133] = x                                   # rows off the 16-byte boundary
+    assert torch.equal(vocab_cross_entropy(wide[:, 5:133], w, y, reduction="none"), want)
+    assert torch.equal(vocab_cross_entropy(x.T.contiguous().T, w.T.contiguous().T, y, reduction="none"), want)
+    lots = torch.stack([y, y], 1)[:, 0]
+    assert torch.equal(vocab_cross_entropy(x, w, lots, reduction="none"), want)
+    row = x[:1].expand(60, 128).requires_grad_()
+    assert vocab_cross_entropy(row, w, y, reduction="none").shape == (60,)
+    for h in (1, 7, 130):                                # widths that are not whole 16-byte lines
+        xs, ws, ys = inputs(37, 333, h, torch.bfloat16, cuda_dev, 10)
+        ys[0] = 5
+        ref = formulas(xs, ws, ys)
+        xs.requires_grad_(), ws.requires_grad_()
+        loss = vocab_cross_entropy(xs, ws, ys)
+        dh, dw = torch.autograd.grad(loss, (xs, ws))
+        within(dh, ref["dh"], ref["tol_h"])
+        within(dw, ref["dw"], ref["tol_w"])
+
+
+@pytest.mark.gpu
+def test_streams_and_repeatability(cuda_dev):
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(300, 2000, 128, torch.bfloat16, cuda_dev, 11)
+    x.requires_grad_(), w.requires_grad_()
+
+    def step():
+        loss = vocab_cross_entropy(x, w, y, piece=512)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w)))
+
+    first = step()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        runs = [step() for _ in range(5)]
+    s.synchronize()
+    for r in runs:
+        assert all(torch.equal(a, b) for a, b in zip(first, r))
+
+
+@pytest.mark.gpu
+def test_empty(cuda_dev):
+    from mpq_b200.loss import vocab_cross_entropy
+    w = torch.randn(30, 16, device=cuda_dev).to(torch.bfloat16).requires_grad_()
+    x = torch.zeros(0, 16, device=cuda_dev, dtype=torch.bfloat16, requires_grad=True)
+    y = torch.zeros(0, device=cuda_dev, dtype=torch.int64)
+    assert vocab_cross_entropy(x, w, y, reduction="none").shape == (0,)
+    assert bool(vocab_cross_entropy(x, w, y).isnan())
+    dh, dw = torch.autograd.grad(vocab_cross_entropy(x, w, y, reduction="sum"), (x, w))
+    assert dh.shape == (0, 16) and not dw.any()
+
+
+def test_refusals_without_a_gpu():
+    from mpq_b200 import _lib
+    from mpq_b200.loss import vocab_cross_entropy
+    with pytest.raises(ValueError, match="CUDA"):
+        vocab_cross_entropy(torch.zeros(2, 8), torch.zeros(4, 8), torch.zeros(2, dtype=torch.int64))
+    lib = _lib.load()
+    f = lambda **k: lib.mpq_xent_forward(*{**dict(T=4, V=9, H=8, dtype=1, h=16, ldh=8, w=16, ldw=8, y=16, ignore=-100,  # noqa: E731
+                                                  part=16, n=8, tgt=16, lse=16, nll=16, status=16, stream=None), **k}.values())
+    assert f(dtype=0) == 10001 and f(ldh=12) == 10001 and f(h=8) == 10001 and f(n=7) == 10001 and f(status=None) == 10001
+    assert f(T=0) == 0
+    b = lambda **k: lib.mpq_xent_backward(*{**dict(T=4, V=600, H=8, dtype=1, h=16, ldh=8, w=16, ldw=8, y=16, ignore=-100,  # noqa: E731
+                                                   lse=16, gout=16, gs=0, count=None, gmax=16, d=16, piece=256, acc=16, dh=16,
+                                                   lddh=8, dw=16, lddw=8, status=16, stream=None), **k}.values())
+    assert b(piece=100) == 10001 and b(acc=None) == 10001 and b(lddh=7) == 10001 and b(d=None) == 10001 and b(dtype=3) == 10001
+
+
+@pytest.mark.gpu
+def test_refusals(cuda_dev):
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(4, 30, 16, torch.bfloat16, cuda_dev)
+    for bad, match in (((x.float(), w.float(), y), "bfloat16 or float16"), ((x, w.half(), y), "one type"),
+                       ((x[:, :8], w, y), "does not fit"), ((x, w[:0], y), "empty"), ((x, w, y[:3]), "labels"),
+                       ((x, w, y.float()), "int64"), ((x, w, y.cpu()), "CUDA")):
+        with pytest.raises(ValueError, match=match):
+            vocab_cross_entropy(*bad)
+    with pytest.raises(ValueError, match="reduction"):
+        vocab_cross_entropy(x, w, y, reduction="avg")
+    with pytest.raises(ValueError, match="piece"):
+        vocab_cross_entropy(x, w, y, piece=0)

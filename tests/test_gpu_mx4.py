@@ -1,0 +1,301 @@
+"""Microscaled 4-bit operators against a plain 64-bit implementation of the format.
+
+The format's own rounding is exact (power-of-two scales, ties defined), so codes and scales are compared bit for bit.
+A product accumulates in the tensor cores' FP32: 1e-5 of sum |a| |b| (the bound that this package's other tensor-core
+products are held to), plus one rounding to the output's type, 2^-8 (bf16), 2^-11 (f16) or 2^-24 (f32) of the result;
+f16 results below its normal range round to multiples of 2^-24.
+"""
+import math
+
+import pytest
+import torch
+
+GRID = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
+ROUND = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+DTYPES = list(ROUND)
+
+
+def plain_quantize(x):
+    """(codes rows x padded cols, scale codes rows x blocks), by search over the grid in 64 bits."""
+    rows, cols = x.shape
+    nb = -(-cols // 32)
+    b = torch.zeros(rows, nb * 32, dtype=torch.float64)
+    b[:, :cols] = x.double().cpu()
+    b = b.view(rows, nb, 32)
+    finite = torch.isfinite(b).all(2)
+    top = torch.where(finite, b.abs().amax(2), 1.0)
+    mantissa, e = torch.frexp(top)  # top = m 2^e, m in [0.5, 1): floor(log2 top) = e - 1
+    c = torch.where(top == 0, 0, (e - 3 + 127).clamp(min=0))
+    a = torch.where(finite[..., None], b.abs() / torch.pow(2.0, c.double() - 127)[..., None], 0.0)
+    gap = (a[..., None] - GRID).abs()
+    near = gap == gap.amin(-1, keepdim=True)
+    even = near & (torch.arange(8) % 2 == 0)
+    code = torch.where(even.any(-1), even.double().argmax(-1), near.double().argmax(-1))
+    code = code + 8 * torch.signbit(b).long()
+    return torch.where(finite[..., None], code, 0).view(rows, -1), torch.where(finite, c.long(), 255)
+
+
+def plain_values(code, c):
+    q = GRID[code & 7] * torch.where(code >= 8, -1.0, 1.0)
+    s = torch.where(c == 255, float("nan"), torch.pow(2.0, c.double() - 127))
+    return (q.view(code.shape[0], -1, 32) * s[..., None]).view(code.shape)
+
+
+def unpack(q):
+    """Codes and scale codes of an Mx4Tensor from its stored form."""
+    codes, scales, (rows, cols) = q.codes.cpu().long(), q.scales.cpu().long(), q.shape
+    nb = -(-cols // 32)
+    code = torch.stack([codes % 16, codes // 16], 2).view(rows, -1)
+    r, j = torch.arange(rows)[:, None], torch.arange(nb)[None]
+    return code, scales[r // 128, j // 4, (r % 32) * 16 + r % 128 // 32 * 4 + j % 4]
+
+
+def same_but_zero_sign(a, b):
+    return bool(((a == b) | ((a & 7) == 0) & ((b & 7) == 0)).all())
+
+
+def values(rows, cols, dtype, dev, seed=0, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g) * torch.exp(spread * torch.randn(rows, max(-(-cols // 8), 1), generator=g)
+                                                         ).repeat_interleave(8, 1)[:, :cols]
+    return x.clamp(-6e4, 6e4).to(dtype).to(dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 32), (3, 31), (2, 33), (127, 100), (129, 256), (257, 1000), (64, 4096)])
+def test_quantize_codes_and_values(cuda_dev, shape, dtype):
+    from mpq_b200.mx4 import dequantize_mx4, quantize_mx4
+    x = values(*shape, dtype, cuda_dev)
+    q = quantize_mx4(x)
+    code, c = unpack(q)
+    want_code, want_c = plain_quantize(x)
+    assert torch.equal(c, want_c)
+    assert same_but_zero_sign(code, want_code)
+    want = plain_values(want_code, want_c)[:, :shape[1]]
+    for out in DTYPES:
+        got = dequantize_mx4(q, out)
+        assert got.dtype == out and torch.equal(got.cpu().double(), want.to(out).double())
+
+
+@pytest.mark.gpu
+def test_quantize_pads_are_zero(cuda_dev):
+    from mpq_b200.mx4 import quantize_mx4, stored_shapes
+    from mpq_b200._lib import call, ptr
+    x = values(130, 70, torch.float32, cuda_dev)
+    codes_shape, scales_shape = stored_shapes(130, 70)
+    codes = torch.full(codes_shape, 0xAB, device=cuda_dev, dtype=torch.uint8)
+    scales = torch.full(scales_shape, 0xFF, device=cuda_dev, dtype=torch.uint8)
+    call("mpq_mx4_quantize", ptr(x), 0, 70, 130, 70, ptr(codes), ptr(scales))
+    q = quantize_mx4(x)
+    assert torch.equal(q.codes, codes) and torch.equal(q.scales, scales)
+    code, _ = unpack(q)
+    assert not (code[:, 70:] & 7).any()
+    real = torch.zeros(scales_shape, dtype=torch.bool)
+    r, j = torch.arange(130)[:, None], torch.arange(3)[None]
+    real[r // 128, j // 4, (r % 32) * 16 + r % 128 // 32 * 4 + j % 4] = True
+    assert not scales.cpu()[~real].any()
+
+
+@pytest.mark.gpu
+def test_every_tie_and_edge_value(cuda_dev):
+    """Midpoints of the grid, their neighbours in bf16 and f32, saturation, and the ends of the scale's range."""
+    from mpq_b200.mx4 import dequantize_mx4, quantize_mx4
+    mids = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 7.9]
+    for dtype in (torch.float32, torch.bfloat16):
+        eps = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -7
+        near = [m * (1 + s * eps) for m in mids for s in (-1, 0, 1)]
+        rows = []
+        for e in (-124, -60, 0, 60, 122):
+            body = [sign * v * 2.0 ** e for v in near for sign in (1, -1)]
+            for i in range(0, len(body), 31):
+                part = body[i:i + 31]
+                rows.append([4.0 * 2.0 ** e] + part + [0.0] * (31 - len(part)))
+        x = torch.tensor(rows, dtype=torch.float64).to(dtype).to(cuda_dev)
+        code, c = unpack(quantize_mx4(x))
+        want_code, want_c = plain_quantize(x)
+        assert torch.equal(c, want_c) and same_but_zero_sign(code, want_code)
+        assert torch.equal(dequantize_mx4(quantize_mx4(x)).cpu().double(), plain_values(want_code, want_c))
+    tiny = torch.zeros(4, 32)
+    tiny[0, 3] = 2.0 ** -149
+    tiny[1, :] = 2.0 ** -127
+    tiny[2, 5] = 3.0e38
+    x = tiny.to(cuda_dev)
+    want_code, want_c = plain_quantize(x)
+    code, c = unpack(quantize_mx4(x))
+    assert torch.equal(c, want_c) and same_but_zero_sign(code, want_code)
+    assert c[3, 0] == 0  # an empty block
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_non_finite_blocks_read_back_as_nan(cuda_dev, dtype):
+    from mpq_b200.mx4 import Mx4Tensor, dequantize_mx4, mx4_linear, quantize_mx4
+    x = values(5, 100, dtype, cuda_dev, spread=0.5)
+    x[1, 40], x[2, 99], x[4, 0] = float("nan"), float("inf"), float("-inf")
+    back = dequantize_mx4(quantize_mx4(x))
+    bad = torch.zeros(5, 100, dtype=torch.bool)
+    bad[1, 32:64] = bad[2, 96:] = bad[4, :32] = True
+    assert torch.equal(back.cpu().isnan(), bad)
+    w = quantize_mx4(values(70, 100, dtype, cuda_dev, 1, 0.5))
+    y = mx4_linear(x, w)
+    assert torch.equal(y.isnan().all(1).cpu(), bad.any(1)) and torch.equal(y.isnan().any(1).cpu(), bad.any(1))
+    assert isinstance(w, Mx4Tensor)
+
+
+def check_linear(x, w, bias=None):
+    from mpq_b200.mx4 import mx4_linear, quantize_mx4
+    k = x.shape[-1]
+    a = plain_values(*plain_quantize(x.reshape(-1, k)))
+    b = plain_values(*plain_quantize(w))
+    ref, size = a @ b.T, a.abs() @ b.abs().T
+    if bias is not None:
+        ref, size = ref + bias.double().cpu(), size + bias.double().cpu().abs()
+    y = mx4_linear(x, quantize_mx4(w), bias)
+    assert y.dtype == x.dtype and y.shape == (*x.shape[:-1], w.shape[0])
+    err = (y.reshape(ref.shape).cpu().double() - ref).abs()
+    tol = 1e-5 * size + ROUND[x.dtype] * ref.abs() + (2.0 ** -24 if x.dtype == torch.float16 else 0)
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 256), (1, 300, 4096), (2, 129, 96), (3, 1000, 520), (7, 257, 2048),
+                                   (8, 64, 33), (9, 512, 1056), (16, 200, 640), (33, 700, 128), (64, 1024, 992),
+                                   (127, 130, 700), (128, 128, 512), (129, 383, 1000), (256, 256, 2304), (333, 1531, 1000),
+                                   (700, 900, 224), (1100, 2100, 160)])
+def test_linear(cuda_dev, m, n, k, dtype):
+    x = values(m, k, dtype, cuda_dev, 2, 0.7)
+    w = values(n, k, dtype, cuda_dev, 3, 0.7) * 0.05
+    check_linear(x, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 5, 40, 200])
+def test_linear_bias_strides_and_leading_dimensions(cuda_dev, m):
+    g = torch.Generator().manual_seed(5)
+    w = (torch.randn(193, 416, generator=g) * 0.1).to(cuda_dev)
+    bias = torch.randn(193, generator=g).to(cuda_dev).to(torch.bfloat16)
+    x = torch.randn(m, 3, 416, generator=g).to(cuda_dev).to(torch.bfloat16)
+    check_linear(x, w, bias)
+    wide = torch.randn(m, 500, generator=g).to(cuda_dev).to(torch.bfloat16)
+    check_linear(wide[:, 3:419], w, bias)                   # rows at odd offsets
+    check_linear(torch.randn(416, m, generator=g).to(cuda_dev).to(torch.bfloat16).T, w)  # columns along the rows
+    check_linear(x[:, 1], w)                                # every third row
+    check_linear(x[:1, :1].expand(m, 1, 416), w)            # one row, broadcast
+
+
+@pytest.mark.gpu
+def test_linear_masked_inputs_of_lowest_value(cuda_dev):
+    """Rows of zeros, and blocks that hold a type's lowest value next to ordinary ones (the scale follows it)."""
+    x = values(6, 256, torch.bfloat16, cuda_dev, 7, 0.5)
+    x[2] = 0
+    x[3, 64:96] = 0
+    x[4, 5] = torch.finfo(torch.bfloat16).min
+    w = values(130, 256, torch.bfloat16, cuda_dev, 8, 0.5) * 0.01
+    check_linear(x[:4], w)
+    check_linear(x.float(), w.float() * 1e-3)
+
+
+@pytest.mark.gpu
+def test_scales_at_the_ends_of_their_range_in_a_product(cuda_dev):
+    """Denormal inputs against large weights: scales 2^-127 .. 2^100, the result in FP32's range."""
+    x = values(4, 96, torch.float32, cuda_dev, 9, 0.3) * 2.0 ** -124
+    w = values(40, 96, torch.float32, cuda_dev, 10, 0.3) * 2.0 ** 100
+    check_linear(x, w)
+    check_linear(x.repeat(20, 1), w)
+
+
+@pytest.mark.gpu
+def test_empty_and_repeatable(cuda_dev):
+    from mpq_b200.mx4 import dequantize_mx4, mx4_linear, quantize_mx4
+    w = quantize_mx4(values(64, 96, torch.bfloat16, cuda_dev))
+    assert mx4_linear(torch.zeros(0, 96, device=cuda_dev), w).shape == (0, 64)
+    assert mx4_linear(torch.zeros(2, 0, 96, device=cuda_dev), w).shape == (2, 0, 64)
+    none = quantize_mx4(torch.zeros(5, 0, device=cuda_dev))
+    assert dequantize_mx4(none).shape == (5, 0)
+    bias = torch.ones(5, device=cuda_dev)
+    assert torch.equal(mx4_linear(torch.zeros(3, 0, device=cuda_dev), none, bias), torch.ones(3, 5, device=cuda_dev))
+    assert dequantize_mx4(quantize_mx4(torch.zeros(0, 33, device=cuda_dev))).shape == (0, 33)
+    for m in (1, 6, 50, 300):
+        x = values(m, 96, torch.bfloat16, cuda_dev, m)
+        assert torch.equal(mx4_linear(x, w), mx4_linear(x, w))
+
+
+@pytest.mark.gpu
+def test_another_stream_and_layers(cuda_dev):
+    """Work queued on a stream of its own, and the module form against the function."""
+    from mpq_b200.mx4 import Mx4Linear, convert_linears_mx4, mx4_linear, quantize_mx4
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Linear(160, 96), torch.nn.Sequential(torch.nn.Linear(96, 40, bias=False))
+                              ).to(cuda_dev).to(torch.bfloat16)
+    x = values(37, 160, torch.bfloat16, cuda_dev, 1, 0.3)
+    want = mx4_linear(mx4_linear(x, quantize_mx4(net[0].weight), net[0].bias), quantize_mx4(net[1][0].weight))
+    assert convert_linears_mx4(net) == 2 and isinstance(net[1][0], Mx4Linear)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        outs = [net(x) for _ in range(20)]
+    s.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    state = net.state_dict()
+    assert math.prod(state["0.codes"].shape) == 96 * 160 // 2
+
+
+@pytest.mark.gpu
+def test_product_in_a_cuda_graph(cuda_dev):
+    from mpq_b200.mx4 import mx4_linear, quantize_mx4
+    w = quantize_mx4(values(300, 512, torch.bfloat16, cuda_dev, 3, 0.3))
+    for m in (1, 30, 150):
+        x = values(m, 512, torch.bfloat16, cuda_dev, 4, 0.3)
+        mx4_linear(x, w)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = mx4_linear(x, w)
+        x.copy_(values(m, 512, torch.bfloat16, cuda_dev, 5, 0.3))
+        graph.replay()
+        assert torch.equal(y, mx4_linear(x, w))
+
+
+def test_refusals_without_a_gpu():
+    from mpq_b200 import _lib
+    from mpq_b200.mx4 import Mx4Tensor, dequantize_mx4, mx4_linear, quantize_mx4
+    x = torch.zeros(4, 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        quantize_mx4(x)
+    with pytest.raises(ValueError, match="uint8"):
+        Mx4Tensor(torch.zeros(4, 32), torch.zeros(1, 1, 512, dtype=torch.uint8), (4, 64))
+    with pytest.raises(ValueError, match="codes"):
+        Mx4Tensor(torch.zeros(4, 31, dtype=torch.uint8), torch.zeros(1, 1, 512, dtype=torch.uint8), (4, 64))
+    q = Mx4Tensor(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(1, 1, 512, dtype=torch.uint8), (4, 64))
+    with pytest.raises(ValueError, match="CUDA"):
+        dequantize_mx4(q)
+    with pytest.raises(ValueError, match="CUDA"):
+        mx4_linear(x, q)
+    lib = _lib.load()
+    assert lib.mpq_mx4_quantize(16, 7, 64, 4, 64, 16, 16, None) == 10001
+    assert lib.mpq_mx4_quantize(16, 0, 63, 4, 64, 16, 16, None) == 10001
+    assert lib.mpq_mx4_quantize(None, 0, 64, 4, 64, 16, 16, None) == 10001
+    assert lib.mpq_mx4_quantize(16, 0, 64, 4, 64, 8, 16, None) == 10001 and b"aligned" in lib.mpq_last_error()
+    assert lib.mpq_mx4_dequantize(16, 16, 4, 64, 16, 0, 63, None) == 10001
+    assert lib.mpq_mx4_gemm(4, 4, 0, 16, 16, 16, 16, None, 16, 0, 4, 16, None) == 10001
+    assert lib.mpq_mx4_gemm(4, 4, 64, 16, 16, 16, 16, None, 16, 0, 4, None, None) == 10001
+    assert lib.mpq_mx4_quantize(None, 0, 64, 0, 64, None, None, None) == 0
+
+
+@pytest.mark.gpu
+def test_refusals(cuda_dev):
+    from mpq_b200.mx4 import mx4_linear, quantize_mx4
+    w = quantize_mx4(torch.zeros(8, 64, device=cuda_dev))
+    with pytest.raises(ValueError, match="columns"):
+        mx4_linear(torch.zeros(2, 65, device=cuda_dev), w)
+    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+        mx4_linear(torch.zeros(2, 64, device=cuda_dev, dtype=torch.float64), w)
+    with pytest.raises(ValueError, match="bias"):
+        mx4_linear(torch.zeros(2, 64, device=cuda_dev), w, torch.zeros(8, device=cuda_dev, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="bias"):
+        mx4_linear(torch.zeros(2, 64, device=cuda_dev), w, torch.zeros(7, device=cuda_dev))
+    with pytest.raises(ValueError, match="different devices"):
+        mx4_linear(torch.zeros(2, 64, device=cuda_dev), w.to("cpu"))
+    with pytest.raises(ValueError, match="dimension"):
+        quantize_mx4(torch.zeros((), device=cuda_dev))
