@@ -461,27 +461,34 @@ int mpq_mx4_gemm(int M, int N, int K, const uint8_t* a_codes, const uint8_t* a_s
 
 /* ---- softmax cross entropy over a vocabulary, from hidden states (T x H) and the output head (V x H) ----
  * No counterpart in the reference (its perplexity scripts call a library's loss on whole logits).  The logits are
- * never stored.  dtype: 1 bfloat16, 2 float16 (hidden, weight and their gradients); operands 16-byte aligned with
+ * not stored.  dtype: 1 bfloat16, 2 float16 (hidden, weight and their gradients); operands 16-byte aligned with
  * leading dimensions that are multiples of 8.  Labels equal to `ignore` do not count; labels outside [0, V) give NaN.
  * `status`: as mpq_gemm_tc. */
 
 /* Columns of `part` below. */
 int mpq_xent_tiles(int V);
-/* lse[t] = log sum_v exp(h_t . w_v), nll[t] = lse[t] - h_t . w_y (0 where ignored).  Workspaces: part, T x
- * mpq_xent_tiles(V) pairs of floats (part_floats: floats it holds); tgt, T floats. */
+/* Planes of T x H floats that mpq_xent_backward needs in `acc` for dhidden (0: none). */
+int mpq_xent_planes(int T, int V, int H, int piece, int keep_cols);
+/* lse[t] = log sum_v exp(h_t . w_v), nll[t] = lse[t] - h_t . w_y (0 where ignored).
+ * reduction: 0 none; 1 loss = sum of nll; 2 loss = that over the number of counted labels (NaN for none); count = that
+ * number.  Workspaces: part, T x
+ * mpq_xent_tiles(V) pairs of floats (part_floats: floats it holds); tgt, T floats.  keep_cols != 0 (V, or a multiple of 256 below it): keep
+ * receives, for mpq_xent_backward, 16-bit distances of those first columns' logits below their tile's largest (T rows,
+ * leading dimension ldk). */
 int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                      const int64_t* labels, int64_t ignore, float* part, int64_t part_floats, float* tgt, float* lse,
-                     float* nll, int* status, void* stream);
-/* loss = sum of nll, divided by the number of counted labels where mean != 0 (NaN for none); count = that number. */
-int mpq_xent_reduce(int T, const float* nll, const int64_t* labels, int64_t ignore, int mean, float* loss, float* count,
-                    void* stream);
+                     float* nll, int reduction, float* loss, float* count, void* keep, int64_t ldk, int keep_cols,
+                     int* status, void* stream);
 /* dhidden (T x H) and dweight (V x H), either may be NULL, from lse and the upstream gradient gout[t * gstride] of
- * each nll (divided by *count where count is given).  Workspaces: gmax, one float; d, T x piece 16-bit values (piece: a
- * multiple of 256 columns); acc, T x H floats, needed for dhidden where V > piece. */
+ * each nll (divided by *count where count is given).  keep, ldk, keep_cols, part and tgt: what mpq_xent_forward left
+ * (keep is overwritten; keep_cols = 0: nothing was kept).  The other columns' logits are computed again, `piece` (a
+ * multiple of 256) columns at a time.  Workspaces: gmax, one float (with gstride != 0); d, T x piece 16-bit values (unless all columns were
+ * kept); acc, mpq_xent_planes(T, V, H, piece, keep_cols) x T x H floats. */
 int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                       const int64_t* labels, int64_t ignore, const float* lse, const float* gout, int gstride,
-                      const float* count, float* gmax, void* d, int piece, float* acc, void* dhidden, int64_t lddh,
-                      void* dweight, int64_t lddw, int* status, void* stream);
+                      const float* count, const float* part, const float* tgt, void* keep, int64_t ldk, int keep_cols,
+                      float* gmax, void* d, int piece, float* acc, void* dhidden, int64_t lddh, void* dweight,
+                      int64_t lddw, int* status, void* stream);
 
 /* ---- rotation ----
  * Block Walsh-Hadamard of the last dim, blocks of `had` (power of two <= 16384), normalized by sqrt(had);

@@ -106,9 +106,9 @@ SIGNATURES: Dict[str, Tuple[Any, ...]] = {
     "mpq_mx4_dequantize": (P, P, I, I, P, I, L, P),
     "mpq_mx4_gemm": (I, I, I, P, P, P, P, P, P, I, L, P, P),
     "mpq_xent_tiles": (I,),
-    "mpq_xent_forward": (I, I, I, I, P, L, P, L, P, L, P, L, P, P, P, P, P),
-    "mpq_xent_reduce": (I, P, P, L, I, P, P, P),
-    "mpq_xent_backward": (I, I, I, I, P, L, P, L, P, L, P, P, I, P, P, P, I, P, P, L, P, L, P, P),
+    "mpq_xent_planes": (I, I, I, I, I),
+    "mpq_xent_forward": (I, I, I, I, P, L, P, L, P, L, P, L, P, P, P, I, P, P, P, L, I, P, P),
+    "mpq_xent_backward": (I, I, I, I, P, L, P, L, P, L, P, P, I, P, P, P, P, L, I, P, P, I, P, P, L, P, L, P, P),
 }
 
 _lib = None
@@ -143,6 +143,20 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call_on(index: int, name: str, *args) -> None:
+    """``call`` on a given device, whichever is current, on that device's current stream.  The raw-stream look-up spares
+    a short operator the microseconds that building a stream object takes."""
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return call_on(index, name, *args)
+    lib = _lib or load()
+    status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    _trace.count_launch()
+    if status != 0:
+        msg = lib.mpq_last_error().decode(errors="replace")
+        raise RuntimeError(f"{name} failed with status {status}: {msg}")
 
 
 def call(name: str, *args) -> None:

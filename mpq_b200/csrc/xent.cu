@@ -3,20 +3,25 @@
 //   l[t, v] = h_t . w_v,   lse_t = log sum_v exp l[t, v],   nll_t = lse_t - l[t, y_t]
 //   d[t, v] = g_t (exp(l[t, v] - lse_t) - [v = y_t]),   dH = d W,   dW = d^T H
 //
-// The logits are never stored.  The forward product reduces each 256-column tile of a token's logits to (max, sum of
-// exp) in its epilogue and picks the label's logit out on the way; a second kernel joins the tiles in order.  The
-// backward pass takes the vocabulary in pieces: it computes a piece's logits again, turns them into d in 16 bits in the
-// epilogue, and multiplies d with the piece of W (dH, summed over the pieces in FP32) and with H (dW's rows of the
-// piece).  Every sum runs in a fixed order, so results repeat bit for bit.
+// The forward product reduces each 128 columns of a token's logits to (max, sum of exp) in its epilogue and picks the
+// label's logit out on the way; a second kernel joins them in order.  The logits are not stored.  Where the caller has
+// room for them, the first columns' distances below the largest of their 128 columns are kept for the backward pass, in
+// 16 bits (log2 units, steps of 2^-11: exp(l) within 2^-12.5 of itself down to 2^-32 of the largest; a bf16 exponential
+// would have rounded d a second time by 2^-9).  They save a quarter of a training step's products for two bytes an
+// entry.  The backward pass takes the vocabulary in pieces: the kept columns first, then pieces whose
+// logits it computes again, with d in 16 bits as the epilogue's result; it multiplies a piece's d with its rows of W
+// (dH, summed over the pieces in FP32) and with H (dW's rows of the piece).  Every sum runs in a fixed order, so
+// results repeat bit for bit.
 //
-// d is held as 2^k d / max|g|, in units of its largest possible magnitude, and the products take the factor back in
-// FP32: in f16 (k = 15) probabilities down to 2^-39 then stay normal numbers, whatever the mean divides by; bf16 has
+// d is held as 2^k d / u, with u = max|g| (or g itself where all tokens share it), in units of its largest possible
+// magnitude, and the products take the factor back in FP32: in f16 (k = 15) probabilities down to 2^-39 then stay normal numbers, whatever the mean divides by; bf16 has
 // the exponent range and takes k = 0.  Rounding d to 16 bits costs each of its entries 2^-9 (bf16) or 2^-12 (f16) of
 // itself, no more than the rounding of the gradients to the same type.
 //
 // A label equal to `ignore` does not count: nll 0, d 0.  A label outside the vocabulary makes the token's nll and its
 // d NaN; no memory is read for it.
 #include <algorithm>
+#include <cmath>
 #include <cuda_bf16.h>
 #include "umma.cuh"
 
@@ -25,15 +30,20 @@ namespace xent {
 
 using namespace tc;
 
-constexpr int kThreads = 192;
-constexpr int kBM = 128, kBN = 256, kStages = 4, kGroup = 16;
-constexpr uint32_t kStageA = kBM * 128, kStageB = kBN * 128;
+// A tile is 256 x 256 NH, computed by a pair of CTAs: each holds 128 rows of A, 128 NH of B and of the accumulator 128
+// rows by 256 NH columns of TMEM.
+constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
+constexpr int kBM = 256, kBN = 256, kGroup = 16;
+__host__ __device__ constexpr int stages_of(int NH) { return NH == 2 ? 4 : 6; }
+constexpr uint32_t kHalf = 128 * 128;  // bytes of an operand's 128 rows of one k-block (64 columns, one swizzle line)
+constexpr int kChunk = 8;              // k-blocks that the forward pass accumulates before it adds in FP32
 constexpr float kLog2e = 1.4426950408889634f;
 
 enum { kLse = 0, kGrad = 1, kOut = 2 };
 
 struct Args {
-  int M, N, K, mt, nt;      // C[M, N] over K; tiles of 128 x 256
+  int M, N, K, mt, nt;      // C[M, N] over K; mt x nt tiles
+  int splits;               // parts of K; more than one only with `acc`
   int f16;                  // 1: f16 operands, 0: bf16
   int* status;
   // kLse, kGrad
@@ -41,18 +51,20 @@ struct Args {
   int64_t ignore;
   int vocab;                // labels in [0, vocab) count
   int v0;                   // first column's vocabulary index
-  float2* part;             // kLse: [M, nt] (max in log2 units, sum of exp2)
+  float2* part;             // kLse: [M, 2 nt] (max in log2 units, sum of exp2) of 128 columns each
   float* tgt;               // kLse: [M] the label's logit
+  uint16_t* keep;           // kLse: distances of the columns below keep_cols (a multiple of 256, or N), [M, ldk]
+  int64_t ldk;
+  int keep_cols;
   const float* lse;         // kGrad: [M]
   const float* gout;        // kGrad: upstream gradient, gout[t * gstride]
   int gstride;
   const float* count;       // kGrad: divides g where given (the mean's number of labels)
-  const float* gmax;        // kGrad, kOut: largest |g| of the counted tokens
+  const float* gmax;        // kGrad, kOut: largest |g| of the counted tokens; null: all share g
   // kGrad, kOut
   void* out;
   int64_t ldo;
-  float* acc;               // kOut: FP32 running sum [M, N], contiguous; null: C goes straight to `out`
-  int first, last;          // kOut with acc: start the sum / round it to `out`
+  float* acc;               // kOut: FP32 planes [splits, M, N], one for each part of K; null: C goes straight to `out`
 };
 
 // MN-major operand in the 128B-swizzled layout: 64 elements of the row dimension to a 128-byte line, one line for each
@@ -77,21 +89,38 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int f16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Tile t of a raster that walks kGroup row tiles down before it takes the next column tile: the tiles in flight share
-// a few row tiles (kept in L2) and stream the columns once for each group.
-__device__ __forceinline__ void tile_at(int t, int mt, int nt, int& mb, int& nb) {
-  const int per = kGroup * nt, g = t / per, r = t - g * per;
-  const int rows = min(kGroup, mt - g * kGroup);
-  mb = g * kGroup + r % rows;
-  nb = r / rows;
+// A token's factor in d, in units of unit_of(), and that unit.
+__device__ __forceinline__ float factor_of(bool inside, const float* gout, int64_t at, const float* count,
+                                           const float* gmax, int f16) {
+  const float top = f16 ? 32768.f : 1.f;
+  if (!inside) return __int_as_float(0x7fc00000);
+  if (!gmax) return top;
+  const float g = count ? gout[at] / *count : gout[at];
+  return *gmax == 0.f && g == 0.f ? 0.f : g / *gmax * top;
+}
+__device__ __forceinline__ float unit_of(const float* gout, const float* count, const float* gmax, int f16) {
+  const float u = gmax ? *gmax : (count ? (*count > 0.f ? *gout / *count : 0.f) : *gout);
+  return f16 ? u * (1.f / 32768.f) : u;
 }
 
-// 32 consecutive 16-bit results of one row.
-__device__ __forceinline__ void store16(void* out, int64_t at, const float (&o)[32], int lim, int f16) {
-  uint16_t* dst = reinterpret_cast<uint16_t*>(out) + at;
-  uint32_t w[16];
-  #pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = pack16(o[2 * i], o[2 * i + 1], f16);
+// Unit u -> its tile and range of k-blocks.  The raster walks kGroup row tiles down before it takes the next column
+// tile: the tiles in flight share a few row tiles (kept in L2) and stream the columns once for each group.
+__device__ __forceinline__ void unit_at(int u, const Args& p, int kblocks, int& mb, int& nb, int& k0, int& k1) {
+  const int t = u / p.splits, s = u - t * p.splits;
+  const int per = kGroup * p.nt, g = t / per, r = t - g * per;
+  const int rows = min(kGroup, p.mt - g * kGroup);
+  mb = g * kGroup + r % rows;
+  nb = r / rows;
+  k0 = (int)((int64_t)kblocks * s / p.splits);
+  k1 = (int)((int64_t)kblocks * (s + 1) / p.splits);
+}
+
+// k-blocks to an accumulator
+template <int EPI>
+__device__ __forceinline__ int chunk_of(int kblocks) { return EPI == kLse ? kChunk : kblocks; }
+
+// 32 consecutive 16-bit values of one row, `lim` of them wanted.
+__device__ __forceinline__ void store_words(uint16_t* dst, const uint32_t (&w)[16], int lim) {
   if (lim >= 32 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
     #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -102,26 +131,57 @@ __device__ __forceinline__ void store16(void* out, int64_t at, const float (&o)[
       if (i < lim) dst[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
   }
 }
+__device__ __forceinline__ void store16(void* out, int64_t at, const float (&o)[32], int lim, int f16) {
+  uint32_t w[16];
+  #pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = pack16(o[2 * i], o[2 * i + 1], f16);
+  store_words(reinterpret_cast<uint16_t*>(out) + at, w, lim);
+}
+
+// 2^t in one instruction (denormal results become 0, 2^-22 relative)
+__device__ __forceinline__ float ex2(float t) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
+
+// Kept distances: t = log2 units below the maximum (t <= 0), in steps of 1 / kStep.  The sum with 2^23 rounds to a whole
+// number, whose bits end the mantissa.
+constexpr float kStep = 2048.f;
+__device__ __forceinline__ uint32_t distance_bits(float t) {
+  return __float_as_uint(fminf(fmaf(t, -kStep, 8388608.f), 8388608.f + 65535.f));
+}
 
 // C[M, N] = A B with an epilogue.  A K-major: [M, K] rows; A_MN: [K, M] rows.  B likewise ([N, K] or [K, N] rows).
-// 16-bit operands, FP32 accumulation in TMEM; persistent over the tiles, two accumulators.  Warp 0 loads (TMA), warp 1
-// issues the MMAs, warps 2..5 are the epilogue, one row to a thread.
-template <int EPI, bool A_MN, bool B_MN>
-__global__ void __launch_bounds__(kThreads, 1)
+// 16-bit operands, FP32 accumulation in TMEM.  Persistent pairs of CTAs walk the 256 x 256 tiles (or, with `splits`,
+// a K range of a tile); in each CTA warp 0 loads its halves of the operands by TMA into a ring, warps 2..9 are the
+// epilogue, a row and 128 columns to a thread; warp 1 of the first CTA issues the MMAs of both (M = 256, N = 256,
+// tcgen05 cta_group::2), so that each CTA's shared memory feeds 128 columns of B instead of 256.
+// NH = 1: two accumulators of 256 columns let the epilogue overlap the next tile's MMAs.  NH = 2: a tile of 512 columns
+// fills TMEM, and each loaded row of A serves twice as many columns (48 KB of operands for 1024 tensor cycles, not
+// 2 x 32 KB); the next tile's first half starts when the epilogue has read the first half.
+//
+// The tensor core's FP32 accumulator truncates, and a score is a small difference of sums of H products; so the
+// forward pass (kLse) accumulates kChunk k-blocks at a time and adds these to nearest in registers.
+template <int EPI, bool A_MN, bool B_MN, int NH>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     k_xent_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * (kStageA + kStageB));
+  constexpr int kStages = stages_of(NH);
+  constexpr uint32_t kStage = (1 + NH) * kHalf;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kStage);
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  auto s_a = [&](int s) { return ring + s * kStageA; };
-  auto s_b = [&](int s) { return ring + kStages * kStageA + s * kStageB; };
+  auto s_a = [&](int s) { return ring + s * kStage; };
+  auto s_b = [&](int s, int h) { return ring + s * kStage + (1 + h) * kHalf; };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int nkb = (p.K + 63) / 64, tiles = p.mt * p.nt;
+  const int rank = (int)cluster_rank(), pairs = gridDim.x >> 1;
+  const int kblocks = (p.K + 63) / 64, units = p.mt * p.nt * p.splits;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -129,18 +189,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4);
+      mbar_init(&acc_empty[b], 2 * kEpiWarps);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u)
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u)
                  : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  cluster_sync();  // both CTAs' barriers are initialised before any is signalled
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
 
@@ -148,79 +209,89 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int64_t it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        int mb, nb;
-        tile_at(t, p.mt, p.nt, mb, nb);
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
+      for (int u = blockIdx.x >> 1; u < units && ok; u += pairs) {
+        int mb, nb, k0, k1;
+        unit_at(u, p, kblocks, mb, nb, k0, k1);
+        const int row_a = mb * kBM + rank * 128;
+        for (int kb = k0; kb < k1; ++kb, ++it) {
           const int s = (int)(it % kStages);
-          if (*abort_flag || !mbar_wait(&empty[s], ((uint32_t)(it / kStages) & 1u) ^ 1u)) {
+          if (*abort_flag || !mbar_wait_cluster(&empty[s], ((uint32_t)(it / kStages) & 1u) ^ 1u)) {
             ok = false;
             break;
           }
-          mbar_expect_tx(&full[s], kStageA + kStageB);
+          // both CTAs' bytes count on the first one's barrier (a peer's copy may land before the expectation)
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * kStage);
+          const uint32_t bar = mapa(smem_u32(&full[s]), 0);
           if constexpr (A_MN) {
-            #pragma unroll
-            for (int i = 0; i < kBM / 64; ++i)
-              tma_load_2d(s_a(s) + i * 8192, &map_a, &full[s], mb * kBM + i * 64, kb * 64);
+            tma_load_2d_pair(s_a(s), &map_a, bar, row_a, kb * 64);
+            tma_load_2d_pair(s_a(s) + 8192, &map_a, bar, row_a + 64, kb * 64);
           } else {
-            tma_load_2d(s_a(s), &map_a, &full[s], kb * 64, mb * kBM);
+            tma_load_2d_pair(s_a(s), &map_a, bar, kb * 64, row_a);
           }
-          if constexpr (B_MN) {
-            #pragma unroll
-            for (int i = 0; i < kBN / 64; ++i)
-              tma_load_2d(s_b(s) + i * 8192, &map_b, &full[s], nb * kBN + i * 64, kb * 64);
-          } else {
-            tma_load_2d(s_b(s), &map_b, &full[s], kb * 64, nb * kBN);
+          #pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            const int row_b = (nb * NH + h) * kBN + rank * 128;
+            if constexpr (B_MN) {
+              tma_load_2d_pair(s_b(s, h), &map_b, bar, row_b, kb * 64);
+              tma_load_2d_pair(s_b(s, h) + 8192, &map_b, bar, row_b + 64, kb * 64);
+            } else {
+              tma_load_2d_pair(s_b(s, h), &map_b, bar, kb * 64, row_b);
+            }
           }
         }
       }
-      if (!ok) {  // drain the copies in flight (each wait bounded) before the CTA may end
+      if (!ok) {  // drain the copies in flight (each wait bounded); the peer leaves only after the cluster barrier
         *abort_flag = 1;
-        for (int64_t k = it < kStages ? 0 : it - kStages; k < it; ++k)
-          mbar_wait(&full[k % kStages], (uint32_t)(k / kStages) & 1u);
+        if (rank == 0)
+          for (int64_t k = it < kStages ? 0 : it - kStages; k < it; ++k)
+            mbar_wait_cluster(&full[k % kStages], (uint32_t)(k / kStages) & 1u);
         atomicCAS(p.status, 0, 2);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       const uint32_t idesc = idesc16(p.f16, A_MN, B_MN, kBM, kBN);
       int64_t it = 0;
       bool ok = true;
-      int n = 0;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++n) {
-        const int b = n & 1;
-        if (*abort_flag || !mbar_wait(&acc_empty[b], ((uint32_t)(n >> 1) & 1u) ^ 1u)) {
-          ok = false;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const int s = (int)(it % kStages);
-          if (*abort_flag || !mbar_wait(&full[s], (uint32_t)(it / kStages) & 1u)) {
-            ok = false;
-            break;
+      int n = 0;  // accumulators handed over
+      for (int u = blockIdx.x >> 1; u < units && ok; u += pairs) {
+        int mb, nb, k0, k1;
+        unit_at(u, p, kblocks, mb, nb, k0, k1);
+        for (int kc = k0; kc < k1 && ok; kc += chunk_of<EPI>(kblocks), n += NH) {
+          const int ke = min(k1, kc + chunk_of<EPI>(kblocks));
+          for (int kb = kc; kb < ke; ++kb, ++it) {
+            const int s = (int)(it % kStages);
+            if (*abort_flag || !mbar_wait_cluster(&full[s], (uint32_t)(it / kStages) & 1u)) {
+              ok = false;
+              break;
+            }
+            const uint32_t a0 = smem_u32(s_a(s));
+            #pragma unroll
+            for (int h = 0; h < NH; ++h) {
+              const int b = (n + h) & 1;
+              if (kb == kc && !mbar_wait_cluster(&acc_empty[b], ((uint32_t)((n + h) >> 1) & 1u) ^ 1u)) {
+                ok = false;
+                break;
+              }
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              const uint32_t b0 = smem_u32(s_b(s, h));
+              #pragma unroll
+              for (int j = 0; j < 4; ++j) {  // K = 16: 32 bytes along a K-major line, 16 lines of an MN-major operand
+                const uint64_t da = A_MN ? smem_desc_mn_sw128(a0 + j * 2048) : smem_desc_k_sw128(a0 + j * 32);
+                const uint64_t db = B_MN ? smem_desc_mn_sw128(b0 + j * 2048) : smem_desc_k_sw128(b0 + j * 32);
+                asm volatile(
+                    "{\n\t.reg .pred p;\n\t"
+                    "setp.ne.b32 p, %4, 0;\n\t"
+                    "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + b * kBN),
+                    "l"(da), "l"(db), "r"(idesc), "r"((kb > kc || j > 0) ? 1u : 0u)
+                    : "memory");
+              }
+              if (kb == ke - 1) commit_pair(&acc_full[b]);
+            }
+            if (!ok) break;
+            commit_pair(&empty[s]);
           }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t a0 = smem_u32(s_a(s)), b0 = smem_u32(s_b(s));
-          #pragma unroll
-          for (int j = 0; j < 4; ++j) {  // K = 16: 32 bytes along a K-major line, 16 lines of an MN-major operand
-            const uint64_t da = A_MN ? smem_desc_mn_sw128(a0 + j * 2048) : smem_desc_k_sw128(a0 + j * 32);
-            const uint64_t db = B_MN ? smem_desc_mn_sw128(b0 + j * 2048) : smem_desc_k_sw128(b0 + j * 32);
-            asm volatile(
-                "{\n\t.reg .pred p;\n\t"
-                "setp.ne.b32 p, %4, 0;\n\t"
-                "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + b * kBN),
-                "l"(da), "l"(db), "r"(idesc), "r"((kb > 0 || j > 0) ? 1u : 0u)
-                : "memory");
-          }
-          asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                           smem_u32(&empty[s]))
-                       : "memory");
         }
-        // the accumulator is complete (or, after an abort, the issued MMAs have retired)
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                         smem_u32(&acc_full[b]))
-                     : "memory");
       }
       if (!ok) {
         *abort_flag = 1;
@@ -228,101 +299,194 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    const int quad = warp & 3;
+    // a warp reads the TMEM lanes of its quadrant (warp % 4); warps 2..5 take columns 0..127, warps 6..9 the others
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * 128);
     int n = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
-      const int b = n & 1;
-      int mb, nb;
-      tile_at(t, p.mt, p.nt, mb, nb);
-      const bool ready = !*abort_flag && mbar_wait(&acc_full[b], (uint32_t)(n >> 1) & 1u);
+    // the next accumulator in TMEM, false after a time-out
+    auto take = [&]() {
+      const bool ready = !*abort_flag && mbar_wait_cluster(&acc_full[n & 1], (uint32_t)(n >> 1) & 1u);
       if (!__all_sync(0xffffffffu, ready) || *abort_flag) {
         if (!*abort_flag) atomicCAS(p.status, 0, 4);
         *abort_flag = 1;
-        break;
+        return false;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int row = mb * kBM + quad * 32 + lane;
+      return true;
+    };
+    auto release = [&]() {
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(&acc_empty[n & 1]), 0));
+      ++n;
+    };
+    for (int u = blockIdx.x >> 1; u < units; u += pairs) {
+      int mb, nb, k0, k1;
+      unit_at(u, p, kblocks, mb, nb, k0, k1);
+      const int row = mb * kBM + rank * 128 + quad * 32 + lane;
       const bool live = row < p.M;
-      const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * kBN);
-      const int n0 = nb * kBN;
-      int64_t label = -1;
-      float g = 0.f, lse2 = 0.f, alpha = 1.f;
-      if constexpr (EPI == kOut) alpha = *p.gmax * (p.f16 ? 1.f / 32768.f : 1.f);
-      if constexpr (EPI != kOut) {
-        if (live) label = p.labels[row];
-        if constexpr (EPI == kGrad) {
-          if (live && label != p.ignore) {
-            g = label >= 0 && label < p.vocab ? p.gout[(int64_t)row * p.gstride] : __int_as_float(0x7fc00000);
-            if (p.count) g /= *p.count;
-            const float top = *p.gmax;
-            g = top == 0.f && g == 0.f ? 0.f : g / top * (p.f16 ? 32768.f : 1.f);
-            lse2 = p.lse[row] * kLog2e;
-          }
-        }
-        if (label == p.ignore || label < 0 || label >= p.vocab) label = -1;
-        else label -= p.v0 + n0;  // the label's column in this tile, if it is in [0, 256)
-      }
-      float m = -INFINITY, sum = 0.f;
+      bool good = true;
       #pragma unroll 1
-      for (int c0 = 0; c0 < kBN; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld32(trow + c0, v);
-        const int lim = p.N - (n0 + c0);
-        if (lim <= 0) continue;
-        if constexpr (EPI == kLse) {
-          float x[32], top = -INFINITY;
-          #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (label == c0 + i && live) p.tgt[row] = __uint_as_float(v[i]);
-            x[i] = i < lim ? __uint_as_float(v[i]) * kLog2e : -INFINITY;
-            top = fmaxf(top, x[i]);
-          }
-          const float mn = fmaxf(m, top);
-          const float base = mn == -INFINITY ? 0.f : mn;
-          sum *= exp2f(m - base);
-          #pragma unroll
-          for (int i = 0; i < 32; ++i) sum += exp2f(x[i] - base);
-          m = mn;
-        } else if constexpr (EPI == kGrad) {
-          float o[32];
-          #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float e = exp2f(fmaf(__uint_as_float(v[i]), kLog2e, -lse2)) - (label == c0 + i ? 1.f : 0.f);
-            o[i] = g == 0.f ? 0.f : g * e;
-          }
-          if (live) store16(p.out, (int64_t)row * p.ldo + n0 + c0, o, lim, p.f16);
-        } else {
-          float o[32];
-          float* acc = p.acc ? p.acc + (int64_t)row * p.N + n0 + c0 : nullptr;
-          #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            o[i] = alpha * __uint_as_float(v[i]);
-            if (acc && !p.first && live && i < lim) o[i] += acc[i];
-          }
-          if (live) {
-            if (!acc || p.last) {
-              store16(p.out, (int64_t)row * p.ldo + n0 + c0, o, lim, p.f16);
-            } else {
-              #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (i < lim) acc[i] = o[i];
+      for (int h = 0; h < NH; ++h) {
+      const int n0 = (nb * NH + h) * kBN + half * 128;
+      int label = -1;  // the label's column among this thread's 128, if it is one of them
+      float g = 0.f, lse2 = 0.f, alpha = 1.f;
+      if constexpr (EPI == kOut) alpha = unit_of(p.gout, p.count, p.gmax, p.f16);
+      if constexpr (EPI != kOut) {
+        if (live) {
+          const int64_t y = p.labels[row];
+          const bool inside = y >= 0 && y < p.vocab;
+          if (inside && y != p.ignore) label = (int)y - (p.v0 + n0);
+          if constexpr (EPI == kGrad) {
+            if (y != p.ignore) {
+              g = factor_of(inside, p.gout, (int64_t)row * p.gstride, p.count, p.gmax, p.f16);
+              lse2 = p.lse[row] * kLog2e;
             }
           }
         }
       }
       if constexpr (EPI == kLse) {
-        if (live) p.part[(int64_t)row * p.nt + nb] = make_float2(m, sum);
+        float x[128];
+        #pragma unroll
+        for (int i = 0; i < 128; ++i) x[i] = 0.f;
+        for (int kc = k0; kc < k1; kc += kChunk) {
+          if (!(good = take())) break;
+          #pragma unroll
+          for (int c0 = 0; c0 < 128; c0 += 16) {
+            uint32_t v[16];
+            tmem_ld16(lanes + (uint32_t)((n & 1) * kBN + c0), v);
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) x[c0 + i] += __uint_as_float(v[i]);
+          }
+          release();
+        }
+        if (!good) break;
+        const int lim = p.N - n0;
+        if (lim < 128) {
+          #pragma unroll
+          for (int i = 0; i < 128; ++i) x[i] = i < lim ? x[i] : -INFINITY;
+        }
+        if (__any_sync(0xffffffffu, label >= 0 && label < 128)) {  // few of the warps' tiles hold a label
+          float own = 0.f;
+          #pragma unroll
+          for (int i = 0; i < 128; ++i) own = label == i ? x[i] : own;
+          if (label >= 0 && label < 128) p.tgt[row] = own;
+        }
+        float m = x[0];
+        #pragma unroll
+        for (int i = 1; i < 128; ++i) m = fmaxf(m, x[i]);
+        const float m2 = m == -INFINITY ? 0.f : m * kLog2e;
+        const bool keep = live && n0 < p.keep_cols;
+        float sum0 = 0.f, sum1 = 0.f;
+        #pragma unroll
+        for (int c0 = 0; c0 < 128; c0 += 32) {
+          uint32_t w[16];
+          #pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float t0 = fmaf(x[c0 + 2 * i], kLog2e, -m2), t1 = fmaf(x[c0 + 2 * i + 1], kLog2e, -m2);
+            sum0 += ex2(t0);
+            sum1 += ex2(t1);
+            w[i] = __byte_perm(distance_bits(t0), distance_bits(t1), 0x5410);
+          }
+          if (keep && lim - c0 > 0) store_words(p.keep + (int64_t)row * p.ldk + n0 + c0, w, lim - c0);
+        }
+        if (live) p.part[(int64_t)row * (2 * p.nt) + 2 * nb + half] = make_float2(lim > 0 ? m2 : -INFINITY, sum0 + sum1);
+      } else {
+        if (!(good = take())) break;
+        #pragma unroll 1
+        for (int c0 = 0; c0 < 128; c0 += 32) {
+          uint32_t v[32];
+          tmem_ld32(lanes + (uint32_t)((n & 1) * kBN + c0), v);
+          const int lim = p.N - (n0 + c0);
+          if (lim <= 0) continue;
+          float o[32];
+          if constexpr (EPI == kGrad) {
+            #pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float e = ex2(fmaf(__uint_as_float(v[i]), kLog2e, -lse2)) - (label == c0 + i ? 1.f : 0.f);
+              o[i] = g == 0.f ? 0.f : g * e;
+            }
+            if (live) store16(p.out, (int64_t)row * p.ldo + n0 + c0, o, lim, p.f16);
+          } else {
+            #pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = alpha * __uint_as_float(v[i]);
+            if (live) {
+              if (!p.acc) {
+                store16(p.out, (int64_t)row * p.ldo + n0 + c0, o, lim, p.f16);
+              } else {
+                float* acc = p.acc + ((int64_t)(u % p.splits) * p.M + row) * p.N + n0 + c0;
+                #pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (i < lim) acc[i] = o[i];
+              }
+            }
+          }
+        }
+        release();
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[b]);
+      }
+      if (!good) break;
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncwarp();
   __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other's loads, MMAs or arrivals may touch its shared memory
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// d of the kept columns, in place of their distances q below the maximum m of 128 columns: g (exp(l - lse) - [v = y]) =
+// g (2^(m - q - lse) - ..); the label's own entry comes from its logit in FP32.  A row to blockIdx.y, eight columns to a
+// thread and step, so that a row's scalars are read once for the columns of a CTA.
+__global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int64_t ldk, int T, int cols,
+                                                   const float2* __restrict__ part, int tiles,
+                                                   const float* __restrict__ tgt, const float* __restrict__ lse,
+                                                   const int64_t* __restrict__ labels, int64_t ignore, int vocab,
+                                                   const float* __restrict__ gout, int gstride,
+                                                   const float* __restrict__ count, const float* __restrict__ gmax,
+                                                   int f16) {
+  for (int row = blockIdx.y; row < T; row += gridDim.y) {
+    const int64_t y = labels[row];
+    const bool inside = y >= 0 && y < vocab;
+    const float lse2 = lse[row] * kLog2e;
+    float g = 0.f, own = 0.f;
+    if (y != ignore) {
+      g = factor_of(inside, gout, (int64_t)row * gstride, count, gmax, f16);
+      if (inside) own = g * (ex2(fmaf(tgt[row], kLog2e, -lse2)) - 1.f);
+    }
+    const int label = inside && y != ignore ? (int)y : -1;
+    #pragma unroll 4
+    for (int c0 = (blockIdx.x * 256 + threadIdx.x) * 8; c0 < cols; c0 += gridDim.x * 2048) {
+      uint4* at = reinterpret_cast<uint4*>(d + row * ldk + c0);
+      uint4 raw = __ldcs(at);
+      const float up = part[(int64_t)row * tiles + (c0 >> 7)].x - lse2;
+      uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float a = g * ex2(fmaf((float)(w[i] & 0xffffu), -1.f / kStep, up));
+        float b = g * ex2(fmaf((float)(w[i] >> 16), -1.f / kStep, up));
+        if (label == c0 + 2 * i) a = own;
+        if (label == c0 + 2 * i + 1) b = own;
+        w[i] = g == 0.f ? 0u : pack16(a, b, f16);
+      }
+      *at = raw;
+    }
+  }
+}
+
+// out (16 bits, ldo) or sum (FP32, contiguous) = (add ? sum : 0) + the planes in order.
+__global__ void __launch_bounds__(256) k_xent_planes(const float* __restrict__ planes, int splits, int M, int N,
+                                                     float* __restrict__ sum, int add, uint16_t* __restrict__ out,
+                                                     int64_t ldo, int f16) {
+  const int64_t total = (int64_t)M * N;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    float a = add ? sum[i] : 0.f;
+    for (int s = 0; s < splits; ++s) a += planes[s * total + i];
+    if (out) out[i / N * ldo + i % N] = (uint16_t)pack16(a, 0.f, f16);
+    else sum[i] = a;
   }
 }
 
@@ -401,25 +565,77 @@ static int map16(CUtensorMap* m, const void* p, int rows, int cols, int64_t ld, 
   return MPQ_OK;
 }
 
-// One operand of a product: [rows, k] K-major or [k, rows] MN-major; `box`: rows of the CTA's tile.
+// One operand of a product: [rows, k] K-major or [k, rows] MN-major; `box`: rows of a CTA's half tile.
 static int operand(CUtensorMap* m, bool mn, const void* p, int rows, int k, int64_t ld, int box, int f16) {
   return mn ? map16(m, p, k, rows, ld, 64, f16) : map16(m, p, rows, k, ld, box, f16);
 }
 
-template <int EPI, bool A_MN, bool B_MN>
+static int num_sms() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!cached[dev]) {
+    int n = 0;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    cached[dev] = n > 1 ? n : 148;
+  }
+  return cached[dev];
+}
+
+// How an M x N product over K is cut: columns of a tile (256 NH) and parts of K.
+struct Plan {
+  int nh, splits;
+};
+
+// The plan with the least estimated time on `pairs` CTA pairs.  A unit takes its k-blocks x columns, a tenth more for
+// 256-column tiles (their operands are loaded twice as often for the same product); parts of K add FP32
+// planes, written and read once, at 3600 bytes a cycle (the memory's rate).
+// Every part has at least 16 k-blocks.
+static Plan plan_for(int M, int N, int K) {
+  const int pairs = num_sms() / 2, kblocks = (K + 63) / 64;
+  const double mt = (M + kBM - 1) / kBM;
+  Plan best{1, 1};
+  double least = 1e300;
+  for (int nh = 1; nh <= 2; ++nh) {
+    const double tiles = mt * ((N + kBN * nh - 1) / (kBN * nh));
+    for (int s = 1; s <= 32 && s * 16 <= std::max(kblocks, 16); ++s) {
+      const double waves = std::ceil(tiles * s / pairs);
+      const double unit = std::ceil((double)kblocks / s) * 512 * nh * (nh == 1 ? 1.1 : 1.0) + 2000;
+      const double planes = s > 1 ? 8.0 * M * N * s / 3600.0 : 0.0;
+      const double t = waves * unit + planes;
+      if (t < 0.98 * least) {
+        least = t;
+        best = {nh, s};
+      }
+    }
+  }
+  return best;
+}
+
+template <int EPI, bool A_MN, bool B_MN, int NH>
 static int product(const void* A, int64_t lda, const void* B, int64_t ldb, Args p, cudaStream_t st) {
   CUtensorMap ma, mb;
-  int r = operand(&ma, A_MN, A, p.M, p.K, lda, kBM, p.f16);
+  int r = operand(&ma, A_MN, A, p.M, p.K, lda, 128, p.f16);
   if (r) return r;
-  if ((r = operand(&mb, B_MN, B, p.N, p.K, ldb, kBN, p.f16))) return r;
+  if ((r = operand(&mb, B_MN, B, p.N, p.K, ldb, 128, p.f16))) return r;
   p.mt = (p.M + kBM - 1) / kBM;
-  p.nt = (p.N + kBN - 1) / kBN;
-  const size_t smem = 1024 + kStages * (kStageA + kStageB) + 256;
-  if ((r = smem_opt_in((const void*)k_xent_gemm<EPI, A_MN, B_MN>, smem, "mpq_xent"))) return r;
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  k_xent_gemm<EPI, A_MN, B_MN><<<std::min(p.mt * p.nt, sms), kThreads, smem, st>>>(ma, mb, p);
+  p.nt = (p.N + kBN * NH - 1) / (kBN * NH);
+  p.splits = std::max(p.splits, 1);
+  const size_t smem = 1024 + stages_of(NH) * (1 + NH) * kHalf + 256;
+  if ((r = smem_opt_in((const void*)k_xent_gemm<EPI, A_MN, B_MN, NH>, smem, "mpq_xent"))) return r;
+  const int grid = 2 * std::min(p.mt * p.nt * p.splits, num_sms() / 2);
+  k_xent_gemm<EPI, A_MN, B_MN, NH><<<grid, kThreads, smem, st>>>(ma, mb, p);
   return launch_status("mpq_xent product");
+}
+
+template <bool A_MN>
+static int out_product(int nh, const void* A, int64_t lda, const void* B, int64_t ldb, const Args& p, cudaStream_t st) {
+  return nh == 2 ? product<kOut, A_MN, true, 2>(A, lda, B, ldb, p, st) : product<kOut, A_MN, true, 1>(A, lda, B, ldb, p, st);
+}
+
+// Width of the piece that starts at column v0.
+static int piece_at(int v0, int V, int piece, int keep_cols) {
+  return v0 < keep_cols ? keep_cols : std::min(piece, V - v0);
 }
 
 static bool operand_ok(const void* p, int64_t ld, int cols) {
@@ -431,21 +647,42 @@ static bool operand_ok(const void* p, int64_t ld, int cols) {
 
 using namespace mpq;
 
-// Vocabulary tiles of the forward pass: `part` holds T x this many float2.
-MPQ_API int mpq_xent_tiles(int V) { return V > 0 ? (int)(((int64_t)V + xent::kBN - 1) / xent::kBN) : 0; }
+// Half tiles of the vocabulary in the forward pass: `part` holds T x this many float2.
+MPQ_API int mpq_xent_tiles(int V) { return V > 0 ? 2 * (int)(((int64_t)V + xent::kBN - 1) / xent::kBN) : 0; }
+
+// FP32 planes of T x H that the backward pass needs for dhidden (0: none): one for each part of K of its largest
+// piece, and the running sum of several pieces.
+MPQ_API int mpq_xent_planes(int T, int V, int H, int piece, int keep_cols) {
+  if (T <= 0 || V <= 0 || H <= 0 || piece <= 0 || keep_cols < 0 || keep_cols > V) return 0;
+  const int rest = V - keep_cols, pieces = (keep_cols > 0) + (rest + piece - 1) / piece;
+  int most = 1;  // over the widths that occur: the kept columns, whole pieces and the last one
+  for (int w : {keep_cols, std::min(piece, rest), rest % piece})
+    if (w > 0) most = std::max(most, xent::plan_for(T, H, w).splits);
+  return pieces > 1 ? most + 1 : (most > 1 ? most : 0);
+}
 
 MPQ_API int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden, int64_t ldh, const void* weight,
                              int64_t ldw, const int64_t* labels, int64_t ignore, float* part, int64_t part_floats,
-                             float* tgt, float* lse, float* nll, int* status, void* stream) {
+                             float* tgt, float* lse, float* nll, int reduction, float* loss,
+                             float* count, void* keep, int64_t ldk, int keep_cols, int* status, void* stream) {
+  MPQ_CHECK_ARG(reduction >= 0 && reduction <= 2 && (reduction == 0 || (loss && count)),
+                "mpq_xent_forward: reduction must be 0 (none), 1 (sum) or 2 (mean); the last two need loss and count");
   MPQ_CHECK_ARG(dtype == 1 || dtype == 2, "mpq_xent_forward: dtype must be 1 (bf16) or 2 (f16)");
   MPQ_CHECK_ARG(T >= 0 && V >= 1 && H >= 1 && T <= (1 << 24) && V <= (1 << 30), "mpq_xent_forward: bad shape %d x %d x %d", T, V, H);
-  if (T == 0) return MPQ_OK;
+  if (T == 0 && reduction == 0) return MPQ_OK;
+  if (T == 0) {
+    xent::k_xent_reduce<<<1, 1024, 0, (cudaStream_t)stream>>>(nullptr, nullptr, ignore, 0, reduction == 2, loss, count);
+    return launch_status("mpq_xent_forward (reduce)");
+  }
   MPQ_CHECK_ARG(hidden && weight && labels && part && tgt && lse && nll && status, "mpq_xent_forward: null pointer");
   MPQ_CHECK_ARG(xent::operand_ok(hidden, ldh, H) && xent::operand_ok(weight, ldw, H),
                 "mpq_xent_forward: operands must be 16-byte aligned with leading dimensions that are multiples of 8");
   MPQ_CHECK_ARG(part_floats >= 2ll * T * mpq_xent_tiles(V) && (reinterpret_cast<uintptr_t>(part) & 7) == 0,
                 "mpq_xent_forward: the workspace needs %lld floats", 2ll * T * mpq_xent_tiles(V));
-  MPQ_CHECK_ARG((int64_t)((T + 127) / 128) * mpq_xent_tiles(V) < (1ll << 31), "mpq_xent_forward: too many tiles");
+  MPQ_CHECK_ARG(keep_cols == 0 || (keep && (keep_cols == V || (keep_cols > 0 && keep_cols < V && keep_cols % 256 == 0)) &&
+                                   xent::operand_ok(keep, ldk, keep_cols)),
+                "mpq_xent_forward: keep_cols must be V or a multiple of 256 below it, kept in rows like the operands");
+  MPQ_CHECK_ARG((int64_t)((T + 255) / 256) * mpq_xent_tiles(V) < (1ll << 31), "mpq_xent_forward: too many tiles");
   int st = tc::get_encoder();
   if (st) return st;
   xent::Args p{};
@@ -455,61 +692,91 @@ MPQ_API int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden,
   p.labels = labels; p.ignore = ignore; p.vocab = V;
   p.part = reinterpret_cast<float2*>(part);
   p.tgt = tgt;
-  st = xent::product<xent::kLse, false, false>(hidden, ldh, weight, ldw, p, (cudaStream_t)stream);
+  p.keep = reinterpret_cast<uint16_t*>(keep); p.ldk = ldk; p.keep_cols = keep_cols;
+  st = xent::product<xent::kLse, false, false, 1>(hidden, ldh, weight, ldw, p, (cudaStream_t)stream);
   if (st) return st;
   xent::k_xent_join<<<T, 128, 0, (cudaStream_t)stream>>>(p.part, (int)mpq_xent_tiles(V), tgt, labels, ignore, V, lse, nll);
-  return launch_status("mpq_xent_forward (join)");
-}
-
-MPQ_API int mpq_xent_reduce(int T, const float* nll, const int64_t* labels, int64_t ignore, int mean, float* loss,
-                            float* count, void* stream) {
-  MPQ_CHECK_ARG(T >= 0 && T <= (1 << 24), "mpq_xent_reduce: bad shape");
-  MPQ_CHECK_ARG(loss && count && (T == 0 || (nll && labels)), "mpq_xent_reduce: null pointer");
-  xent::k_xent_reduce<<<1, 1024, 0, (cudaStream_t)stream>>>(nll, labels, ignore, T, mean, loss, count);
-  return launch_status("mpq_xent_reduce");
+  if ((st = launch_status("mpq_xent_forward (join)")) || reduction == 0) return st;
+  xent::k_xent_reduce<<<1, 1024, 0, (cudaStream_t)stream>>>(nll, labels, ignore, T, reduction == 2, loss, count);
+  return launch_status("mpq_xent_forward (reduce)");
 }
 
 MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden, int64_t ldh, const void* weight,
                               int64_t ldw, const int64_t* labels, int64_t ignore, const float* lse, const float* gout,
-                              int gstride, const float* count, float* gmax, void* d, int piece, float* acc,
-                              void* dhidden, int64_t lddh, void* dweight, int64_t lddw, int* status, void* stream) {
+                              int gstride, const float* count, const float* part, const float* tgt, void* keep,
+                              int64_t ldk, int keep_cols, float* gmax, void* d, int piece, float* acc, void* dhidden,
+                              int64_t lddh, void* dweight, int64_t lddw, int* status, void* stream) {
   MPQ_CHECK_ARG(dtype == 1 || dtype == 2, "mpq_xent_backward: dtype must be 1 (bf16) or 2 (f16)");
   MPQ_CHECK_ARG(T >= 0 && V >= 1 && H >= 1 && T <= (1 << 24) && V <= (1 << 30), "mpq_xent_backward: bad shape %d x %d x %d", T, V, H);
   MPQ_CHECK_ARG(piece >= 256 && piece % 256 == 0, "mpq_xent_backward: the piece must be a multiple of 256 columns");
+  MPQ_CHECK_ARG(keep_cols == 0 || keep_cols == V || (keep_cols > 0 && keep_cols < V && keep_cols % 256 == 0),
+                "mpq_xent_backward: keep_cols must be V or a multiple of 256 below it");
   if (T == 0) return MPQ_OK;
-  MPQ_CHECK_ARG(hidden && weight && labels && lse && gout && gmax && d && status, "mpq_xent_backward: null pointer");
-  MPQ_CHECK_ARG(xent::operand_ok(hidden, ldh, H) && xent::operand_ok(weight, ldw, H) && xent::operand_ok(d, piece, 0),
+  MPQ_CHECK_ARG(hidden && weight && labels && lse && gout && (gmax || gstride == 0) && status, "mpq_xent_backward: null pointer");
+  MPQ_CHECK_ARG(xent::operand_ok(hidden, ldh, H) && xent::operand_ok(weight, ldw, H),
                 "mpq_xent_backward: operands must be 16-byte aligned with leading dimensions that are multiples of 8");
+  MPQ_CHECK_ARG(keep_cols == 0 || (keep && part && tgt && xent::operand_ok(keep, ldk, keep_cols)),
+                "mpq_xent_backward: the kept columns need their rows, part and tgt");
+  MPQ_CHECK_ARG(keep_cols == V || (d && xent::operand_ok(d, piece, 0)), "mpq_xent_backward: a piece needs its workspace");
   MPQ_CHECK_ARG(!dhidden || lddh >= H, "mpq_xent_backward: lddh < H");
   MPQ_CHECK_ARG(!dweight || lddw >= H, "mpq_xent_backward: lddw < H");
-  MPQ_CHECK_ARG(!dhidden || V <= piece || acc, "mpq_xent_backward: several pieces need the FP32 sum of dhidden");
+  const int planes = mpq_xent_planes(T, V, H, piece, keep_cols);
+  MPQ_CHECK_ARG(!dhidden || planes == 0 || acc, "mpq_xent_backward: dhidden needs %d planes of workspace", planes);
+  cudaStream_t cs = (cudaStream_t)stream;
   int st = tc::get_encoder();
   if (st) return st;
-  xent::k_xent_gmax<<<1, 1024, 0, (cudaStream_t)stream>>>(gout, gstride, labels, ignore, V, T, count, gmax);
-  if ((st = launch_status("mpq_xent_backward (scale)"))) return st;
-  for (int v0 = 0; v0 < V; v0 += piece) {
-    const int w = std::min(piece, V - v0);
+  const int f16 = dtype == 2;
+  if (gstride == 0) {
+    gmax = nullptr;
+  } else {
+    xent::k_xent_gmax<<<1, 1024, 0, cs>>>(gout, gstride, labels, ignore, V, T, count, gmax);
+    if ((st = launch_status("mpq_xent_backward (scale)"))) return st;
+  }
+  for (int v0 = 0, w; v0 < V; v0 += w) {
+    w = xent::piece_at(v0, V, piece, keep_cols);
     const uint16_t* W = reinterpret_cast<const uint16_t*>(weight) + (int64_t)v0 * ldw;
+    const void* dv = d;
+    int64_t ldd = piece;
     xent::Args p{};
-    p.f16 = dtype == 2;
+    p.f16 = f16;
     p.status = status;
-    p.M = T; p.N = w; p.K = H;
-    p.labels = labels; p.ignore = ignore; p.vocab = V; p.v0 = v0;
-    p.lse = lse; p.gout = gout; p.gstride = gstride; p.count = count; p.gmax = gmax;
-    p.out = d; p.ldo = piece;
-    if ((st = xent::product<xent::kGrad, false, false>(hidden, ldh, W, ldw, p, (cudaStream_t)stream))) return st;
+    p.gout = gout; p.gstride = gstride; p.count = count; p.gmax = gmax;
+    if (v0 < keep_cols) {
+      dim3 grid(std::min((keep_cols + 2047) / 2048, 4), std::min(T, 32768));
+      xent::k_xent_kept<<<grid, 256, 0, cs>>>((uint16_t*)keep, ldk, T, keep_cols, (const float2*)part, mpq_xent_tiles(V),
+                                              tgt, lse, labels, ignore, V, gout, gstride, count, gmax, f16);
+      if ((st = launch_status("mpq_xent_backward (kept)"))) return st;
+      dv = keep;
+      ldd = ldk;
+    } else {
+      p.M = T; p.N = w; p.K = H;
+      p.labels = labels; p.ignore = ignore; p.vocab = V; p.v0 = v0;
+      p.lse = lse;
+      p.out = d; p.ldo = piece;
+      if ((st = xent::product<xent::kGrad, false, false, 1>(hidden, ldh, W, ldw, p, cs))) return st;
+    }
     if (dhidden) {
+      const xent::Plan plan = xent::plan_for(T, H, w);
       p.M = T; p.N = H; p.K = w;
       p.out = dhidden; p.ldo = lddh;
-      p.acc = V > piece ? acc : nullptr;
-      p.first = v0 == 0; p.last = v0 + w == V;
-      if ((st = xent::product<xent::kOut, false, true>(d, piece, W, ldw, p, (cudaStream_t)stream))) return st;
+      p.acc = planes ? acc : nullptr;
+      p.splits = plan.splits;
+      if ((st = xent::out_product<false>(plan.nh, dv, ldd, W, ldw, p, cs))) return st;
+      if (planes) {
+        const int64_t n = (int64_t)T * H;
+        const int grid = (int)std::min<int64_t>((n + 255) / 256, 8 * xent::num_sms());
+        xent::k_xent_planes<<<grid, 256, 0, cs>>>(acc, plan.splits, T, H, acc + (planes - 1) * n, v0 > 0,
+                                                  v0 + w == V ? (uint16_t*)dhidden : nullptr, lddh, f16);
+        if ((st = launch_status("mpq_xent_backward (planes)"))) return st;
+      }
     }
     if (dweight) {
       p.M = w; p.N = H; p.K = T;
       p.out = reinterpret_cast<uint16_t*>(dweight) + (int64_t)v0 * lddw; p.ldo = lddw;
       p.acc = nullptr;
-      if ((st = xent::product<xent::kOut, true, true>(d, piece, hidden, ldh, p, (cudaStream_t)stream))) return st;
+      p.splits = 1;
+      const int nh = xent::plan_for(w, H, T).nh;
+      if ((st = xent::out_product<true>(nh, dv, ldd, hidden, ldh, p, cs))) return st;
     }
   }
   return MPQ_OK;

@@ -3,8 +3,9 @@
     loss = vocab_cross_entropy(hidden, model.lm_head.weight, labels)        # mean over the labels that count
     nll = vocab_cross_entropy(hidden, weight, labels, reduction="none")     # scores of tokens, for a perplexity
 
-The logits (tokens x vocabulary) are never stored: the forward pass reduces them tile by tile inside the product, and
-the backward pass computes them again a piece of the vocabulary at a time.
+The logits (tokens x vocabulary) are not stored: the forward pass reduces them tile by tile inside the product.  The
+backward pass takes the vocabulary in pieces.  It computes a piece's logits again, except for the first columns, which
+the forward pass keeps in 16 bits where a gradient is wanted and ``keep_bytes`` has room: that saves their product.  With ``keep_bytes=0`` nothing of the logits' size outlives a call.
 """
 from __future__ import annotations
 
@@ -14,11 +15,12 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import ops
-from ._lib import call, load, ptr
+from ._lib import call_on, load, ptr
 
 _DTYPES = {torch.bfloat16: 1, torch.float16: 2}
-_REDUCTIONS = ("mean", "sum", "none")
+_REDUCTIONS = ("none", "sum", "mean")
 PIECE_BYTES = 1 << 30  # default room for the piece of the logits' gradient that the backward pass holds at a time
+KEEP_BYTES = 1 << 31   # default room for what the forward pass keeps for the backward pass
 
 
 def _operand(x: torch.Tensor) -> torch.Tensor:
@@ -40,32 +42,41 @@ def _piece(tokens: int, vocab: int, piece: Optional[int]) -> int:
     return max(256, min((int(piece) + 255) // 256 * 256, most))
 
 
+def _keep(tokens: int, vocab: int, keep_bytes: int) -> int:
+    """Columns of the vocabulary that fit in keep_bytes at two bytes a token: all, or a multiple of 256."""
+    cols = int(keep_bytes) // (2 * max(tokens, 1))
+    return vocab if cols >= (vocab + 7) // 8 * 8 else cols // 256 * 256
+
+
+def _forward(hidden, weight, labels, ignore_index, reduction, keep_bytes):
+    """(result, count, lse, part, tgt, keep, keep_cols) of a checked call."""
+    t, h = hidden.shape
+    v = weight.shape[0]
+    dev = hidden.device
+    x, w = _operand(hidden), _operand(weight)
+    tiles = load().mpq_xent_tiles(v)
+    each = reduction == "none"
+    out = torch.empty((t,) if each else (), device=dev, dtype=torch.float32)
+    small = torch.empty(2 * t + 1, device=dev, dtype=torch.float32)        # lse, count, nll
+    part = torch.empty(2 * t * tiles + t, device=dev, dtype=torch.float32)  # the tiles' partial sums, the labels' logits
+    at, at_part = small.data_ptr(), part.data_ptr()
+    keep_cols = _keep(t, v, keep_bytes) if keep_bytes and t else 0
+    keep = torch.empty(t, (keep_cols + 7) // 8 * 8, device=dev, dtype=hidden.dtype) if keep_cols else None
+    call_on(dev.index, "mpq_xent_forward", t, v, h, _DTYPES[hidden.dtype], ptr(x), x.stride(0), ptr(w), w.stride(0),
+            ptr(labels), ignore_index, at_part, 2 * t * tiles, at_part + 8 * t * tiles, at,
+            out.data_ptr() if each else at + 4 * t + 4, _REDUCTIONS.index(reduction), out.data_ptr(), at + 4 * t, ptr(keep),
+            keep.shape[1] if keep_cols else 0, keep_cols, ptr(ops.status_word(dev)))
+    return out, small[t:t + 1], small[:t], part, part[2 * t * tiles:], keep, keep_cols
+
+
 class _VocabCrossEntropy(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, hidden, weight, labels, ignore_index, reduction, piece):
-        t, h = hidden.shape
-        v = weight.shape[0]
-        dev = hidden.device
-        code = _DTYPES[hidden.dtype]
-        x, w = _operand(hidden), _operand(weight)
-        tiles = int(load().mpq_xent_tiles(v))
-        lse = torch.empty(t, device=dev, dtype=torch.float32)
-        nll = torch.empty(t, device=dev, dtype=torch.float32)
-        part = torch.empty(2 * t * tiles + t, device=dev, dtype=torch.float32)
-        tgt = part[2 * t * tiles:]
-        with torch.cuda.device(dev):
-            call("mpq_xent_forward", t, v, h, code, ptr(x), x.stride(0), ptr(w), w.stride(0), ptr(labels), ignore_index,
-                 ptr(part), 2 * t * tiles, ptr(tgt), ptr(lse), ptr(nll), ptr(ops.status_word(dev)))
-            if reduction == "none":
-                out, count = nll, None
-            else:
-                both = torch.empty(2, device=dev, dtype=torch.float32)
-                out, count = both[0], both[1]
-                call("mpq_xent_reduce", t, ptr(nll), ptr(labels), ignore_index, int(reduction == "mean"), ptr(out),
-                     ptr(count))
+    def forward(ctx, hidden, weight, labels, ignore_index, reduction, piece, keep_bytes):
+        out, count, lse, part, tgt, keep, keep_cols = _forward(hidden, weight, labels, ignore_index, reduction, keep_bytes)
         ctx.save_for_backward(hidden, weight, labels, lse, count if reduction == "mean" else None)
         ctx.ignore_index, ctx.piece = ignore_index, piece
+        ctx.kept = (keep, keep_cols, part, tgt) if keep_cols else None
         return out
 
     @staticmethod
@@ -79,29 +90,35 @@ class _VocabCrossEntropy(torch.autograd.Function):
         dh = torch.empty(t, h, device=dev, dtype=hidden.dtype) if need_h else None
         dw = torch.empty(v, h, device=dev, dtype=weight.dtype) if need_w else None
         if t == 0:
-            return dh, dw if dw is None else dw.zero_(), None, None, None, None
+            return dh, dw if dw is None else dw.zero_(), None, None, None, None, None
         x, w = _operand(hidden), _operand(weight)
         gout = gout.to(torch.float32).contiguous()
-        piece = _piece(t, v, ctx.piece)
-        d = torch.empty(t, piece, device=dev, dtype=hidden.dtype)
-        gmax = torch.empty(1, device=dev, dtype=torch.float32)
-        acc = torch.empty(t, h, device=dev, dtype=torch.float32) if need_h and v > piece else None
-        with torch.cuda.device(dev):
-            call("mpq_xent_backward", t, v, h, _DTYPES[hidden.dtype], ptr(x), x.stride(0), ptr(w), w.stride(0),
-                 ptr(labels), ctx.ignore_index, ptr(lse), ptr(gout), int(gout.dim() > 0), ptr(count), ptr(gmax), ptr(d),
-                 piece, ptr(acc), ptr(dh), h, ptr(dw), h, ptr(ops.status_word(dev)))
-        return dh, dw, None, None, None, None
+        # the kept columns turn into their gradient in place: a second pass through the graph computes them again
+        (keep, keep_cols, part, tgt), ctx.kept = ctx.kept or (None, 0, None, None), None
+        piece = _piece(t, v - keep_cols, ctx.piece)
+        d = torch.empty(t, piece, device=dev, dtype=hidden.dtype) if keep_cols < v else None
+        each = gout.dim() > 0  # one upstream gradient a token: d is scaled by the largest
+        gmax = torch.empty(1, device=dev, dtype=torch.float32) if each else None
+        planes = load().mpq_xent_planes(t, v, h, piece, keep_cols) if need_h else 0
+        acc = torch.empty(planes, t, h, device=dev, dtype=torch.float32) if planes else None
+        call_on(dev.index, "mpq_xent_backward", t, v, h, _DTYPES[hidden.dtype], ptr(x), x.stride(0), ptr(w), w.stride(0),
+                ptr(labels), ctx.ignore_index, ptr(lse), ptr(gout), int(each), ptr(count), ptr(part), ptr(tgt), ptr(keep),
+                keep.shape[1] if keep_cols else 0, keep_cols, ptr(gmax), ptr(d), piece, ptr(acc), ptr(dh), h, ptr(dw), h,
+                ptr(ops.status_word(dev)))
+        return dh, dw, None, None, None, None, None
 
 
 def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, ignore_index: int = -100,
-                        reduction: str = "mean", piece: Optional[int] = None) -> torch.Tensor:
+                        reduction: str = "mean", piece: Optional[int] = None, keep_bytes: int = KEEP_BYTES) -> torch.Tensor:
     """Cross entropy of softmax(hidden @ weight.T) at ``labels``, in float32.
 
     ``hidden`` (..., H) and ``weight`` (V, H): bfloat16 or float16; ``labels`` (...): integers.  Labels equal to
     ``ignore_index`` do not count (their score is 0, their gradient 0; the mean over no labels is NaN); labels outside
     the vocabulary give NaN.  ``reduction``: "mean" over the labels that count, "sum" or "none" (one score a token).
-    Differentiable once in ``hidden`` and ``weight``, whose gradients come in their own type; ``piece`` sets how many
-    columns of the vocabulary the backward pass holds at a time (by default what fits in 1 GiB)."""
+    Differentiable once in ``hidden`` and ``weight``, whose gradients come in their own type (for the head's, rows of
+    ``hidden`` that do not count must be finite all the same: they meet a zero).  ``keep_bytes`` bounds what the forward
+    pass keeps for the backward pass (by default 2 GiB; 0: nothing), ``piece`` the columns of the vocabulary that the
+    backward pass computes again at a time (by default what fits in 1 GiB)."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
     if not (hidden.is_cuda and weight.is_cuda and labels.is_cuda):
@@ -121,8 +138,14 @@ def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torc
         raise ValueError(f"labels must be int64 or int32, got {labels.dtype}")
     if piece is not None and int(piece) < 1:
         raise ValueError("piece must be positive")
+    if int(keep_bytes) < 0:
+        raise ValueError("keep_bytes must not be negative")
     flat = labels.reshape(-1).to(torch.int64).contiguous()
-    out = _VocabCrossEntropy.apply(hidden.reshape(-1, hidden.shape[-1]), weight, flat, int(ignore_index), reduction, piece)
+    rows = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        out = _VocabCrossEntropy.apply(rows, weight, flat, int(ignore_index), reduction, piece, int(keep_bytes))
+    else:
+        out = _forward(rows, weight, flat, int(ignore_index), reduction, 0)[0]
     return out.view(labels.shape) if reduction == "none" else out
 
 

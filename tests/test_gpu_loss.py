@@ -74,22 +74,22 @@ def test_scores(cuda_dev, t, v, h, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("piece", [None, 256, 600])
+@pytest.mark.parametrize("piece,keep", [(None, 1 << 31), (None, 0), (256, 0), (600, 0), (256, 150000), (None, 700000)])
 @pytest.mark.parametrize("dtype", list(U), ids=str)
 @pytest.mark.parametrize("t,v,h", SHAPES)
-def test_gradients(cuda_dev, t, v, h, dtype, piece):
+def test_gradients(cuda_dev, t, v, h, dtype, piece, keep):
     from mpq_b200.loss import vocab_cross_entropy
     x, w, y = inputs(t, v, h, dtype, cuda_dev, 1)
     y[0] = v - 1
     x.requires_grad_(), w.requires_grad_()
     ref = formulas(x.detach(), w.detach(), y)
-    dh, dw = torch.autograd.grad(vocab_cross_entropy(x, w, y, piece=piece), (x, w))
+    dh, dw = torch.autograd.grad(vocab_cross_entropy(x, w, y, piece=piece, keep_bytes=keep), (x, w))
     assert dh.dtype == dtype and dw.dtype == dtype
     within(dh, ref["dh"], ref["tol_h"])
     within(dw, ref["dw"], ref["tol_w"])
     gout = torch.randn(t, generator=torch.Generator().manual_seed(3)).to(cuda_dev)
     ref = formulas(x.detach(), w.detach(), y, gout, "none")
-    nll = vocab_cross_entropy(x, w, y, reduction="none", piece=piece)
+    nll = vocab_cross_entropy(x, w, y, reduction="none", piece=piece, keep_bytes=keep)
     dh, dw = torch.autograd.grad(nll, (x, w), gout)
     within(dh, ref["dh"], ref["tol_h"])
     within(dw, ref["dw"], ref["tol_w"])
@@ -126,6 +126,21 @@ def test_one_gradient_at_a_time_and_scaled_loss(cuda_dev):
     assert torch.equal(both[0], only_h) and torch.equal(both[1], only_w)
     scaled = torch.autograd.grad(64.0 * vocab_cross_entropy(x, w, y), (x, w))
     assert torch.equal(scaled[0], 64 * both[0]) and torch.equal(scaled[1], 64 * both[1])
+
+
+@pytest.mark.gpu
+def test_a_second_pass_through_the_graph(cuda_dev):
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(90, 1200, 64, torch.bfloat16, cuda_dev, 12)
+    x.requires_grad_(), w.requires_grad_()
+    loss = vocab_cross_entropy(x, w, y)
+    one = torch.autograd.grad(loss, (x, w), retain_graph=True)
+    two = torch.autograd.grad(loss, (x, w))
+    again = torch.autograd.grad(vocab_cross_entropy(x, w, y, keep_bytes=0), (x, w))
+    ref = formulas(x.detach(), w.detach(), y)
+    within(one[0], ref["dh"], ref["tol_h"])
+    within(one[1], ref["dw"], ref["tol_w"])
+    assert torch.equal(two[0], again[0]) and torch.equal(two[1], again[1])
 
 
 @pytest.mark.gpu
@@ -260,12 +275,19 @@ def test_refusals_without_a_gpu():
         vocab_cross_entropy(torch.zeros(2, 8), torch.zeros(4, 8), torch.zeros(2, dtype=torch.int64))
     lib = _lib.load()
     f = lambda **k: lib.mpq_xent_forward(*{**dict(T=4, V=9, H=8, dtype=1, h=16, ldh=8, w=16, ldw=8, y=16, ignore=-100,  # noqa: E731
-                                                  part=16, n=8, tgt=16, lse=16, nll=16, status=16, stream=None), **k}.values())
-    assert f(dtype=0) == 10001 and f(ldh=12) == 10001 and f(h=8) == 10001 and f(n=7) == 10001 and f(status=None) == 10001
+                                                  part=16, n=16, tgt=16, lse=16, nll=16, red=0, loss=None,
+                                                  count=None, keep=None, ldk=0, kc=0,
+                                                  status=16, stream=None), **k}.values())
+    assert f(red=1) == 10001 and f(red=3) == 10001
+    assert f(kc=9) == 10001 and f(keep=16, ldk=8, kc=9) == 10001 and f(keep=16, ldk=8, kc=8) == 10001
+    assert f(dtype=0) == 10001 and f(ldh=12) == 10001 and f(h=8) == 10001 and f(n=15) == 10001 and f(status=None) == 10001
     assert f(T=0) == 0
     b = lambda **k: lib.mpq_xent_backward(*{**dict(T=4, V=600, H=8, dtype=1, h=16, ldh=8, w=16, ldw=8, y=16, ignore=-100,  # noqa: E731
-                                                   lse=16, gout=16, gs=0, count=None, gmax=16, d=16, piece=256, acc=16, dh=16,
+                                                   lse=16, gout=16, gs=0, count=None, part=16, tgt=16,
+                                                   keep=None, ldk=0, kc=0, gmax=16, d=16, piece=256, acc=16, dh=16,
                                                    lddh=8, dw=16, lddw=8, status=16, stream=None), **k}.values())
+    assert b(gs=1, gmax=None) == 10001
+    assert b(kc=256) == 10001 and b(keep=16, ldk=256, kc=256, part=None) == 10001
     assert b(piece=100) == 10001 and b(acc=None) == 10001 and b(lddh=7) == 10001 and b(d=None) == 10001 and b(dtype=3) == 10001
 
 
@@ -282,3 +304,5 @@ def test_refusals(cuda_dev):
         vocab_cross_entropy(x, w, y, reduction="avg")
     with pytest.raises(ValueError, match="piece"):
         vocab_cross_entropy(x, w, y, piece=0)
+    with pytest.raises(ValueError, match="keep_bytes"):
+        vocab_cross_entropy(x, w, y, keep_bytes=-1)
