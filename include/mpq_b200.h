@@ -459,6 +459,13 @@ int mpq_mx4_gemm(int M, int N, int K, const uint8_t* a_codes, const uint8_t* a_s
                  const uint8_t* b_scales, const void* bias, void* out, int dtype, int64_t ldo, int* status,
                  void* stream);
 
+/* y (M x N, dtype) = Q(x) W^T + bias with x (M x K, dtype, leading dimension ldx) quantised within the call; one launch
+ * for a few tokens.  work: mpq_mx4_linear_work(M, K) bytes, 16-byte aligned (NULL where that is 0). */
+int64_t mpq_mx4_linear_work(int M, int K);
+int mpq_mx4_linear(const void* x, int dtype, int64_t ldx, int M, int N, int K, const uint8_t* w_codes,
+                   const uint8_t* w_scales, const void* bias, uint8_t* work, void* out, int64_t ldo, int* status,
+                   void* stream);
+
 /* ---- softmax cross entropy over a vocabulary, from hidden states (T x H) and the output head (V x H) ----
  * No counterpart in the reference (its perplexity scripts call a library's loss on whole logits).  The logits are
  * not stored.  dtype: 1 bfloat16, 2 float16 (hidden, weight and their gradients); operands 16-byte aligned with

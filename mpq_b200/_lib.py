@@ -105,6 +105,8 @@ SIGNATURES: Dict[str, Tuple[Any, ...]] = {
     "mpq_mx4_quantize": (P, I, L, I, I, P, P, P),
     "mpq_mx4_dequantize": (P, P, I, I, P, I, L, P),
     "mpq_mx4_gemm": (I, I, I, P, P, P, P, P, P, I, L, P, P),
+    "mpq_mx4_linear_work": (I, I),
+    "mpq_mx4_linear": (P, I, L, I, I, I, P, P, P, P, P, L, P, P),
     "mpq_xent_tiles": (I,),
     "mpq_xent_planes": (I, I, I, I, I),
     "mpq_xent_forward": (I, I, I, I, P, L, P, L, P, L, P, L, P, P, P, I, P, P, P, L, I, P, P),
@@ -128,6 +130,7 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = list(argtypes)
         fn.restype = ctypes.c_int
+    lib.mpq_mx4_linear_work.restype = L
     lib.mpq_last_error.restype = ctypes.c_char_p
     lib.mpq_last_error.argtypes = []
     lib.mpq_abi_version.restype = ctypes.c_int

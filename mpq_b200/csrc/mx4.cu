@@ -11,6 +11,7 @@
 // That is the layout in which the tensor cores take scales (32 lanes x 16 bytes), so a tile moves from memory to TMEM
 // as it is.  Blocks and rows that pad a tile carry c = 0.
 #include <algorithm>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp4.h>
 #include "umma.cuh"
@@ -37,6 +38,9 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+template <class T>
+constexpr int type_code() { return sizeof(T) == 4 ? kF32 : (std::is_same<T, __half>::value ? kF16 : kBF16); }
 
 // 2^(c - 127), NaN for c = 255 (2^-127 is a denormal)
 __device__ __forceinline__ float scale_value(uint32_t c) {
@@ -91,54 +95,69 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int c, int cols
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Quantisation: four lanes to a block, eight elements to a lane
+// Quantisation and reading back: eight elements to a lane (four lanes to a block), kRows rows to a thread
 // ------------------------------------------------------------------------------------------------------------------
+//
+// Both move memory: 4 or 2 bytes in and 17/32 out for an element, or the reverse.  A thread issues its kRows loads
+// before it uses the first, and a CTA of 256 threads covers as many rows side by side as a narrow matrix leaves room for.
+
+constexpr int kRows = 4;
 
 template <class T>
 __global__ void __launch_bounds__(256) k_mx4_quantize(const T* __restrict__ x, int64_t ldx, int rows, int cols, bool vec,
                                                       uint8_t* __restrict__ codes, int64_t ldc,
                                                       uint8_t* __restrict__ scales, int kt) {
+  asm volatile("griddepcontrol.launch_dependents;");  // a product launched behind may set itself up
+  // blockDim.x is a multiple of 16 (a scale tile's width in quarter blocks), so the shuffles stay inside a block's lanes
   const int nb = (cols + 31) >> 5, rows_pad = (rows + 127) & ~127;
-  const int q = blockIdx.x * 256 + threadIdx.x;  // quarter block along the row; kt tiles hold 16 of them
-  const int block = q >> 2;
-  const bool any = block < 4 * kt;  // whole warps agree: 16 kt quarters and 256 threads are multiples of 16, the
-                                    // shuffles below stay inside groups of four
-  for (int64_t row = blockIdx.y; row < rows_pad; row += gridDim.y) {
-    const bool real = any && row < rows && block < nb;
-    float v[8];
+  const int q = blockIdx.y * blockDim.x + threadIdx.x, block = q >> 2;
+  const int64_t row0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * kRows;
+  const uint32_t four = 0xfu << ((threadIdx.y * blockDim.x + threadIdx.x) & 28);  // the block's lanes
+  float v[kRows][8];
+  #pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) v[r][i] = 0.f;
+    if (row0 + r < rows && block < nb) load8(x + (row0 + r) * ldx, q * 8, cols, vec, v[r]);
+  }
+  #pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int64_t row = row0 + r;
     uint32_t mag = 0;
-    if (real) {
-      load8(x + row * ldx, q * 8, cols, vec, v);
-      #pragma unroll
-      for (int i = 0; i < 8; ++i) mag = max(mag, __float_as_uint(v[i]) & 0x7fffffffu);
-    }
-    mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 1));
-    mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 2));
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) mag = max(mag, __float_as_uint(v[r][i]) & 0x7fffffffu);
+    mag = max(mag, __shfl_xor_sync(four, mag, 1));
+    mag = max(mag, __shfl_xor_sync(four, mag, 2));
     const uint32_t c = scale_code(mag);
     const float inv = c == 255 ? 0.f : scale_inverse(c);
     #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = real && c != 255 ? v[i] * inv : 0.f;
-    const uint32_t word = encode8(v);
-    if (real) *reinterpret_cast<uint32_t*>(codes + row * ldc + q * 4) = word;
-    if (any && (q & 3) == 0) scales[scale_at(row, block, kt)] = real ? (uint8_t)c : 0;
+    for (int i = 0; i < 8; ++i) v[r][i] = c == 255 ? 0.f : v[r][i] * inv;
+    const uint32_t word = encode8(v[r]);
+    if (row < rows && block < nb) *reinterpret_cast<uint32_t*>(codes + row * ldc + q * 4) = word;
+    if (row < rows_pad && block < 4 * kt && (q & 3) == 0) scales[scale_at(row, block, kt)] = (uint8_t)c;
   }
 }
-
-// ------------------------------------------------------------------------------------------------------------------
-// Reading back: eight elements to a thread
-// ------------------------------------------------------------------------------------------------------------------
 
 template <class T>
 __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restrict__ codes, int64_t ldc,
                                                         const uint8_t* __restrict__ scales, int kt, int rows, int cols,
                                                         bool vec, T* __restrict__ out, int64_t ldo) {
-  const int c0 = (blockIdx.x * 256 + threadIdx.x) * 8;
+  const int c0 = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
+  const int64_t row0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * kRows;
   if (c0 >= cols) return;
-  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + row * ldc + c0 / 2);
-    const float s = scale_value(scales[scale_at(row, c0 >> 5, kt)]);
+  uint32_t w[kRows], c[kRows];
+  #pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int64_t row = min(row0 + r, (int64_t)rows - 1);
+    w[r] = *reinterpret_cast<const uint32_t*>(codes + row * ldc + c0 / 2);
+    c[r] = scales[scale_at(row, c0 >> 5, kt)];
+  }
+  #pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    if (row0 + r >= rows) break;
+    const float s = scale_value(c[r]);
     __half2 h[4];
-    decode8(w, h);
+    decode8(w[r], h);
     alignas(16) T v[8];
     #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -146,7 +165,7 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restric
       v[2 * i] = from_f32<T>(f.x * s);
       v[2 * i + 1] = from_f32<T>(f.y * s);
     }
-    T* dst = out + row * ldo + c0;
+    T* dst = out + (row0 + r) * ldo + c0;
     if (vec && c0 + 8 <= cols) {
       #pragma unroll
       for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i)
@@ -160,20 +179,193 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restric
 }
 
 // ------------------------------------------------------------------------------------------------------------------
+// Product for one to four tokens: y[t, n] = sum_k Q(x)[t, k] W[n, k] (+ bias[n]), x quantised in the same launch
+// ------------------------------------------------------------------------------------------------------------------
+//
+// W is read once (17 bytes for 32 weights), which bounds it.  Twice an E2M1 value is a small integer, so a block's 32
+// products are summed exactly in integers by dp4a and only then scaled: y += 2^(cx + cw - 256) sum (2 q_x) (2 q_w).
+// Every CTA quantises x for itself into shared memory (bytes 2 q_x, two planes of 16 bytes a block so that a warp's
+// reads are free of conflicts).  A warp takes whole rows of W, kFewRows at a time, a lane every 32nd block; each lane
+// copies its blocks ahead into a ring of kFewDepth steps of its own (cp.async, no barrier between lanes), so that the
+// reads from memory never wait for the arithmetic, nor for the quantisation of x at the start.  A weight's magnitude
+// comes from a byte permutation of the eight magnitudes; its sign is left to a second dp4a over the negative ones:
+// sum = all - 2 negative.
+
+constexpr int kFewRows = 2, kFewThreads = 256, kFewDepth = 6;
+constexpr int kFewStep = kFewRows * 32 * 20;  // bytes of a warp's step: 16 of codes and 4 of scales for a lane and row
+
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// Codes -> bytes 2 q (signed), eight to two words
+__device__ __forceinline__ void bytes_of(uint32_t w, uint32_t (&b)[2]) {
+  #pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t r = 0;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t c = w >> (16 * i + 4 * j), m = __byte_perm(0x03020100u, 0x0c080604u, c & 7u) & 0xffu;
+      r |= ((c & 8u ? 0u - m : m) & 0xffu) << (8 * j);
+    }
+    b[i] = r;
+  }
+}
+
+template <class T, int TOK>
+__global__ void __launch_bounds__(kFewThreads, 2)
+    k_mx4_few(const T* __restrict__ x, int64_t ldx, int tokens, int N, int K, bool vec, const uint8_t* __restrict__ codes,
+              const uint8_t* __restrict__ scales, const T* __restrict__ bias, T* __restrict__ out, int64_t ldo) {
+  extern __shared__ __align__(16) unsigned char sm[];
+  const int nb = (K + 31) >> 5, kt = (nb + 3) >> 2;
+  uint4* xb = reinterpret_cast<uint4*>(sm);                        // [TOK][2][nb]
+  float* xs = reinterpret_cast<float*>(xb + (size_t)TOK * 2 * nb);  // [TOK][nb], a quarter of the scale
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned char* ring = sm + (((size_t)TOK * nb * 36 + 15) & ~(size_t)15) + warp * kFewDepth * kFewStep;
+  const int warps = gridDim.x * (kFewThreads / 32), me = blockIdx.x * (kFewThreads / 32) + warp;
+  const int n0 = (int)((int64_t)N * me / warps), n1 = (int)((int64_t)N * (me + 1) / warps);
+  const int iters = (nb + 31) >> 5, steps = (n1 - n0 + kFewRows - 1) / kFewRows * iters;
+  int ln = n0, lb = lane, ls = 0;  // next step to load: row, this lane's block, slot
+  auto load_step = [&](int step) {
+    if (step < steps) {
+      unsigned char* at = ring + ls * kFewStep;
+      if (lb < nb) {
+        #pragma unroll
+        for (int r = 0; r < kFewRows; ++r) {
+          const int64_t row = min(ln + r, n1 - 1);
+          copy_async16(at + (r * 32 + lane) * 16, codes + (row * nb + lb) * 16);
+          copy_async4(at + kFewRows * 512 + (r * 32 + lane) * 4, scales + (scale_at(row, lb, kt) & ~(int64_t)3));
+        }
+      }
+      lb += 32;
+      if (lb - lane >= iters * 32) {
+        lb = lane;
+        ln += kFewRows;
+      }
+      ls = ls + 1 == kFewDepth ? 0 : ls + 1;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  #pragma unroll
+  for (int i = 0; i < kFewDepth - 1; ++i) load_step(i);
+
+  for (int i = threadIdx.x; i < TOK * 16 * kt; i += kFewThreads) {  // quarter blocks; 16 kt of them to a token
+    const int t = i / (16 * kt), q = i - t * 16 * kt, block = q >> 2;
+    const bool real = t < tokens && block < nb;
+    float v[8];
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    if (real) load8(x + t * ldx, q * 8, K, vec, v);
+    uint32_t mag = 0;
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) mag = max(mag, __float_as_uint(v[j]) & 0x7fffffffu);
+    const uint32_t four = 0xfu << (lane & ~3);  // the block's lanes: a warp's last pass may be partial
+    mag = max(mag, __shfl_xor_sync(four, mag, 1));
+    mag = max(mag, __shfl_xor_sync(four, mag, 2));
+    const uint32_t c = scale_code(mag);
+    const float inv = c == 255 ? 0.f : scale_inverse(c);
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c == 255 ? 0.f : v[j] * inv;
+    const uint32_t word = encode8(v);
+    if (block < nb) {
+      uint32_t b[2];
+      bytes_of(word, b);
+      reinterpret_cast<uint2*>(xb + ((size_t)t * 2 + ((q >> 1) & 1)) * nb + block)[q & 1] = make_uint2(b[0], b[1]);
+      if ((q & 3) == 0) xs[t * nb + block] = 0.25f * scale_value(c);
+    }
+  }
+  __syncthreads();
+
+  int step = 0, slot = 0;
+  for (int n = n0; n < n1; n += kFewRows) {
+    float acc[kFewRows][TOK];
+    #pragma unroll
+    for (int r = 0; r < kFewRows; ++r)
+      #pragma unroll
+      for (int t = 0; t < TOK; ++t) acc[r][t] = 0.f;
+    for (int i = 0, b = lane; i < iters; ++i, b += 32, ++step) {
+      load_step(step + kFewDepth - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kFewDepth - 1) : "memory");
+      const unsigned char* at = ring + slot * kFewStep;
+      slot = slot + 1 == kFewDepth ? 0 : slot + 1;
+      if (b >= nb) continue;
+      uint4 raw[kFewRows];
+      uint32_t c[kFewRows];
+      #pragma unroll
+      for (int r = 0; r < kFewRows; ++r) {
+        raw[r] = *reinterpret_cast<const uint4*>(at + (r * 32 + lane) * 16);
+        c[r] = at[kFewRows * 512 + (r * 32 + lane) * 4 + (b & 3)];
+      }
+      int all[kFewRows][TOK], neg[kFewRows][TOK];
+      #pragma unroll
+      for (int r = 0; r < kFewRows; ++r)
+        #pragma unroll
+        for (int t = 0; t < TOK; ++t) all[r][t] = neg[r][t] = 0;
+      #pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 xv[TOK];
+        #pragma unroll
+        for (int t = 0; t < TOK; ++t) xv[t] = xb[((size_t)t * 2 + h) * nb + b];
+        #pragma unroll
+        for (int r = 0; r < kFewRows; ++r) {
+          #pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t word = h == 0 ? (k == 0 ? raw[r].x : raw[r].y) : (k == 0 ? raw[r].z : raw[r].w);
+            const uint32_t size = word & 0x77777777u;
+            const uint32_t m0 = __byte_perm(0x03020100u, 0x0c080604u, size), m1 = __byte_perm(0x03020100u, 0x0c080604u, size >> 16);
+            uint32_t s0, s1;  // a code's bit 3 replicates the sign of a 0x80 byte: 0xff where negative, 0x80 elsewhere
+            asm("prmt.b32 %0, %1, %1, %2;" : "=r"(s0) : "r"(0x80808080u), "r"(word));
+            asm("prmt.b32 %0, %1, %1, %2;" : "=r"(s1) : "r"(0x80808080u), "r"(word >> 16));
+            #pragma unroll
+            for (int t = 0; t < TOK; ++t) {
+              const int x0 = (int)(k == 0 ? xv[t].x : xv[t].z), x1 = (int)(k == 0 ? xv[t].y : xv[t].w);
+              all[r][t] = __dp4a((int)m1, x1, __dp4a((int)m0, x0, all[r][t]));
+              neg[r][t] = __dp4a((int)(m1 & s1), x1, __dp4a((int)(m0 & s0), x0, neg[r][t]));
+            }
+          }
+        }
+      }
+      #pragma unroll
+      for (int r = 0; r < kFewRows; ++r) {
+        const float sw = scale_value(c[r]);
+        #pragma unroll
+        for (int t = 0; t < TOK; ++t) acc[r][t] = fmaf((float)(all[r][t] - 2 * neg[r][t]), sw * xs[t * nb + b], acc[r][t]);
+      }
+    }
+    #pragma unroll
+    for (int r = 0; r < kFewRows; ++r)
+      #pragma unroll
+      for (int t = 0; t < TOK; ++t) {
+        const float y = warp_sum(acc[r][t]);
+        if (lane == 0 && n + r < n1 && t < tokens)
+          out[(int64_t)t * ldo + n + r] = from_f32<T>(bias ? y + to_f32(bias[n + r]) : y);
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
 // Product: y[t, n] = sum_k A[t, k] B[n, k] (+ bias[n]), A and B in the stored form, on the block-scaled tensor cores
 // ------------------------------------------------------------------------------------------------------------------
 //
-// One CTA per SM walks 128 x 128 output tiles.  A k-block is one 128-byte swizzle row per operand row = 256 codes, with
+// Two kernels.  k_mx4_tile, for few rows of A:
+// One CTA per SM walks 128 x BN output tiles (BN = 64 or 128: narrow tiles spread few
+// tokens' work over more SMs; a narrower one's scales would start at an odd TMEM column, which the MMA refuses).  A k-block is one 128-byte swizzle row per operand row = 256 codes, with
 // two 512-byte scale tiles for each operand.  Warp 0 fills a ring of stages by TMA; warp 1's elected thread copies the
 // stage's scales from shared memory to TMEM (tcgen05.cp, replicated to the four lane quadrants) and issues four MMAs
 // of K = 64; warps 2..5 read the FP32 accumulator, add the bias, round once and store.  Two accumulators let the
 // epilogue overlap the next tile.  Scale columns in TMEM belong to the stage, so they are not rewritten before the
-// MMAs that read them are done.
+// MMAs that read them are done.  With at most 128 rows of A only those are loaded (a tile load takes two to three cycles a
+// 128-byte row; what the others' shared memory holds stays in their rows of the accumulator), and a cluster of up to
+// four CTAs may share a tile, each with a part of K: the others leave their FP32 parts in shared memory and the first
+// adds them in order.
 
 constexpr int kThreads = 192;
-constexpr int kBM = 128, kBN = 128, kStages = 6;
-constexpr uint32_t kOperand = 128 * 128, kScale = 1024, kStage = 2 * kOperand + 2 * kScale;
-constexpr uint32_t kScaleCols = 256, kStageCols = 16;  // TMEM: accumulators [0, 256), 16 scale columns a stage above
+constexpr int kBM = 128, kStages = 6;
+constexpr uint32_t kOperand = 128 * 128, kScale = 1024;
+constexpr uint32_t kScaleCols = 256, kStageCols = 16;   // TMEM: accumulators [0, 256), 16 scale columns a stage above
 
 // kind::mxf4 with E8M0 scales of 32 elements: A = B = E2M1, K-major, D = F32, M = m, N = n; `sf`: which half of the
 // four scales of a 128-element tile this K = 64 step takes (0 or 2, the same for A and B).
@@ -188,11 +380,28 @@ __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
          ((uint64_t)1 << 46);
 }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
+template <int CTAS>
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
+  if constexpr (CTAS == 2)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t add) {
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(add)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(add)
+        : "memory");
 }
 
 struct GemmArgs {
@@ -200,28 +409,83 @@ struct GemmArgs {
   const void* bias;
   void* out;
   int64_t ldo;
-  int M, N, kt, mt, nt;
+  int M, N, kt, mt, nt;  // kt: scale tiles along K; mt x nt output tiles
+  int a_rows;            // k_mx4_tile: rows of A that a tile loads
+  int tile_out;          // the result's rows are aligned for tile stores
   int* status;
 };
 
+// kCols<T> columns of the accumulator are 128 bytes of a row.  Columns col.. of a warp's 32 rows from row0 on (`lane`: the
+// thread's row): bias, one rounding, and off as a tile, or by the thread where the result's rows are not aligned.
 template <class T>
+constexpr int kCols = 128 / sizeof(T);
+
+template <class T>
+__device__ __forceinline__ void store_rows(const GemmArgs& p, const CUtensorMap* map, unsigned char* buf, int lane, int row0,
+                                           int col, const uint32_t (&v)[kCols<T>]) {
+  const int lim = p.N - col;
+  if (lim <= 0 || row0 >= p.M) return;  // the same for the warp
+  const T* bias = reinterpret_cast<const T*>(p.bias);
+  alignas(16) T o[kCols<T>];
+  #pragma unroll
+  for (int i = 0; i < kCols<T>; ++i) {
+    float f = __uint_as_float(v[i]);
+    if (bias && i < lim) f += to_f32(bias[col + i]);
+    o[i] = from_f32<T>(f);
+  }
+  if (p.tile_out) {
+    uint32_t w[32];
+    #pragma unroll
+    for (int i = 0; i < 32; ++i) w[i] = reinterpret_cast<const uint32_t*>(o)[i];
+    chunk_put(buf, lane, w);
+    chunk_send(buf, lane, map, col, row0, 0);
+  } else if (row0 + lane < p.M) {
+    T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(row0 + lane) * p.ldo + col;
+    #pragma unroll
+    for (int i = 0; i < kCols<T>; ++i)
+      if (i < lim) dst[i] = o[i];
+  }
+}
+
+// kCols<T> columns of TMEM
+template <int C>
+__device__ __forceinline__ void tmem_cols(uint32_t at, uint32_t (&v)[C]) {
+  #pragma unroll
+  for (int c = 0; c < C; c += 32) {
+    uint32_t t[32];
+    tmem_ld32(at + c, t);
+    #pragma unroll
+    for (int i = 0; i < 32; ++i) v[c + i] = t[i];
+  }
+}
+
+template <class T, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_mx4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs p) {
+    k_mx4_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfb,
+               const __grid_constant__ CUtensorMap map_o, const GemmArgs p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kStage);
+  constexpr uint32_t kOperandB = BN * 128;
+  constexpr uint32_t kStage = kOperand + kOperandB + 2 * kScale;
+  unsigned char* out_buf = ring + kStages * kStage;  // 4 KB to an epilogue warp
+  uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + 4 * 4096);
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // a stage: A codes, B codes (1024-byte aligned), then the scales of all stages behind the operands of all stages
-  auto s_a = [&](int s) { return ring + s * 2 * kOperand; };
-  auto s_b = [&](int s) { return ring + s * 2 * kOperand + kOperand; };
-  auto s_sf = [&](int s) { return ring + kStages * 2 * kOperand + s * 2 * kScale; };
+  auto s_a = [&](int s) { return ring + s * (kOperand + kOperandB); };
+  auto s_b = [&](int s) { return s_a(s) + kOperand; };
+  auto s_sf = [&](int s) { return ring + kStages * (kOperand + kOperandB) + s * 2 * kScale; };
+  float* part_sum = reinterpret_cast<float*>(ring);  // [BN][128] at the end of a part of K
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int nkb = (p.kt + 1) / 2, tiles = p.mt * p.nt;
+  // a cluster of `parts` CTAs shares a tile (more than one only where the grid holds every tile once)
+  const int rank = (int)cluster_rank(), parts = (int)cluster_size();
+  const int nkb = (p.kt + 1) / 2, kb0 = nkb * rank / parts, kb1 = nkb * (rank + 1) / parts;
+  const int tiles = p.mt * p.nt, first_tile = blockIdx.x / parts, stride = gridDim.x / parts;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -246,130 +510,143 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
+      const uint32_t bytes = p.a_rows * 128 + kOperandB + 2 * kScale;
       int64_t it = 0;
+      Ring<kStages> r;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int t = first_tile; t < tiles && ok; t += stride) {
         const int mb = t % p.mt, nb = t / p.mt;
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const int s = (int)(it % kStages);
-          if (*abort_flag || !mbar_wait(&empty[s], ((uint32_t)(it / kStages) & 1u) ^ 1u)) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it, r.next()) {
+          if (!mbar_wait_fast(&empty[r.s], r.ph ^ 1u) || *abort_flag) {
             ok = false;
             break;
           }
-          const uint32_t sf_bytes = 512u * min(2, p.kt - 2 * kb);
-          mbar_expect_tx(&full[s], 2 * kOperand + 2 * sf_bytes);
-          tma_load_2d(s_a(s), &map_a, &full[s], kb * 128, mb * kBM);
-          tma_load_2d(s_b(s), &map_b, &full[s], kb * 128, nb * kBN);
-          bulk_load(s_sf(s), p.sfa + ((int64_t)mb * p.kt + 2 * kb) * 512, sf_bytes, &full[s]);
-          bulk_load(s_sf(s) + kScale, p.sfb + ((int64_t)nb * p.kt + 2 * kb) * 512, sf_bytes, &full[s]);
+          uint64_t* bar = &full[r.s];
+          mbar_expect_tx(bar, bytes);
+          tma_load_2d(s_b(r.s), &map_b, bar, kb * 128, nb * BN);
+          tma_load_2d(s_sf(r.s) + kScale, &map_sfb, bar, kb * 256, nb * BN >> 7);
+          // A may come from the kernel before: wait for its end once the first weights are on their way
+          if (it == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+          tma_load_2d(s_a(r.s), &map_a, bar, kb * 128, mb * kBM);
+          tma_load_2d(s_sf(r.s), &map_sfa, bar, kb * 256, mb);
         }
       }
       if (!ok) {  // drain the copies in flight (each wait bounded) before the CTA may end
         *abort_flag = 1;
-        for (int64_t k = it < kStages ? 0 : it - kStages; k < it; ++k)
-          mbar_wait(&full[k % kStages], (uint32_t)(k / kStages) & 1u);
+        for (int i = 0; i < kStages && i < it; ++i) {
+          r.back();
+          mbar_wait_fast(&full[r.s], r.ph);
+        }
         atomicCAS(p.status, 0, 2);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int64_t it = 0;
-      bool ok = true;
-      int n = 0;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++n) {
-        const int b = n & 1;
-        if (*abort_flag || !mbar_wait(&acc_empty[b], ((uint32_t)(n >> 1) & 1u) ^ 1u)) {
+    const bool lead = elect_one();
+    const uint64_t da0 = smem_desc_k_sw128(smem_u32(s_a(0))), db0 = smem_desc_k_sw128(smem_u32(s_b(0)));
+    const uint64_t ds0 = scale_desc(smem_u32(s_sf(0)));
+    const uint32_t i0 = idesc_mxf4(kBM, BN, 0), i2 = idesc_mxf4(kBM, BN, 2);
+    Ring<kStages> r;
+    bool ok = true;
+    int n = 0;
+    for (int t = first_tile; t < tiles && ok; t += stride, ++n) {
+      const uint32_t acc = tmem + (n & 1) * BN;
+      if (!warp_agrees(mbar_wait_fast(&acc_empty[n & 1], ((uint32_t)(n >> 1) & 1u) ^ 1u) && !*abort_flag)) {
+        ok = false;
+        break;
+      }
+      const uint32_t part = (uint32_t)((t / p.mt) * BN & 127) >> 5;  // the tile's column in its scale tile
+      for (int kb = kb0; kb < kb1; ++kb, r.next()) {
+        if (!warp_agrees(mbar_wait_fast(&full[r.s], r.ph) && !*abort_flag)) {
           ok = false;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const int s = (int)(it % kStages);
-          if (*abort_flag || !mbar_wait(&full[s], (uint32_t)(it / kStages) & 1u)) {
-            ok = false;
-            break;
+        const uint32_t sf = tmem + kScaleCols + r.s * kStageCols;
+        const uint64_t ds = desc_add(ds0, r.s * 2 * kScale);
+        const uint64_t da = desc_add(da0, r.s * (kOperand + kOperandB)), db = desc_add(db0, r.s * (kOperand + kOperandB));
+        if (lead) {  // scales beyond the matrix are zeros, as are its codes
+          #pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            copy_scales<1>(sf + j * 4, desc_add(ds, j * 512));
+            copy_scales<1>(sf + 8 + j * 4, desc_add(ds, kScale + j * 512));
           }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t sf = tmem + kScaleCols + s * kStageCols;
-          const int ktiles = min(2, p.kt - 2 * kb);
-          for (int j = 0; j < ktiles; ++j) {
-            asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(sf + j * 4),
-                         "l"(scale_desc(smem_u32(s_sf(s)) + j * 512))
-                         : "memory");
-            asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(sf + 8 + j * 4),
-                         "l"(scale_desc(smem_u32(s_sf(s)) + kScale + j * 512))
-                         : "memory");
-          }
-          const uint32_t a0 = smem_u32(s_a(s)), b0 = smem_u32(s_b(s));
-          for (int j = 0; j < 2 * ktiles; ++j) {  // steps beyond the last scale tile hold no elements
-            asm volatile(
-                "{\n\t.reg .pred p;\n\t"
-                "setp.ne.b32 p, %6, 0;\n\t"
-                "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-                    tmem + b * kBN),
-                "l"(smem_desc_k_sw128(a0 + j * 32)), "l"(smem_desc_k_sw128(b0 + j * 32)),
-                "r"(idesc_mxf4(kBM, kBN, (j & 1) * 2)), "r"(sf + (j >> 1) * 4), "r"(sf + 8 + (j >> 1) * 4),
-                "r"((kb > 0 || j > 0) ? 1u : 0u)
-                : "memory");
-          }
+          #pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_mxf4<1>(acc, desc_add(da, j * 32), desc_add(db, j * 32), j & 1 ? i2 : i0, sf + (j >> 1) * 4,
+                        sf + 8 + (j >> 1) * 4 + part, j > 0 || kb > kb0);
           asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                           smem_u32(&empty[s]))
+                           smem_u32(&empty[r.s]))
                        : "memory");
         }
-        // the accumulator is complete (or, after an abort, the issued MMAs have retired)
+        __syncwarp();
+      }
+      // the accumulator is complete (or, after an abort, the issued MMAs have retired)
+      if (lead)
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                         smem_u32(&acc_full[b]))
+                         smem_u32(&acc_full[n & 1]))
                      : "memory");
-      }
-      if (!ok) {
-        *abort_flag = 1;
-        atomicCAS(p.status, 0, 3);
-      }
+      __syncwarp();
+    }
+    if (!ok && lead) {
+      *abort_flag = 1;
+      atomicCAS(p.status, 0, 3);
     }
   } else {
     const int quad = warp & 3;
     int n = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
+    for (int t = first_tile; t < tiles; t += stride, ++n) {
       const int b = n & 1, mb = t % p.mt, nb = t / p.mt;
-      const bool ready = !*abort_flag && mbar_wait(&acc_full[b], (uint32_t)(n >> 1) & 1u);
+      const bool ready = !*abort_flag && mbar_wait_fast(&acc_full[b], (uint32_t)(n >> 1) & 1u);
       if (!__all_sync(0xffffffffu, ready) || *abort_flag) {
         if (!*abort_flag) atomicCAS(p.status, 0, 4);
         *abort_flag = 1;
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int row = mb * kBM + quad * 32 + lane;
+      if (parts > 1 && rank == 0) break;  // finishes below
+      const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * BN);
       #pragma unroll 1
-      for (int c0 = 0; c0 < kBN; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * kBN + c0), v);
-        const int col = nb * kBN + c0;
-        if (row < p.M && col < p.N) {
-          T* dst = reinterpret_cast<T*>(p.out) + (int64_t)row * p.ldo + col;
-          const T* bias = reinterpret_cast<const T*>(p.bias);
-          const int lim = min(32, p.N - col);
-          alignas(16) T o[32];
+      for (int c0 = 0; c0 < BN; c0 += kCols<T>) {
+        uint32_t v[kCols<T>];
+        tmem_cols(at + c0, v);
+        if (parts > 1) {  // every load of the ring has been consumed: it holds this part, column by column
           #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float f = __uint_as_float(v[i]);
-            if (bias && i < lim) f += to_f32(bias[col + i]);
-            o[i] = from_f32<T>(f);
-          }
-          if (lim == 32 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-            #pragma unroll
-            for (int i = 0; i < (int)(32 * sizeof(T) / 16); ++i)
-              reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(o)[i];
-          } else {
-            #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < lim) dst[i] = o[i];
-          }
+          for (int i = 0; i < kCols<T>; ++i) part_sum[(c0 + i) * kBM + quad * 32 + lane] = __uint_as_float(v[i]);
+        } else {
+          store_rows<T>(p, &map_o, out_buf + quad * 4096, lane, mb * kBM + quad * 32, nb * BN + c0, v);
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[b]);
     }
+  }
+  if (warp >= 2 && parts == 1) chunk_drain(lane);
+  __syncwarp();
+  if (parts > 1) {
+    cluster_sync();  // the parts are complete
+    if (rank == 0 && warp >= 2 && !*abort_flag) {
+      const int quad = warp & 3, row = quad * 32 + lane;  // one row tile
+      #pragma unroll 1
+      for (int c0 = 0; c0 < BN; c0 += kCols<T>) {
+        uint32_t v[kCols<T>];
+        tmem_cols(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c0, v);
+        for (int r = 1; r < parts; ++r) {
+          const uint32_t at = mapa(smem_u32(part_sum + c0 * kBM + row), r);
+          #pragma unroll
+          for (int i = 0; i < kCols<T>; ++i) {
+            float f;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(at + i * kBM * 4));
+            v[i] = __float_as_uint(__uint_as_float(v[i]) + f);
+          }
+        }
+        store_rows<T>(p, &map_o, out_buf + quad * 4096, lane, quad * 32, first_tile * BN + c0, v);
+      }
+      chunk_drain(lane);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    __syncwarp();
+    cluster_sync();  // the parts have been read
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -379,11 +656,207 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Codes as rows of bytes: box = 128 bytes x 128 rows, 128B swizzle, zeros (codes of 0) beyond the matrix.
-static int code_map(CUtensorMap* m, const void* p, int rows, int64_t ldc) {
+// k_mx4_pair, for many rows of A: a pair of CTAs computes 256 x 384 tiles (tcgen05 cta_group::2, M = 256, two products of
+// N = 192 a step).  Each CTA loads 128 rows of A and 192 of B a k-block: what bounds these products is the operands'
+// way from L2 to shared memory (two to three cycles a 128-byte row), so the tile is as wide as TMEM allows: 384 columns of
+// accumulator and 4 stages x 32 columns of scales (8 of A's 128 rows, 24 of B's 384, the latter in both CTAs).  The
+// accumulator is not doubled: the next tile's first half starts when the epilogue has read that half.
+
+constexpr int kPairWarps = 8, kPairThreads = 64 + 32 * kPairWarps, kPairStages = 4, kPairGroup = 8;
+constexpr int kPM = 256, kPN = 384, kPHalf = 192;
+constexpr uint32_t kPairB = 96 * 128, kPairOps = kOperand + 2 * kPairB, kPairSf = 4 * kScale;
+constexpr uint32_t kPairCols = 32;  // TMEM columns of a stage's scales, above the accumulator's 384
+
+template <class T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    k_mx4_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfb,
+               const __grid_constant__ CUtensorMap map_o, const GemmArgs p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* out_buf = ring + kPairStages * (kPairOps + kPairSf);  // 4 KB to an epilogue warp
+  uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + kPairWarps * 4096);
+  uint64_t* empty = full + kPairStages;
+  uint64_t* acc_full = empty + kPairStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  auto s_a = [&](int s) { return ring + s * kPairOps; };
+  auto s_b = [&](int s, int h) { return ring + s * kPairOps + kOperand + h * kPairB; };
+  auto s_sf = [&](int s) { return ring + kPairStages * kPairOps + s * kPairSf; };  // A's tile pair, then B's three
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank(), pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
+  const int nkb = (p.kt + 1) / 2, tiles = p.mt * p.nt;
+  auto tile_at = [&](int t, int& mb, int& nb) {  // kPairGroup row tiles down, then the next column tile
+    const int per = kPairGroup * p.nt, g = t / per, r = t - g * per;
+    const int rows = min(kPairGroup, p.mt - g * kPairGroup);
+    mb = g * kPairGroup + r % rows;
+    nb = r / rows;
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], kPairWarps);  // four warps of each CTA read a half
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are initialised before any is signalled
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // A may come from the kernel before
+      const uint32_t bar0 = mapa(smem_u32(full), 0);
+      int64_t it = 0;
+      Ring<kPairStages> r;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int mb, nb;
+        tile_at(t, mb, nb);
+        const int row_a = mb * kPM + rank * 128, row_b = nb * kPN + rank * 96, tile_a = mb * 2 + rank, tile_b = nb * 3;
+        for (int kb = 0; kb < nkb; ++kb, ++it, r.next()) {
+          if (!mbar_wait_cluster(&empty[r.s], r.ph ^ 1u) || *abort_flag) {
+            ok = false;
+            break;
+          }
+          // both CTAs' bytes count on the first one's barrier (a peer's copy may land before the expectation)
+          if (rank == 0) mbar_expect_tx(&full[r.s], 2 * (kPairOps + kPairSf));
+          const uint32_t bar = bar0 + r.s * 8;
+          tma_load_2d_pair(s_a(r.s), &map_a, bar, kb * 128, row_a);
+          tma_load_2d_pair(s_b(r.s, 0), &map_b, bar, kb * 128, row_b);
+          tma_load_2d_pair(s_b(r.s, 1), &map_b, bar, kb * 128, row_b + kPHalf);
+          tma_load_2d_pair(s_sf(r.s), &map_sfa, bar, kb * 256, tile_a);
+          tma_load_2d_pair(s_sf(r.s) + kScale, &map_sfb, bar, kb * 256, tile_b);
+        }
+      }
+      if (!ok) {  // drain the copies in flight (each wait bounded); the peer leaves only after the cluster barrier
+        *abort_flag = 1;
+        for (int i = 0; rank == 0 && i < kPairStages && i < it; ++i) {
+          r.back();
+          mbar_wait_cluster(&full[r.s], r.ph);
+        }
+        atomicCAS(p.status, 0, 2);
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool lead = elect_one();
+      const uint64_t da0 = smem_desc_k_sw128(smem_u32(s_a(0))), ds0 = scale_desc(smem_u32(s_sf(0)));
+      const uint32_t i0 = idesc_mxf4(kPM, kPHalf, 0), i2 = idesc_mxf4(kPM, kPHalf, 2);
+      Ring<kPairStages> r;
+      bool ok = true;
+      uint32_t n = 0;  // tiles
+      for (int t = pair; t < tiles && ok; t += pairs, ++n) {
+        for (int kb = 0; kb < nkb; ++kb, r.next()) {
+          if (!warp_agrees(mbar_wait_cluster(&full[r.s], r.ph) && !*abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (kb == 0 && !warp_agrees(mbar_wait_cluster(&acc_empty[0], (n & 1u) ^ 1u))) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t sf = tmem + kPN + r.s * kPairCols;  // A's 2 x 4 columns, then B's 2 x 12
+          const uint64_t ds = desc_add(ds0, r.s * kPairSf), da = desc_add(da0, r.s * kPairOps), db = desc_add(da, kOperand);
+          const uint32_t add = kb > 0;
+          if (lead) {  // scales beyond the matrix are zeros, as are its codes
+            #pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              copy_scales<2>(sf + j * 4, desc_add(ds, j * 512));
+              #pragma unroll
+              for (int i = 0; i < 3; ++i)
+                copy_scales<2>(sf + 8 + j * 12 + i * 4, desc_add(ds, kScale * (1 + i) + j * 512));
+            }
+            #pragma unroll
+            for (int j = 0; j < 4; ++j)
+              mma_mxf4<2>(tmem, desc_add(da, j * 32), desc_add(db, j * 32), j & 1 ? i2 : i0, sf + (j >> 1) * 4,
+                          sf + 8 + (j >> 1) * 12, j > 0 ? 1u : add);
+            if (kb == nkb - 1) commit_pair(&acc_full[0]);
+          }
+          __syncwarp();
+          if (kb == 0) {
+            if (!warp_agrees(mbar_wait_cluster(&acc_empty[1], (n & 1u) ^ 1u))) {
+              ok = false;
+              break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          }
+          if (lead) {
+            #pragma unroll
+            for (int j = 0; j < 4; ++j)
+              mma_mxf4<2>(tmem + kPHalf, desc_add(da, j * 32), desc_add(db, kPairB + j * 32), j & 1 ? i2 : i0,
+                          sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 12 + 6, j > 0 ? 1u : add);
+            if (kb == nkb - 1) commit_pair(&acc_full[1]);
+            commit_pair(&empty[r.s]);
+          }
+          __syncwarp();
+        }
+      }
+      if (!ok && lead) {
+        *abort_flag = 1;
+        atomicCAS(p.status, 0, 3);
+      }
+    }
+  } else {
+    // a warp reads the TMEM lanes of its quadrant (warp % 4); warps 2..5 take the first half's columns, 6..9 the second's
+    const int quad = warp & 3, h = (warp - 2) >> 2;
+    unsigned char* buf = out_buf + (warp - 2) * 4096;
+    uint32_t n = 0;
+    for (int t = pair; t < tiles; t += pairs, ++n) {
+      int mb, nb;
+      tile_at(t, mb, nb);
+      const bool ready = !*abort_flag && mbar_wait_cluster(&acc_full[h], n & 1u);
+      if (!__all_sync(0xffffffffu, ready) || *abort_flag) {
+        if (!*abort_flag) atomicCAS(p.status, 0, 4);
+        *abort_flag = 1;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(h * kPHalf);
+      #pragma unroll 1
+      for (int c0 = 0; c0 < kPHalf; c0 += kCols<T>) {
+        uint32_t v[kCols<T>];
+        tmem_cols(at + c0, v);
+        if (c0 + kCols<T> == kPHalf) {  // all read: the tensor cores may go on
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(&acc_empty[h]), 0));
+        }
+        store_rows<T>(p, &map_o, buf, lane, mb * kPM + rank * 128 + quad * 32, nb * kPN + h * kPHalf + c0, v);
+      }
+    }
+    chunk_drain(lane);
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncwarp();
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other's loads, MMAs or arrivals may touch its shared memory
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// Codes as rows of bytes: box = 128 bytes x box_rows, 128B swizzle, zeros (codes of 0) beyond the matrix.
+static int code_map(CUtensorMap* m, const void* p, int rows, int64_t ldc, int box_rows) {
   cuuint64_t dims[2] = {(cuuint64_t)ldc, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)ldc};
-  cuuint32_t box[2] = {128, 128};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   const CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, estr,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -397,12 +870,33 @@ static int code_map(CUtensorMap* m, const void* p, int rows, int64_t ldc) {
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+static int num_sms() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!cached[dev]) {
+    int n = 0;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    cached[dev] = n > 0 ? n : 148;
+  }
+  return cached[dev];
+}
+
+// CTAs of 256 threads: `wide` threads along a row (all of a narrow one), the others on further rows.
+static void shape_of(int wide, int rows, dim3* grid, dim3* block) {
+  const int bx = std::min(wide, 256), by = 256 / bx;
+  *block = dim3(bx, by);
+  *grid = dim3((rows + by * kRows - 1) / (by * kRows), (wide + bx - 1) / bx);
+}
+
 template <class T>
 static int quantize(const void* x, int64_t ldx, int rows, int cols, uint8_t* codes, uint8_t* scales, cudaStream_t st) {
   const int nb = (cols + 31) / 32, kt = (nb + 3) / 4;
   const bool vec = aligned16(x) && (ldx * (int64_t)sizeof(T)) % 16 == 0;
-  dim3 grid((16 * kt + 255) / 256, std::min((rows + 127) / 128 * 128, 65535));
-  k_mx4_quantize<T><<<grid, 256, 0, st>>>((const T*)x, ldx, rows, cols, vec, codes, 16 * (int64_t)nb, scales, kt);
+  dim3 grid, block;
+  shape_of(16 * kt, (rows + 127) / 128 * 128, &grid, &block);
+  MPQ_CHECK_ARG(grid.y <= 65535, "mpq_mx4_quantize: %d columns are too many", cols);
+  k_mx4_quantize<T><<<grid, block, 0, st>>>((const T*)x, ldx, rows, cols, vec, codes, 16 * (int64_t)nb, scales, kt);
   return launch_status("mpq_mx4_quantize");
 }
 
@@ -411,21 +905,160 @@ static int dequantize(const uint8_t* codes, const uint8_t* scales, int rows, int
                       cudaStream_t st) {
   const int nb = (cols + 31) / 32, kt = (nb + 3) / 4;
   const bool vec = aligned16(out) && (ldo * (int64_t)sizeof(T)) % 16 == 0;
-  dim3 grid((cols + 2047) / 2048, std::min(rows, 65535));
-  k_mx4_dequantize<T><<<grid, 256, 0, st>>>(codes, 16 * (int64_t)nb, scales, kt, rows, cols, vec, (T*)out, ldo);
+  dim3 grid, block;
+  shape_of((cols + 7) / 8, rows, &grid, &block);
+  MPQ_CHECK_ARG(grid.y <= 65535, "mpq_mx4_dequantize: %d columns are too many", cols);
+  k_mx4_dequantize<T><<<grid, block, 0, st>>>(codes, 16 * (int64_t)nb, scales, kt, rows, cols, vec, (T*)out, ldo);
   return launch_status("mpq_mx4_dequantize");
 }
 
+// Scales as rows of tiles: box = `rows` row tiles x two block tiles (1024 bytes), zeros beyond the matrix.
+static int scale_map(CUtensorMap* m, const void* p, int row_tiles, int kt, int rows) {
+  cuuint64_t dims[2] = {(cuuint64_t)kt * 128, (cuuint64_t)row_tiles};
+  cuuint64_t strides[1] = {(cuuint64_t)kt * 512};
+  cuuint32_t box[2] = {256, (cuuint32_t)rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(p), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_last_error("mpq_mx4_gemm: cuTensorMapEncodeTiled failed (%d) for scales, tiles %d x %d", (int)r, row_tiles, kt);
+    return MPQ_ERR_ARG;
+  }
+  return MPQ_OK;
+}
+
+// Launch of a product: `cluster` CTAs to a cluster (0: the kernel says), started while the kernel before still runs
+// where `behind` says that it is this call's quantisation.
+template <class... P, class... A>
+static int launch_product(void (*kernel)(P...), int grid, int threads, size_t smem, int cluster, bool behind,
+                          cudaStream_t st, A... args) {
+  const int r = smem_opt_in((const void*)kernel, smem, "mpq_mx4_gemm");
+  if (r) return r;
+  cudaLaunchAttribute at[2];
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  if (cluster) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = cluster;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (behind) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_last_error("mpq_mx4_gemm: %s", cudaGetErrorString(e));
+    return (int)e;
+  }
+  return MPQ_OK;
+}
+
+template <class T, int BN>
+static int gemm_tile(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc, GemmArgs p, int parts, bool behind,
+                     cudaStream_t st) {
+  p.a_rows = std::min((p.M + 7) / 8 * 8, kBM);
+  CUtensorMap a, b;
+  int r = code_map(&a, a_codes, p.M, ldc, p.a_rows);
+  if (r) return r;
+  if ((r = code_map(&b, b_codes, p.N, ldc, BN))) return r;
+  CUtensorMap sa, sb;
+  if ((r = scale_map(&sa, p.sfa, (p.M + 127) / 128, p.kt, 1))) return r;
+  if ((r = scale_map(&sb, p.sfb, (p.N + 127) / 128, p.kt, 1))) return r;
+  p.mt = (p.M + kBM - 1) / kBM;
+  p.nt = (p.N + BN - 1) / BN;
+  MPQ_CHECK_ARG((int64_t)p.mt * p.nt <= 0x1fffffff, "mpq_mx4_gemm: too many tiles");
+  CUtensorMap o{};
+  p.tile_out = result_map(&o, p.out, type_code<T>(), 1, p.M, p.N, p.ldo);
+  const size_t smem = 1024 + kStages * (kOperand + BN * 128 + 2 * kScale) + 4 * 4096 + 256;
+  const int grid = parts > 1 ? p.mt * p.nt * parts : std::min(p.mt * p.nt, num_sms());
+  return launch_product(k_mx4_tile<T, BN>, grid, kThreads, smem, parts, behind, st, a, b, sa, sb, o, p);
+}
+
 template <class T>
-static int gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& p, cudaStream_t st) {
-  const size_t smem = 1024 + kStages * kStage + 256;
-  const int ast = smem_opt_in((const void*)k_mx4_gemm<T>, smem, "mpq_mx4_gemm");
-  if (ast) return ast;
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int grid = std::min(p.mt * p.nt, sms);
-  k_mx4_gemm<T><<<grid, kThreads, smem, st>>>(a, b, p);
-  return launch_status("mpq_mx4_gemm");
+static int gemm_pair(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc, GemmArgs p, bool behind, cudaStream_t st) {
+  CUtensorMap a, b, sa, sb;
+  int r = code_map(&a, a_codes, p.M, ldc, 128);
+  if (r) return r;
+  if ((r = code_map(&b, b_codes, p.N, ldc, 96))) return r;
+  if ((r = scale_map(&sa, p.sfa, (p.M + 127) / 128, p.kt, 1))) return r;
+  if ((r = scale_map(&sb, p.sfb, (p.N + 127) / 128, p.kt, 3))) return r;
+  p.mt = (p.M + kPM - 1) / kPM;
+  p.nt = (p.N + kPN - 1) / kPN;
+  MPQ_CHECK_ARG((int64_t)p.mt * p.nt <= 0x7fffffff, "mpq_mx4_gemm: too many tiles");
+  CUtensorMap o{};
+  p.tile_out = result_map(&o, p.out, type_code<T>(), 1, p.M, p.N, p.ldo);
+  const size_t smem = 1024 + kPairStages * (kPairOps + kPairSf) + kPairWarps * 4096 + 256;
+  return launch_product(k_mx4_pair<T>, 2 * std::min(p.mt * p.nt, num_sms() / 2), kPairThreads, smem, 0, behind, st, a, b,
+                        sa, sb, o, p);
+}
+
+// The kernel with the shortest estimate: waves of CTAs (or pairs) x k-blocks x the cycles of one, which are those of its
+// operands' rows (a tile load takes about 2.5 cycles a row), and at least 300 for its steps one after the other; parts
+// of K on a cluster pay for their sum.  (Measured at K = 4096: 128 x 128 tiles 1140 cycles a k-block.)
+template <class T>
+static int gemm(const uint8_t* a_codes, const uint8_t* b_codes, const GemmArgs& p, int K, bool behind, cudaStream_t st) {
+  const int64_t ldc = 16 * (int64_t)((K + 31) / 32);
+  const int sms = num_sms(), nkb = (p.kt + 1) / 2;
+  auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  int bn = 0, parts = 1;  // 0: pairs
+  double least = (double)up(up(p.M, kPM) * up(p.N, kPN), sms / 2) * (nkb * 900.0 + 1500.0);
+  for (int w : {128, 64})
+    for (int s : {1, 2, 4}) {
+      const int64_t tiles = up(p.M, kBM) * up(p.N, w);
+      if (s > 1 && (p.M > kBM || tiles * s > sms || nkb < 4 * s)) break;
+      const double kb = std::max(300.0, 4.5 * (std::min(p.M, kBM) + w));
+      const double t = (double)up(tiles, sms / s) * (up(nkb, s) * kb + 1000.0) + (s > 1 ? 1500.0 + 500.0 * s : 0.0);
+      if (t < least) {
+        least = t;
+        bn = w;
+        parts = s;
+      }
+    }
+  return bn == 0     ? gemm_pair<T>(a_codes, b_codes, ldc, p, behind, st)
+         : bn == 128 ? gemm_tile<T, 128>(a_codes, b_codes, ldc, p, parts, behind, st)
+                     : gemm_tile<T, 64>(a_codes, b_codes, ldc, p, parts, behind, st);
+}
+
+template <class T, int TOK>
+static int few_tokens(const void* x, int64_t ldx, int M, int N, int K, const uint8_t* codes, const uint8_t* scales,
+                      const void* bias, void* out, int64_t ldo, cudaStream_t st) {
+  const int nb = (K + 31) / 32;
+  const size_t smem = (((size_t)TOK * nb * 36 + 15) & ~(size_t)15) + kFewThreads / 32 * kFewDepth * kFewStep;
+  const int r = smem_opt_in((const void*)k_mx4_few<T, TOK>, smem, "mpq_mx4_linear");
+  if (r) return r;
+  const bool vec = aligned16(x) && (ldx * (int64_t)sizeof(T)) % 16 == 0;
+  const int grid = std::min((N + 7) / 8, num_sms() * (smem <= 112 * 1024 ? 2 : 1));
+  k_mx4_few<T, TOK><<<grid, kFewThreads, smem, st>>>((const T*)x, ldx, M, N, K, vec, codes, scales, (const T*)bias,
+                                                     (T*)out, ldo);
+  return launch_status("mpq_mx4_linear (few tokens)");
+}
+
+constexpr int kFewTokens = 4;
+// x has to fit in shared memory
+static bool takes_few(int M, int K) { return M <= kFewTokens && (M <= 2 ? M : 4) * ((K + 31ll) / 32) * 36 <= 160 * 1024; }
+
+template <class T>
+static int linear(const void* x, int dtype, int64_t ldx, int M, int N, int K, const uint8_t* codes, const uint8_t* scales,
+                  const void* bias, uint8_t* work, void* out, int64_t ldo, int* status, cudaStream_t st) {
+  if (takes_few(M, K)) {
+    return M == 1   ? few_tokens<T, 1>(x, ldx, M, N, K, codes, scales, bias, out, ldo, st)
+           : M == 2 ? few_tokens<T, 2>(x, ldx, M, N, K, codes, scales, bias, out, ldo, st)
+                    : few_tokens<T, 4>(x, ldx, M, N, K, codes, scales, bias, out, ldo, st);
+  }
+  const int nb = (K + 31) / 32;
+  uint8_t* x_scales = work + 16 * (int64_t)nb * M;
+  const int r = quantize<T>(x, ldx, M, K, work, x_scales, st);
+  if (r) return r;
+  return gemm<T>(work, codes, GemmArgs{x_scales, scales, bias, out, ldo, M, N, (nb + 3) / 4, 0, 0, 0, 0, status}, K, true, st);
 }
 
 }  // namespace mx4
@@ -470,13 +1103,32 @@ MPQ_API int mpq_mx4_gemm(int M, int N, int K, const uint8_t* a_codes, const uint
   MPQ_CHECK_ARG(a_codes && a_scales && b_codes && b_scales && out && status, "mpq_mx4_gemm: null pointer");
   MPQ_CHECK_ARG(mx4::aligned16(a_codes) && mx4::aligned16(a_scales) && mx4::aligned16(b_codes) && mx4::aligned16(b_scales),
                 "mpq_mx4_gemm: codes and scales must be 16-byte aligned");
-  int st = tc::get_encoder();
+  const int st = tc::get_encoder();
   if (st) return st;
-  const int nb = (K + 31) / 32;
-  mx4::GemmArgs p{a_scales, b_scales, bias, out, ldo, M, N, (nb + 3) / 4, (M + 127) / 128, (N + 127) / 128, status};
-  MPQ_CHECK_ARG((int64_t)p.mt * p.nt <= 0x7fffffff, "mpq_mx4_gemm: too many tiles");
-  CUtensorMap ma, mb;
-  if ((st = mx4::code_map(&ma, a_codes, M, 16 * (int64_t)nb))) return st;
-  if ((st = mx4::code_map(&mb, b_codes, N, 16 * (int64_t)nb))) return st;
-  return MX4_BY_TYPE(dtype, gemm, ma, mb, p, (cudaStream_t)stream);
+  const mx4::GemmArgs p{a_scales, b_scales, bias, out, ldo, M, N, ((K + 31) / 32 + 3) / 4, 0, 0, 0, 0, status};
+  return MX4_BY_TYPE(dtype, gemm, a_codes, b_codes, p, K, false, (cudaStream_t)stream);
+}
+
+// Bytes of workspace that mpq_mx4_linear needs: the quantised x, or none.
+MPQ_API int64_t mpq_mx4_linear_work(int M, int K) {
+  if (M <= 0 || K <= 0 || mx4::takes_few(M, K)) return 0;
+  const int64_t nb = ((int64_t)K + 31) / 32;
+  return 16 * nb * M + (M + 127ll) / 128 * ((nb + 3) / 4) * 512;
+}
+
+MPQ_API int mpq_mx4_linear(const void* x, int dtype, int64_t ldx, int M, int N, int K, const uint8_t* w_codes,
+                           const uint8_t* w_scales, const void* bias, uint8_t* work, void* out, int64_t ldo, int* status,
+                           void* stream) {
+  MPQ_CHECK_ARG(dtype >= 0 && dtype <= 2, "mpq_mx4_linear: dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+  MPQ_CHECK_ARG(M >= 0 && N >= 0 && K >= 1 && K <= 0x7fffff00 && M <= 0x7fffff00 && ldx >= K && ldo >= N,
+                "mpq_mx4_linear: bad shape %d x %d x %d", M, N, K);
+  if (M == 0 || N == 0) return MPQ_OK;
+  MPQ_CHECK_ARG(x && w_codes && w_scales && out && status, "mpq_mx4_linear: null pointer");
+  MPQ_CHECK_ARG(mpq_mx4_linear_work(M, K) == 0 || work, "mpq_mx4_linear: the workspace is missing");
+  MPQ_CHECK_ARG(mx4::aligned16(w_codes) && mx4::aligned16(w_scales) && mx4::aligned16(work),
+                "mpq_mx4_linear: codes, scales and workspace must be 16-byte aligned");
+  const int st = tc::get_encoder();
+  if (st) return st;
+  return MX4_BY_TYPE(dtype, linear, x, dtype, ldx, M, N, K, w_codes, w_scales, bias, work, out, ldo, status,
+                     (cudaStream_t)stream);
 }

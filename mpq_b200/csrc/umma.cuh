@@ -45,6 +45,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   return true;
 }
 
+// The same wait with the clock read only once the first try has failed: %globaltimer takes hundreds of cycles, which a
+// pipeline with short steps would pay at each.
+__device__ __forceinline__ bool mbar_wait_fast(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity);
+}
+
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
@@ -74,6 +81,11 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
 __device__ __forceinline__ void cluster_sync() {
@@ -147,6 +159,74 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// ---- results: a warp's 32 rows x 128 bytes through shared memory ----
+//
+// A thread holds a row of the accumulator; stored as it is, each 16 bytes of a warp go to 32 different lines, and the
+// stores, not the products, bound a kernel (measured on a 4-bit product: 418 us of stores, 231 us without).  So a warp
+// lays 128 bytes of each of its rows out in a 4 KB buffer of its own, swizzled as a tile load would (no bank is hit
+// twice), and one lane sends them off as a tile.
+
+__device__ __forceinline__ void chunk_put(unsigned char* buf, int lane, const uint32_t (&w)[32]) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last chunk has left the buffer
+  __syncwarp();
+  #pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+}
+// x: first column, y: first row, z: plane.  Rows and columns beyond the map's are not written.
+__device__ __forceinline__ void chunk_send(const unsigned char* buf, int lane, const CUtensorMap* map, int x, int y, int z) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(smem_u32(buf)), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+// Before the buffer's CTA ends.
+__device__ __forceinline__ void chunk_drain(int lane) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  __syncwarp();
+}
+
+// ---- issue ----
+//
+// One thread issues the MMAs, but the whole warp walks its loop: the loop's values stay uniform, and what is left to the
+// elected thread is straight-line.  (In a loop of lane 0 alone, with descriptors made for each MMA, an MMA of 96 tensor
+// cycles took 233 to issue.)
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// A wait's outcome, the same for all lanes (they leave a loop together).
+__device__ __forceinline__ bool warp_agrees(bool ok) { return __all_sync(0xffffffffu, ok); }
+// K-major / MN-major descriptors advance by their low word: (byte offset) / 16.
+__device__ __forceinline__ uint64_t desc_add(uint64_t d, uint32_t bytes) { return d + (bytes >> 4); }
+
+// Position in a ring of N stages: slot and phase parity.
+template <int N>
+struct Ring {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      ph ^= 1u;
+    }
+  }
+  __device__ __forceinline__ void back() {
+    if (s-- == 0) {
+      s = N - 1;
+      ph ^= 1u;
+    }
+  }
+};
+
 // ---- host: tensor maps through the driver entry point (no libcuda link dependency) ----
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
@@ -161,6 +241,22 @@ inline int get_encoder() {
   }
   g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   return MPQ_OK;
+}
+
+// Map of a result [planes, rows, cols] (leading dimension ld, planes contiguous) for chunk_send: type 0 f32, 1 bf16, 2
+// f16.  False where a tile store cannot take it (rows that do not start on 16 bytes).
+inline bool result_map(CUtensorMap* m, void* p, int type, int64_t planes, int64_t rows, int64_t cols, int64_t ld) {
+  const int size = type == 0 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(p) & 15) || (ld * size) % 16 || (ld * size * rows) >> 40) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  cuuint64_t strides[2] = {(cuuint64_t)(ld * size), (cuuint64_t)(ld * size * rows)};
+  cuuint32_t box[3] = {(cuuint32_t)(128 / size), 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType t = type == 0   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : type == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return g_encode(m, t, 3, p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace tc

@@ -207,93 +207,98 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
+      const uint32_t bar0 = mapa(smem_u32(full), 0);
       int64_t it = 0;
+      Ring<kStages> r;
       bool ok = true;
       for (int u = blockIdx.x >> 1; u < units && ok; u += pairs) {
         int mb, nb, k0, k1;
         unit_at(u, p, kblocks, mb, nb, k0, k1);
-        const int row_a = mb * kBM + rank * 128;
-        for (int kb = k0; kb < k1; ++kb, ++it) {
-          const int s = (int)(it % kStages);
-          if (*abort_flag || !mbar_wait_cluster(&empty[s], ((uint32_t)(it / kStages) & 1u) ^ 1u)) {
+        const int row_a = mb * kBM + rank * 128, row_b = nb * NH * kBN + rank * 128;
+        for (int kb = k0; kb < k1; ++kb, ++it, r.next()) {
+          if (!mbar_wait_cluster(&empty[r.s], r.ph ^ 1u) || *abort_flag) {
             ok = false;
             break;
           }
           // both CTAs' bytes count on the first one's barrier (a peer's copy may land before the expectation)
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * kStage);
-          const uint32_t bar = mapa(smem_u32(&full[s]), 0);
+          if (rank == 0) mbar_expect_tx(&full[r.s], 2 * kStage);
+          const uint32_t bar = bar0 + r.s * 8;
           if constexpr (A_MN) {
-            tma_load_2d_pair(s_a(s), &map_a, bar, row_a, kb * 64);
-            tma_load_2d_pair(s_a(s) + 8192, &map_a, bar, row_a + 64, kb * 64);
+            tma_load_2d_pair(s_a(r.s), &map_a, bar, row_a, kb * 64);
+            tma_load_2d_pair(s_a(r.s) + 8192, &map_a, bar, row_a + 64, kb * 64);
           } else {
-            tma_load_2d_pair(s_a(s), &map_a, bar, kb * 64, row_a);
+            tma_load_2d_pair(s_a(r.s), &map_a, bar, kb * 64, row_a);
           }
           #pragma unroll
           for (int h = 0; h < NH; ++h) {
-            const int row_b = (nb * NH + h) * kBN + rank * 128;
             if constexpr (B_MN) {
-              tma_load_2d_pair(s_b(s, h), &map_b, bar, row_b, kb * 64);
-              tma_load_2d_pair(s_b(s, h) + 8192, &map_b, bar, row_b + 64, kb * 64);
+              tma_load_2d_pair(s_b(r.s, h), &map_b, bar, row_b + h * kBN, kb * 64);
+              tma_load_2d_pair(s_b(r.s, h) + 8192, &map_b, bar, row_b + h * kBN + 64, kb * 64);
             } else {
-              tma_load_2d_pair(s_b(s, h), &map_b, bar, kb * 64, row_b);
+              tma_load_2d_pair(s_b(r.s, h), &map_b, bar, kb * 64, row_b + h * kBN);
             }
           }
         }
       }
       if (!ok) {  // drain the copies in flight (each wait bounded); the peer leaves only after the cluster barrier
         *abort_flag = 1;
-        if (rank == 0)
-          for (int64_t k = it < kStages ? 0 : it - kStages; k < it; ++k)
-            mbar_wait_cluster(&full[k % kStages], (uint32_t)(k / kStages) & 1u);
+        for (int i = 0; rank == 0 && i < kStages && i < it; ++i) {
+          r.back();
+          mbar_wait_cluster(&full[r.s], r.ph);
+        }
         atomicCAS(p.status, 0, 2);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const bool lead = elect_one();
       const uint32_t idesc = idesc16(p.f16, A_MN, B_MN, kBM, kBN);
-      int64_t it = 0;
+      const uint64_t da0 = A_MN ? smem_desc_mn_sw128(smem_u32(s_a(0))) : smem_desc_k_sw128(smem_u32(s_a(0)));
+      const uint64_t db0 = B_MN ? smem_desc_mn_sw128(smem_u32(s_b(0, 0))) : smem_desc_k_sw128(smem_u32(s_b(0, 0)));
+      constexpr uint32_t kStepA = A_MN ? 2048 : 32, kStepB = B_MN ? 2048 : 32;  // K = 16: 16 lines, or 32 bytes of a line
+      const int chunk = chunk_of<EPI>(kblocks);
+      Ring<kStages> r;
       bool ok = true;
       int n = 0;  // accumulators handed over
       for (int u = blockIdx.x >> 1; u < units && ok; u += pairs) {
         int mb, nb, k0, k1;
         unit_at(u, p, kblocks, mb, nb, k0, k1);
-        for (int kc = k0; kc < k1 && ok; kc += chunk_of<EPI>(kblocks), n += NH) {
-          const int ke = min(k1, kc + chunk_of<EPI>(kblocks));
-          for (int kb = kc; kb < ke; ++kb, ++it) {
-            const int s = (int)(it % kStages);
-            if (*abort_flag || !mbar_wait_cluster(&full[s], (uint32_t)(it / kStages) & 1u)) {
+        for (int kc = k0; kc < k1 && ok; kc += chunk, n += NH) {
+          const int ke = min(k1, kc + chunk);
+          for (int kb = kc; kb < ke; ++kb, r.next()) {
+            if (!warp_agrees(mbar_wait_cluster(&full[r.s], r.ph) && !*abort_flag)) {
               ok = false;
               break;
             }
-            const uint32_t a0 = smem_u32(s_a(s));
+            const uint64_t da = desc_add(da0, r.s * kStage), db = desc_add(db0, r.s * kStage);
+            const uint32_t add = kb > kc;
             #pragma unroll
             for (int h = 0; h < NH; ++h) {
               const int b = (n + h) & 1;
-              if (kb == kc && !mbar_wait_cluster(&acc_empty[b], ((uint32_t)((n + h) >> 1) & 1u) ^ 1u)) {
+              if (kb == kc && !warp_agrees(mbar_wait_cluster(&acc_empty[b], ((uint32_t)((n + h) >> 1) & 1u) ^ 1u))) {
                 ok = false;
                 break;
               }
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              const uint32_t b0 = smem_u32(s_b(s, h));
-              #pragma unroll
-              for (int j = 0; j < 4; ++j) {  // K = 16: 32 bytes along a K-major line, 16 lines of an MN-major operand
-                const uint64_t da = A_MN ? smem_desc_mn_sw128(a0 + j * 2048) : smem_desc_k_sw128(a0 + j * 32);
-                const uint64_t db = B_MN ? smem_desc_mn_sw128(b0 + j * 2048) : smem_desc_k_sw128(b0 + j * 32);
-                asm volatile(
-                    "{\n\t.reg .pred p;\n\t"
-                    "setp.ne.b32 p, %4, 0;\n\t"
-                    "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + b * kBN),
-                    "l"(da), "l"(db), "r"(idesc), "r"((kb > kc || j > 0) ? 1u : 0u)
-                    : "memory");
+              if (lead) {
+                #pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  asm volatile(
+                      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + b * kBN),
+                      "l"(desc_add(da, j * kStepA)), "l"(desc_add(db, h * kHalf + j * kStepB)), "r"(idesc),
+                      "r"(j > 0 ? 1u : add)
+                      : "memory");
+                if (kb == ke - 1) commit_pair(&acc_full[b]);
+                if (h == NH - 1) commit_pair(&empty[r.s]);
               }
-              if (kb == ke - 1) commit_pair(&acc_full[b]);
+              __syncwarp();
             }
             if (!ok) break;
-            commit_pair(&empty[s]);
           }
         }
       }
-      if (!ok) {
+      if (!ok && lead) {
         *abort_flag = 1;
         atomicCAS(p.status, 0, 3);
       }

@@ -17,7 +17,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import ops
-from ._lib import call, ptr
+from ._lib import call_on, load, ptr
 
 BLOCK = 32
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -63,6 +63,13 @@ class Mx4Tensor:
     def device(self) -> torch.device:
         return self.codes.device
 
+    @classmethod
+    def _checked(cls, codes, scales, shape) -> "Mx4Tensor":
+        """A tensor whose parts are known to fit (they were just made)."""
+        q = cls.__new__(cls)
+        q.codes, q.scales, q.shape = codes, scales, shape
+        return q
+
     def to(self, device) -> "Mx4Tensor":
         return Mx4Tensor(self.codes.to(device), self.scales.to(device), self.shape)
 
@@ -76,7 +83,6 @@ def _rows_of(x: torch.Tensor, what: str) -> torch.Tensor:
         raise ValueError("mpq_b200 kernels require CUDA tensors (there is no CPU path)")
     if x.dim() < 1:
         raise ValueError(f"{what} needs at least one dimension")
-    x = x.detach()
     if x.dim() != 2:
         x = x.reshape(x.numel() // x.shape[-1] if x.shape[-1] else 0, x.shape[-1])
     if x.numel() and (x.stride(1) != 1 and x.shape[1] != 1 or x.stride(0) < x.shape[1]):
@@ -93,9 +99,9 @@ def quantize_mx4(x: torch.Tensor) -> Mx4Tensor:
     shape_codes, shape_scales = stored_shapes(rows, cols)
     codes = torch.empty(shape_codes, device=x.device, dtype=torch.uint8)
     scales = torch.empty(shape_scales, device=x.device, dtype=torch.uint8)
-    with torch.cuda.device(x.device):
-        call("mpq_mx4_quantize", ptr(x), code, max(x.stride(0), cols), rows, cols, ptr(codes), ptr(scales))
-    return Mx4Tensor(codes, scales, (rows, cols))
+    call_on(x.device.index, "mpq_mx4_quantize", x.data_ptr(), code, max(x.stride(0), cols), rows, cols, codes.data_ptr(),
+            scales.data_ptr())
+    return Mx4Tensor._checked(codes, scales, (rows, cols))
 
 
 def dequantize_mx4(q: Mx4Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -106,8 +112,8 @@ def dequantize_mx4(q: Mx4Tensor, dtype: torch.dtype = torch.float32) -> torch.Te
         raise ValueError("mpq_b200 kernels require CUDA tensors (there is no CPU path)")
     rows, cols = q.shape
     out = torch.empty(rows, cols, device=q.device, dtype=dtype)
-    with torch.cuda.device(q.device):
-        call("mpq_mx4_dequantize", ptr(q.codes), ptr(q.scales), rows, cols, ptr(out), code, max(cols, 1))
+    call_on(out.device.index, "mpq_mx4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, out.data_ptr(), code,
+            max(cols, 1))
     return out
 
 
@@ -131,11 +137,12 @@ def mx4_linear(x: torch.Tensor, weight: Mx4Tensor, bias: Optional[torch.Tensor] 
         if k == 0:
             out.zero_() if bias is None else out.copy_(bias.expand(m, n))
         else:
-            q = quantize_mx4(rows)
-            with torch.cuda.device(x.device):
-                call("mpq_mx4_gemm", m, n, k, ptr(q.codes), ptr(q.scales), ptr(weight.codes), ptr(weight.scales),
-                     ptr(bias), ptr(out), code, n, ptr(ops.status_word(x.device)))
-    return out.view(*x.shape[:-1], n)
+            need = load().mpq_mx4_linear_work(m, k)
+            work = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
+            call_on(x.device.index, "mpq_mx4_linear", rows.data_ptr(), code, max(rows.stride(0), k), m, n, k,
+                    weight.codes.data_ptr(), weight.scales.data_ptr(), ptr(bias), ptr(work), out.data_ptr(), n,
+                    ops.status_word(x.device).data_ptr())
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
 
 
 class Mx4Linear(torch.nn.Module):

@@ -171,6 +171,17 @@ def test_linear(cuda_dev, m, n, k, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m,n,k", [(12, 4096, 2048), (5, 192, 4128), (128, 1000, 8200), (4, 96, 32), (2, 31, 20000), (3, 40, 20000),
+                                   (1, 5, 180000), (2600, 1153, 288), (3000, 2000, 1000), (2049, 4097, 96), (1537, 3900, 2080)])
+def test_linear_split_and_wide(cuda_dev, m, n, k, dtype):
+    """K shared by a cluster, K too long for the kernel of few tokens, and tiles of CTA pairs with ragged ends."""
+    x = values(m, k, dtype, cuda_dev, 4, 0.4)
+    w = values(n, k, dtype, cuda_dev, 5, 0.4) * 0.05
+    check_linear(x, w)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 5, 40, 200])
 def test_linear_bias_strides_and_leading_dimensions(cuda_dev, m):
     g = torch.Generator().manual_seed(5)
