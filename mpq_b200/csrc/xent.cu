@@ -44,6 +44,7 @@ enum { kLse = 0, kGrad = 1, kOut = 2 };
 struct Args {
   int M, N, K, mt, nt;      // C[M, N] over K; mt x nt tiles
   int splits;               // parts of K; more than one only with `acc`
+  int tile_out;             // the result's rows are aligned for tile stores
   int f16;                  // 1: f16 operands, 0: bf16
   int* status;
   // kLse, kGrad
@@ -119,23 +120,20 @@ __device__ __forceinline__ void unit_at(int u, const Args& p, int kblocks, int& 
 template <int EPI>
 __device__ __forceinline__ int chunk_of(int kblocks) { return EPI == kLse ? kChunk : kblocks; }
 
-// 32 consecutive 16-bit values of one row, `lim` of them wanted.
-__device__ __forceinline__ void store_words(uint16_t* dst, const uint32_t (&w)[16], int lim) {
-  if (lim >= 32 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+// 64 16-bit values (32 words) of each of a warp's rows from (row0, col) on, `lim` columns wanted: as a tile, or by the
+// threads where the result's rows are not aligned.
+__device__ __forceinline__ void store_half_rows(const Args& p, const CUtensorMap* map, unsigned char* buf, int lane, int row0,
+                                                int col, uint16_t* out, int64_t ld, const uint32_t (&w)[32], int lim) {
+  if (lim <= 0 || row0 >= p.M) return;  // the same for the warp
+  if (p.tile_out) {
+    chunk_put(buf, lane, w);
+    chunk_send(buf, lane, map, col, row0, 0);
+  } else if (row0 + lane < p.M) {
+    uint16_t* dst = out + (int64_t)(row0 + lane) * ld + col;
     #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-  } else {
-    #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 64; ++i)
       if (i < lim) dst[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
   }
-}
-__device__ __forceinline__ void store16(void* out, int64_t at, const float (&o)[32], int lim, int f16) {
-  uint32_t w[16];
-  #pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = pack16(o[2 * i], o[2 * i + 1], f16);
-  store_words(reinterpret_cast<uint16_t*>(out) + at, w, lim);
 }
 
 // 2^t in one instruction (denormal results become 0, 2^-22 relative)
@@ -165,12 +163,14 @@ __device__ __forceinline__ uint32_t distance_bits(float t) {
 // forward pass (kLse) accumulates kChunk k-blocks at a time and adds these to nearest in registers.
 template <int EPI, bool A_MN, bool B_MN, int NH>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    k_xent_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args p) {
+    k_xent_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ CUtensorMap map_o, const Args p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr int kStages = stages_of(NH);
   constexpr uint32_t kStage = (1 + NH) * kHalf;
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kStage);
+  unsigned char* out_buf = ring + kStages * kStage;  // 4 KB to an epilogue warp
+  uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + kEpiWarps * 4096);
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;
   uint64_t* acc_empty = acc_full + 2;
@@ -306,6 +306,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else {
     // a warp reads the TMEM lanes of its quadrant (warp % 4); warps 2..5 take columns 0..127, warps 6..9 the others
     const int quad = warp & 3, half = (warp - 2) >> 2;
+    unsigned char* buf = out_buf + (warp - 2) * 4096;
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * 128);
     int n = 0;
     // the next accumulator in TMEM, false after a time-out
@@ -328,7 +329,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int u = blockIdx.x >> 1; u < units; u += pairs) {
       int mb, nb, k0, k1;
       unit_at(u, p, kblocks, mb, nb, k0, k1);
-      const int row = mb * kBM + rank * 128 + quad * 32 + lane;
+      const int row0 = mb * kBM + rank * 128 + quad * 32, row = row0 + lane;
       const bool live = row < p.M;
       bool good = true;
       #pragma unroll 1
@@ -381,50 +382,69 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         #pragma unroll
         for (int i = 1; i < 128; ++i) m = fmaxf(m, x[i]);
         const float m2 = m == -INFINITY ? 0.f : m * kLog2e;
-        const bool keep = live && n0 < p.keep_cols;
+        const bool keep = n0 < p.keep_cols;
         float sum0 = 0.f, sum1 = 0.f;
         #pragma unroll
-        for (int c0 = 0; c0 < 128; c0 += 32) {
-          uint32_t w[16];
+        for (int c0 = 0; c0 < 128; c0 += 64) {
+          uint32_t w[32];
           #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 32; ++i) {
             const float t0 = fmaf(x[c0 + 2 * i], kLog2e, -m2), t1 = fmaf(x[c0 + 2 * i + 1], kLog2e, -m2);
             sum0 += ex2(t0);
             sum1 += ex2(t1);
             w[i] = __byte_perm(distance_bits(t0), distance_bits(t1), 0x5410);
           }
-          if (keep && lim - c0 > 0) store_words(p.keep + (int64_t)row * p.ldk + n0 + c0, w, lim - c0);
+          if (keep) store_half_rows(p, &map_o, buf, lane, row0, n0 + c0, p.keep, p.ldk, w, lim - c0);
         }
         if (live) p.part[(int64_t)row * (2 * p.nt) + 2 * nb + half] = make_float2(lim > 0 ? m2 : -INFINITY, sum0 + sum1);
       } else {
         if (!(good = take())) break;
-        #pragma unroll 1
-        for (int c0 = 0; c0 < 128; c0 += 32) {
-          uint32_t v[32];
-          tmem_ld32(lanes + (uint32_t)((n & 1) * kBN + c0), v);
-          const int lim = p.N - (n0 + c0);
-          if (lim <= 0) continue;
-          float o[32];
-          if constexpr (EPI == kGrad) {
+        const uint32_t at = lanes + (uint32_t)((n & 1) * kBN);
+        if (EPI == kOut && p.acc) {
+          float* acc = p.acc + (int64_t)(u % p.splits) * p.M * p.N;
+          #pragma unroll 1
+          for (int c0 = 0; c0 < 128; c0 += 32) {
+            uint32_t v[32];
+            tmem_ld32(at + c0, v);
+            const int lim = p.N - (n0 + c0);
+            if (lim <= 0 || row0 >= p.M) continue;
             #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float e = ex2(fmaf(__uint_as_float(v[i]), kLog2e, -lse2)) - (label == c0 + i ? 1.f : 0.f);
-              o[i] = g == 0.f ? 0.f : g * e;
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(alpha * __uint_as_float(v[i]));
+            if (p.tile_out) {
+              chunk_put(buf, lane, v);
+              chunk_send(buf, lane, &map_o, n0 + c0, row0, u % p.splits);
+            } else if (live) {
+              #pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i < lim) acc[(int64_t)row * p.N + n0 + c0 + i] = __uint_as_float(v[i]);
             }
-            if (live) store16(p.out, (int64_t)row * p.ldo + n0 + c0, o, lim, p.f16);
-          } else {
+          }
+        } else {
+          #pragma unroll 1
+          for (int c0 = 0; c0 < 128; c0 += 64) {
+            uint32_t w[32];
             #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = alpha * __uint_as_float(v[i]);
-            if (live) {
-              if (!p.acc) {
-                store16(p.out, (int64_t)row * p.ldo + n0 + c0, o, lim, p.f16);
-              } else {
-                float* acc = p.acc + ((int64_t)(u % p.splits) * p.M + row) * p.N + n0 + c0;
-                #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (i < lim) acc[i] = o[i];
+            for (int q = 0; q < 2; ++q) {
+              uint32_t v[32];
+              tmem_ld32(at + c0 + 32 * q, v);
+              #pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float a, b;
+                if constexpr (EPI == kGrad) {
+                  const int c = c0 + 32 * q + i;
+                  a = ex2(fmaf(__uint_as_float(v[i]), kLog2e, -lse2)) - (label == c ? 1.f : 0.f);
+                  b = ex2(fmaf(__uint_as_float(v[i + 1]), kLog2e, -lse2)) - (label == c + 1 ? 1.f : 0.f);
+                  a = g == 0.f ? 0.f : g * a;
+                  b = g == 0.f ? 0.f : g * b;
+                } else {
+                  a = alpha * __uint_as_float(v[i]);
+                  b = alpha * __uint_as_float(v[i + 1]);
+                }
+                w[16 * q + i / 2] = pack16(a, b, p.f16);
               }
             }
+            store_half_rows(p, &map_o, buf, lane, row0, n0 + c0, reinterpret_cast<uint16_t*>(p.out), p.ldo, w,
+                            p.N - (n0 + c0));
           }
         }
         release();
@@ -432,6 +452,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if (!good) break;
     }
+    chunk_drain(lane);
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncwarp();
@@ -626,10 +647,18 @@ static int product(const void* A, int64_t lda, const void* B, int64_t ldb, Args 
   p.mt = (p.M + kBM - 1) / kBM;
   p.nt = (p.N + kBN * NH - 1) / (kBN * NH);
   p.splits = std::max(p.splits, 1);
-  const size_t smem = 1024 + stages_of(NH) * (1 + NH) * kHalf + 256;
+  CUtensorMap mo{};
+  const int type = p.f16 ? 2 : 1;
+  if (EPI == kLse)
+    p.tile_out = p.keep_cols && result_map(&mo, p.keep, type, 1, p.M, p.keep_cols, p.ldk);
+  else if (p.acc)
+    p.tile_out = result_map(&mo, p.acc, 0, p.splits, p.M, p.N, p.N);
+  else
+    p.tile_out = result_map(&mo, p.out, type, 1, p.M, p.N, p.ldo);
+  const size_t smem = 1024 + stages_of(NH) * (1 + NH) * kHalf + kEpiWarps * 4096 + 256;
   if ((r = smem_opt_in((const void*)k_xent_gemm<EPI, A_MN, B_MN, NH>, smem, "mpq_xent"))) return r;
   const int grid = 2 * std::min(p.mt * p.nt * p.splits, num_sms() / 2);
-  k_xent_gemm<EPI, A_MN, B_MN, NH><<<grid, kThreads, smem, st>>>(ma, mb, p);
+  k_xent_gemm<EPI, A_MN, B_MN, NH><<<grid, kThreads, smem, st>>>(ma, mb, mo, p);
   return launch_status("mpq_xent product");
 }
 
