@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       const uint32_t bytes = p.a_rows * 128 + kOperandB + 2 * kScale;
       int64_t it = 0;
-      Ring<kStages> r;
+      Ring r(kStages);
       bool ok = true;
       for (int t = first_tile; t < tiles && ok; t += stride) {
         const int mb = t % p.mt, nb = t / p.mt;
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t da0 = smem_desc_k_sw128(smem_u32(s_a(0))), db0 = smem_desc_k_sw128(smem_u32(s_b(0)));
     const uint64_t ds0 = scale_desc(smem_u32(s_sf(0)));
     const uint32_t i0 = idesc_mxf4(kBM, BN, 0), i2 = idesc_mxf4(kBM, BN, 2);
-    Ring<kStages> r;
+    Ring r(kStages);
     bool ok = true;
     int n = 0;
     for (int t = first_tile; t < tiles && ok; t += stride, ++n) {
@@ -722,7 +722,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       asm volatile("griddepcontrol.wait;" ::: "memory");  // A may come from the kernel before
       const uint32_t bar0 = mapa(smem_u32(full), 0);
       int64_t it = 0;
-      Ring<kPairStages> r;
+      Ring r(kPairStages);
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += pairs) {
         int mb, nb;
@@ -757,7 +757,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const bool lead = elect_one();
       const uint64_t da0 = smem_desc_k_sw128(smem_u32(s_a(0))), ds0 = scale_desc(smem_u32(s_sf(0)));
       const uint32_t i0 = idesc_mxf4(kPM, kPHalf, 0), i2 = idesc_mxf4(kPM, kPHalf, 2);
-      Ring<kPairStages> r;
+      Ring r(kPairStages);
       bool ok = true;
       uint32_t n = 0;  // tiles
       for (int t = pair; t < tiles && ok; t += pairs, ++n) {

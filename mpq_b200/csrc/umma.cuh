@@ -159,6 +159,26 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// 128 columns at once, one wait for all of them.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&x)[128]) {
+  #pragma unroll
+  for (int c = 0; c < 128; c += 32)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(x[c + 0]), "=f"(x[c + 1]), "=f"(x[c + 2]), "=f"(x[c + 3]),
+          "=f"(x[c + 4]), "=f"(x[c + 5]), "=f"(x[c + 6]), "=f"(x[c + 7]),
+          "=f"(x[c + 8]), "=f"(x[c + 9]), "=f"(x[c + 10]), "=f"(x[c + 11]),
+          "=f"(x[c + 12]), "=f"(x[c + 13]), "=f"(x[c + 14]), "=f"(x[c + 15]),
+          "=f"(x[c + 16]), "=f"(x[c + 17]), "=f"(x[c + 18]), "=f"(x[c + 19]),
+          "=f"(x[c + 20]), "=f"(x[c + 21]), "=f"(x[c + 22]), "=f"(x[c + 23]),
+          "=f"(x[c + 24]), "=f"(x[c + 25]), "=f"(x[c + 26]), "=f"(x[c + 27]),
+          "=f"(x[c + 28]), "=f"(x[c + 29]), "=f"(x[c + 30]), "=f"(x[c + 31])
+        : "r"(taddr + c));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
 // ---- results: a warp's 32 rows x 128 bytes through shared memory ----
 //
 // A thread holds a row of the accumulator; stored as it is, each 16 bytes of a warp go to 32 different lines, and the
@@ -166,13 +186,18 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
 // lays 128 bytes of each of its rows out in a 4 KB buffer of its own, swizzled as a tile load would (no bank is hit
 // twice), and one lane sends them off as a tile.
 
-__device__ __forceinline__ void chunk_put(unsigned char* buf, int lane, const uint32_t (&w)[32]) {
+__device__ __forceinline__ void chunk_begin(int lane) {
   if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last chunk has left the buffer
   __syncwarp();
+}
+// 16 bytes of the lane's row, j = 0..7
+__device__ __forceinline__ void chunk_unit(unsigned char* buf, int lane, int j, uint4 w) {
+  *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = w;
+}
+__device__ __forceinline__ void chunk_put(unsigned char* buf, int lane, const uint32_t (&w)[32]) {
+  chunk_begin(lane);
   #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  for (int j = 0; j < 8; ++j) chunk_unit(buf, lane, j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
 }
 // x: first column, y: first row, z: plane.  Rows and columns beyond the map's are not written.
 __device__ __forceinline__ void chunk_send(const unsigned char* buf, int lane, const CUtensorMap* map, int x, int y, int z) {
@@ -208,20 +233,20 @@ __device__ __forceinline__ bool warp_agrees(bool ok) { return __all_sync(0xfffff
 // K-major / MN-major descriptors advance by their low word: (byte offset) / 16.
 __device__ __forceinline__ uint64_t desc_add(uint64_t d, uint32_t bytes) { return d + (bytes >> 4); }
 
-// Position in a ring of N stages: slot and phase parity.
-template <int N>
+// Position in a ring of n stages: slot and phase parity.
 struct Ring {
-  int s = 0;
+  int n, s = 0;
   uint32_t ph = 0;
+  __device__ __forceinline__ explicit Ring(int stages) : n(stages) {}
   __device__ __forceinline__ void next() {
-    if (++s == N) {
+    if (++s == n) {
       s = 0;
       ph ^= 1u;
     }
   }
   __device__ __forceinline__ void back() {
     if (s-- == 0) {
-      s = N - 1;
+      s = n - 1;
       ph ^= 1u;
     }
   }

@@ -30,11 +30,11 @@ namespace xent {
 
 using namespace tc;
 
-// A tile is 256 x 256 NH, computed by a pair of CTAs: each holds 128 rows of A, 128 NH of B and of the accumulator 128
-// rows by 256 NH columns of TMEM.
+// A tile is 256 x 256, computed by a pair of CTAs: each holds 128 rows of A, 128 of B and 128 rows of the accumulator.
 constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
 constexpr int kBM = 256, kBN = 256, kGroup = 16;
-__host__ __device__ constexpr int stages_of(int NH) { return NH == 2 ? 4 : 6; }
+constexpr uint32_t kRingBytes = 192 * 1024;
+constexpr int kMostStages = 11;  // of 16 KB of B and 1 KB of A
 constexpr uint32_t kHalf = 128 * 128;  // bytes of an operand's 128 rows of one k-block (64 columns, one swizzle line)
 constexpr int kChunk = 8;              // k-blocks that the forward pass accumulates before it adds in FP32
 constexpr float kLog2e = 1.4426950408889634f;
@@ -45,6 +45,8 @@ struct Args {
   int M, N, K, mt, nt;      // C[M, N] over K; mt x nt tiles
   int splits;               // parts of K; more than one only with `acc`
   int tile_out;             // the result's rows are aligned for tile stores
+  int a_rows;               // rows of A that a CTA loads
+  int stages;               // of the ring, each 16 KB of B and a_rows x 128 bytes of A
   int f16;                  // 1: f16 operands, 0: bf16
   int* status;
   // kLse, kGrad
@@ -154,36 +156,39 @@ __device__ __forceinline__ uint32_t distance_bits(float t) {
 // 16-bit operands, FP32 accumulation in TMEM.  Persistent pairs of CTAs walk the 256 x 256 tiles (or, with `splits`,
 // a K range of a tile); in each CTA warp 0 loads its halves of the operands by TMA into a ring, warps 2..9 are the
 // epilogue, a row and 128 columns to a thread; warp 1 of the first CTA issues the MMAs of both (M = 256, N = 256,
-// tcgen05 cta_group::2), so that each CTA's shared memory feeds 128 columns of B instead of 256.
-// NH = 1: two accumulators of 256 columns let the epilogue overlap the next tile's MMAs.  NH = 2: a tile of 512 columns
-// fills TMEM, and each loaded row of A serves twice as many columns (48 KB of operands for 1024 tensor cycles, not
-// 2 x 32 KB); the next tile's first half starts when the epilogue has read the first half.
+// tcgen05 cta_group::2), so that each CTA's shared memory feeds 128 columns of B instead of 256.  Two accumulators let
+// the epilogue overlap the next tile's MMAs.  (A tile of 512 columns, which halves A's loads but fills TMEM, gained
+// nothing once the MMAs were issued fast enough: 6075 us against 6970 for dH at 8192 x 128256 x 4096.)
+//
+// With at most 128 rows of A only those are loaded: a tile load takes two to three cycles a 128-byte row, and 128 rows of
+// zeros would cost as much as the columns of B that bound such a product (1 x 128256 x 4096: 263 us with them, 209
+// without), and the ring takes more stages for it.  What the other rows' shared memory holds stays in their rows of
+// the accumulator.
 //
 // The tensor core's FP32 accumulator truncates, and a score is a small difference of sums of H products; so the
 // forward pass (kLse) accumulates kChunk k-blocks at a time and adds these to nearest in registers.
-template <int EPI, bool A_MN, bool B_MN, int NH>
+template <int EPI, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     k_xent_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_o, const Args p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kStages = stages_of(NH);
-  constexpr uint32_t kStage = (1 + NH) * kHalf;
-  unsigned char* out_buf = ring + kStages * kStage;  // 4 KB to an epilogue warp
+  unsigned char* out_buf = ring + kRingBytes;  // 4 KB to an epilogue warp
   uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + kEpiWarps * 4096);
-  uint64_t* empty = full + kStages;
-  uint64_t* acc_full = empty + kStages;
+  uint64_t* empty = full + kMostStages;
+  uint64_t* acc_full = empty + kMostStages;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  auto s_a = [&](int s) { return ring + s * kStage; };
-  auto s_b = [&](int s, int h) { return ring + s * kStage + (1 + h) * kHalf; };
+  const uint32_t a_bytes = p.a_rows * 128, stage = kHalf + a_bytes;
+  auto s_b = [&](int s) { return ring + s * stage; };
+  auto s_a = [&](int s) { return ring + s * stage + kHalf; };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), pairs = gridDim.x >> 1;
   const int kblocks = (p.K + 63) / 64, units = p.mt * p.nt * p.splits;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -209,19 +214,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       const uint32_t bar0 = mapa(smem_u32(full), 0);
       int64_t it = 0;
-      Ring<kStages> r;
+      Ring r(p.stages);
       bool ok = true;
       for (int u = blockIdx.x >> 1; u < units && ok; u += pairs) {
         int mb, nb, k0, k1;
         unit_at(u, p, kblocks, mb, nb, k0, k1);
-        const int row_a = mb * kBM + rank * 128, row_b = nb * NH * kBN + rank * 128;
+        const int row_a = mb * kBM + rank * 128, row_b = nb * kBN + rank * 128;
         for (int kb = k0; kb < k1; ++kb, ++it, r.next()) {
           if (!mbar_wait_cluster(&empty[r.s], r.ph ^ 1u) || *abort_flag) {
             ok = false;
             break;
           }
           // both CTAs' bytes count on the first one's barrier (a peer's copy may land before the expectation)
-          if (rank == 0) mbar_expect_tx(&full[r.s], 2 * kStage);
+          if (rank == 0) mbar_expect_tx(&full[r.s], 2 * stage);
           const uint32_t bar = bar0 + r.s * 8;
           if constexpr (A_MN) {
             tma_load_2d_pair(s_a(r.s), &map_a, bar, row_a, kb * 64);
@@ -229,20 +234,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           } else {
             tma_load_2d_pair(s_a(r.s), &map_a, bar, kb * 64, row_a);
           }
-          #pragma unroll
-          for (int h = 0; h < NH; ++h) {
-            if constexpr (B_MN) {
-              tma_load_2d_pair(s_b(r.s, h), &map_b, bar, row_b + h * kBN, kb * 64);
-              tma_load_2d_pair(s_b(r.s, h) + 8192, &map_b, bar, row_b + h * kBN + 64, kb * 64);
-            } else {
-              tma_load_2d_pair(s_b(r.s, h), &map_b, bar, kb * 64, row_b + h * kBN);
-            }
+          if constexpr (B_MN) {
+            tma_load_2d_pair(s_b(r.s), &map_b, bar, row_b, kb * 64);
+            tma_load_2d_pair(s_b(r.s) + 8192, &map_b, bar, row_b + 64, kb * 64);
+          } else {
+            tma_load_2d_pair(s_b(r.s), &map_b, bar, kb * 64, row_b);
           }
         }
       }
       if (!ok) {  // drain the copies in flight (each wait bounded); the peer leaves only after the cluster barrier
         *abort_flag = 1;
-        for (int i = 0; rank == 0 && i < kStages && i < it; ++i) {
+        for (int i = 0; rank == 0 && i < p.stages && i < it; ++i) {
           r.back();
           mbar_wait_cluster(&full[r.s], r.ph);
         }
@@ -254,47 +256,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const bool lead = elect_one();
       const uint32_t idesc = idesc16(p.f16, A_MN, B_MN, kBM, kBN);
       const uint64_t da0 = A_MN ? smem_desc_mn_sw128(smem_u32(s_a(0))) : smem_desc_k_sw128(smem_u32(s_a(0)));
-      const uint64_t db0 = B_MN ? smem_desc_mn_sw128(smem_u32(s_b(0, 0))) : smem_desc_k_sw128(smem_u32(s_b(0, 0)));
+      const uint64_t db0 = B_MN ? smem_desc_mn_sw128(smem_u32(s_b(0))) : smem_desc_k_sw128(smem_u32(s_b(0)));
       constexpr uint32_t kStepA = A_MN ? 2048 : 32, kStepB = B_MN ? 2048 : 32;  // K = 16: 16 lines, or 32 bytes of a line
       const int chunk = chunk_of<EPI>(kblocks);
-      Ring<kStages> r;
+      Ring r(p.stages);
       bool ok = true;
       int n = 0;  // accumulators handed over
       for (int u = blockIdx.x >> 1; u < units && ok; u += pairs) {
         int mb, nb, k0, k1;
         unit_at(u, p, kblocks, mb, nb, k0, k1);
-        for (int kc = k0; kc < k1 && ok; kc += chunk, n += NH) {
-          const int ke = min(k1, kc + chunk);
+        for (int kc = k0; kc < k1 && ok; kc += chunk, ++n) {
+          const int ke = min(k1, kc + chunk), b = n & 1;
+          if (!warp_agrees(mbar_wait_cluster(&acc_empty[b], ((uint32_t)(n >> 1) & 1u) ^ 1u))) {
+            ok = false;
+            break;
+          }
           for (int kb = kc; kb < ke; ++kb, r.next()) {
             if (!warp_agrees(mbar_wait_cluster(&full[r.s], r.ph) && !*abort_flag)) {
               ok = false;
               break;
             }
-            const uint64_t da = desc_add(da0, r.s * kStage), db = desc_add(db0, r.s * kStage);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint64_t da = desc_add(da0, r.s * stage), db = desc_add(db0, r.s * stage);
             const uint32_t add = kb > kc;
-            #pragma unroll
-            for (int h = 0; h < NH; ++h) {
-              const int b = (n + h) & 1;
-              if (kb == kc && !warp_agrees(mbar_wait_cluster(&acc_empty[b], ((uint32_t)((n + h) >> 1) & 1u) ^ 1u))) {
-                ok = false;
-                break;
-              }
-              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              if (lead) {
-                #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  asm volatile(
-                      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + b * kBN),
-                      "l"(desc_add(da, j * kStepA)), "l"(desc_add(db, h * kHalf + j * kStepB)), "r"(idesc),
-                      "r"(j > 0 ? 1u : add)
-                      : "memory");
-                if (kb == ke - 1) commit_pair(&acc_full[b]);
-                if (h == NH - 1) commit_pair(&empty[r.s]);
-              }
-              __syncwarp();
+            if (lead) {
+              #pragma unroll
+              for (int j = 0; j < 4; ++j)
+                asm volatile(
+                    "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                    "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + b * kBN),
+                    "l"(desc_add(da, j * kStepA)), "l"(desc_add(db, j * kStepB)), "r"(idesc), "r"(j > 0 ? 1u : add)
+                    : "memory");
+              commit_pair(&empty[r.s]);
+              if (kb == ke - 1) commit_pair(&acc_full[b]);
             }
-            if (!ok) break;
+            __syncwarp();
           }
         }
       }
@@ -309,6 +305,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     unsigned char* buf = out_buf + (warp - 2) * 4096;
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * 128);
     int n = 0;
+    const float alpha = EPI == kOut ? unit_of(p.gout, p.count, p.gmax, p.f16) : 1.f;
     // the next accumulator in TMEM, false after a time-out
     auto take = [&]() {
       const bool ready = !*abort_flag && mbar_wait_cluster(&acc_full[n & 1], (uint32_t)(n >> 1) & 1u);
@@ -331,13 +328,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       unit_at(u, p, kblocks, mb, nb, k0, k1);
       const int row0 = mb * kBM + rank * 128 + quad * 32, row = row0 + lane;
       const bool live = row < p.M;
-      bool good = true;
-      #pragma unroll 1
-      for (int h = 0; h < NH; ++h) {
-      const int n0 = (nb * NH + h) * kBN + half * 128;
+      const int n0 = nb * kBN + half * 128;
       int label = -1;  // the label's column among this thread's 128, if it is one of them
-      float g = 0.f, lse2 = 0.f, alpha = 1.f;
-      if constexpr (EPI == kOut) alpha = unit_of(p.gout, p.count, p.gmax, p.f16);
+      float g = 0.f, lse2 = 0.f;
       if constexpr (EPI != kOut) {
         if (live) {
           const int64_t y = p.labels[row];
@@ -353,9 +346,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if constexpr (EPI == kLse) {
         float x[128];
-        #pragma unroll
-        for (int i = 0; i < 128; ++i) x[i] = 0.f;
-        for (int kc = k0; kc < k1; kc += kChunk) {
+        if (!take()) break;
+        tmem_ld128(lanes + (uint32_t)((n & 1) * kBN), x);
+        release();
+        bool good = true;
+        #pragma unroll 1
+        for (int kc = k0 + kChunk; kc < k1; kc += kChunk) {
           if (!(good = take())) break;
           #pragma unroll
           for (int c0 = 0; c0 < 128; c0 += 16) {
@@ -382,23 +378,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         #pragma unroll
         for (int i = 1; i < 128; ++i) m = fmaxf(m, x[i]);
         const float m2 = m == -INFINITY ? 0.f : m * kLog2e;
-        const bool keep = n0 < p.keep_cols;
+        if (n0 < p.keep_cols && row0 < p.M) {
+          #pragma unroll
+          for (int c0 = 0; c0 < 128; c0 += 64) {
+            if (lim <= c0) break;
+            chunk_begin(lane);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) {  // 16 bytes at a time: the sums leave no registers for more
+              uint32_t w[4];
+              #pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int c = c0 + 8 * j + 2 * i;
+                w[i] = __byte_perm(distance_bits(fmaf(x[c], kLog2e, -m2)), distance_bits(fmaf(x[c + 1], kLog2e, -m2)), 0x5410);
+              }
+              chunk_unit(buf, lane, j, make_uint4(w[0], w[1], w[2], w[3]));
+            }
+            chunk_send(buf, lane, &map_o, n0 + c0, row0, 0);
+          }
+        }
         float sum0 = 0.f, sum1 = 0.f;
         #pragma unroll
-        for (int c0 = 0; c0 < 128; c0 += 64) {
-          uint32_t w[32];
-          #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float t0 = fmaf(x[c0 + 2 * i], kLog2e, -m2), t1 = fmaf(x[c0 + 2 * i + 1], kLog2e, -m2);
-            sum0 += ex2(t0);
-            sum1 += ex2(t1);
-            w[i] = __byte_perm(distance_bits(t0), distance_bits(t1), 0x5410);
-          }
-          if (keep) store_half_rows(p, &map_o, buf, lane, row0, n0 + c0, p.keep, p.ldk, w, lim - c0);
+        for (int i = 0; i < 128; i += 2) {
+          sum0 += ex2(fmaf(x[i], kLog2e, -m2));
+          sum1 += ex2(fmaf(x[i + 1], kLog2e, -m2));
         }
         if (live) p.part[(int64_t)row * (2 * p.nt) + 2 * nb + half] = make_float2(lim > 0 ? m2 : -INFINITY, sum0 + sum1);
       } else {
-        if (!(good = take())) break;
+        if (!take()) break;
         const uint32_t at = lanes + (uint32_t)((n & 1) * kBN);
         if (EPI == kOut && p.acc) {
           float* acc = p.acc + (int64_t)(u % p.splits) * p.M * p.N;
@@ -449,8 +455,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         release();
       }
-      }
-      if (!good) break;
     }
     chunk_drain(lane);
   }
@@ -608,63 +612,51 @@ static int num_sms() {
   return cached[dev];
 }
 
-// How an M x N product over K is cut: columns of a tile (256 NH) and parts of K.
-struct Plan {
-  int nh, splits;
-};
-
-// The plan with the least estimated time on `pairs` CTA pairs.  A unit takes its k-blocks x columns, a tenth more for
-// 256-column tiles (their operands are loaded twice as often for the same product); parts of K add FP32
-// planes, written and read once, at 3600 bytes a cycle (the memory's rate).
-// Every part has at least 16 k-blocks.
-static Plan plan_for(int M, int N, int K) {
+// Parts of K for an M x N product: the number with the least estimated cycles.  A unit takes 512 a k-block and 2000 for
+// its start and end; parts add FP32 planes, written and read once at 3600 bytes a cycle (the memory's rate), and the
+// launch that sums them.  Every part has at least 16 k-blocks.  (dH at 511 x 32003 x 2048, us: 1 part 190, 2 96, 4 65,
+// 8 73; at 8192 x 128256 x 4096: 1 part 6075, 2 7600.)
+static int splits_for(int M, int N, int K) {
   const int pairs = num_sms() / 2, kblocks = (K + 63) / 64;
-  const double mt = (M + kBM - 1) / kBM;
-  Plan best{1, 1};
+  const double tiles = (double)((M + kBM - 1) / kBM) * ((N + kBN - 1) / kBN);
+  int best = 1;
   double least = 1e300;
-  for (int nh = 1; nh <= 2; ++nh) {
-    const double tiles = mt * ((N + kBN * nh - 1) / (kBN * nh));
-    for (int s = 1; s <= 32 && s * 16 <= std::max(kblocks, 16); ++s) {
-      const double waves = std::ceil(tiles * s / pairs);
-      const double unit = std::ceil((double)kblocks / s) * 512 * nh * (nh == 1 ? 1.1 : 1.0) + 2000;
-      const double planes = s > 1 ? 8.0 * M * N * s / 3600.0 : 0.0;
-      const double t = waves * unit + planes;
-      if (t < 0.98 * least) {
-        least = t;
-        best = {nh, s};
-      }
+  for (int s = 1; s <= 32 && (s == 1 || s * 16 <= kblocks); ++s) {
+    const double planes = s > 1 ? 8.0 * M * N * s / 3600.0 + 5000.0 : 0.0;
+    const double t = std::ceil(tiles * s / pairs) * (std::ceil((double)kblocks / s) * 512 + 2000) + planes;
+    if (t < 0.98 * least) {
+      least = t;
+      best = s;
     }
   }
   return best;
 }
 
-template <int EPI, bool A_MN, bool B_MN, int NH>
+template <int EPI, bool A_MN, bool B_MN>
 static int product(const void* A, int64_t lda, const void* B, int64_t ldb, Args p, cudaStream_t st) {
-  CUtensorMap ma, mb;
-  int r = operand(&ma, A_MN, A, p.M, p.K, lda, 128, p.f16);
+  CUtensorMap ma, mb, mo{};
+  p.a_rows = A_MN ? 128 : std::min((p.M + 7) / 8 * 8, 128);
+  p.stages = std::min<int>(kMostStages, kRingBytes / (kHalf + p.a_rows * 128));
+  int r = operand(&ma, A_MN, A, p.M, p.K, lda, p.a_rows, p.f16);
   if (r) return r;
   if ((r = operand(&mb, B_MN, B, p.N, p.K, ldb, 128, p.f16))) return r;
   p.mt = (p.M + kBM - 1) / kBM;
-  p.nt = (p.N + kBN * NH - 1) / (kBN * NH);
+  p.nt = (p.N + kBN - 1) / kBN;
   p.splits = std::max(p.splits, 1);
-  CUtensorMap mo{};
   const int type = p.f16 ? 2 : 1;
-  if (EPI == kLse)
-    p.tile_out = p.keep_cols && result_map(&mo, p.keep, type, 1, p.M, p.keep_cols, p.ldk);
-  else if (p.acc)
+  if (EPI == kLse) {
+    MPQ_CHECK_ARG(p.keep_cols == 0 || result_map(&mo, p.keep, type, 1, p.M, p.keep_cols, p.ldk),
+                  "mpq_xent_forward: no tensor map for %d kept columns", p.keep_cols);
+  } else if (p.acc) {
     p.tile_out = result_map(&mo, p.acc, 0, p.splits, p.M, p.N, p.N);
-  else
+  } else {
     p.tile_out = result_map(&mo, p.out, type, 1, p.M, p.N, p.ldo);
-  const size_t smem = 1024 + stages_of(NH) * (1 + NH) * kHalf + kEpiWarps * 4096 + 256;
-  if ((r = smem_opt_in((const void*)k_xent_gemm<EPI, A_MN, B_MN, NH>, smem, "mpq_xent"))) return r;
+  }
+  const size_t smem = 1024 + kRingBytes + kEpiWarps * 4096 + 256;
+  if ((r = smem_opt_in((const void*)k_xent_gemm<EPI, A_MN, B_MN>, smem, "mpq_xent"))) return r;
   const int grid = 2 * std::min(p.mt * p.nt * p.splits, num_sms() / 2);
-  k_xent_gemm<EPI, A_MN, B_MN, NH><<<grid, kThreads, smem, st>>>(ma, mb, mo, p);
+  k_xent_gemm<EPI, A_MN, B_MN><<<grid, kThreads, smem, st>>>(ma, mb, mo, p);
   return launch_status("mpq_xent product");
-}
-
-template <bool A_MN>
-static int out_product(int nh, const void* A, int64_t lda, const void* B, int64_t ldb, const Args& p, cudaStream_t st) {
-  return nh == 2 ? product<kOut, A_MN, true, 2>(A, lda, B, ldb, p, st) : product<kOut, A_MN, true, 1>(A, lda, B, ldb, p, st);
 }
 
 // Width of the piece that starts at column v0.
@@ -691,7 +683,7 @@ MPQ_API int mpq_xent_planes(int T, int V, int H, int piece, int keep_cols) {
   const int rest = V - keep_cols, pieces = (keep_cols > 0) + (rest + piece - 1) / piece;
   int most = 1;  // over the widths that occur: the kept columns, whole pieces and the last one
   for (int w : {keep_cols, std::min(piece, rest), rest % piece})
-    if (w > 0) most = std::max(most, xent::plan_for(T, H, w).splits);
+    if (w > 0) most = std::max(most, xent::splits_for(T, H, w));
   return pieces > 1 ? most + 1 : (most > 1 ? most : 0);
 }
 
@@ -727,7 +719,7 @@ MPQ_API int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden,
   p.part = reinterpret_cast<float2*>(part);
   p.tgt = tgt;
   p.keep = reinterpret_cast<uint16_t*>(keep); p.ldk = ldk; p.keep_cols = keep_cols;
-  st = xent::product<xent::kLse, false, false, 1>(hidden, ldh, weight, ldw, p, (cudaStream_t)stream);
+  st = xent::product<xent::kLse, false, false>(hidden, ldh, weight, ldw, p, (cudaStream_t)stream);
   if (st) return st;
   xent::k_xent_join<<<T, 128, 0, (cudaStream_t)stream>>>(p.part, (int)mpq_xent_tiles(V), tgt, labels, ignore, V, lse, nll);
   if ((st = launch_status("mpq_xent_forward (join)")) || reduction == 0) return st;
@@ -787,19 +779,18 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
       p.labels = labels; p.ignore = ignore; p.vocab = V; p.v0 = v0;
       p.lse = lse;
       p.out = d; p.ldo = piece;
-      if ((st = xent::product<xent::kGrad, false, false, 1>(hidden, ldh, W, ldw, p, cs))) return st;
+      if ((st = xent::product<xent::kGrad, false, false>(hidden, ldh, W, ldw, p, cs))) return st;
     }
     if (dhidden) {
-      const xent::Plan plan = xent::plan_for(T, H, w);
       p.M = T; p.N = H; p.K = w;
       p.out = dhidden; p.ldo = lddh;
       p.acc = planes ? acc : nullptr;
-      p.splits = plan.splits;
-      if ((st = xent::out_product<false>(plan.nh, dv, ldd, W, ldw, p, cs))) return st;
+      p.splits = xent::splits_for(T, H, w);
+      if ((st = xent::product<xent::kOut, false, true>(dv, ldd, W, ldw, p, cs))) return st;
       if (planes) {
         const int64_t n = (int64_t)T * H;
         const int grid = (int)std::min<int64_t>((n + 255) / 256, 8 * xent::num_sms());
-        xent::k_xent_planes<<<grid, 256, 0, cs>>>(acc, plan.splits, T, H, acc + (planes - 1) * n, v0 > 0,
+        xent::k_xent_planes<<<grid, 256, 0, cs>>>(acc, p.splits, T, H, acc + (planes - 1) * n, v0 > 0,
                                                   v0 + w == V ? (uint16_t*)dhidden : nullptr, lddh, f16);
         if ((st = launch_status("mpq_xent_backward (planes)"))) return st;
       }
@@ -809,8 +800,7 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
       p.out = reinterpret_cast<uint16_t*>(dweight) + (int64_t)v0 * lddw; p.ldo = lddw;
       p.acc = nullptr;
       p.splits = 1;
-      const int nh = xent::plan_for(w, H, T).nh;
-      if ((st = xent::out_product<true>(nh, dv, ldd, hidden, ldh, p, cs))) return st;
+      if ((st = xent::product<xent::kOut, true, true>(dv, ldd, hidden, ldh, p, cs))) return st;
     }
   }
   return MPQ_OK;
