@@ -95,46 +95,88 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int c, int cols
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Quantisation and reading back: eight elements to a lane (four lanes to a block), kRows rows to a thread
+// Quantisation and reading back
 // ------------------------------------------------------------------------------------------------------------------
 //
-// Both move memory: 4 or 2 bytes in and 17/32 out for an element, or the reverse.  A thread issues its kRows loads
-// before it uses the first, and a CTA of 256 threads covers as many rows side by side as a narrow matrix leaves room for.
+// Both move memory: 4 or 2 bytes in and 17/32 out for an element, or the reverse, which at the memory's rate leaves some
+// ten instructions an element.  Quantisation gives half a block to a thread: its partner's maximum is one shuffle away,
+// and for 16-bit types the maximum is taken two elements at a time.  (With a quarter block to a thread and every
+// element in 32 bits it ran 17 instructions an element, 2.5 TB/s.)  Reading back gives 16 bytes of the result to a
+// thread.  A thread issues its kRows rows' loads before it uses the first, and a CTA of 256 threads covers as many rows
+// side by side as a narrow matrix leaves room for.
 
-constexpr int kRows = 4;
+constexpr int kRows = 2;
+
+// Sixteen elements of a row as they are stored.
+template <class T>
+struct Half {
+  static constexpr int kWords = 16 * sizeof(T) / 4;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const T* __restrict__ row, int c, int cols, bool vec) {
+    if (vec && c + 16 <= cols) {
+      #pragma unroll
+      for (int i = 0; i < kWords / 4; ++i)
+        *reinterpret_cast<uint4*>(w + 4 * i) = __ldcs(reinterpret_cast<const uint4*>(row + c) + i);
+    } else {
+      #pragma unroll
+      for (int i = 0; i < 16; ++i) reinterpret_cast<T*>(w)[i] = c + i < cols ? row[c + i] : T(0.f);
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return to_f32(reinterpret_cast<const T*>(w)[i]); }
+  // the largest magnitude's FP32 bits
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t m = 0;
+    if constexpr (sizeof(T) == 4) {
+      #pragma unroll
+      for (int i = 0; i < kWords; ++i) m = max(m, w[i] & 0x7fffffffu);
+      return m;
+    } else {
+      #pragma unroll
+      for (int i = 0; i < kWords; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+      m = max(m & 0xffffu, m >> 16);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) return m << 16;
+      else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+    }
+  }
+};
 
 template <class T>
 __global__ void __launch_bounds__(256) k_mx4_quantize(const T* __restrict__ x, int64_t ldx, int rows, int cols, bool vec,
                                                       uint8_t* __restrict__ codes, int64_t ldc,
                                                       uint8_t* __restrict__ scales, int kt) {
   asm volatile("griddepcontrol.launch_dependents;");  // a product launched behind may set itself up
-  // blockDim.x is a multiple of 16 (a scale tile's width in quarter blocks), so the shuffles stay inside a block's lanes
+  // blockDim.x is a multiple of 8 (a scale tile's width in half blocks): partners sit in one warp
   const int nb = (cols + 31) >> 5, rows_pad = (rows + 127) & ~127;
-  const int q = blockIdx.y * blockDim.x + threadIdx.x, block = q >> 2;
-  const int64_t row0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * kRows;
-  const uint32_t four = 0xfu << ((threadIdx.y * blockDim.x + threadIdx.x) & 28);  // the block's lanes
-  float v[kRows][8];
+  const int q = blockIdx.y * blockDim.x + threadIdx.x, block = q >> 1;
+  const int row0 = (blockIdx.x * blockDim.y + threadIdx.y) * kRows;
+  const uint32_t two = 3u << ((threadIdx.y * blockDim.x + threadIdx.x) & 30);  // the block's lanes
+  if (block >= 4 * kt) return;
+  Half<T> h[kRows];
   #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     #pragma unroll
-    for (int i = 0; i < 8; ++i) v[r][i] = 0.f;
-    if (row0 + r < rows && block < nb) load8(x + (row0 + r) * ldx, q * 8, cols, vec, v[r]);
+    for (int i = 0; i < Half<T>::kWords; ++i) h[r].w[i] = 0;
+    if (row0 + r < rows && block < nb) h[r].load(x + (int64_t)(row0 + r) * ldx, q * 16, cols, vec);
   }
+  uint8_t* code = codes + (int64_t)row0 * ldc + q * 8;
   #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    const int64_t row = row0 + r;
-    uint32_t mag = 0;
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) mag = max(mag, __float_as_uint(v[r][i]) & 0x7fffffffu);
-    mag = max(mag, __shfl_xor_sync(four, mag, 1));
-    mag = max(mag, __shfl_xor_sync(four, mag, 2));
+    const int row = row0 + r;
+    uint32_t mag = h[r].largest();
+    mag = max(mag, __shfl_xor_sync(two, mag, 1));
     const uint32_t c = scale_code(mag);
-    const float inv = c == 255 ? 0.f : scale_inverse(c);
+    const float inv = c == 255 ? 0.f : scale_inverse(c);  // a block that is not finite reads back as NaN whatever it holds
+    uint2 word;
     #pragma unroll
-    for (int i = 0; i < 8; ++i) v[r][i] = c == 255 ? 0.f : v[r][i] * inv;
-    const uint32_t word = encode8(v[r]);
-    if (row < rows && block < nb) *reinterpret_cast<uint32_t*>(codes + row * ldc + q * 4) = word;
-    if (row < rows_pad && block < 4 * kt && (q & 3) == 0) scales[scale_at(row, block, kt)] = (uint8_t)c;
+    for (int k = 0; k < 2; ++k) {
+      float v[8];
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = h[r].at(8 * k + i) * inv;
+      (k ? word.y : word.x) = encode8(v);
+    }
+    if (row < rows && block < nb) *reinterpret_cast<uint2*>(code + r * ldc) = word;
+    if (row < rows_pad && (q & 1) == 0) scales[scale_at(row, block, kt)] = (uint8_t)c;
   }
 }
 
@@ -142,37 +184,37 @@ template <class T>
 __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restrict__ codes, int64_t ldc,
                                                         const uint8_t* __restrict__ scales, int kt, int rows, int cols,
                                                         bool vec, T* __restrict__ out, int64_t ldo) {
-  const int c0 = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
-  const int64_t row0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * kRows;
+  constexpr int kPer = 16 / sizeof(T);  // elements of a thread and row
+  const int c0 = (blockIdx.y * blockDim.x + threadIdx.x) * kPer;
+  const int row0 = (blockIdx.x * blockDim.y + threadIdx.y) * kRows * 2;
   if (c0 >= cols) return;
-  uint32_t w[kRows], c[kRows];
+  uint32_t w[kRows * 2], c[kRows * 2];
   #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int64_t row = min(row0 + r, (int64_t)rows - 1);
-    w[r] = *reinterpret_cast<const uint32_t*>(codes + row * ldc + c0 / 2);
+  for (int r = 0; r < kRows * 2; ++r) {
+    const int row = min(row0 + r, rows - 1);
+    const uint8_t* at = codes + (int64_t)row * ldc + c0 / 2;
+    w[r] = kPer == 8 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
     c[r] = scales[scale_at(row, c0 >> 5, kt)];
   }
   #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
+  for (int r = 0; r < kRows * 2; ++r) {
     if (row0 + r >= rows) break;
     const float s = scale_value(c[r]);
     __half2 h[4];
     decode8(w[r], h);
-    alignas(16) T v[8];
+    alignas(16) T v[kPer];
     #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kPer / 2; ++i) {
       const float2 f = __half22float2(h[i]);
       v[2 * i] = from_f32<T>(f.x * s);
       v[2 * i + 1] = from_f32<T>(f.y * s);
     }
-    T* dst = out + (row0 + r) * ldo + c0;
-    if (vec && c0 + 8 <= cols) {
-      #pragma unroll
-      for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i)
-        reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(v)[i];
+    T* dst = out + (int64_t)(row0 + r) * ldo + c0;
+    if (vec && c0 + kPer <= cols) {
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
     } else {
       #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < kPer; ++i)
         if (c0 + i < cols) dst[i] = v[i];
     }
   }
@@ -185,21 +227,12 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restric
 // W is read once (17 bytes for 32 weights), which bounds it.  Twice an E2M1 value is a small integer, so a block's 32
 // products are summed exactly in integers by dp4a and only then scaled: y += 2^(cx + cw - 256) sum (2 q_x) (2 q_w).
 // Every CTA quantises x for itself into shared memory (bytes 2 q_x, two planes of 16 bytes a block so that a warp's
-// reads are free of conflicts).  A warp takes whole rows of W, kFewRows at a time, a lane every 32nd block; each lane
-// copies its blocks ahead into a ring of kFewDepth steps of its own (cp.async, no barrier between lanes), so that the
-// reads from memory never wait for the arithmetic, nor for the quantisation of x at the start.  A weight's magnitude
-// comes from a byte permutation of the eight magnitudes; its sign is left to a second dp4a over the negative ones:
-// sum = all - 2 negative.
+// reads are free of conflicts) while its first weights are on their way.  A warp takes kFewRows rows of W and one of
+// `slices` parts of K (so that all warps have work whatever N is), a lane every 32nd block; the next blocks are loaded
+// before the last are used.  A weight's magnitude comes from a byte permutation of the eight magnitudes; its sign is
+// left to a second dp4a over the negative ones: sum = all - 2 negative.
 
-constexpr int kFewRows = 2, kFewThreads = 256, kFewDepth = 6;
-constexpr int kFewStep = kFewRows * 32 * 20;  // bytes of a warp's step: 16 of codes and 4 of scales for a lane and row
-
-__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_async4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
+constexpr int kFewRows = 4, kFewThreads = 256, kFewWarps = kFewThreads / 32;
 
 // Codes -> bytes 2 q (signed), eight to two words
 __device__ __forceinline__ void bytes_of(uint32_t w, uint32_t (&b)[2]) {
@@ -218,39 +251,35 @@ __device__ __forceinline__ void bytes_of(uint32_t w, uint32_t (&b)[2]) {
 template <class T, int TOK>
 __global__ void __launch_bounds__(kFewThreads, 2)
     k_mx4_few(const T* __restrict__ x, int64_t ldx, int tokens, int N, int K, bool vec, const uint8_t* __restrict__ codes,
-              const uint8_t* __restrict__ scales, const T* __restrict__ bias, T* __restrict__ out, int64_t ldo) {
+              const uint8_t* __restrict__ scales, const T* __restrict__ bias, T* __restrict__ out, int64_t ldo, int slices) {
   extern __shared__ __align__(16) unsigned char sm[];
+  __shared__ float part[2][kFewWarps][kFewRows * TOK];
   const int nb = (K + 31) >> 5, kt = (nb + 3) >> 2;
   uint4* xb = reinterpret_cast<uint4*>(sm);                        // [TOK][2][nb]
   float* xs = reinterpret_cast<float*>(xb + (size_t)TOK * 2 * nb);  // [TOK][nb], a quarter of the scale
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned char* ring = sm + (((size_t)TOK * nb * 36 + 15) & ~(size_t)15) + warp * kFewDepth * kFewStep;
-  const int warps = gridDim.x * (kFewThreads / 32), me = blockIdx.x * (kFewThreads / 32) + warp;
-  const int n0 = (int)((int64_t)N * me / warps), n1 = (int)((int64_t)N * (me + 1) / warps);
-  const int iters = (nb + 31) >> 5, steps = (n1 - n0 + kFewRows - 1) / kFewRows * iters;
-  int ln = n0, lb = lane, ls = 0;  // next step to load: row, this lane's block, slot
-  auto load_step = [&](int step) {
-    if (step < steps) {
-      unsigned char* at = ring + ls * kFewStep;
-      if (lb < nb) {
-        #pragma unroll
-        for (int r = 0; r < kFewRows; ++r) {
-          const int64_t row = min(ln + r, n1 - 1);
-          copy_async16(at + (r * 32 + lane) * 16, codes + (row * nb + lb) * 16);
-          copy_async4(at + kFewRows * 512 + (r * 32 + lane) * 4, scales + (scale_at(row, lb, kt) & ~(int64_t)3));
-        }
+  const int slice = warp % slices, wide = kFewWarps / slices;  // a CTA takes `wide` groups of rows at a time
+  const int iters = (nb + 31) >> 5, i0 = iters * slice / slices, i1 = iters * (slice + 1) / slices;
+  const int groups = (N + kFewRows - 1) / kFewRows, rounds = (groups + wide - 1) / wide;
+
+  uint4 raw[kFewRows];
+  uint32_t sc[kFewRows];
+  auto load = [&](int n0, int i) {
+    const int b = lane + 32 * i;
+    #pragma unroll
+    for (int r = 0; r < kFewRows; ++r) {
+      const int row = min(n0 + r, N - 1);
+      raw[r] = make_uint4(0, 0, 0, 0);
+      sc[r] = 0;
+      if (b < nb) {
+        raw[r] = __ldcs(reinterpret_cast<const uint4*>(codes) + (int64_t)row * nb + b);
+        sc[r] = scales[scale_at(row, b, kt)];
       }
-      lb += 32;
-      if (lb - lane >= iters * 32) {
-        lb = lane;
-        ln += kFewRows;
-      }
-      ls = ls + 1 == kFewDepth ? 0 : ls + 1;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  #pragma unroll
-  for (int i = 0; i < kFewDepth - 1; ++i) load_step(i);
+  int round = blockIdx.x;
+  int n0 = (round * wide + warp / slices) * kFewRows;
+  if (n0 < N) load(n0, i0);
 
   for (int i = threadIdx.x; i < TOK * 16 * kt; i += kFewThreads) {  // quarter blocks; 16 kt of them to a token
     const int t = i / (16 * kt), q = i - t * 16 * kt, block = q >> 2;
@@ -268,7 +297,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     const uint32_t c = scale_code(mag);
     const float inv = c == 255 ? 0.f : scale_inverse(c);
     #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c == 255 ? 0.f : v[j] * inv;
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * inv;
     const uint32_t word = encode8(v);
     if (block < nb) {
       uint32_t b[2];
@@ -279,70 +308,75 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   }
   __syncthreads();
 
-  int step = 0, slot = 0;
-  for (int n = n0; n < n1; n += kFewRows) {
-    float acc[kFewRows][TOK];
+  for (int turn = 0; round < rounds; round += gridDim.x, turn ^= 1) {
+    float acc[kFewRows * TOK];
     #pragma unroll
-    for (int r = 0; r < kFewRows; ++r)
-      #pragma unroll
-      for (int t = 0; t < TOK; ++t) acc[r][t] = 0.f;
-    for (int i = 0, b = lane; i < iters; ++i, b += 32, ++step) {
-      load_step(step + kFewDepth - 1);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kFewDepth - 1) : "memory");
-      const unsigned char* at = ring + slot * kFewStep;
-      slot = slot + 1 == kFewDepth ? 0 : slot + 1;
-      if (b >= nb) continue;
-      uint4 raw[kFewRows];
-      uint32_t c[kFewRows];
-      #pragma unroll
-      for (int r = 0; r < kFewRows; ++r) {
-        raw[r] = *reinterpret_cast<const uint4*>(at + (r * 32 + lane) * 16);
-        c[r] = at[kFewRows * 512 + (r * 32 + lane) * 4 + (b & 3)];
-      }
-      int all[kFewRows][TOK], neg[kFewRows][TOK];
-      #pragma unroll
-      for (int r = 0; r < kFewRows; ++r)
-        #pragma unroll
-        for (int t = 0; t < TOK; ++t) all[r][t] = neg[r][t] = 0;
-      #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4 xv[TOK];
-        #pragma unroll
-        for (int t = 0; t < TOK; ++t) xv[t] = xb[((size_t)t * 2 + h) * nb + b];
+    for (int j = 0; j < kFewRows * TOK; ++j) acc[j] = 0.f;
+    const int next = ((round + gridDim.x) * wide + warp / slices) * kFewRows;
+    if (n0 < N) {
+      for (int i = i0; i < i1; ++i) {
+        const int b = min(lane + 32 * i, nb - 1);  // beyond the last block the weights are zeros
+        uint4 w[kFewRows];
+        float sw[kFewRows];
         #pragma unroll
         for (int r = 0; r < kFewRows; ++r) {
+          w[r] = raw[r];
+          sw[r] = scale_value(sc[r]);
+        }
+        if (i + 1 < i1) load(n0, i + 1);
+        else if (next < N) load(next, i0);
+        #pragma unroll
+        for (int t = 0; t < TOK; ++t) {
+          const uint4 x0 = xb[((size_t)t * 2) * nb + b], x1 = xb[((size_t)t * 2 + 1) * nb + b];
+          const float s = xs[t * nb + b];
           #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t word = h == 0 ? (k == 0 ? raw[r].x : raw[r].y) : (k == 0 ? raw[r].z : raw[r].w);
-            const uint32_t size = word & 0x77777777u;
-            const uint32_t m0 = __byte_perm(0x03020100u, 0x0c080604u, size), m1 = __byte_perm(0x03020100u, 0x0c080604u, size >> 16);
-            uint32_t s0, s1;  // a code's bit 3 replicates the sign of a 0x80 byte: 0xff where negative, 0x80 elsewhere
-            asm("prmt.b32 %0, %1, %1, %2;" : "=r"(s0) : "r"(0x80808080u), "r"(word));
-            asm("prmt.b32 %0, %1, %1, %2;" : "=r"(s1) : "r"(0x80808080u), "r"(word >> 16));
+          for (int r = 0; r < kFewRows; ++r) {
+            int all = 0, neg = 0;
             #pragma unroll
-            for (int t = 0; t < TOK; ++t) {
-              const int x0 = (int)(k == 0 ? xv[t].x : xv[t].z), x1 = (int)(k == 0 ? xv[t].y : xv[t].w);
-              all[r][t] = __dp4a((int)m1, x1, __dp4a((int)m0, x0, all[r][t]));
-              neg[r][t] = __dp4a((int)(m1 & s1), x1, __dp4a((int)(m0 & s0), x0, neg[r][t]));
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t word = k == 0 ? w[r].x : (k == 1 ? w[r].y : (k == 2 ? w[r].z : w[r].w));
+              const int xa = (int)(k == 0 ? x0.x : (k == 1 ? x0.z : (k == 2 ? x1.x : x1.z)));
+              const int xc = (int)(k == 0 ? x0.y : (k == 1 ? x0.w : (k == 2 ? x1.y : x1.w)));
+              const uint32_t size = word & 0x77777777u;
+              const uint32_t m0 = __byte_perm(0x03020100u, 0x0c080604u, size), m1 = __byte_perm(0x03020100u, 0x0c080604u, size >> 16);
+              uint32_t s0, s1;  // a code's bit 3 replicates the sign of a 0x80 byte: 0xff where negative, 0x80 elsewhere
+              asm("prmt.b32 %0, %1, %1, %2;" : "=r"(s0) : "r"(0x80808080u), "r"(word));
+              asm("prmt.b32 %0, %1, %1, %2;" : "=r"(s1) : "r"(0x80808080u), "r"(word >> 16));
+              all = __dp4a((int)m1, xc, __dp4a((int)m0, xa, all));
+              neg = __dp4a((int)(m1 & s1), xc, __dp4a((int)(m0 & s0), xa, neg));
             }
+            acc[r * TOK + t] = fmaf((float)(all - 2 * neg), sw[r] * s, acc[r * TOK + t]);
           }
         }
       }
-      #pragma unroll
-      for (int r = 0; r < kFewRows; ++r) {
-        const float sw = scale_value(c[r]);
-        #pragma unroll
-        for (int t = 0; t < TOK; ++t) acc[r][t] = fmaf((float)(all[r][t] - 2 * neg[r][t]), sw * xs[t * nb + b], acc[r][t]);
-      }
     }
     #pragma unroll
-    for (int r = 0; r < kFewRows; ++r)
-      #pragma unroll
-      for (int t = 0; t < TOK; ++t) {
-        const float y = warp_sum(acc[r][t]);
-        if (lane == 0 && n + r < n1 && t < tokens)
-          out[(int64_t)t * ldo + n + r] = from_f32<T>(bias ? y + to_f32(bias[n + r]) : y);
+    for (int j = 0; j < kFewRows * TOK; ++j) acc[j] = warp_sum(acc[j]);
+    if (slices == 1) {
+      if (n0 < N && lane == 0) {
+        #pragma unroll
+        for (int j = 0; j < kFewRows * TOK; ++j) {
+          const int n = n0 + j / TOK, t = j % TOK;
+          if (n < N && t < tokens) out[(int64_t)t * ldo + n] = from_f32<T>(bias ? acc[j] + to_f32(bias[n]) : acc[j]);
+        }
       }
+    } else {  // the parts in order; the other buffer takes the next round's, so one barrier is enough
+      if (lane == 0) {
+        #pragma unroll
+        for (int j = 0; j < kFewRows * TOK; ++j) part[turn][warp][j] = acc[j];
+      }
+      __syncthreads();
+      for (int j = threadIdx.x; j < wide * kFewRows * TOK; j += kFewThreads) {
+        const int g = j / (kFewRows * TOK), e = j - g * kFewRows * TOK;
+        const int n = (round * wide + g) * kFewRows + e / TOK, t = e % TOK;
+        if (n < N && t < tokens) {
+          float y = 0.f;
+          for (int k = 0; k < slices; ++k) y += part[turn][g * slices + k][e];
+          out[(int64_t)t * ldo + n] = from_f32<T>(bias ? y + to_f32(bias[n]) : y);
+        }
+      }
+    }
+    n0 = next;
   }
 }
 
@@ -883,10 +917,10 @@ static int num_sms() {
 }
 
 // CTAs of 256 threads: `wide` threads along a row (all of a narrow one), the others on further rows.
-static void shape_of(int wide, int rows, dim3* grid, dim3* block) {
+static void shape_of(int wide, int rows, int rows_each, dim3* grid, dim3* block) {
   const int bx = std::min(wide, 256), by = 256 / bx;
   *block = dim3(bx, by);
-  *grid = dim3((rows + by * kRows - 1) / (by * kRows), (wide + bx - 1) / bx);
+  *grid = dim3((rows + by * rows_each - 1) / (by * rows_each), (wide + bx - 1) / bx);
 }
 
 template <class T>
@@ -894,7 +928,7 @@ static int quantize(const void* x, int64_t ldx, int rows, int cols, uint8_t* cod
   const int nb = (cols + 31) / 32, kt = (nb + 3) / 4;
   const bool vec = aligned16(x) && (ldx * (int64_t)sizeof(T)) % 16 == 0;
   dim3 grid, block;
-  shape_of(16 * kt, (rows + 127) / 128 * 128, &grid, &block);
+  shape_of(8 * kt, (rows + 127) / 128 * 128, kRows, &grid, &block);
   MPQ_CHECK_ARG(grid.y <= 65535, "mpq_mx4_quantize: %d columns are too many", cols);
   k_mx4_quantize<T><<<grid, block, 0, st>>>((const T*)x, ldx, rows, cols, vec, codes, 16 * (int64_t)nb, scales, kt);
   return launch_status("mpq_mx4_quantize");
@@ -906,7 +940,7 @@ static int dequantize(const uint8_t* codes, const uint8_t* scales, int rows, int
   const int nb = (cols + 31) / 32, kt = (nb + 3) / 4;
   const bool vec = aligned16(out) && (ldo * (int64_t)sizeof(T)) % 16 == 0;
   dim3 grid, block;
-  shape_of((cols + 7) / 8, rows, &grid, &block);
+  shape_of((int)((cols * sizeof(T) + 15) / 16), rows, 2 * kRows, &grid, &block);
   MPQ_CHECK_ARG(grid.y <= 65535, "mpq_mx4_dequantize: %d columns are too many", cols);
   k_mx4_dequantize<T><<<grid, block, 0, st>>>(codes, 16 * (int64_t)nb, scales, kt, rows, cols, vec, (T*)out, ldo);
   return launch_status("mpq_mx4_dequantize");
@@ -1031,20 +1065,31 @@ static int gemm(const uint8_t* a_codes, const uint8_t* b_codes, const GemmArgs& 
 template <class T, int TOK>
 static int few_tokens(const void* x, int64_t ldx, int M, int N, int K, const uint8_t* codes, const uint8_t* scales,
                       const void* bias, void* out, int64_t ldo, cudaStream_t st) {
-  const int nb = (K + 31) / 32;
-  const size_t smem = (((size_t)TOK * nb * 36 + 15) & ~(size_t)15) + kFewThreads / 32 * kFewDepth * kFewStep;
+  const int nb = (K + 31) / 32, iters = (nb + 31) / 32, groups = (N + kFewRows - 1) / kFewRows;
+  const size_t smem = (size_t)TOK * nb * 36;
   const int r = smem_opt_in((const void*)k_mx4_few<T, TOK>, smem, "mpq_mx4_linear");
   if (r) return r;
   const bool vec = aligned16(x) && (ldx * (int64_t)sizeof(T)) % 16 == 0;
-  const int grid = std::min((N + 7) / 8, num_sms() * (smem <= 112 * 1024 ? 2 : 1));
+  const int ctas = num_sms() * (smem <= 100 * 1024 ? 2 : 1);
+  // the parts of K with the fewest steps for the busiest warp; a round's sum counts as one
+  int slices = 1, least = 1 << 30;
+  for (int s = 1; s <= kFewWarps && s <= iters; s *= 2) {
+    const int rounds = (groups * s + ctas * kFewWarps - 1) / (ctas * kFewWarps);
+    const int steps = rounds * ((iters + s - 1) / s + 1);
+    if (steps < least) {
+      least = steps;
+      slices = s;
+    }
+  }
+  const int wide = kFewWarps / slices, grid = std::min((groups + wide - 1) / wide, ctas);
   k_mx4_few<T, TOK><<<grid, kFewThreads, smem, st>>>((const T*)x, ldx, M, N, K, vec, codes, scales, (const T*)bias,
-                                                     (T*)out, ldo);
+                                                     (T*)out, ldo, slices);
   return launch_status("mpq_mx4_linear (few tokens)");
 }
 
 constexpr int kFewTokens = 4;
 // x has to fit in shared memory
-static bool takes_few(int M, int K) { return M <= kFewTokens && (M <= 2 ? M : 4) * ((K + 31ll) / 32) * 36 <= 160 * 1024; }
+static bool takes_few(int M, int K) { return M <= kFewTokens && (M <= 2 ? M : 4) * ((K + 31ll) / 32) * 36 <= 200 * 1024; }
 
 template <class T>
 static int linear(const void* x, int dtype, int64_t ldx, int M, int N, int K, const uint8_t* codes, const uint8_t* scales,

@@ -405,55 +405,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (live) p.part[(int64_t)row * (2 * p.nt) + 2 * nb + half] = make_float2(lim > 0 ? m2 : -INFINITY, sum0 + sum1);
       } else {
         if (!take()) break;
-        const uint32_t at = lanes + (uint32_t)((n & 1) * kBN);
+        float x[128];
+        tmem_ld128(lanes + (uint32_t)((n & 1) * kBN), x);
+        release();
         if (EPI == kOut && p.acc) {
           float* acc = p.acc + (int64_t)(u % p.splits) * p.M * p.N;
-          #pragma unroll 1
+          #pragma unroll
           for (int c0 = 0; c0 < 128; c0 += 32) {
-            uint32_t v[32];
-            tmem_ld32(at + c0, v);
             const int lim = p.N - (n0 + c0);
-            if (lim <= 0 || row0 >= p.M) continue;
-            #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(alpha * __uint_as_float(v[i]));
+            if (lim <= 0 || row0 >= p.M) break;
             if (p.tile_out) {
-              chunk_put(buf, lane, v);
+              chunk_begin(lane);
+              #pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float* e = x + c0 + 4 * j;
+                chunk_unit(buf, lane, j, make_uint4(__float_as_uint(alpha * e[0]), __float_as_uint(alpha * e[1]),
+                                                    __float_as_uint(alpha * e[2]), __float_as_uint(alpha * e[3])));
+              }
               chunk_send(buf, lane, &map_o, n0 + c0, row0, u % p.splits);
             } else if (live) {
               #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (i < lim) acc[(int64_t)row * p.N + n0 + c0 + i] = __uint_as_float(v[i]);
+                if (i < lim) acc[(int64_t)row * p.N + n0 + c0 + i] = alpha * x[c0 + i];
             }
           }
         } else {
-          #pragma unroll 1
+          #pragma unroll
           for (int c0 = 0; c0 < 128; c0 += 64) {
             uint32_t w[32];
             #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t v[32];
-              tmem_ld32(at + c0 + 32 * q, v);
-              #pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                float a, b;
-                if constexpr (EPI == kGrad) {
-                  const int c = c0 + 32 * q + i;
-                  a = ex2(fmaf(__uint_as_float(v[i]), kLog2e, -lse2)) - (label == c ? 1.f : 0.f);
-                  b = ex2(fmaf(__uint_as_float(v[i + 1]), kLog2e, -lse2)) - (label == c + 1 ? 1.f : 0.f);
-                  a = g == 0.f ? 0.f : g * a;
-                  b = g == 0.f ? 0.f : g * b;
-                } else {
-                  a = alpha * __uint_as_float(v[i]);
-                  b = alpha * __uint_as_float(v[i + 1]);
-                }
-                w[16 * q + i / 2] = pack16(a, b, p.f16);
+            for (int i = 0; i < 64; i += 2) {
+              float a = x[c0 + i], b = x[c0 + i + 1];
+              if constexpr (EPI == kGrad) {
+                a = ex2(fmaf(a, kLog2e, -lse2)) - (label == c0 + i ? 1.f : 0.f);
+                b = ex2(fmaf(b, kLog2e, -lse2)) - (label == c0 + i + 1 ? 1.f : 0.f);
+                a = g == 0.f ? 0.f : g * a;
+                b = g == 0.f ? 0.f : g * b;
+              } else {
+                a *= alpha;
+                b *= alpha;
               }
+              w[i / 2] = pack16(a, b, p.f16);
             }
             store_half_rows(p, &map_o, buf, lane, row0, n0 + c0, reinterpret_cast<uint16_t*>(p.out), p.ldo, w,
                             p.N - (n0 + c0));
           }
         }
-        release();
       }
     }
     chunk_drain(lane);

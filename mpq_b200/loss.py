@@ -49,7 +49,8 @@ def _keep(tokens: int, vocab: int, keep_bytes: int) -> int:
 
 
 def _forward(hidden, weight, labels, ignore_index, reduction, keep_bytes):
-    """(result, count, lse, part, tgt, keep, keep_cols) of a checked call."""
+    """(result, work, keep, keep_cols) of a checked call.  ``work`` holds, as floats: lse (T), the count of labels, the
+    labels' logits (T), the scores (T, unless they are the result) and, from 8 bytes on, the tiles' partial sums."""
     t, h = hidden.shape
     v = weight.shape[0]
     dev = hidden.device
@@ -57,32 +58,36 @@ def _forward(hidden, weight, labels, ignore_index, reduction, keep_bytes):
     tiles = load().mpq_xent_tiles(v)
     each = reduction == "none"
     out = torch.empty((t,) if each else (), device=dev, dtype=torch.float32)
-    small = torch.empty(2 * t + 1, device=dev, dtype=torch.float32)        # lse, count, nll
-    part = torch.empty(2 * t * tiles + t, device=dev, dtype=torch.float32)  # the tiles' partial sums, the labels' logits
-    at, at_part = small.data_ptr(), part.data_ptr()
+    work = torch.empty(_part_at(t) + 2 * t * tiles, device=dev, dtype=torch.float32)
+    at, at_out = work.data_ptr(), out.data_ptr()
     keep_cols = _keep(t, v, keep_bytes) if keep_bytes and t else 0
-    keep = torch.empty(t, (keep_cols + 7) // 8 * 8, device=dev, dtype=hidden.dtype) if keep_cols else None
-    call_on(dev.index, "mpq_xent_forward", t, v, h, _DTYPES[hidden.dtype], ptr(x), x.stride(0), ptr(w), w.stride(0),
-            ptr(labels), ignore_index, at_part, 2 * t * tiles, at_part + 8 * t * tiles, at,
-            out.data_ptr() if each else at + 4 * t + 4, _REDUCTIONS.index(reduction), out.data_ptr(), at + 4 * t, ptr(keep),
-            keep.shape[1] if keep_cols else 0, keep_cols, ptr(ops.status_word(dev)))
-    return out, small[t:t + 1], small[:t], part, part[2 * t * tiles:], keep, keep_cols
+    ldk = (keep_cols + 7) // 8 * 8
+    keep = torch.empty(t, ldk, device=dev, dtype=hidden.dtype) if keep_cols else None
+    call_on(dev.index, "mpq_xent_forward", t, v, h, _DTYPES[hidden.dtype], x.data_ptr(), x.stride(0), w.data_ptr(),
+            w.stride(0), labels.data_ptr(), ignore_index, at + 4 * _part_at(t), 2 * t * tiles, at + 4 * (t + 1), at,
+            at_out if each else at + 4 * (2 * t + 1), _REDUCTIONS.index(reduction), at_out, at + 4 * t, ptr(keep), ldk,
+            keep_cols, ops.status_word(dev).data_ptr())
+    return out, work, keep, keep_cols
+
+
+def _part_at(t: int) -> int:
+    return (3 * t + 2) // 2 * 2
 
 
 class _VocabCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, labels, ignore_index, reduction, piece, keep_bytes):
-        out, count, lse, part, tgt, keep, keep_cols = _forward(hidden, weight, labels, ignore_index, reduction, keep_bytes)
-        ctx.save_for_backward(hidden, weight, labels, lse, count if reduction == "mean" else None)
-        ctx.ignore_index, ctx.piece = ignore_index, piece
-        ctx.kept = (keep, keep_cols, part, tgt) if keep_cols else None
+        out, work, keep, keep_cols = _forward(hidden, weight, labels, ignore_index, reduction, keep_bytes)
+        ctx.save_for_backward(hidden, weight, labels)
+        ctx.ignore_index, ctx.piece, ctx.mean = ignore_index, piece, reduction == "mean"
+        ctx.work, ctx.kept = work, (keep, keep_cols)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        hidden, weight, labels, lse, count = ctx.saved_tensors
+        hidden, weight, labels = ctx.saved_tensors
         t, h = hidden.shape
         v = weight.shape[0]
         dev = hidden.device
@@ -94,17 +99,20 @@ class _VocabCrossEntropy(torch.autograd.Function):
         x, w = _operand(hidden), _operand(weight)
         gout = gout.to(torch.float32).contiguous()
         # the kept columns turn into their gradient in place: a second pass through the graph computes them again
-        (keep, keep_cols, part, tgt), ctx.kept = ctx.kept or (None, 0, None, None), None
+        (keep, keep_cols), ctx.kept = ctx.kept, (None, 0)
         piece = _piece(t, v - keep_cols, ctx.piece)
-        d = torch.empty(t, piece, device=dev, dtype=hidden.dtype) if keep_cols < v else None
         each = gout.dim() > 0  # one upstream gradient a token: d is scaled by the largest
-        gmax = torch.empty(1, device=dev, dtype=torch.float32) if each else None
         planes = load().mpq_xent_planes(t, v, h, piece, keep_cols) if need_h else 0
-        acc = torch.empty(planes, t, h, device=dev, dtype=torch.float32) if planes else None
-        call_on(dev.index, "mpq_xent_backward", t, v, h, _DTYPES[hidden.dtype], ptr(x), x.stride(0), ptr(w), w.stride(0),
-                ptr(labels), ctx.ignore_index, ptr(lse), ptr(gout), int(each), ptr(count), ptr(part), ptr(tgt), ptr(keep),
-                keep.shape[1] if keep_cols else 0, keep_cols, ptr(gmax), ptr(d), piece, ptr(acc), ptr(dh), h, ptr(dw), h,
-                ptr(ops.status_word(dev)))
+        # FP32 sums of dhidden, and the scale
+        acc = torch.empty(planes * t * h + 1, device=dev, dtype=torch.float32) if planes or each else None
+        d = torch.empty(t, piece, device=dev, dtype=hidden.dtype) if keep_cols < v else None
+        at = ctx.work.data_ptr()
+        at_acc = 0 if acc is None else acc.data_ptr()
+        call_on(dev.index, "mpq_xent_backward", t, v, h, _DTYPES[hidden.dtype], x.data_ptr(), x.stride(0), w.data_ptr(),
+                w.stride(0), labels.data_ptr(), ctx.ignore_index, at, gout.data_ptr(), int(each),
+                at + 4 * t if ctx.mean else None, at + 4 * _part_at(t), at + 4 * (t + 1), ptr(keep),
+                0 if keep is None else keep.shape[1], keep_cols, at_acc + 4 * planes * t * h if each else None, ptr(d), piece,
+                at_acc if planes else None, ptr(dh), h, ptr(dw), h, ops.status_word(dev).data_ptr())
         return dh, dw, None, None, None, None, None
 
 
