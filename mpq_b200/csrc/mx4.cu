@@ -221,31 +221,33 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restric
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Product for one to four tokens: y[t, n] = sum_k Q(x)[t, k] W[n, k] (+ bias[n]), x quantised in the same launch
+// Product for one or two tokens: y[t, n] = sum_k Q(x)[t, k] W[n, k] (+ bias[n]), x quantised in the same launch
 // ------------------------------------------------------------------------------------------------------------------
 //
-// W is read once (17 bytes for 32 weights), which bounds it.  Twice an E2M1 value is a small integer, so a block's 32
-// products are summed exactly in integers by dp4a and only then scaled: y += 2^(cx + cw - 256) sum (2 q_x) (2 q_w).
-// Every CTA quantises x for itself into shared memory (bytes 2 q_x, two planes of 16 bytes a block so that a warp's
+// W is read once (17 bytes for 32 weights), and the arithmetic has to keep up with that: a block of a row takes 16
+// conversions of two codes to an f16 pair and 16 f16 products a token.  The products are exact: they are multiples of
+// 1/4 up to 36, and the eight that a half of an accumulator adds stay below 2^11 quarters; a block's four sums are
+// added in FP32 and scaled by 2^(cx + cw - 254) once.  (Decoded by byte permutations for dp4a a block took twice the
+// instructions: 14.1 us at 1 x 14336 x 4096.)
+// Every CTA quantises x for itself into shared memory (f16 values in four planes of 16 bytes a block, so that a warp's
 // reads are free of conflicts) while its first weights are on their way.  A warp takes kFewRows rows of W and one of
 // `slices` parts of K (so that all warps have work whatever N is), a lane every 32nd block; the next blocks are loaded
-// before the last are used.  A weight's magnitude comes from a byte permutation of the eight magnitudes; its sign is
-// left to a second dp4a over the negative ones: sum = all - 2 negative.
+// before the last are used.  (A deeper ring in shared memory was slower, 15.0 us against 13.0: the arithmetic bounds it,
+// which is why larger products go to the tensor cores even for one token.)
 
 constexpr int kFewRows = 4, kFewThreads = 256, kFewWarps = kFewThreads / 32;
 
-// Codes -> bytes 2 q (signed), eight to two words
-__device__ __forceinline__ void bytes_of(uint32_t w, uint32_t (&b)[2]) {
+// Sums of four values over a warp: lane l gets the total of value l & 3.
+__device__ __forceinline__ float warp_sum4(const float (&v)[4], int lane) {
+  const bool odd = lane & 1, high = lane & 2;
+  float a = odd ? v[1] : v[0], b = odd ? v[3] : v[2];
+  a += __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[1], 1);
+  b += __shfl_xor_sync(0xffffffffu, odd ? v[2] : v[3], 1);
+  float c = high ? b : a;
+  c += __shfl_xor_sync(0xffffffffu, high ? a : b, 2);
   #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint32_t r = 0;
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t c = w >> (16 * i + 4 * j), m = __byte_perm(0x03020100u, 0x0c080604u, c & 7u) & 0xffu;
-      r |= ((c & 8u ? 0u - m : m) & 0xffu) << (8 * j);
-    }
-    b[i] = r;
-  }
+  for (int o = 4; o < 32; o <<= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+  return c;
 }
 
 template <class T, int TOK>
@@ -255,8 +257,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   extern __shared__ __align__(16) unsigned char sm[];
   __shared__ float part[2][kFewWarps][kFewRows * TOK];
   const int nb = (K + 31) >> 5, kt = (nb + 3) >> 2;
-  uint4* xb = reinterpret_cast<uint4*>(sm);                        // [TOK][2][nb]
-  float* xs = reinterpret_cast<float*>(xb + (size_t)TOK * 2 * nb);  // [TOK][nb], a quarter of the scale
+  uint4* xb = reinterpret_cast<uint4*>(sm);                        // [TOK][4][nb]
+  float* xs = reinterpret_cast<float*>(xb + (size_t)TOK * 4 * nb);  // [TOK][nb]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slice = warp % slices, wide = kFewWarps / slices;  // a CTA takes `wide` groups of rows at a time
   const int iters = (nb + 31) >> 5, i0 = iters * slice / slices, i1 = iters * (slice + 1) / slices;
@@ -264,16 +266,20 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 
   uint4 raw[kFewRows];
   uint32_t sc[kFewRows];
-  auto load = [&](int n0, int i) {
+  auto load = [&](int n0, int i) {  // n0 is a multiple of 4: a group's rows are neighbours in their scale tile
     const int b = lane + 32 * i;
     #pragma unroll
     for (int r = 0; r < kFewRows; ++r) {
-      const int row = min(n0 + r, N - 1);
       raw[r] = make_uint4(0, 0, 0, 0);
       sc[r] = 0;
-      if (b < nb) {
-        raw[r] = __ldcs(reinterpret_cast<const uint4*>(codes) + (int64_t)row * nb + b);
-        sc[r] = scales[scale_at(row, b, kt)];
+    }
+    if (b < nb) {
+      const uint4* at = reinterpret_cast<const uint4*>(codes) + (int64_t)n0 * nb + b;
+      const uint8_t* s = scales + scale_at(n0, b, kt);
+      #pragma unroll
+      for (int r = 0; r < kFewRows; ++r) {
+        raw[r] = __ldcs(at + min(r, N - 1 - n0) * nb);
+        sc[r] = s[r * 16];
       }
     }
   };
@@ -298,22 +304,24 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     const float inv = c == 255 ? 0.f : scale_inverse(c);
     #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = v[j] * inv;
-    const uint32_t word = encode8(v);
+    __half2 h[4];
+    decode8(encode8(v), h);
     if (block < nb) {
-      uint32_t b[2];
-      bytes_of(word, b);
-      reinterpret_cast<uint2*>(xb + ((size_t)t * 2 + ((q >> 1) & 1)) * nb + block)[q & 1] = make_uint2(b[0], b[1]);
-      if ((q & 3) == 0) xs[t * nb + block] = 0.25f * scale_value(c);
+      xb[((size_t)t * 4 + (q & 3)) * nb + block] = *reinterpret_cast<const uint4*>(h);
+      if ((q & 3) == 0) xs[t * nb + block] = scale_value(c);
     }
   }
   __syncthreads();
 
   for (int turn = 0; round < rounds; round += gridDim.x, turn ^= 1) {
-    float acc[kFewRows * TOK];
+    float acc[TOK][kFewRows];
     #pragma unroll
-    for (int j = 0; j < kFewRows * TOK; ++j) acc[j] = 0.f;
+    for (int t = 0; t < TOK; ++t)
+      #pragma unroll
+      for (int r = 0; r < kFewRows; ++r) acc[t][r] = 0.f;
     const int next = ((round + gridDim.x) * wide + warp / slices) * kFewRows;
     if (n0 < N) {
+      #pragma unroll 1
       for (int i = i0; i < i1; ++i) {
         const int b = min(lane + 32 * i, nb - 1);  // beyond the last block the weights are zeros
         uint4 w[kFewRows];
@@ -325,50 +333,51 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         }
         if (i + 1 < i1) load(n0, i + 1);
         else if (next < N) load(next, i0);
+        __half2 lo[TOK][kFewRows], hi[TOK][kFewRows];  // sums of the block's first and last 16 products
+        #pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          __half2 xv[TOK][4];
+          #pragma unroll
+          for (int t = 0; t < TOK; ++t) *reinterpret_cast<uint4*>(xv[t]) = xb[((size_t)t * 4 + q) * nb + b];
+          #pragma unroll
+          for (int r = 0; r < kFewRows; ++r) {
+            __half2 h[4];
+            decode8(q == 0 ? w[r].x : (q == 1 ? w[r].y : (q == 2 ? w[r].z : w[r].w)), h);
+            #pragma unroll
+            for (int t = 0; t < TOK; ++t) {
+              __half2& sum = q < 2 ? lo[t][r] : hi[t][r];
+              sum = (q & 1) ? __hfma2(h[0], xv[t][0], sum) : __hmul2(h[0], xv[t][0]);
+              #pragma unroll
+              for (int j = 1; j < 4; ++j) sum = __hfma2(h[j], xv[t][j], sum);
+            }
+          }
+        }
         #pragma unroll
         for (int t = 0; t < TOK; ++t) {
-          const uint4 x0 = xb[((size_t)t * 2) * nb + b], x1 = xb[((size_t)t * 2 + 1) * nb + b];
           const float s = xs[t * nb + b];
           #pragma unroll
           for (int r = 0; r < kFewRows; ++r) {
-            int all = 0, neg = 0;
-            #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t word = k == 0 ? w[r].x : (k == 1 ? w[r].y : (k == 2 ? w[r].z : w[r].w));
-              const int xa = (int)(k == 0 ? x0.x : (k == 1 ? x0.z : (k == 2 ? x1.x : x1.z)));
-              const int xc = (int)(k == 0 ? x0.y : (k == 1 ? x0.w : (k == 2 ? x1.y : x1.w)));
-              const uint32_t size = word & 0x77777777u;
-              const uint32_t m0 = __byte_perm(0x03020100u, 0x0c080604u, size), m1 = __byte_perm(0x03020100u, 0x0c080604u, size >> 16);
-              uint32_t s0, s1;  // a code's bit 3 replicates the sign of a 0x80 byte: 0xff where negative, 0x80 elsewhere
-              asm("prmt.b32 %0, %1, %1, %2;" : "=r"(s0) : "r"(0x80808080u), "r"(word));
-              asm("prmt.b32 %0, %1, %1, %2;" : "=r"(s1) : "r"(0x80808080u), "r"(word >> 16));
-              all = __dp4a((int)m1, xc, __dp4a((int)m0, xa, all));
-              neg = __dp4a((int)(m1 & s1), xc, __dp4a((int)(m0 & s0), xa, neg));
-            }
-            acc[r * TOK + t] = fmaf((float)(all - 2 * neg), sw[r] * s, acc[r * TOK + t]);
+            const float2 f = __half22float2(lo[t][r]), g = __half22float2(hi[t][r]);
+            acc[t][r] = fmaf((f.x + f.y) + (g.x + g.y), sw[r] * s, acc[t][r]);
           }
         }
       }
     }
     #pragma unroll
-    for (int j = 0; j < kFewRows * TOK; ++j) acc[j] = warp_sum(acc[j]);
-    if (slices == 1) {
-      if (n0 < N && lane == 0) {
-        #pragma unroll
-        for (int j = 0; j < kFewRows * TOK; ++j) {
-          const int n = n0 + j / TOK, t = j % TOK;
-          if (n < N && t < tokens) out[(int64_t)t * ldo + n] = from_f32<T>(bias ? acc[j] + to_f32(bias[n]) : acc[j]);
-        }
+    for (int t = 0; t < TOK; ++t) {
+      const float y = warp_sum4(acc[t], lane);  // lane r: row r
+      if (slices > 1) {
+        if (lane < kFewRows) part[turn][warp][t * kFewRows + lane] = y;
+      } else if (lane < kFewRows && n0 + lane < N && t < tokens) {
+        const int n = n0 + lane;
+        out[(int64_t)t * ldo + n] = from_f32<T>(bias ? y + to_f32(bias[n]) : y);
       }
-    } else {  // the parts in order; the other buffer takes the next round's, so one barrier is enough
-      if (lane == 0) {
-        #pragma unroll
-        for (int j = 0; j < kFewRows * TOK; ++j) part[turn][warp][j] = acc[j];
-      }
+    }
+    if (slices > 1) {  // the parts in order; the other buffer takes the next round's, so one barrier is enough
       __syncthreads();
       for (int j = threadIdx.x; j < wide * kFewRows * TOK; j += kFewThreads) {
         const int g = j / (kFewRows * TOK), e = j - g * kFewRows * TOK;
-        const int n = (round * wide + g) * kFewRows + e / TOK, t = e % TOK;
+        const int n = (round * wide + g) * kFewRows + e % kFewRows, t = e / kFewRows;
         if (n < N && t < tokens) {
           float y = 0.f;
           for (int k = 0; k < slices; ++k) y += part[turn][g * slices + k][e];
@@ -392,12 +401,14 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 // of K = 64; warps 2..5 read the FP32 accumulator, add the bias, round once and store.  Two accumulators let the
 // epilogue overlap the next tile.  Scale columns in TMEM belong to the stage, so they are not rewritten before the
 // MMAs that read them are done.  With at most 128 rows of A only those are loaded (a tile load takes two to three cycles a
-// 128-byte row; what the others' shared memory holds stays in their rows of the accumulator), and a cluster of up to
-// four CTAs may share a tile, each with a part of K: the others leave their FP32 parts in shared memory and the first
-// adds them in order.
+// 128-byte row; what the others' shared memory holds stays in their rows of the accumulator), the ring takes the
+// more stages for it, and a cluster of up to
+// four CTAs may share a tile, each with a part of K: they leave their FP32 sums in shared memory, and each adds the parts
+// of its share of the columns, in order.
 
 constexpr int kThreads = 192;
-constexpr int kBM = 128, kStages = 6;
+constexpr int kBM = 128, kMostStages = 16;
+constexpr uint32_t kTileRing = 204 * 1024;
 constexpr uint32_t kOperand = 128 * 128, kScale = 1024;
 constexpr uint32_t kScaleCols = 256, kStageCols = 16;   // TMEM: accumulators [0, 256), 16 scale columns a stage above
 
@@ -445,12 +456,13 @@ struct GemmArgs {
   int64_t ldo;
   int M, N, kt, mt, nt;  // kt: scale tiles along K; mt x nt output tiles
   int a_rows;            // k_mx4_tile: rows of A that a tile loads
+  int stages;            // k_mx4_tile: of the ring
   int tile_out;          // the result's rows are aligned for tile stores
   int* status;
 };
 
 // kCols<T> columns of the accumulator are 128 bytes of a row.  Columns col.. of a warp's 32 rows from row0 on (`lane`: the
-// thread's row): bias, one rounding, and off as a tile, or by the thread where the result's rows are not aligned.
+// thread's row): bias, one rounding, and off as a tile, or row by row where the result's rows are not aligned.
 template <class T>
 constexpr int kCols = 128 / sizeof(T);
 
@@ -467,18 +479,15 @@ __device__ __forceinline__ void store_rows(const GemmArgs& p, const CUtensorMap*
     if (bias && i < lim) f += to_f32(bias[col + i]);
     o[i] = from_f32<T>(f);
   }
-  if (p.tile_out) {
-    uint32_t w[32];
-    #pragma unroll
-    for (int i = 0; i < 32; ++i) w[i] = reinterpret_cast<const uint32_t*>(o)[i];
-    chunk_put(buf, lane, w);
+  uint32_t w[32];
+  #pragma unroll
+  for (int i = 0; i < 32; ++i) w[i] = reinterpret_cast<const uint32_t*>(o)[i];
+  chunk_put(buf, lane, w);
+  if (p.tile_out)
     chunk_send(buf, lane, map, col, row0, 0);
-  } else if (row0 + lane < p.M) {
-    T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(row0 + lane) * p.ldo + col;
-    #pragma unroll
-    for (int i = 0; i < kCols<T>; ++i)
-      if (i < lim) dst[i] = o[i];
-  }
+  else
+    chunk_rows<sizeof(T)>(buf, lane, reinterpret_cast<T*>(p.out) + (int64_t)row0 * p.ldo + col, p.ldo * sizeof(T),
+                          p.M - row0, lim);
 }
 
 // kCols<T> columns of TMEM
@@ -501,18 +510,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr uint32_t kOperandB = BN * 128;
-  constexpr uint32_t kStage = kOperand + kOperandB + 2 * kScale;
-  unsigned char* out_buf = ring + kStages * kStage;  // 4 KB to an epilogue warp
+  const uint32_t stage = kOperandB + p.a_rows * 128;
+  // ring: B then A of each stage (1024-byte aligned), then the scales of all stages (A's, B's)
+  unsigned char* out_buf = ring + kTileRing;  // 4 KB to an epilogue warp
   uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + 4 * 4096);
-  uint64_t* empty = full + kStages;
-  uint64_t* acc_full = empty + kStages;
+  uint64_t* empty = full + kMostStages;
+  uint64_t* acc_full = empty + kMostStages;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  // a stage: A codes, B codes (1024-byte aligned), then the scales of all stages behind the operands of all stages
-  auto s_a = [&](int s) { return ring + s * (kOperand + kOperandB); };
-  auto s_b = [&](int s) { return s_a(s) + kOperand; };
-  auto s_sf = [&](int s) { return ring + kStages * (kOperand + kOperandB) + s * 2 * kScale; };
+  auto s_b = [&](int s) { return ring + s * stage; };
+  auto s_a = [&](int s) { return ring + s * stage + kOperandB; };
+  auto s_sf = [&](int s) { return ring + p.stages * stage + s * 2 * kScale; };
   float* part_sum = reinterpret_cast<float*>(ring);  // [BN][128] at the end of a part of K
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -521,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int nkb = (p.kt + 1) / 2, kb0 = nkb * rank / parts, kb1 = nkb * (rank + 1) / parts;
   const int tiles = p.mt * p.nt, first_tile = blockIdx.x / parts, stride = gridDim.x / parts;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -544,30 +553,39 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      const uint32_t bytes = p.a_rows * 128 + kOperandB + 2 * kScale;
+      const uint32_t bytes = stage + 2 * kScale;
       int64_t it = 0;
-      Ring r(kStages);
+      Ring r(p.stages);
       bool ok = true;
+      // The first tile's first weights, which no kernel before has made; A may come from one, so its loads wait for
+      // that kernel's end.
+      const int ahead = first_tile < tiles ? min(p.stages, kb1 - kb0) : 0, nb0 = first_tile / p.mt;
+      for (int i = 0; i < ahead; ++i) {
+        mbar_expect_tx(&full[i], bytes);
+        tma_load_2d(s_b(i), &map_b, &full[i], (kb0 + i) * 128, nb0 * BN);
+        tma_load_2d(s_sf(i) + kScale, &map_sfb, &full[i], (kb0 + i) * 256, nb0 * BN >> 7);
+      }
+      asm volatile("griddepcontrol.wait;" ::: "memory");
       for (int t = first_tile; t < tiles && ok; t += stride) {
         const int mb = t % p.mt, nb = t / p.mt;
         for (int kb = kb0; kb < kb1; ++kb, ++it, r.next()) {
-          if (!mbar_wait_fast(&empty[r.s], r.ph ^ 1u) || *abort_flag) {
-            ok = false;
-            break;
-          }
           uint64_t* bar = &full[r.s];
-          mbar_expect_tx(bar, bytes);
-          tma_load_2d(s_b(r.s), &map_b, bar, kb * 128, nb * BN);
-          tma_load_2d(s_sf(r.s) + kScale, &map_sfb, bar, kb * 256, nb * BN >> 7);
-          // A may come from the kernel before: wait for its end once the first weights are on their way
-          if (it == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+          if (it >= ahead) {
+            if (!mbar_wait_fast(&empty[r.s], r.ph ^ 1u) || *abort_flag) {
+              ok = false;
+              break;
+            }
+            mbar_expect_tx(bar, bytes);
+            tma_load_2d(s_b(r.s), &map_b, bar, kb * 128, nb * BN);
+            tma_load_2d(s_sf(r.s) + kScale, &map_sfb, bar, kb * 256, nb * BN >> 7);
+          }
           tma_load_2d(s_a(r.s), &map_a, bar, kb * 128, mb * kBM);
           tma_load_2d(s_sf(r.s), &map_sfa, bar, kb * 256, mb);
         }
       }
       if (!ok) {  // drain the copies in flight (each wait bounded) before the CTA may end
         *abort_flag = 1;
-        for (int i = 0; i < kStages && i < it; ++i) {
+        for (int i = 0; i < p.stages && i < it; ++i) {
           r.back();
           mbar_wait_fast(&full[r.s], r.ph);
         }
@@ -579,8 +597,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t da0 = smem_desc_k_sw128(smem_u32(s_a(0))), db0 = smem_desc_k_sw128(smem_u32(s_b(0)));
     const uint64_t ds0 = scale_desc(smem_u32(s_sf(0)));
     const uint32_t i0 = idesc_mxf4(kBM, BN, 0), i2 = idesc_mxf4(kBM, BN, 2);
-    Ring r(kStages);
-    bool ok = true;
+    Ring r(p.stages), c(p.stages);
+    // Scales of the next step, put in line behind the MMAs in flight: copied right before their own MMAs they would
+    // hold those up (57 cycles a copy).
+    auto copy = [&]() {
+      if (!warp_agrees(mbar_wait_fast(&full[c.s], c.ph) && !*abort_flag)) return false;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t sf = tmem + kScaleCols + c.s * kStageCols;
+      const uint64_t ds = desc_add(ds0, c.s * 2 * kScale);
+      if (lead) {
+        #pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          copy_scales<1>(sf + j * 4, desc_add(ds, j * 512));
+          copy_scales<1>(sf + 8 + j * 4, desc_add(ds, kScale + j * 512));
+        }
+      }
+      __syncwarp();
+      c.next();
+      return true;
+    };
+    int64_t left = (int64_t)((tiles - first_tile + stride - 1) / stride) * (kb1 - kb0);  // steps
+    bool ok = first_tile >= tiles || copy();
     int n = 0;
     for (int t = first_tile; t < tiles && ok; t += stride, ++n) {
       const uint32_t acc = tmem + (n & 1) * BN;
@@ -588,26 +625,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = false;
         break;
       }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t part = (uint32_t)((t / p.mt) * BN & 127) >> 5;  // the tile's column in its scale tile
       for (int kb = kb0; kb < kb1; ++kb, r.next()) {
-        if (!warp_agrees(mbar_wait_fast(&full[r.s], r.ph) && !*abort_flag)) {
+        const uint32_t sf = tmem + kScaleCols + r.s * kStageCols;
+        const uint64_t da = desc_add(da0, r.s * stage), db = desc_add(db0, r.s * stage);
+        const uint32_t add = kb > kb0;
+        if (lead) {  // scales beyond the matrix are zeros, as are its codes
+          #pragma unroll
+          for (int j = 0; j < 2; ++j)
+            mma_mxf4<1>(acc, desc_add(da, j * 32), desc_add(db, j * 32), j ? i2 : i0, sf, sf + 8 + part, j ? 1u : add);
+        }
+        __syncwarp();
+        if (--left > 0 && !copy()) {
           ok = false;
           break;
         }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t sf = tmem + kScaleCols + r.s * kStageCols;
-        const uint64_t ds = desc_add(ds0, r.s * 2 * kScale);
-        const uint64_t da = desc_add(da0, r.s * (kOperand + kOperandB)), db = desc_add(db0, r.s * (kOperand + kOperandB));
-        if (lead) {  // scales beyond the matrix are zeros, as are its codes
+        if (lead) {
           #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            copy_scales<1>(sf + j * 4, desc_add(ds, j * 512));
-            copy_scales<1>(sf + 8 + j * 4, desc_add(ds, kScale + j * 512));
-          }
-          #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_mxf4<1>(acc, desc_add(da, j * 32), desc_add(db, j * 32), j & 1 ? i2 : i0, sf + (j >> 1) * 4,
-                        sf + 8 + (j >> 1) * 4 + part, j > 0 || kb > kb0);
+          for (int j = 2; j < 4; ++j)
+            mma_mxf4<1>(acc, desc_add(da, j * 32), desc_add(db, j * 32), j & 1 ? i2 : i0, sf + 4, sf + 12 + part, 1u);
           asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                            smem_u32(&empty[r.s]))
                        : "memory");
@@ -637,15 +674,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (parts > 1 && rank == 0) break;  // finishes below
       const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * BN);
       #pragma unroll 1
       for (int c0 = 0; c0 < BN; c0 += kCols<T>) {
         uint32_t v[kCols<T>];
         tmem_cols(at + c0, v);
         if (parts > 1) {  // every load of the ring has been consumed: it holds this part, column by column
-          #pragma unroll
-          for (int i = 0; i < kCols<T>; ++i) part_sum[(c0 + i) * kBM + quad * 32 + lane] = __uint_as_float(v[i]);
+          if (quad * 32 < p.M) {
+            #pragma unroll
+            for (int i = 0; i < kCols<T>; ++i) part_sum[(c0 + i) * kBM + quad * 32 + lane] = __uint_as_float(v[i]);
+          }
         } else {
           store_rows<T>(p, &map_o, out_buf + quad * 4096, lane, mb * kBM + quad * 32, nb * BN + c0, v);
         }
@@ -659,13 +697,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   if (parts > 1) {
     cluster_sync();  // the parts are complete
-    if (rank == 0 && warp >= 2 && !*abort_flag) {
-      const int quad = warp & 3, row = quad * 32 + lane;  // one row tile
+    const int quad = warp & 3, row = quad * 32 + lane;  // one row tile
+    if (warp >= 2 && quad * 32 < p.M && !*abort_flag) {
+      // each CTA adds the parts of its share of the columns, in order
       #pragma unroll 1
-      for (int c0 = 0; c0 < BN; c0 += kCols<T>) {
+      for (int c0 = rank * kCols<T>; c0 < BN; c0 += parts * kCols<T>) {
         uint32_t v[kCols<T>];
-        tmem_cols(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c0, v);
-        for (int r = 1; r < parts; ++r) {
+        #pragma unroll
+        for (int i = 0; i < kCols<T>; ++i) v[i] = 0;
+        for (int r = 0; r < parts; ++r) {
           const uint32_t at = mapa(smem_u32(part_sum + c0 * kBM + row), r);
           #pragma unroll
           for (int i = 0; i < kCols<T>; ++i) {
@@ -677,7 +717,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         store_rows<T>(p, &map_o, out_buf + quad * 4096, lane, quad * 32, first_tile * BN + c0, v);
       }
       chunk_drain(lane);
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     }
     __syncwarp();
     cluster_sync();  // the parts have been read
@@ -791,54 +830,56 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const bool lead = elect_one();
       const uint64_t da0 = smem_desc_k_sw128(smem_u32(s_a(0))), ds0 = scale_desc(smem_u32(s_sf(0)));
       const uint32_t i0 = idesc_mxf4(kPM, kPHalf, 0), i2 = idesc_mxf4(kPM, kPHalf, 2);
-      Ring r(kPairStages);
-      bool ok = true;
+      Ring r(kPairStages), c(kPairStages);
+      auto copy = [&]() {  // the next step's scales, as in k_mx4_tile
+        if (!warp_agrees(mbar_wait_cluster(&full[c.s], c.ph) && !*abort_flag)) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t sf = tmem + kPN + c.s * kPairCols;  // A's 2 x 4 columns, then B's 2 x 12
+        const uint64_t ds = desc_add(ds0, c.s * kPairSf);
+        if (lead) {
+          #pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            copy_scales<2>(sf + j * 4, desc_add(ds, j * 512));
+            #pragma unroll
+            for (int i = 0; i < 3; ++i)
+              copy_scales<2>(sf + 8 + j * 12 + i * 4, desc_add(ds, kScale * (1 + i) + j * 512));
+          }
+        }
+        __syncwarp();
+        c.next();
+        return true;
+      };
+      int64_t left = (int64_t)((tiles - pair + pairs - 1) / pairs) * nkb;  // steps
+      bool ok = pair >= tiles || copy();
       uint32_t n = 0;  // tiles
       for (int t = pair; t < tiles && ok; t += pairs, ++n) {
-        for (int kb = 0; kb < nkb; ++kb, r.next()) {
-          if (!warp_agrees(mbar_wait_cluster(&full[r.s], r.ph) && !*abort_flag)) {
-            ok = false;
-            break;
-          }
-          if (kb == 0 && !warp_agrees(mbar_wait_cluster(&acc_empty[0], (n & 1u) ^ 1u))) {
-            ok = false;
-            break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t sf = tmem + kPN + r.s * kPairCols;  // A's 2 x 4 columns, then B's 2 x 12
-          const uint64_t ds = desc_add(ds0, r.s * kPairSf), da = desc_add(da0, r.s * kPairOps), db = desc_add(da, kOperand);
+        for (int kb = 0; kb < nkb && ok; ++kb, r.next()) {
+          const uint32_t sf = tmem + kPN + r.s * kPairCols;
+          const uint64_t da = desc_add(da0, r.s * kPairOps), db = desc_add(da, kOperand);
           const uint32_t add = kb > 0;
-          if (lead) {  // scales beyond the matrix are zeros, as are its codes
-            #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              copy_scales<2>(sf + j * 4, desc_add(ds, j * 512));
-              #pragma unroll
-              for (int i = 0; i < 3; ++i)
-                copy_scales<2>(sf + 8 + j * 12 + i * 4, desc_add(ds, kScale * (1 + i) + j * 512));
+          #pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (kb == 0) {
+              if (!warp_agrees(mbar_wait_cluster(&acc_empty[h], (n & 1u) ^ 1u))) {
+                ok = false;
+                break;
+              }
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
-            #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              mma_mxf4<2>(tmem, desc_add(da, j * 32), desc_add(db, j * 32), j & 1 ? i2 : i0, sf + (j >> 1) * 4,
-                          sf + 8 + (j >> 1) * 12, j > 0 ? 1u : add);
-            if (kb == nkb - 1) commit_pair(&acc_full[0]);
-          }
-          __syncwarp();
-          if (kb == 0) {
-            if (!warp_agrees(mbar_wait_cluster(&acc_empty[1], (n & 1u) ^ 1u))) {
+            if (lead) {  // scales beyond the matrix are zeros, as are its codes
+              #pragma unroll
+              for (int j = 0; j < 4; ++j)
+                mma_mxf4<2>(tmem + h * kPHalf, desc_add(da, j * 32), desc_add(db, h * kPairB + j * 32), j & 1 ? i2 : i0,
+                            sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 12 + h * 6, j > 0 ? 1u : add);
+              if (h) commit_pair(&empty[r.s]);
+              if (kb == nkb - 1) commit_pair(&acc_full[h]);
+            }
+            __syncwarp();
+            if (h == 0 && --left > 0 && !copy()) {
               ok = false;
               break;
             }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           }
-          if (lead) {
-            #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              mma_mxf4<2>(tmem + kPHalf, desc_add(da, j * 32), desc_add(db, kPairB + j * 32), j & 1 ? i2 : i0,
-                          sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 12 + 6, j > 0 ? 1u : add);
-            if (kb == nkb - 1) commit_pair(&acc_full[1]);
-            commit_pair(&empty[r.s]);
-          }
-          __syncwarp();
         }
       }
       if (!ok && lead) {
@@ -1012,7 +1053,8 @@ static int gemm_tile(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc
   MPQ_CHECK_ARG((int64_t)p.mt * p.nt <= 0x1fffffff, "mpq_mx4_gemm: too many tiles");
   CUtensorMap o{};
   p.tile_out = result_map(&o, p.out, type_code<T>(), 1, p.M, p.N, p.ldo);
-  const size_t smem = 1024 + kStages * (kOperand + BN * 128 + 2 * kScale) + 4 * 4096 + 256;
+  p.stages = std::min<int>(kMostStages, kTileRing / (BN * 128 + p.a_rows * 128 + 2 * kScale));
+  const size_t smem = 1024 + kTileRing + 4 * 4096 + 512;
   const int grid = parts > 1 ? p.mt * p.nt * parts : std::min(p.mt * p.nt, num_sms());
   return launch_product(k_mx4_tile<T, BN>, grid, kThreads, smem, parts, behind, st, a, b, sa, sb, o, p);
 }
@@ -1066,16 +1108,16 @@ template <class T, int TOK>
 static int few_tokens(const void* x, int64_t ldx, int M, int N, int K, const uint8_t* codes, const uint8_t* scales,
                       const void* bias, void* out, int64_t ldo, cudaStream_t st) {
   const int nb = (K + 31) / 32, iters = (nb + 31) / 32, groups = (N + kFewRows - 1) / kFewRows;
-  const size_t smem = (size_t)TOK * nb * 36;
+  const size_t smem = (size_t)TOK * nb * 68;
   const int r = smem_opt_in((const void*)k_mx4_few<T, TOK>, smem, "mpq_mx4_linear");
   if (r) return r;
   const bool vec = aligned16(x) && (ldx * (int64_t)sizeof(T)) % 16 == 0;
   const int ctas = num_sms() * (smem <= 100 * 1024 ? 2 : 1);
-  // the parts of K with the fewest steps for the busiest warp; a round's sum counts as one
+  // the parts of K with the fewest steps for the busiest warp; a round's sum counts as half of one
   int slices = 1, least = 1 << 30;
   for (int s = 1; s <= kFewWarps && s <= iters; s *= 2) {
     const int rounds = (groups * s + ctas * kFewWarps - 1) / (ctas * kFewWarps);
-    const int steps = rounds * ((iters + s - 1) / s + 1);
+    const int steps = rounds * (2 * ((iters + s - 1) / s) + 1);
     if (steps < least) {
       least = steps;
       slices = s;
@@ -1087,23 +1129,22 @@ static int few_tokens(const void* x, int64_t ldx, int M, int N, int K, const uin
   return launch_status("mpq_mx4_linear (few tokens)");
 }
 
-constexpr int kFewTokens = 4;
+constexpr int kFewTokens = 2;
 // x has to fit in shared memory
-static bool takes_few(int M, int K) { return M <= kFewTokens && (M <= 2 ? M : 4) * ((K + 31ll) / 32) * 36 <= 200 * 1024; }
+static bool takes_few(int M, int K) { return M <= kFewTokens && M * ((K + 31ll) / 32) * 68 <= 200 * 1024; }
 
 template <class T>
 static int linear(const void* x, int dtype, int64_t ldx, int M, int N, int K, const uint8_t* codes, const uint8_t* scales,
                   const void* bias, uint8_t* work, void* out, int64_t ldo, int* status, cudaStream_t st) {
   if (takes_few(M, K)) {
-    return M == 1   ? few_tokens<T, 1>(x, ldx, M, N, K, codes, scales, bias, out, ldo, st)
-           : M == 2 ? few_tokens<T, 2>(x, ldx, M, N, K, codes, scales, bias, out, ldo, st)
-                    : few_tokens<T, 4>(x, ldx, M, N, K, codes, scales, bias, out, ldo, st);
+    return M == 1 ? few_tokens<T, 1>(x, ldx, M, N, K, codes, scales, bias, out, ldo, st)
+                  : few_tokens<T, 2>(x, ldx, M, N, K, codes, scales, bias, out, ldo, st);
   }
   const int nb = (K + 31) / 32;
   uint8_t* x_scales = work + 16 * (int64_t)nb * M;
   const int r = quantize<T>(x, ldx, M, K, work, x_scales, st);
   if (r) return r;
-  return gemm<T>(work, codes, GemmArgs{x_scales, scales, bias, out, ldo, M, N, (nb + 3) / 4, 0, 0, 0, 0, status}, K, true, st);
+  return gemm<T>(work, codes, GemmArgs{x_scales, scales, bias, out, ldo, M, N, (nb + 3) / 4, 0, 0, 0, 0, 0, status}, K, true, st);
 }
 
 }  // namespace mx4
@@ -1150,7 +1191,7 @@ MPQ_API int mpq_mx4_gemm(int M, int N, int K, const uint8_t* a_codes, const uint
                 "mpq_mx4_gemm: codes and scales must be 16-byte aligned");
   const int st = tc::get_encoder();
   if (st) return st;
-  const mx4::GemmArgs p{a_scales, b_scales, bias, out, ldo, M, N, ((K + 31) / 32 + 3) / 4, 0, 0, 0, 0, status};
+  const mx4::GemmArgs p{a_scales, b_scales, bias, out, ldo, M, N, ((K + 31) / 32 + 3) / 4, 0, 0, 0, 0, 0, status};
   return MX4_BY_TYPE(dtype, gemm, a_codes, b_codes, p, K, false, (cudaStream_t)stream);
 }
 

@@ -211,6 +211,23 @@ __device__ __forceinline__ void chunk_send(const unsigned char* buf, int lane, c
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   }
 }
+// The same chunk where the result's rows do not start on 16 bytes: the lanes go along the rows, E bytes an element.
+template <int E>
+__device__ __forceinline__ void chunk_rows(const unsigned char* buf, int lane, void* dst, int64_t ld_bytes, int rows,
+                                           int cols) {
+  __syncwarp();
+  for (int r = 0; r < rows && r < 32; ++r) {
+    #pragma unroll
+    for (int b = lane * E; b < 128; b += 32 * E) {
+      if (b >= cols * E) break;
+      const unsigned char* at = buf + r * 128 + ((((b >> 4) ^ (r & 7)) << 4) | (b & 15));
+      unsigned char* to = reinterpret_cast<unsigned char*>(dst) + r * ld_bytes + b;
+      if constexpr (E == 2) *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(at);
+      else *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(at);
+    }
+  }
+  __syncwarp();
+}
 // Before the buffer's CTA ends.
 __device__ __forceinline__ void chunk_drain(int lane) {
   if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");

@@ -122,20 +122,16 @@ __device__ __forceinline__ void unit_at(int u, const Args& p, int kblocks, int& 
 template <int EPI>
 __device__ __forceinline__ int chunk_of(int kblocks) { return EPI == kLse ? kChunk : kblocks; }
 
-// 64 16-bit values (32 words) of each of a warp's rows from (row0, col) on, `lim` columns wanted: as a tile, or by the
-// threads where the result's rows are not aligned.
+// 64 16-bit values (32 words) of each of a warp's rows from (row0, col) on, `lim` columns wanted: as a tile, or row by
+// row where the result's rows are not aligned.
 __device__ __forceinline__ void store_half_rows(const Args& p, const CUtensorMap* map, unsigned char* buf, int lane, int row0,
                                                 int col, uint16_t* out, int64_t ld, const uint32_t (&w)[32], int lim) {
   if (lim <= 0 || row0 >= p.M) return;  // the same for the warp
-  if (p.tile_out) {
-    chunk_put(buf, lane, w);
+  chunk_put(buf, lane, w);
+  if (p.tile_out)
     chunk_send(buf, lane, map, col, row0, 0);
-  } else if (row0 + lane < p.M) {
-    uint16_t* dst = out + (int64_t)(row0 + lane) * ld + col;
-    #pragma unroll
-    for (int i = 0; i < 64; ++i)
-      if (i < lim) dst[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-  }
+  else
+    chunk_rows<2>(buf, lane, out + row0 * ld + col, ld * 2, p.M - row0, lim);
 }
 
 // 2^t in one instruction (denormal results become 0, 2^-22 relative)
@@ -414,20 +410,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int c0 = 0; c0 < 128; c0 += 32) {
             const int lim = p.N - (n0 + c0);
             if (lim <= 0 || row0 >= p.M) break;
-            if (p.tile_out) {
-              chunk_begin(lane);
-              #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float* e = x + c0 + 4 * j;
-                chunk_unit(buf, lane, j, make_uint4(__float_as_uint(alpha * e[0]), __float_as_uint(alpha * e[1]),
-                                                    __float_as_uint(alpha * e[2]), __float_as_uint(alpha * e[3])));
-              }
-              chunk_send(buf, lane, &map_o, n0 + c0, row0, u % p.splits);
-            } else if (live) {
-              #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (i < lim) acc[(int64_t)row * p.N + n0 + c0 + i] = alpha * x[c0 + i];
+            chunk_begin(lane);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float* e = x + c0 + 4 * j;
+              chunk_unit(buf, lane, j, make_uint4(__float_as_uint(alpha * e[0]), __float_as_uint(alpha * e[1]),
+                                                  __float_as_uint(alpha * e[2]), __float_as_uint(alpha * e[3])));
             }
+            if (p.tile_out)
+              chunk_send(buf, lane, &map_o, n0 + c0, row0, u % p.splits);
+            else
+              chunk_rows<4>(buf, lane, acc + (int64_t)row0 * p.N + n0 + c0, (int64_t)p.N * 4, p.M - row0, lim);
           }
         } else {
           #pragma unroll
