@@ -468,14 +468,14 @@ constexpr int kCols = 128 / sizeof(T);
 
 template <class T>
 __device__ __forceinline__ void store_rows(const GemmArgs& p, const CUtensorMap* map, unsigned char* buf, int lane, int row0,
-                                           int col, const uint32_t (&v)[kCols<T>]) {
+                                           int col, const float* v) {
   const int lim = p.N - col;
   if (lim <= 0 || row0 >= p.M) return;  // the same for the warp
   const T* bias = reinterpret_cast<const T*>(p.bias);
   alignas(16) T o[kCols<T>];
   #pragma unroll
   for (int i = 0; i < kCols<T>; ++i) {
-    float f = __uint_as_float(v[i]);
+    float f = v[i];
     if (bias && i < lim) f += to_f32(bias[col + i]);
     o[i] = from_f32<T>(f);
   }
@@ -492,13 +492,13 @@ __device__ __forceinline__ void store_rows(const GemmArgs& p, const CUtensorMap*
 
 // kCols<T> columns of TMEM
 template <int C>
-__device__ __forceinline__ void tmem_cols(uint32_t at, uint32_t (&v)[C]) {
+__device__ __forceinline__ void tmem_cols(uint32_t at, float (&v)[C]) {
   #pragma unroll
   for (int c = 0; c < C; c += 32) {
     uint32_t t[32];
     tmem_ld32(at + c, t);
     #pragma unroll
-    for (int i = 0; i < 32; ++i) v[c + i] = t[i];
+    for (int i = 0; i < 32; ++i) v[c + i] = __uint_as_float(t[i]);
   }
 }
 
@@ -677,12 +677,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * BN);
       #pragma unroll 1
       for (int c0 = 0; c0 < BN; c0 += kCols<T>) {
-        uint32_t v[kCols<T>];
+        float v[kCols<T>];
         tmem_cols(at + c0, v);
         if (parts > 1) {  // every load of the ring has been consumed: it holds this part, column by column
           if (quad * 32 < p.M) {
             #pragma unroll
-            for (int i = 0; i < kCols<T>; ++i) part_sum[(c0 + i) * kBM + quad * 32 + lane] = __uint_as_float(v[i]);
+            for (int i = 0; i < kCols<T>; ++i) part_sum[(c0 + i) * kBM + quad * 32 + lane] = v[i];
           }
         } else {
           store_rows<T>(p, &map_o, out_buf + quad * 4096, lane, mb * kBM + quad * 32, nb * BN + c0, v);
@@ -702,16 +702,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       // each CTA adds the parts of its share of the columns, in order
       #pragma unroll 1
       for (int c0 = rank * kCols<T>; c0 < BN; c0 += parts * kCols<T>) {
-        uint32_t v[kCols<T>];
+        float v[kCols<T>];
         #pragma unroll
-        for (int i = 0; i < kCols<T>; ++i) v[i] = 0;
+        for (int i = 0; i < kCols<T>; ++i) v[i] = 0.f;
         for (int r = 0; r < parts; ++r) {
           const uint32_t at = mapa(smem_u32(part_sum + c0 * kBM + row), r);
           #pragma unroll
           for (int i = 0; i < kCols<T>; ++i) {
             float f;
             asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(at + i * kBM * 4));
-            v[i] = __float_as_uint(__uint_as_float(v[i]) + f);
+            v[i] += f;
           }
         }
         store_rows<T>(p, &map_o, out_buf + quad * 4096, lane, quad * 32, first_tile * BN + c0, v);
@@ -729,16 +729,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// k_mx4_pair, for many rows of A: a pair of CTAs computes 256 x 384 tiles (tcgen05 cta_group::2, M = 256, two products of
-// N = 192 a step).  Each CTA loads 128 rows of A and 192 of B a k-block: what bounds these products is the operands'
-// way from L2 to shared memory (two to three cycles a 128-byte row), so the tile is as wide as TMEM allows: 384 columns of
-// accumulator and 4 stages x 32 columns of scales (8 of A's 128 rows, 24 of B's 384, the latter in both CTAs).  The
-// accumulator is not doubled: the next tile's first half starts when the epilogue has read that half.
+// k_mx4_pair, for many rows of A: a pair of CTAs computes 256 x 256 tiles (tcgen05 cta_group::2, M = N = 256), each CTA
+// loading 128 rows of A and of B a k-block.  A step costs the tensor cores about 128 cycles an MMA, whatever its N, and
+// 57 a scale copy (measured; the two do not overlap), so N is the full 256: 4 MMAs and 6 copies for 256 columns against
+// 8 and 8 for 384.  TMEM holds one accumulator and the scales of 5 stages (24 columns each: 8 of A's 128 rows, 16 of
+// B's 256, the latter in both CTAs); the epilogue takes the accumulator into registers at once, so that the next tile's
+// MMAs wait for the reading only.
 
-constexpr int kPairWarps = 8, kPairThreads = 64 + 32 * kPairWarps, kPairStages = 4, kPairGroup = 8;
-constexpr int kPM = 256, kPN = 384, kPHalf = 192;
-constexpr uint32_t kPairB = 96 * 128, kPairOps = kOperand + 2 * kPairB, kPairSf = 4 * kScale;
-constexpr uint32_t kPairCols = 32;  // TMEM columns of a stage's scales, above the accumulator's 384
+constexpr int kPairWarps = 8, kPairThreads = 64 + 32 * kPairWarps, kPairStages = 5, kPairGroup = 8;
+constexpr int kPM = 256, kPN = 256;
+constexpr uint32_t kPairOps = 2 * kOperand, kPairSf = 3 * kScale;
+constexpr uint32_t kPairCols = 24;  // TMEM columns of a stage's scales, above the accumulator's 256
 
 template <class T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
@@ -751,12 +752,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + kPairWarps * 4096);
   uint64_t* empty = full + kPairStages;
   uint64_t* acc_full = empty + kPairStages;
-  uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* acc_empty = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto s_a = [&](int s) { return ring + s * kPairOps; };
-  auto s_b = [&](int s, int h) { return ring + s * kPairOps + kOperand + h * kPairB; };
-  auto s_sf = [&](int s) { return ring + kPairStages * kPairOps + s * kPairSf; };  // A's tile pair, then B's three
+  auto s_b = [&](int s) { return ring + s * kPairOps + kOperand; };
+  auto s_sf = [&](int s) { return ring + kPairStages * kPairOps + s * kPairSf; };  // A's tile pair, then B's two
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
@@ -772,10 +773,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], kPairWarps);  // four warps of each CTA read a half
-    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 2 * kPairWarps);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -800,7 +799,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       for (int t = pair; t < tiles && ok; t += pairs) {
         int mb, nb;
         tile_at(t, mb, nb);
-        const int row_a = mb * kPM + rank * 128, row_b = nb * kPN + rank * 96, tile_a = mb * 2 + rank, tile_b = nb * 3;
+        const int row_a = mb * kPM + rank * 128, row_b = nb * kPN + rank * 128, tile_a = mb * 2 + rank, tile_b = nb * 2;
         for (int kb = 0; kb < nkb; ++kb, ++it, r.next()) {
           if (!mbar_wait_cluster(&empty[r.s], r.ph ^ 1u) || *abort_flag) {
             ok = false;
@@ -810,8 +809,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           if (rank == 0) mbar_expect_tx(&full[r.s], 2 * (kPairOps + kPairSf));
           const uint32_t bar = bar0 + r.s * 8;
           tma_load_2d_pair(s_a(r.s), &map_a, bar, kb * 128, row_a);
-          tma_load_2d_pair(s_b(r.s, 0), &map_b, bar, kb * 128, row_b);
-          tma_load_2d_pair(s_b(r.s, 1), &map_b, bar, kb * 128, row_b + kPHalf);
+          tma_load_2d_pair(s_b(r.s), &map_b, bar, kb * 128, row_b);
           tma_load_2d_pair(s_sf(r.s), &map_sfa, bar, kb * 256, tile_a);
           tma_load_2d_pair(s_sf(r.s) + kScale, &map_sfb, bar, kb * 256, tile_b);
         }
@@ -829,20 +827,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (rank == 0) {
       const bool lead = elect_one();
       const uint64_t da0 = smem_desc_k_sw128(smem_u32(s_a(0))), ds0 = scale_desc(smem_u32(s_sf(0)));
-      const uint32_t i0 = idesc_mxf4(kPM, kPHalf, 0), i2 = idesc_mxf4(kPM, kPHalf, 2);
+      const uint32_t i0 = idesc_mxf4(kPM, kPN, 0), i2 = idesc_mxf4(kPM, kPN, 2);
       Ring r(kPairStages), c(kPairStages);
       auto copy = [&]() {  // the next step's scales, as in k_mx4_tile
         if (!warp_agrees(mbar_wait_cluster(&full[c.s], c.ph) && !*abort_flag)) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t sf = tmem + kPN + c.s * kPairCols;  // A's 2 x 4 columns, then B's 2 x 12
+        const uint32_t sf = tmem + kPN + c.s * kPairCols;  // A's 2 x 4 columns, then B's 2 x 8
         const uint64_t ds = desc_add(ds0, c.s * kPairSf);
         if (lead) {
           #pragma unroll
           for (int j = 0; j < 2; ++j) {
             copy_scales<2>(sf + j * 4, desc_add(ds, j * 512));
             #pragma unroll
-            for (int i = 0; i < 3; ++i)
-              copy_scales<2>(sf + 8 + j * 12 + i * 4, desc_add(ds, kScale * (1 + i) + j * 512));
+            for (int i = 0; i < 2; ++i)
+              copy_scales<2>(sf + 8 + j * 8 + i * 4, desc_add(ds, kScale * (1 + i) + j * 512));
           }
         }
         __syncwarp();
@@ -857,29 +855,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           const uint32_t sf = tmem + kPN + r.s * kPairCols;
           const uint64_t da = desc_add(da0, r.s * kPairOps), db = desc_add(da, kOperand);
           const uint32_t add = kb > 0;
-          #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (kb == 0) {
-              if (!warp_agrees(mbar_wait_cluster(&acc_empty[h], (n & 1u) ^ 1u))) {
-                ok = false;
-                break;
-              }
-              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            }
-            if (lead) {  // scales beyond the matrix are zeros, as are its codes
-              #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                mma_mxf4<2>(tmem + h * kPHalf, desc_add(da, j * 32), desc_add(db, h * kPairB + j * 32), j & 1 ? i2 : i0,
-                            sf + (j >> 1) * 4, sf + 8 + (j >> 1) * 12 + h * 6, j > 0 ? 1u : add);
-              if (h) commit_pair(&empty[r.s]);
-              if (kb == nkb - 1) commit_pair(&acc_full[h]);
-            }
-            __syncwarp();
-            if (h == 0 && --left > 0 && !copy()) {
+          if (kb == 0) {
+            if (!warp_agrees(mbar_wait_cluster(acc_empty, (n & 1u) ^ 1u))) {
               ok = false;
               break;
             }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           }
+          if (lead) {  // scales beyond the matrix are zeros, as are its codes
+            #pragma unroll
+            for (int j = 0; j < 2; ++j)
+              mma_mxf4<2>(tmem, desc_add(da, j * 32), desc_add(db, j * 32), j ? i2 : i0, sf, sf + 8, j ? 1u : add);
+          }
+          __syncwarp();
+          if (--left > 0 && !copy()) {
+            ok = false;
+            break;
+          }
+          if (lead) {
+            #pragma unroll
+            for (int j = 2; j < 4; ++j)
+              mma_mxf4<2>(tmem, desc_add(da, j * 32), desc_add(db, j * 32), j & 1 ? i2 : i0, sf + 4, sf + 16, 1u);
+            commit_pair(&empty[r.s]);
+            if (kb == nkb - 1) commit_pair(acc_full);
+          }
+          __syncwarp();
         }
       }
       if (!ok && lead) {
@@ -888,32 +888,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
     }
   } else {
-    // a warp reads the TMEM lanes of its quadrant (warp % 4); warps 2..5 take the first half's columns, 6..9 the second's
-    const int quad = warp & 3, h = (warp - 2) >> 2;
+    // a warp reads the TMEM lanes of its quadrant (warp % 4); warps 2..5 take columns 0..127, warps 6..9 the others
+    const int quad = warp & 3, half = (warp - 2) >> 2;
     unsigned char* buf = out_buf + (warp - 2) * 4096;
     uint32_t n = 0;
     for (int t = pair; t < tiles; t += pairs, ++n) {
       int mb, nb;
       tile_at(t, mb, nb);
-      const bool ready = !*abort_flag && mbar_wait_cluster(&acc_full[h], n & 1u);
+      const bool ready = !*abort_flag && mbar_wait_cluster(acc_full, n & 1u);
       if (!__all_sync(0xffffffffu, ready) || *abort_flag) {
         if (!*abort_flag) atomicCAS(p.status, 0, 4);
         *abort_flag = 1;
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(h * kPHalf);
-      #pragma unroll 1
-      for (int c0 = 0; c0 < kPHalf; c0 += kCols<T>) {
-        uint32_t v[kCols<T>];
-        tmem_cols(at + c0, v);
-        if (c0 + kCols<T> == kPHalf) {  // all read: the tensor cores may go on
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(&acc_empty[h]), 0));
-        }
-        store_rows<T>(p, &map_o, buf, lane, mb * kPM + rank * 128 + quad * 32, nb * kPN + h * kPHalf + c0, v);
-      }
+      float x[128];
+      tmem_ld128(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * 128), x);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(acc_empty), 0));
+      #pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += kCols<T>)
+        store_rows<T>(p, &map_o, buf, lane, mb * kPM + rank * 128 + quad * 32, nb * kPN + half * 128 + c0, x + c0);
     }
     chunk_drain(lane);
   }
@@ -1064,9 +1060,9 @@ static int gemm_pair(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc
   CUtensorMap a, b, sa, sb;
   int r = code_map(&a, a_codes, p.M, ldc, 128);
   if (r) return r;
-  if ((r = code_map(&b, b_codes, p.N, ldc, 96))) return r;
+  if ((r = code_map(&b, b_codes, p.N, ldc, 128))) return r;
   if ((r = scale_map(&sa, p.sfa, (p.M + 127) / 128, p.kt, 1))) return r;
-  if ((r = scale_map(&sb, p.sfb, (p.N + 127) / 128, p.kt, 3))) return r;
+  if ((r = scale_map(&sb, p.sfb, (p.N + 127) / 128, p.kt, 2))) return r;
   p.mt = (p.M + kPM - 1) / kPM;
   p.nt = (p.N + kPN - 1) / kPN;
   MPQ_CHECK_ARG((int64_t)p.mt * p.nt <= 0x7fffffff, "mpq_mx4_gemm: too many tiles");
@@ -1077,22 +1073,22 @@ static int gemm_pair(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc
                         sa, sb, o, p);
 }
 
-// The kernel with the shortest estimate: waves of CTAs (or pairs) x k-blocks x the cycles of one, which are those of its
-// operands' rows (a tile load takes about 2.5 cycles a row), and at least 300 for its steps one after the other; parts
-// of K on a cluster pay for their sum.  (Measured at K = 4096: 128 x 128 tiles 1140 cycles a k-block.)
+// The kernel with the shortest estimate in cycles, from measured parts: a k-block takes 740 in k_mx4_tile (4 MMAs, 4
+// scale copies, whatever the tile's width) and 860 in k_mx4_pair, the pair's launch 3000 more; a cluster's sum of two
+// parts of K takes 4000, of four 6000.  (us, 512 x 4096 x 4096: 128 columns 13.7, 64 18.7, pair 17.9; 8 x 14336 x 4096:
+// 128 columns in 4 parts 16.3, 2 parts 18.6, whole 26.4.)
 template <class T>
 static int gemm(const uint8_t* a_codes, const uint8_t* b_codes, const GemmArgs& p, int K, bool behind, cudaStream_t st) {
   const int64_t ldc = 16 * (int64_t)((K + 31) / 32);
   const int sms = num_sms(), nkb = (p.kt + 1) / 2;
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   int bn = 0, parts = 1;  // 0: pairs
-  double least = (double)up(up(p.M, kPM) * up(p.N, kPN), sms / 2) * (nkb * 900.0 + 1500.0);
+  double least = (double)up(up(p.M, kPM) * up(p.N, kPN), sms / 2) * (nkb * 860.0 + 1000.0) + 3000.0;
   for (int w : {128, 64})
     for (int s : {1, 2, 4}) {
       const int64_t tiles = up(p.M, kBM) * up(p.N, w);
-      if (s > 1 && (p.M > kBM || tiles * s > sms || nkb < 4 * s)) break;
-      const double kb = std::max(300.0, 4.5 * (std::min(p.M, kBM) + w));
-      const double t = (double)up(tiles, sms / s) * (up(nkb, s) * kb + 1000.0) + (s > 1 ? 1500.0 + 500.0 * s : 0.0);
+      if (s > 1 && (p.M > kBM || tiles * s > sms || nkb < s)) break;
+      const double t = (double)up(tiles, s > 1 ? tiles : sms) * up(nkb, s) * 740.0 + (s > 1 ? 2000.0 + 1000.0 * s : 0.0) + w;
       if (t < least) {
         least = t;
         bn = w;
