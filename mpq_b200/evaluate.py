@@ -1,0 +1,115 @@
+"""Scores of token sequences under a decoder LM, in floating point or with its linears in microscaled 4 bits.
+
+    perplexity(model, ids)                       # of a loaded decoder
+    convert_linears_mx4(model.model)             # every linear of the layers in MX4, in place
+    perplexity(model, ids)
+    tune_head(model, ids, steps=20)              # final norm and output head, the 4-bit layers as they are
+
+and the same from the command line, on a registered synthetic shape or a local checkpoint directory:
+
+    python -m mpq_b200.evaluate --model tiny_llama --sequences 8 --seqlen 512 --tune 20
+
+The output head's logits are not stored: the loss is ``vocab_cross_entropy`` on the hidden states.
+"""
+from __future__ import annotations
+
+import argparse
+import json
+import math
+from typing import Any, Dict, List, Optional
+
+import torch
+
+from . import ops
+from .loss import vocab_cross_entropy
+from .mx4 import convert_linears_mx4
+
+
+def _checked_ids(model, ids: torch.Tensor) -> torch.Tensor:
+    dev = next(model.parameters()).device
+    if dev.type != "cuda":
+        raise ValueError("mpq_b200 kernels require CUDA tensors (there is no CPU path)")
+    ids = torch.as_tensor(ids, dtype=torch.long)
+    if ids.dim() != 2 or ids.shape[1] < 2:
+        raise ValueError("ids must be (sequences, tokens) with two tokens at least")
+    return ids.to(dev)
+
+
+@torch.no_grad()
+def token_scores(model, ids: torch.Tensor, batch_size: int = 8) -> torch.Tensor:
+    """Negative log-likelihood of every token but the first of each sequence: (sequences, tokens - 1) in float32."""
+    ids = _checked_ids(model, ids)
+    head = model.lm_head.weight
+    out: List[torch.Tensor] = []
+    for part in ids.split(int(batch_size)):
+        hidden = model.model(part[:, :-1]).last_hidden_state.to(head.dtype)
+        out.append(vocab_cross_entropy(hidden, head, part[:, 1:], reduction="none"))
+    ops.check_status(ids.device)
+    return torch.cat(out)
+
+
+def perplexity(model, ids: torch.Tensor, batch_size: int = 8) -> float:
+    """exp of the mean score over all scored tokens."""
+    return math.exp(float(token_scores(model, ids, batch_size).double().mean()))
+
+
+def tune_head(model, ids: torch.Tensor, steps: int = 20, lr: float = 1e-3, batch_size: int = 8) -> List[float]:
+    """Train the final norm and the output head on ``ids`` (SGD on the mean loss), with the layers as they are; returns
+    the loss of each step.  The layers run forward only, so their linears may be in any format."""
+    ids = _checked_ids(model, ids)
+    inner, head = model.model, model.lm_head.weight
+    params = [p for p in (*inner.norm.parameters(), head)]
+    wanted = [p.requires_grad for p in params]
+    seen: Dict[str, torch.Tensor] = {}
+    hook = inner.norm.register_forward_pre_hook(lambda mod, args: seen.__setitem__("x", args[0].detach()))
+    losses: List[torch.Tensor] = []
+    try:
+        for p in params:
+            p.requires_grad_(True)
+        parts = ids.split(int(batch_size))
+        for step in range(int(steps)):
+            part = parts[step % len(parts)]
+            with torch.no_grad():
+                inner(part[:, :-1])
+            loss = vocab_cross_entropy(inner.norm(seen["x"]).to(head.dtype), head, part[:, 1:])
+            grads = torch.autograd.grad(loss, params)
+            with torch.no_grad():
+                for p, g in zip(params, grads):
+                    p.add_(g.to(p.dtype), alpha=-float(lr))
+            losses.append(loss.detach())
+    finally:
+        hook.remove()
+        for p, w in zip(params, wanted):
+            p.requires_grad_(w)
+    ops.check_status(ids.device)
+    return [float(v) for v in losses]
+
+
+def main(argv: Optional[List[str]] = None) -> Dict[str, Any]:
+    from .model import calibration_ids
+    from .quantization import _load_model
+    ap = argparse.ArgumentParser(prog="mpq_b200.evaluate", description=__doc__.split("\n\n")[0])
+    ap.add_argument("--model", default="tiny_llama", help="a registered synthetic shape or a local checkpoint directory")
+    ap.add_argument("--sequences", type=int, default=8)
+    ap.add_argument("--seqlen", type=int, default=512)
+    ap.add_argument("--batch-size", type=int, default=8)
+    ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--tune", type=int, default=0, help="training steps of the final norm and the head afterwards")
+    ap.add_argument("--lr", type=float, default=1e-3)
+    a = ap.parse_args(argv)
+    dev = torch.device("cuda", torch.cuda.current_device())
+    model, name = _load_model(a.model, dev, a.seed)
+    ids = calibration_ids(a.sequences, a.seqlen, int(model.config.vocab_size), seed=a.seed + 1)
+    out: Dict[str, Any] = {"model": name, "tokens": a.sequences * (a.seqlen - 1),
+                           "perplexity": perplexity(model, ids, a.batch_size)}
+    out["mx4_linears"] = convert_linears_mx4(model.model)
+    out["perplexity_mx4"] = perplexity(model, ids, a.batch_size)
+    if a.tune:
+        out["tune_losses"] = tune_head(model, ids, a.tune, a.lr, a.batch_size)
+        out["perplexity_mx4_tuned"] = perplexity(model, ids, a.batch_size)
+    print(json.dumps(out))
+    return out
+
+
+if __name__ == "__main__":
+    main()
