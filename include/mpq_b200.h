@@ -473,15 +473,14 @@ int mpq_mx4_linear(const void* x, int dtype, int64_t ldx, int M, int N, int K, c
  * `status`: as mpq_gemm_tc. */
 
 /* Columns of `part` below. */
-int mpq_xent_tiles(int V);
+int mpq_xent_tiles(int T, int V);
 /* Planes of T x H floats that mpq_xent_backward needs in `acc` for dhidden (0: none). */
 int mpq_xent_planes(int T, int V, int H, int piece, int keep_cols);
 /* lse[t] = log sum_v exp(h_t . w_v), nll[t] = lse[t] - h_t . w_y (0 where ignored).
  * reduction: 0 none; 1 loss = sum of nll; 2 loss = that over the number of counted labels (NaN for none); count = that
- * number.  Workspaces: part, T x
- * mpq_xent_tiles(V) pairs of floats (part_floats: floats it holds); tgt, T floats.  keep_cols != 0 (V, or a multiple of 256 below it): keep
- * receives, for mpq_xent_backward, 16-bit distances of those first columns' logits below their tile's largest (T rows,
- * leading dimension ldk). */
+ * number.  Workspaces: part, T x mpq_xent_tiles(T, V) pairs of floats (part_floats: floats it holds); tgt, T floats.
+ * keep_cols != 0 (V, or a multiple of 256 below it): keep receives, for mpq_xent_backward, 16-bit distances of those
+ * first columns' logits below their tile's largest (T rows, leading dimension ldk). */
 int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                      const int64_t* labels, int64_t ignore, float* part, int64_t part_floats, float* tgt, float* lse,
                      float* nll, int reduction, float* loss, float* count, void* keep, int64_t ldk, int keep_cols,

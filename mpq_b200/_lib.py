@@ -107,7 +107,7 @@ SIGNATURES: Dict[str, Tuple[Any, ...]] = {
     "mpq_mx4_gemm": (I, I, I, P, P, P, P, P, P, I, L, P, P),
     "mpq_mx4_linear_work": (I, I),
     "mpq_mx4_linear": (P, I, L, I, I, I, P, P, P, P, P, L, P, P),
-    "mpq_xent_tiles": (I,),
+    "mpq_xent_tiles": (I, I),
     "mpq_xent_planes": (I, I, I, I, I),
     "mpq_xent_forward": (I, I, I, I, P, L, P, L, P, L, P, L, P, P, P, I, P, P, P, L, I, P, P),
     "mpq_xent_backward": (I, I, I, I, P, L, P, L, P, L, P, P, I, P, P, P, P, L, I, P, P, I, P, P, L, P, L, P, P),

@@ -18,6 +18,10 @@
 // the exponent range and takes k = 0.  Rounding d to 16 bits costs each of its entries 2^-9 (bf16) or 2^-12 (f16) of
 // itself, no more than the rounding of the gradients to the same type.
 //
+// Few tokens (T <= kFew) take the narrow side of the products: the weights fill the 256 rows of a tile and the tokens its
+// columns, 16 at least.  As rows, T tokens would still cost the tensor cores 256 rows: 1 x 128256 x 4096 is bound by
+// reading W, but drew the full 1000 W doing so, which lowered the clock to 1.1 GHz and W to 4.1 TB/s.
+//
 // A label equal to `ignore` does not count: nll 0, d 0.  A label outside the vocabulary makes the token's nll and its
 // d NaN; no memory is read for it.
 #include <algorithm>
@@ -34,8 +38,8 @@ using namespace tc;
 constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
 constexpr int kBM = 256, kBN = 256, kGroup = 16;
 constexpr uint32_t kRingBytes = 192 * 1024;
-constexpr int kMostStages = 11;  // of 16 KB of B and 1 KB of A
-constexpr uint32_t kHalf = 128 * 128;  // bytes of an operand's 128 rows of one k-block (64 columns, one swizzle line)
+constexpr int kMostStages = 11;  // of 16 KB of one operand and 1 KB of the other
+constexpr int kFew = 128;
 constexpr int kChunk = 8;              // k-blocks that the forward pass accumulates before it adds in FP32
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -45,8 +49,9 @@ struct Args {
   int M, N, K, mt, nt;      // C[M, N] over K; mt x nt tiles
   int splits;               // parts of K; more than one only with `acc`
   int tile_out;             // the result's rows are aligned for tile stores
-  int a_rows;               // rows of A that a CTA loads
-  int stages;               // of the ring, each 16 KB of B and a_rows x 128 bytes of A
+  int a_rows, b_rows;       // rows of A and of B that a CTA loads
+  int tile_n;               // columns of a tile (256, or the tokens' 16 .. 128)
+  int stages;               // of the ring, each (a_rows + b_rows) x 128 bytes
   int f16;                  // 1: f16 operands, 0: bf16
   int* status;
   // kLse, kGrad
@@ -54,9 +59,10 @@ struct Args {
   int64_t ignore;
   int vocab;                // labels in [0, vocab) count
   int v0;                   // first column's vocabulary index
-  float2* part;             // kLse: [M, 2 nt] (max in log2 units, sum of exp2) of 128 columns each
+  float2* part;             // kLse: [tokens, parts] (max in log2 units, sum of exp2) of 128 columns each, 32 if few
+  int parts;
   float* tgt;               // kLse: [M] the label's logit
-  uint16_t* keep;           // kLse: distances of the columns below keep_cols (a multiple of 256, or N), [M, ldk]
+  uint16_t* keep;           // kLse: distances of the columns below keep_cols (a multiple of 256, or V), [tokens, ldk]
   int64_t ldk;
   int keep_cols;
   const float* lse;         // kGrad: [M]
@@ -163,7 +169,10 @@ __device__ __forceinline__ uint32_t distance_bits(float t) {
 //
 // The tensor core's FP32 accumulator truncates, and a score is a small difference of sums of H products; so the
 // forward pass (kLse) accumulates kChunk k-blocks at a time and adds these to nearest in registers.
-template <int EPI, bool A_MN, bool B_MN>
+//
+// FEW: A is the weights' side and B the tokens', one tile of p.tile_n columns; a thread holds a vocabulary row (kLse) or
+// a column of dH (kOut) for half of the tokens.
+template <int EPI, bool A_MN, bool B_MN, bool FEW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     k_xent_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_o, const Args p) {
@@ -176,9 +185,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const uint32_t a_bytes = p.a_rows * 128, stage = kHalf + a_bytes;
-  auto s_b = [&](int s) { return ring + s * stage; };
-  auto s_a = [&](int s) { return ring + s * stage + kHalf; };
+  // the full operand of a stage comes first: what the MMA reads beyond a short A belongs to this kernel's memory
+  const uint32_t stage = (p.a_rows + p.b_rows) * 128, lead_a = FEW ? 0 : p.b_rows * 128, lead_b = FEW ? p.a_rows * 128 : 0;
+  auto s_b = [&](int s) { return ring + s * stage + lead_b; };
+  auto s_a = [&](int s) { return ring + s * stage + lead_a; };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), pairs = gridDim.x >> 1;
@@ -215,7 +225,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int u = blockIdx.x >> 1; u < units && ok; u += pairs) {
         int mb, nb, k0, k1;
         unit_at(u, p, kblocks, mb, nb, k0, k1);
-        const int row_a = mb * kBM + rank * 128, row_b = nb * kBN + rank * 128;
+        const int row_a = mb * kBM + rank * 128, row_b = nb * kBN + rank * p.b_rows;
         for (int kb = k0; kb < k1; ++kb, ++it, r.next()) {
           if (!mbar_wait_cluster(&empty[r.s], r.ph ^ 1u) || *abort_flag) {
             ok = false;
@@ -250,7 +260,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     if (rank == 0) {
       const bool lead = elect_one();
-      const uint32_t idesc = idesc16(p.f16, A_MN, B_MN, kBM, kBN);
+      const uint32_t idesc = idesc16(p.f16, A_MN, B_MN, kBM, p.tile_n);
       const uint64_t da0 = A_MN ? smem_desc_mn_sw128(smem_u32(s_a(0))) : smem_desc_k_sw128(smem_u32(s_a(0)));
       const uint64_t db0 = B_MN ? smem_desc_mn_sw128(smem_u32(s_b(0))) : smem_desc_k_sw128(smem_u32(s_b(0)));
       constexpr uint32_t kStepA = A_MN ? 2048 : 32, kStepB = B_MN ? 2048 : 32;  // K = 16: 16 lines, or 32 bytes of a line
@@ -322,6 +332,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int u = blockIdx.x >> 1; u < units; u += pairs) {
       int mb, nb, k0, k1;
       unit_at(u, p, kblocks, mb, nb, k0, k1);
+      if constexpr (FEW) {
+        const int cw = p.tile_n >> 1, t0 = half * cw;  // this warp's tokens
+        const int col = mb * kBM + rank * 128 + quad * 32 + lane;  // vocabulary index, or column of dH
+        const bool inside = col < p.M;
+        const uint32_t at0 = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)t0;
+        float x[kFew / 2];
+        bool good = true;
+        const int chunk = chunk_of<EPI>(kblocks);
+        for (int kc = k0; kc < k1; kc += chunk) {
+          if (!(good = take())) break;
+          #pragma unroll
+          for (int c = 0; c < kFew / 2; c += 8) {
+            if (c < cw) {
+              float v[8];
+              tmem_ld8(at0 + (uint32_t)((n & 1) * kBN + c), v);
+              #pragma unroll
+              for (int i = 0; i < 8; ++i) x[c + i] = kc == k0 ? v[i] : x[c + i] + v[i];
+            }
+          }
+          release();
+        }
+        if (!good) break;
+        #pragma unroll
+        for (int j = 0; j < kFew / 2; ++j) {
+          const int t = t0 + j;
+          if (j >= cw || t >= p.N) break;
+          if constexpr (EPI == kLse) {
+            const float v = inside ? x[j] : -INFINITY;
+            float m = v;
+            #pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const float m2 = m == -INFINITY ? 0.f : m * kLog2e, e = fmaf(v, kLog2e, -m2);
+            const float sum = warp_sum(ex2(e));
+            const int first = col - lane;
+            if (lane == 0 && first < p.M) p.part[(int64_t)t * p.parts + (first >> 5)] = make_float2(m2, sum);
+            if (p.labels[t] == col && inside) p.tgt[t] = v;
+            if (col < p.keep_cols) p.keep[t * p.ldk + col] = (uint16_t)(distance_bits(e) & 0xffffu);
+          } else {
+            const float v = alpha * x[j];
+            if (inside) {
+              if (p.acc) p.acc[((int64_t)(u % p.splits) * p.N + t) * p.M + col] = v;
+              else reinterpret_cast<uint16_t*>(p.out)[t * p.ldo + col] = (uint16_t)pack16(v, 0.f, p.f16);
+            }
+          }
+        }
+        continue;
+      }
       const int row0 = mb * kBM + rank * 128 + quad * 32, row = row0 + lane;
       const bool live = row < p.M;
       const int n0 = nb * kBN + half * 128;
@@ -398,7 +455,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           sum0 += ex2(fmaf(x[i], kLog2e, -m2));
           sum1 += ex2(fmaf(x[i + 1], kLog2e, -m2));
         }
-        if (live) p.part[(int64_t)row * (2 * p.nt) + 2 * nb + half] = make_float2(lim > 0 ? m2 : -INFINITY, sum0 + sum1);
+        if (live) p.part[(int64_t)row * p.parts + 2 * nb + half] = make_float2(lim > 0 ? m2 : -INFINITY, sum0 + sum1);
       } else {
         if (!take()) break;
         float x[128];
@@ -458,11 +515,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-// d of the kept columns, in place of their distances q below the maximum m of 128 columns: g (exp(l - lse) - [v = y]) =
+// d of the kept columns, in place of their distances q below the maximum m of their part of the columns (2^shift): g (exp(l - lse) - [v = y]) =
 // g (2^(m - q - lse) - ..); the label's own entry comes from its logit in FP32.  A row to blockIdx.y, eight columns to a
 // thread and step, so that a row's scalars are read once for the columns of a CTA.
 __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int64_t ldk, int T, int cols,
-                                                   const float2* __restrict__ part, int tiles,
+                                                   const float2* __restrict__ part, int parts, int shift,
                                                    const float* __restrict__ tgt, const float* __restrict__ lse,
                                                    const int64_t* __restrict__ labels, int64_t ignore, int vocab,
                                                    const float* __restrict__ gout, int gstride,
@@ -482,7 +539,7 @@ __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int
     for (int c0 = (blockIdx.x * 256 + threadIdx.x) * 8; c0 < cols; c0 += gridDim.x * 2048) {
       uint4* at = reinterpret_cast<uint4*>(d + row * ldk + c0);
       uint4 raw = __ldcs(at);
-      const float up = part[(int64_t)row * tiles + (c0 >> 7)].x - lse2;
+      const float up = part[(int64_t)row * parts + (c0 >> shift)].x - lse2;
       uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
       #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -511,21 +568,21 @@ __global__ void __launch_bounds__(256) k_xent_planes(const float* __restrict__ p
 }
 
 // Joins a token's tiles: lse = log2-domain maximum and sum -> natural log; one CTA a token, fixed order.
-__global__ void __launch_bounds__(128) k_xent_join(const float2* __restrict__ part, int nt, const float* __restrict__ tgt,
+__global__ void __launch_bounds__(512) k_xent_join(const float2* __restrict__ part, int ld, int nt, const float* __restrict__ tgt,
                                                    const int64_t* __restrict__ labels, int64_t ignore, int vocab,
                                                    float* __restrict__ lse, float* __restrict__ nll) {
-  __shared__ float red[4];
+  __shared__ float red[16];
   __shared__ float top_s;
   const int64_t t = blockIdx.x;
-  const float2* row = part + t * nt;
+  const float2* row = part + t * ld;
   float m = -INFINITY;
-  for (int i = threadIdx.x; i < nt; i += 128) m = fmaxf(m, row[i].x);
+  for (int i = threadIdx.x; i < nt; i += blockDim.x) m = fmaxf(m, row[i].x);
   m = block_max(m, red);
   if (threadIdx.x == 0) top_s = m;
   __syncthreads();
   const float top = top_s, base = top == -INFINITY ? 0.f : top;
   float s = 0.f;
-  for (int i = threadIdx.x; i < nt; i += 128) s += row[i].y * exp2f(row[i].x - base);
+  for (int i = threadIdx.x; i < nt; i += blockDim.x) s += row[i].y * exp2f(row[i].x - base);
   s = block_sum(s, red);
   if (threadIdx.x == 0) {
     const float l = (base + log2f(s)) * 0.69314718055994531f;
@@ -622,19 +679,23 @@ static int splits_for(int M, int N, int K) {
   return best;
 }
 
-template <int EPI, bool A_MN, bool B_MN>
+template <int EPI, bool A_MN, bool B_MN, bool FEW = false>
 static int product(const void* A, int64_t lda, const void* B, int64_t ldb, Args p, cudaStream_t st) {
   CUtensorMap ma, mb, mo{};
-  p.a_rows = A_MN ? 128 : std::min((p.M + 7) / 8 * 8, 128);
-  p.stages = std::min<int>(kMostStages, kRingBytes / (kHalf + p.a_rows * 128));
+  p.tile_n = FEW ? (p.N + 15) / 16 * 16 : kBN;
+  p.a_rows = A_MN || FEW ? 128 : std::min((p.M + 7) / 8 * 8, 128);
+  p.b_rows = p.tile_n / 2;
+  p.stages = std::min<int>(kMostStages, kRingBytes / ((p.a_rows + p.b_rows) * 128));
   int r = operand(&ma, A_MN, A, p.M, p.K, lda, p.a_rows, p.f16);
   if (r) return r;
-  if ((r = operand(&mb, B_MN, B, p.N, p.K, ldb, 128, p.f16))) return r;
+  if ((r = operand(&mb, B_MN, B, p.N, p.K, ldb, p.b_rows, p.f16))) return r;
   p.mt = (p.M + kBM - 1) / kBM;
   p.nt = (p.N + kBN - 1) / kBN;
   p.splits = std::max(p.splits, 1);
   const int type = p.f16 ? 2 : 1;
-  if (EPI == kLse) {
+  if (FEW) {
+    // the threads store: a warp's 32 columns of a token are neighbours
+  } else if (EPI == kLse) {
     MPQ_CHECK_ARG(p.keep_cols == 0 || result_map(&mo, p.keep, type, 1, p.M, p.keep_cols, p.ldk),
                   "mpq_xent_forward: no tensor map for %d kept columns", p.keep_cols);
   } else if (p.acc) {
@@ -643,9 +704,9 @@ static int product(const void* A, int64_t lda, const void* B, int64_t ldb, Args 
     p.tile_out = result_map(&mo, p.out, type, 1, p.M, p.N, p.ldo);
   }
   const size_t smem = 1024 + kRingBytes + kEpiWarps * 4096 + 256;
-  if ((r = smem_opt_in((const void*)k_xent_gemm<EPI, A_MN, B_MN>, smem, "mpq_xent"))) return r;
+  if ((r = smem_opt_in((const void*)k_xent_gemm<EPI, A_MN, B_MN, FEW>, smem, "mpq_xent"))) return r;
   const int grid = 2 * std::min(p.mt * p.nt * p.splits, num_sms() / 2);
-  k_xent_gemm<EPI, A_MN, B_MN><<<grid, kThreads, smem, st>>>(ma, mb, mo, p);
+  k_xent_gemm<EPI, A_MN, B_MN, FEW><<<grid, kThreads, smem, st>>>(ma, mb, mo, p);
   return launch_status("mpq_xent product");
 }
 
@@ -663,8 +724,10 @@ static bool operand_ok(const void* p, int64_t ld, int cols) {
 
 using namespace mpq;
 
-// Half tiles of the vocabulary in the forward pass: `part` holds T x this many float2.
-MPQ_API int mpq_xent_tiles(int V) { return V > 0 ? 2 * (int)(((int64_t)V + xent::kBN - 1) / xent::kBN) : 0; }
+// Parts of the vocabulary in the forward pass: `part` holds T x this many float2.
+MPQ_API int mpq_xent_tiles(int T, int V) {
+  return T > 0 && V > 0 ? (T <= xent::kFew ? 8 : 2) * (int)(((int64_t)V + xent::kBN - 1) / xent::kBN) : 0;
+}
 
 // FP32 planes of T x H that the backward pass needs for dhidden (0: none): one for each part of K of its largest
 // piece, and the running sum of several pieces.
@@ -693,25 +756,34 @@ MPQ_API int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden,
   MPQ_CHECK_ARG(hidden && weight && labels && part && tgt && lse && nll && status, "mpq_xent_forward: null pointer");
   MPQ_CHECK_ARG(xent::operand_ok(hidden, ldh, H) && xent::operand_ok(weight, ldw, H),
                 "mpq_xent_forward: operands must be 16-byte aligned with leading dimensions that are multiples of 8");
-  MPQ_CHECK_ARG(part_floats >= 2ll * T * mpq_xent_tiles(V) && (reinterpret_cast<uintptr_t>(part) & 7) == 0,
-                "mpq_xent_forward: the workspace needs %lld floats", 2ll * T * mpq_xent_tiles(V));
+  MPQ_CHECK_ARG(part_floats >= 2ll * T * mpq_xent_tiles(T, V) && (reinterpret_cast<uintptr_t>(part) & 7) == 0,
+                "mpq_xent_forward: the workspace needs %lld floats", 2ll * T * mpq_xent_tiles(T, V));
   MPQ_CHECK_ARG(keep_cols == 0 || (keep && (keep_cols == V || (keep_cols > 0 && keep_cols < V && keep_cols % 256 == 0)) &&
                                    xent::operand_ok(keep, ldk, keep_cols)),
                 "mpq_xent_forward: keep_cols must be V or a multiple of 256 below it, kept in rows like the operands");
-  MPQ_CHECK_ARG((int64_t)((T + 255) / 256) * mpq_xent_tiles(V) < (1ll << 31), "mpq_xent_forward: too many tiles");
+  MPQ_CHECK_ARG((int64_t)((T + 255) / 256) * mpq_xent_tiles(T, V) < (1ll << 31), "mpq_xent_forward: too many tiles");
   int st = tc::get_encoder();
   if (st) return st;
   xent::Args p{};
-  p.M = T; p.N = V; p.K = H;
+  p.K = H;
   p.f16 = dtype == 2;
   p.status = status;
   p.labels = labels; p.ignore = ignore; p.vocab = V;
   p.part = reinterpret_cast<float2*>(part);
+  p.parts = mpq_xent_tiles(T, V);
   p.tgt = tgt;
   p.keep = reinterpret_cast<uint16_t*>(keep); p.ldk = ldk; p.keep_cols = keep_cols;
-  st = xent::product<xent::kLse, false, false>(hidden, ldh, weight, ldw, p, (cudaStream_t)stream);
+  if (T <= xent::kFew) {
+    p.M = V; p.N = T;
+    st = xent::product<xent::kLse, false, false, true>(weight, ldw, hidden, ldh, p, (cudaStream_t)stream);
+  } else {
+    p.M = T; p.N = V;
+    st = xent::product<xent::kLse, false, false>(hidden, ldh, weight, ldw, p, (cudaStream_t)stream);
+  }
   if (st) return st;
-  xent::k_xent_join<<<T, 128, 0, (cudaStream_t)stream>>>(p.part, (int)mpq_xent_tiles(V), tgt, labels, ignore, V, lse, nll);
+  const int live = T <= xent::kFew ? (V + 31) / 32 : p.parts;  // parts that hold columns
+  xent::k_xent_join<<<T, live > 1024 && T <= 512 ? 512 : 128, 0, (cudaStream_t)stream>>>(p.part, p.parts, live, tgt, labels,
+                                                                                         ignore, V, lse, nll);
   if ((st = launch_status("mpq_xent_forward (join)")) || reduction == 0) return st;
   xent::k_xent_reduce<<<1, 1024, 0, (cudaStream_t)stream>>>(nll, labels, ignore, T, reduction == 2, loss, count);
   return launch_status("mpq_xent_forward (reduce)");
@@ -759,8 +831,8 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
     p.gout = gout; p.gstride = gstride; p.count = count; p.gmax = gmax;
     if (v0 < keep_cols) {
       dim3 grid(std::min((keep_cols + 2047) / 2048, 4), std::min(T, 32768));
-      xent::k_xent_kept<<<grid, 256, 0, cs>>>((uint16_t*)keep, ldk, T, keep_cols, (const float2*)part, mpq_xent_tiles(V),
-                                              tgt, lse, labels, ignore, V, gout, gstride, count, gmax, f16);
+      xent::k_xent_kept<<<grid, 256, 0, cs>>>((uint16_t*)keep, ldk, T, keep_cols, (const float2*)part, mpq_xent_tiles(T, V),
+                                              T <= xent::kFew ? 5 : 7, tgt, lse, labels, ignore, V, gout, gstride, count, gmax, f16);
       if ((st = launch_status("mpq_xent_backward (kept)"))) return st;
       dv = keep;
       ldd = ldk;
@@ -772,11 +844,18 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
       if ((st = xent::product<xent::kGrad, false, false>(hidden, ldh, W, ldw, p, cs))) return st;
     }
     if (dhidden) {
-      p.M = T; p.N = H; p.K = w;
+      p.K = w;
       p.out = dhidden; p.ldo = lddh;
       p.acc = planes ? acc : nullptr;
-      p.splits = xent::splits_for(T, H, w);
-      if ((st = xent::product<xent::kOut, false, true>(dv, ldd, W, ldw, p, cs))) return st;
+      p.splits = xent::splits_for(T, H, w);  // no more for a narrower last piece
+      if (T <= xent::kFew) {
+        p.M = H; p.N = T;
+        st = xent::product<xent::kOut, true, false, true>(W, ldw, dv, ldd, p, cs);
+      } else {
+        p.M = T; p.N = H;
+        st = xent::product<xent::kOut, false, true>(dv, ldd, W, ldw, p, cs);
+      }
+      if (st) return st;
       if (planes) {
         const int64_t n = (int64_t)T * H;
         const int grid = (int)std::min<int64_t>((n + 255) / 256, 8 * xent::num_sms());

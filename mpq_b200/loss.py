@@ -55,7 +55,7 @@ def _forward(hidden, weight, labels, ignore_index, reduction, keep_bytes):
     v = weight.shape[0]
     dev = hidden.device
     x, w = _operand(hidden), _operand(weight)
-    tiles = load().mpq_xent_tiles(v)
+    tiles = load().mpq_xent_tiles(t, v)
     each = reduction == "none"
     out = torch.empty((t,) if each else (), device=dev, dtype=torch.float32)
     work = torch.empty(_part_at(t) + 2 * t * tiles, device=dev, dtype=torch.float32)
