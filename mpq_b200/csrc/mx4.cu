@@ -237,19 +237,6 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restric
 
 constexpr int kFewRows = 4, kFewThreads = 256, kFewWarps = kFewThreads / 32;
 
-// Sums of four values over a warp: lane l gets the total of value l & 3.
-__device__ __forceinline__ float warp_sum4(const float (&v)[4], int lane) {
-  const bool odd = lane & 1, high = lane & 2;
-  float a = odd ? v[1] : v[0], b = odd ? v[3] : v[2];
-  a += __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[1], 1);
-  b += __shfl_xor_sync(0xffffffffu, odd ? v[2] : v[3], 1);
-  float c = high ? b : a;
-  c += __shfl_xor_sync(0xffffffffu, high ? a : b, 2);
-  #pragma unroll
-  for (int o = 4; o < 32; o <<= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-  return c;
-}
-
 template <class T, int TOK>
 __global__ void __launch_bounds__(kFewThreads, 2)
     k_mx4_few(const T* __restrict__ x, int64_t ldx, int tokens, int N, int K, bool vec, const uint8_t* __restrict__ codes,

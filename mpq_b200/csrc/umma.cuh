@@ -76,6 +76,19 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// Sums of four values over a warp: lane l gets the total of value l & 3.
+__device__ __forceinline__ float warp_sum4(const float (&v)[4], int lane) {
+  const bool odd = lane & 1, high = lane & 2;
+  float a = odd ? v[1] : v[0], b = odd ? v[3] : v[2];
+  a += __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[1], 1);
+  b += __shfl_xor_sync(0xffffffffu, odd ? v[2] : v[3], 1);
+  float c = high ? b : a;
+  c += __shfl_xor_sync(0xffffffffu, high ? a : b, 2);
+  #pragma unroll
+  for (int o = 4; o < 32; o <<= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+  return c;
+}
+
 // ---- CTA pairs (clusters of two whose tensor cores work on one tile) ----
 
 __device__ __forceinline__ uint32_t cluster_rank() {

@@ -18,9 +18,11 @@
 // the exponent range and takes k = 0.  Rounding d to 16 bits costs each of its entries 2^-9 (bf16) or 2^-12 (f16) of
 // itself, no more than the rounding of the gradients to the same type.
 //
-// Few tokens (T <= kFew) take the narrow side of the products: the weights fill the 256 rows of a tile and the tokens its
-// columns, 16 at least.  As rows, T tokens would still cost the tensor cores 256 rows: 1 x 128256 x 4096 is bound by
-// reading W, but drew the full 1000 W doing so, which lowered the clock to 1.1 GHz and W to 4.1 TB/s.
+// Few tokens take the narrow side of the products: the weights fill the 256 rows of a tile and the tokens its columns, 16
+// at least.  As rows, T tokens would still cost the tensor cores 256 rows: 1 x 128256 x 4096 is bound by reading W, but
+// drew the full 1000 W doing so, which lowered the clock to 1.1 GHz and W to 4.1 TB/s.  The limits were measured,
+// sustained, at 128256 x 4096 (us, few against many): scores of 32 tokens 203 and 273, of 48 242 and 273, of 64 283 and
+// 254 (each token's maximum and sum cross the lanes then); dH of 64 tokens 202 and 241, of 128 229 and 261.
 //
 // A label equal to `ignore` does not count: nll 0, d 0.  A label outside the vocabulary makes the token's nll and its
 // d NaN; no memory is read for it.
@@ -39,7 +41,7 @@ constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
 constexpr int kBM = 256, kBN = 256, kGroup = 16;
 constexpr uint32_t kRingBytes = 192 * 1024;
 constexpr int kMostStages = 11;  // of 16 KB of one operand and 1 KB of the other
-constexpr int kFew = 128;
+constexpr int kFewScored = 32, kFewGrads = 128;
 constexpr int kChunk = 8;              // k-blocks that the forward pass accumulates before it adds in FP32
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -115,13 +117,19 @@ __device__ __forceinline__ float unit_of(const float* gout, const float* count, 
 // Unit u -> its tile and range of k-blocks.  The raster walks kGroup row tiles down before it takes the next column
 // tile: the tiles in flight share a few row tiles (kept in L2) and stream the columns once for each group.
 __device__ __forceinline__ void unit_at(int u, const Args& p, int kblocks, int& mb, int& nb, int& k0, int& k1) {
-  const int t = u / p.splits, s = u - t * p.splits;
+  int t = u, s = 0;
+  k0 = 0;
+  k1 = kblocks;
+  if (p.splits > 1) {
+    t = u / p.splits;
+    s = u - t * p.splits;
+    k0 = (int)((int64_t)kblocks * s / p.splits);
+    k1 = (int)((int64_t)kblocks * (s + 1) / p.splits);
+  }
   const int per = kGroup * p.nt, g = t / per, r = t - g * per;
   const int rows = min(kGroup, p.mt - g * kGroup);
-  mb = g * kGroup + r % rows;
   nb = r / rows;
-  k0 = (int)((int64_t)kblocks * s / p.splits);
-  k1 = (int)((int64_t)kblocks * (s + 1) / p.splits);
+  mb = g * kGroup + r - nb * rows;
 }
 
 // k-blocks to an accumulator
@@ -145,6 +153,13 @@ __device__ __forceinline__ float ex2(float t) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
+}
+
+// Largest of a warp's values, NaN if one is: order-preserving whole numbers for the integer reduction.
+__device__ __forceinline__ float warp_max(float v) {
+  const int b = __float_as_int(v);
+  const int m = __reduce_max_sync(0xffffffffu, b ^ ((b >> 31) & 0x7fffffff));
+  return __int_as_float(m ^ ((m >> 31) & 0x7fffffff));
 }
 
 // Kept distances: t = log2 units below the maximum (t <= 0), in steps of 1 / kStep.  The sum with 2^23 rounds to a whole
@@ -311,6 +326,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     unsigned char* buf = out_buf + (warp - 2) * 4096;
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * 128);
     int n = 0;
+    int token_label = -1;  // FEW: lane i holds the label of this warp's token i, -1 where it does not count
+    if constexpr (FEW && EPI == kLse) {
+      const int cw = p.tile_n >> 1, t = half * cw + lane;
+      const int64_t y = lane < cw && t < p.N ? p.labels[t] : -1;
+      if (y >= 0 && y < p.vocab && y != p.ignore) token_label = (int)y;
+    }
     const float alpha = EPI == kOut ? unit_of(p.gout, p.count, p.gmax, p.f16) : 1.f;
     // the next accumulator in TMEM, false after a time-out
     auto take = [&]() {
@@ -337,13 +358,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int col = mb * kBM + rank * 128 + quad * 32 + lane;  // vocabulary index, or column of dH
         const bool inside = col < p.M;
         const uint32_t at0 = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)t0;
-        float x[kFew / 2];
+        constexpr int kMost = (EPI == kLse ? kFewScored : kFewGrads) / 2;
+        float x[kMost];
         bool good = true;
         const int chunk = chunk_of<EPI>(kblocks);
         for (int kc = k0; kc < k1; kc += chunk) {
           if (!(good = take())) break;
           #pragma unroll
-          for (int c = 0; c < kFew / 2; c += 8) {
+          for (int c = 0; c < kMost; c += 8) {
             if (c < cw) {
               float v[8];
               tmem_ld8(at0 + (uint32_t)((n & 1) * kBN + c), v);
@@ -354,27 +376,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           release();
         }
         if (!good) break;
-        #pragma unroll
-        for (int j = 0; j < kFew / 2; ++j) {
-          const int t = t0 + j;
-          if (j >= cw || t >= p.N) break;
-          if constexpr (EPI == kLse) {
-            const float v = inside ? x[j] : -INFINITY;
-            float m = v;
+        if constexpr (EPI == kLse) {
+          const int first = col - lane;
+          #pragma unroll
+          for (int j = 0; j < kMost; j += 4) {
+            if (j >= cw || t0 + j >= p.N) break;
+            float e[4], m2 = 0.f;  // lane i keeps token j + i's maximum
             #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float m2 = m == -INFINITY ? 0.f : m * kLog2e, e = fmaf(v, kLog2e, -m2);
-            const float sum = warp_sum(ex2(e));
-            const int first = col - lane;
-            if (lane == 0 && first < p.M) p.part[(int64_t)t * p.parts + (first >> 5)] = make_float2(m2, sum);
-            if (p.labels[t] == col && inside) p.tgt[t] = v;
-            if (col < p.keep_cols) p.keep[t * p.ldk + col] = (uint16_t)(distance_bits(e) & 0xffffu);
-          } else {
-            const float v = alpha * x[j];
-            if (inside) {
-              if (p.acc) p.acc[((int64_t)(u % p.splits) * p.N + t) * p.M + col] = v;
-              else reinterpret_cast<uint16_t*>(p.out)[t * p.ldo + col] = (uint16_t)pack16(v, 0.f, p.f16);
+            for (int i = 0; i < 4; ++i) {
+              const float v = inside ? x[j + i] : -INFINITY, m = warp_max(v), top = m == -INFINITY ? 0.f : m * kLog2e;
+              e[i] = fmaf(v, kLog2e, -top);
+              if (lane == i) m2 = top;
+              const int t = t0 + j + i;
+              const int y = __shfl_sync(0xffffffffu, token_label, j + i);
+              if (y == col && t < p.N) p.tgt[t] = v;
+              if (col < p.keep_cols && t < p.N) p.keep[t * p.ldk + col] = (uint16_t)(distance_bits(e[i]) & 0xffffu);
+              e[i] = ex2(e[i]);
             }
+            const float sum = warp_sum4(e, lane);  // lane i: token j + i
+            const int t = t0 + j + lane;
+            if (lane < 4 && t < p.N && first < p.M) p.part[(int64_t)t * p.parts + (first >> 5)] = make_float2(m2, sum);
+          }
+        } else if (inside) {
+          #pragma unroll
+          for (int j = 0; j < kMost; ++j) {
+            const int t = t0 + j;
+            if (j >= cw || t >= p.N) break;
+            const float v = alpha * x[j];
+            if (p.acc) p.acc[((int64_t)(u % p.splits) * p.N + t) * p.M + col] = v;
+            else reinterpret_cast<uint16_t*>(p.out)[t * p.ldo + col] = (uint16_t)pack16(v, 0.f, p.f16);
           }
         }
         continue;
@@ -726,7 +756,7 @@ using namespace mpq;
 
 // Parts of the vocabulary in the forward pass: `part` holds T x this many float2.
 MPQ_API int mpq_xent_tiles(int T, int V) {
-  return T > 0 && V > 0 ? (T <= xent::kFew ? 8 : 2) * (int)(((int64_t)V + xent::kBN - 1) / xent::kBN) : 0;
+  return T > 0 && V > 0 ? (T <= xent::kFewScored ? 8 : 2) * (int)(((int64_t)V + xent::kBN - 1) / xent::kBN) : 0;
 }
 
 // FP32 planes of T x H that the backward pass needs for dhidden (0: none): one for each part of K of its largest
@@ -773,7 +803,7 @@ MPQ_API int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden,
   p.parts = mpq_xent_tiles(T, V);
   p.tgt = tgt;
   p.keep = reinterpret_cast<uint16_t*>(keep); p.ldk = ldk; p.keep_cols = keep_cols;
-  if (T <= xent::kFew) {
+  if (T <= xent::kFewScored) {
     p.M = V; p.N = T;
     st = xent::product<xent::kLse, false, false, true>(weight, ldw, hidden, ldh, p, (cudaStream_t)stream);
   } else {
@@ -781,7 +811,7 @@ MPQ_API int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden,
     st = xent::product<xent::kLse, false, false>(hidden, ldh, weight, ldw, p, (cudaStream_t)stream);
   }
   if (st) return st;
-  const int live = T <= xent::kFew ? (V + 31) / 32 : p.parts;  // parts that hold columns
+  const int live = T <= xent::kFewScored ? (V + 31) / 32 : p.parts;  // parts that hold columns
   xent::k_xent_join<<<T, live > 1024 && T <= 512 ? 512 : 128, 0, (cudaStream_t)stream>>>(p.part, p.parts, live, tgt, labels,
                                                                                          ignore, V, lse, nll);
   if ((st = launch_status("mpq_xent_forward (join)")) || reduction == 0) return st;
@@ -832,7 +862,7 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
     if (v0 < keep_cols) {
       dim3 grid(std::min((keep_cols + 2047) / 2048, 4), std::min(T, 32768));
       xent::k_xent_kept<<<grid, 256, 0, cs>>>((uint16_t*)keep, ldk, T, keep_cols, (const float2*)part, mpq_xent_tiles(T, V),
-                                              T <= xent::kFew ? 5 : 7, tgt, lse, labels, ignore, V, gout, gstride, count, gmax, f16);
+                                              T <= xent::kFewScored ? 5 : 7, tgt, lse, labels, ignore, V, gout, gstride, count, gmax, f16);
       if ((st = launch_status("mpq_xent_backward (kept)"))) return st;
       dv = keep;
       ldd = ldk;
@@ -848,7 +878,7 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
       p.out = dhidden; p.ldo = lddh;
       p.acc = planes ? acc : nullptr;
       p.splits = xent::splits_for(T, H, w);  // no more for a narrower last piece
-      if (T <= xent::kFew) {
+      if (T <= xent::kFewGrads) {
         p.M = H; p.N = T;
         st = xent::product<xent::kOut, true, false, true>(W, ldw, dv, ldd, p, cs);
       } else {
