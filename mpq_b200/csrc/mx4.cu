@@ -70,6 +70,22 @@ __device__ __forceinline__ void decode8(uint32_t codes, __half2 (&h)[4]) {
   for (int i = 0; i < 4; ++i)
     h[i] = __half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(codes >> (8 * i)), __NV_E2M1));
 }
+// The same with one instruction a pair, each taking its byte out of the word by itself, where the function above adds a
+// shift and a mask.  Only for code that a warp runs together: in code that diverges, ptxas 12.9.86 has lost the
+// operands of this form (seen in reading back and, with the opposite conversion, in quantisation).
+__device__ __forceinline__ void decode8_together(uint32_t codes, __half2 (&h)[4]) {
+  uint32_t r[4];
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(codes));
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<__half2*>(&r[i]);
+}
 
 // Byte of the scale of (row, block) inside the tiled scales of a matrix with kt tiles along its blocks.
 __device__ __forceinline__ int64_t scale_at(int64_t row, int block, int kt) {
@@ -232,13 +248,12 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restric
 // Every CTA quantises x for itself into shared memory (f16 values in four planes of 16 bytes a block, so that a warp's
 // reads are free of conflicts) while its first weights are on their way.  A warp takes kFewRows rows of W and one of
 // `slices` parts of K (so that all warps have work whatever N is), a lane every 32nd block; the next blocks are loaded
-// before the last are used.  (A deeper ring in shared memory was slower, 15.0 us against 13.0: the arithmetic bounds it,
-// which is why larger products go to the tensor cores even for one token.)
+// before the last are used.  (A deeper ring in shared memory was slower, 15.0 us against 13.0: the arithmetic bounds it.)
 
 constexpr int kFewRows = 4, kFewThreads = 256, kFewWarps = kFewThreads / 32;
 
 template <class T, int TOK>
-__global__ void __launch_bounds__(kFewThreads, 2)
+__global__ void __launch_bounds__(kFewThreads, 3)
     k_mx4_few(const T* __restrict__ x, int64_t ldx, int tokens, int N, int K, bool vec, const uint8_t* __restrict__ codes,
               const uint8_t* __restrict__ scales, const T* __restrict__ bias, T* __restrict__ out, int64_t ldo, int slices) {
   extern __shared__ __align__(16) unsigned char sm[];
@@ -329,7 +344,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
           #pragma unroll
           for (int r = 0; r < kFewRows; ++r) {
             __half2 h[4];
-            decode8(q == 0 ? w[r].x : (q == 1 ? w[r].y : (q == 2 ? w[r].z : w[r].w)), h);
+            decode8_together(q == 0 ? w[r].x : (q == 1 ? w[r].y : (q == 2 ? w[r].z : w[r].w)), h);
             #pragma unroll
             for (int t = 0; t < TOK; ++t) {
               __half2& sum = q < 2 ? lo[t][r] : hi[t][r];
@@ -1095,7 +1110,7 @@ static int few_tokens(const void* x, int64_t ldx, int M, int N, int K, const uin
   const int r = smem_opt_in((const void*)k_mx4_few<T, TOK>, smem, "mpq_mx4_linear");
   if (r) return r;
   const bool vec = aligned16(x) && (ldx * (int64_t)sizeof(T)) % 16 == 0;
-  const int ctas = num_sms() * (smem <= 100 * 1024 ? 2 : 1);
+  const int ctas = num_sms() * (smem <= 70 * 1024 ? 3 : 1);
   // the parts of K with the fewest steps for the busiest warp; a round's sum counts as half of one
   int slices = 1, least = 1 << 30;
   for (int s = 1; s <= kFewWarps && s <= iters; s *= 2) {
@@ -1112,14 +1127,16 @@ static int few_tokens(const void* x, int64_t ldx, int M, int N, int K, const uin
   return launch_status("mpq_mx4_linear (few tokens)");
 }
 
-constexpr int kFewTokens = 2;
-// x has to fit in shared memory
-static bool takes_few(int M, int K) { return M <= kFewTokens && M * ((K + 31ll) / 32) * 68 <= 200 * 1024; }
+// x has to fit in shared memory; a second token's arithmetic costs more than k_mx4_tile's start from 40 M weights on
+// (us, few against tile: 4096 x 4096 7.4 and 10.3, 14336 x 4096 15.1 and 13.8; one token 10.0 and 13.8).
+static bool takes_few(int M, int N, int K) {
+  return M <= 2 && M * ((K + 31ll) / 32) * 68 <= 200 * 1024 && (M == 1 || (int64_t)N * K <= 40000000);
+}
 
 template <class T>
 static int linear(const void* x, int dtype, int64_t ldx, int M, int N, int K, const uint8_t* codes, const uint8_t* scales,
                   const void* bias, uint8_t* work, void* out, int64_t ldo, int* status, cudaStream_t st) {
-  if (takes_few(M, K)) {
+  if (takes_few(M, N, K)) {
     return M == 1 ? few_tokens<T, 1>(x, ldx, M, N, K, codes, scales, bias, out, ldo, st)
                   : few_tokens<T, 2>(x, ldx, M, N, K, codes, scales, bias, out, ldo, st);
   }
@@ -1180,7 +1197,7 @@ MPQ_API int mpq_mx4_gemm(int M, int N, int K, const uint8_t* a_codes, const uint
 
 // Bytes of workspace that mpq_mx4_linear needs: the quantised x, or none.
 MPQ_API int64_t mpq_mx4_linear_work(int M, int K) {
-  if (M <= 0 || K <= 0 || mx4::takes_few(M, K)) return 0;
+  if (M <= 0 || K <= 0 || (M == 1 && mx4::takes_few(M, 1, K))) return 0;
   const int64_t nb = ((int64_t)K + 31) / 32;
   return 16 * nb * M + (M + 127ll) / 128 * ((nb + 3) / 4) * 512;
 }

@@ -218,6 +218,31 @@ def test_scales_at_the_ends_of_their_range_in_a_product(cuda_dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2, 3, 130])
+def test_every_code_at_every_place_of_a_block(cuda_dev, m):
+    """Products with a single element of x: y is the weight itself, exactly, for each of the 16 codes at each of the 96
+    places of a row (three blocks of different scales), whichever kernel the number of tokens selects."""
+    from mpq_b200.mx4 import Mx4Tensor, mx4_linear, stored_shapes
+    rows, cols = 16 * 3 + 1, 96
+    r, j = torch.arange(rows)[:, None], torch.arange(cols)[None]
+    code = (r * 5 + j * 7 + j // 16) % 16
+    c = (120 + 5 * (j // 32) + r % 3).expand(rows, cols)[:, ::32]
+    pairs = code.view(rows, -1, 2)
+    codes = (pairs[..., 0] + 16 * pairs[..., 1]).to(torch.uint8)
+    scales = torch.zeros(stored_shapes(rows, cols)[1], dtype=torch.uint8)
+    b = torch.arange(3)[None]
+    scales[r // 128, b // 4, (r % 32) * 16 + r % 128 // 32 * 4 + b % 4] = c.to(torch.uint8)
+    w = Mx4Tensor(codes.to(cuda_dev), scales.to(cuda_dev), (rows, cols))
+    want = plain_values(code, c)
+    for start in range(0, cols, m):
+        x = torch.zeros(m, cols)
+        places = [(start + t) % cols for t in range(m)]
+        x[torch.arange(m), places] = 1.0
+        y = mx4_linear(x.to(cuda_dev), w)
+        assert torch.equal(y.cpu().double(), want[:, places].T + 0.0)
+
+
+@pytest.mark.gpu
 def test_empty_and_repeatable(cuda_dev):
     from mpq_b200.mx4 import dequantize_mx4, mx4_linear, quantize_mx4
     w = quantize_mx4(values(64, 96, torch.bfloat16, cuda_dev))
