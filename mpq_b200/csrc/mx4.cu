@@ -161,7 +161,7 @@ template <class T>
 __global__ void __launch_bounds__(256) k_mx4_quantize(const T* __restrict__ x, int64_t ldx, int rows, int cols, bool vec,
                                                       uint8_t* __restrict__ codes, int64_t ldc,
                                                       uint8_t* __restrict__ scales, int kt) {
-  asm volatile("griddepcontrol.launch_dependents;");  // a product launched behind may set itself up
+  allow_behind();  // a product launched behind may set itself up
   // blockDim.x is a multiple of 8 (a scale tile's width in half blocks): partners sit in one warp
   const int nb = (cols + 31) >> 5, rows_pad = (rows + 127) & ~127;
   const int q = blockIdx.y * blockDim.x + threadIdx.x, block = q >> 1;
@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_2d(s_b(i), &map_b, &full[i], (kb0 + i) * 128, nb0 * BN);
         tma_load_2d(s_sf(i) + kScale, &map_sfb, &full[i], (kb0 + i) * 256, nb0 * BN >> 7);
       }
-      asm volatile("griddepcontrol.wait;" ::: "memory");
+      wait_before();
       for (int t = first_tile; t < tiles && ok; t += stride) {
         const int mb = t % p.mt, nb = t / p.mt;
         for (int kb = kb0; kb < kb1; ++kb, ++it, r.next()) {
@@ -793,7 +793,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");  // A may come from the kernel before
+      wait_before();  // A may come from the kernel before
       const uint32_t bar0 = mapa(smem_u32(full), 0);
       int64_t it = 0;
       Ring r(kPairStages);
@@ -1001,40 +1001,6 @@ static int scale_map(CUtensorMap* m, const void* p, int row_tiles, int kt, int r
   return MPQ_OK;
 }
 
-// Launch of a product: `cluster` CTAs to a cluster (0: the kernel says), started while the kernel before still runs
-// where `behind` says that it is this call's quantisation.
-template <class... P, class... A>
-static int launch_product(void (*kernel)(P...), int grid, int threads, size_t smem, int cluster, bool behind,
-                          cudaStream_t st, A... args) {
-  const int r = smem_opt_in((const void*)kernel, smem, "mpq_mx4_gemm");
-  if (r) return r;
-  cudaLaunchAttribute at[2];
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = at;
-  if (cluster) {
-    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    at[cfg.numAttrs].val.clusterDim.x = cluster;
-    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
-    ++cfg.numAttrs;
-  }
-  if (behind) {
-    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-    ++cfg.numAttrs;
-  }
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    set_last_error("mpq_mx4_gemm: %s", cudaGetErrorString(e));
-    return (int)e;
-  }
-  return MPQ_OK;
-}
-
 template <class T, int BN>
 static int gemm_tile(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc, GemmArgs p, int parts, bool behind,
                      cudaStream_t st) {
@@ -1054,7 +1020,7 @@ static int gemm_tile(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc
   p.stages = std::min<int>(kMostStages, kTileRing / (BN * 128 + p.a_rows * 128 + 2 * kScale));
   const size_t smem = 1024 + kTileRing + 4 * 4096 + 512;
   const int grid = parts > 1 ? p.mt * p.nt * parts : std::min(p.mt * p.nt, num_sms());
-  return launch_product(k_mx4_tile<T, BN>, grid, kThreads, smem, parts, behind, st, a, b, sa, sb, o, p);
+  return launch("mpq_mx4_gemm", k_mx4_tile<T, BN>, grid, kThreads, smem, parts, behind, st, a, b, sa, sb, o, p);
 }
 
 template <class T>
@@ -1071,7 +1037,7 @@ static int gemm_pair(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc
   CUtensorMap o{};
   p.tile_out = result_map(&o, p.out, type_code<T>(), 1, p.M, p.N, p.ldo);
   const size_t smem = 1024 + kPairStages * (kPairOps + kPairSf) + kPairWarps * 4096 + 256;
-  return launch_product(k_mx4_pair<T>, 2 * std::min(p.mt * p.nt, num_sms() / 2), kPairThreads, smem, 0, behind, st, a, b,
+  return launch("mpq_mx4_gemm", k_mx4_pair<T>, 2 * std::min(p.mt * p.nt, num_sms() / 2), kPairThreads, smem, 0, behind, st, a, b,
                         sa, sb, o, p);
 }
 

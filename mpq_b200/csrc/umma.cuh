@@ -320,5 +320,43 @@ inline bool result_map(CUtensorMap* m, void* p, int type, int64_t planes, int64_
                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Launch of a kernel: `cluster` CTAs to a cluster (0: the kernel says).  `behind`: it may start while the kernel before
+// it on the stream still runs (where that one allows it), and waits for its end by wait_before().
+template <class... P, class... A>
+static int launch(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int cluster, bool behind,
+                  cudaStream_t st, A... args) {
+  int r = MPQ_OK;
+  if (smem > 48 * 1024 && (r = smem_opt_in((const void*)kernel, smem, what))) return r;
+  cudaLaunchAttribute at[2];
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  if (cluster) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = cluster;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (behind) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_last_error("%s: %s", what, cudaGetErrorString(e));
+    return (int)e;
+  }
+  return MPQ_OK;
+}
+
+// The kernel behind this one may be started once all of this grid's CTAs are here; and: wait for the kernel before.
+__device__ __forceinline__ void allow_behind() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 }  // namespace tc
 }  // namespace mpq

@@ -208,6 +208,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), pairs = gridDim.x >> 1;
   const int kblocks = (p.K + 63) / 64, units = p.mt * p.nt * p.splits;
+  allow_behind();
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(&full[s], 1);
@@ -230,6 +231,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync();  // both CTAs' barriers are initialised before any is signalled
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
+  wait_before();  // operands, scalars and workspaces may be those of the kernel before
 
   if (warp == 0) {
     if (lane == 0) {
@@ -555,6 +557,8 @@ __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int
                                                    const float* __restrict__ gout, int gstride,
                                                    const float* __restrict__ count, const float* __restrict__ gmax,
                                                    int f16) {
+  allow_behind();
+  wait_before();
   for (int row = blockIdx.y; row < T; row += gridDim.y) {
     const int64_t y = labels[row];
     const bool inside = y >= 0 && y < vocab;
@@ -584,35 +588,78 @@ __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int
   }
 }
 
-// out (16 bits, ldo) or sum (FP32, contiguous) = (add ? sum : 0) + the planes in order.
-__global__ void __launch_bounds__(256) k_xent_planes(const float* __restrict__ planes, int splits, int M, int N,
-                                                     float* __restrict__ sum, int add, uint16_t* __restrict__ out,
-                                                     int64_t ldo, int f16) {
+// out (16 bits, ldo) or sum (FP32, contiguous) = (add ? sum : 0) + the planes in order.  W columns to a thread: 4 where
+// the rows are aligned for it, else 1; rows to blockIdx.y.
+template <int W>
+__global__ void __launch_bounds__(256) k_xent_planes(const float* __restrict__ planes, int splits, int M, int N, float* sum,
+                                                     int add, uint16_t* __restrict__ out, int64_t ldo, int f16) {
+  allow_behind();
+  wait_before();
+  const int c = (blockIdx.x * 256 + threadIdx.x) * W;
+  if (c >= N) return;
   const int64_t total = (int64_t)M * N;
-  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    float a = add ? sum[i] : 0.f;
-    for (int s = 0; s < splits; ++s) a += planes[s * total + i];
-    if (out) out[i / N * ldo + i % N] = (uint16_t)pack16(a, 0.f, f16);
-    else sum[i] = a;
+  for (int row = blockIdx.y; row < M; row += gridDim.y) {
+    const int64_t at = (int64_t)row * N + c;
+    float a[W];
+    auto load = [&](const float* from, float (&v)[W]) {
+      if constexpr (W == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(from);
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+      } else {
+        v[0] = *from;
+      }
+    };
+    #pragma unroll
+    for (int i = 0; i < W; ++i) a[i] = 0.f;
+    if (add) load(sum + at, a);
+    #pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      float v[W];
+      load(planes + s * total + at, v);
+      #pragma unroll
+      for (int i = 0; i < W; ++i) a[i] += v[i];
+    }
+    if constexpr (W == 4) {
+      if (out) *reinterpret_cast<uint2*>(out + row * ldo + c) = make_uint2(pack16(a[0], a[1], f16), pack16(a[2], a[3], f16));
+      else *reinterpret_cast<float4*>(sum + at) = make_float4(a[0], a[1], a[2], a[3]);
+    } else {
+      if (out) out[row * ldo + c] = (uint16_t)pack16(a[0], 0.f, f16);
+      else sum[at] = a[0];
+    }
   }
 }
 
-// Joins a token's tiles: lse = log2-domain maximum and sum -> natural log; one CTA a token, fixed order.
-__global__ void __launch_bounds__(512) k_xent_join(const float2* __restrict__ part, int ld, int nt, const float* __restrict__ tgt,
-                                                   const int64_t* __restrict__ labels, int64_t ignore, int vocab,
-                                                   float* __restrict__ lse, float* __restrict__ nll) {
-  __shared__ float red[16];
+// Joins a token's parts: lse = log2-domain maximum and sum -> natural log; one CTA a token, fixed order.  A thread's
+// first kHeld parts stay in registers between the two passes: all of them up to kHeld parts a thread.
+constexpr int kHeld = 8;
+__global__ void __launch_bounds__(1024) k_xent_join(const float2* __restrict__ part, int ld, int nt,
+                                                    const float* __restrict__ tgt, const int64_t* __restrict__ labels,
+                                                    int64_t ignore, int vocab, float* __restrict__ lse,
+                                                    float* __restrict__ nll) {
+  __shared__ float red[32];
   __shared__ float top_s;
+  allow_behind();
+  wait_before();
   const int64_t t = blockIdx.x;
   const float2* row = part + t * ld;
+  float2 v[kHeld];
+  #pragma unroll
+  for (int j = 0; j < kHeld; ++j) {
+    const int i = threadIdx.x + j * blockDim.x;
+    v[j] = i < nt ? row[i] : make_float2(-INFINITY, 0.f);
+  }
   float m = -INFINITY;
-  for (int i = threadIdx.x; i < nt; i += blockDim.x) m = fmaxf(m, row[i].x);
+  #pragma unroll
+  for (int j = 0; j < kHeld; ++j) m = fmaxf(m, v[j].x);
+  for (int i = threadIdx.x + kHeld * blockDim.x; i < nt; i += blockDim.x) m = fmaxf(m, row[i].x);
   m = block_max(m, red);
   if (threadIdx.x == 0) top_s = m;
   __syncthreads();
   const float top = top_s, base = top == -INFINITY ? 0.f : top;
   float s = 0.f;
-  for (int i = threadIdx.x; i < nt; i += blockDim.x) s += row[i].y * exp2f(row[i].x - base);
+  #pragma unroll
+  for (int j = 0; j < kHeld; ++j) s += v[j].y * exp2f(v[j].x - base);
+  for (int i = threadIdx.x + kHeld * blockDim.x; i < nt; i += blockDim.x) s += row[i].y * exp2f(row[i].x - base);
   s = block_sum(s, red);
   if (threadIdx.x == 0) {
     const float l = (base + log2f(s)) * 0.69314718055994531f;
@@ -627,6 +674,8 @@ __global__ void __launch_bounds__(1024) k_xent_reduce(const float* __restrict__ 
                                                       int64_t ignore, int T, int mean, float* __restrict__ loss,
                                                       float* __restrict__ count) {
   __shared__ float red[32];
+  allow_behind();
+  wait_before();
   float s = 0.f, c = 0.f;
   for (int t = threadIdx.x; t < T; t += 1024) {
     s += nll[t];
@@ -645,6 +694,7 @@ __global__ void __launch_bounds__(1024) k_xent_gmax(const float* __restrict__ go
                                                     const int64_t* __restrict__ labels, int64_t ignore, int vocab, int T,
                                                     const float* __restrict__ count, float* __restrict__ gmax) {
   __shared__ float red[32];
+  allow_behind();
   float m = 0.f;
   for (int t = threadIdx.x; t < T; t += 1024) {
     const int64_t y = labels[t];
@@ -710,7 +760,7 @@ static int splits_for(int M, int N, int K) {
 }
 
 template <int EPI, bool A_MN, bool B_MN, bool FEW = false>
-static int product(const void* A, int64_t lda, const void* B, int64_t ldb, Args p, cudaStream_t st) {
+static int product(const void* A, int64_t lda, const void* B, int64_t ldb, Args p, bool behind, cudaStream_t st) {
   CUtensorMap ma, mb, mo{};
   p.tile_n = FEW ? (p.N + 15) / 16 * 16 : kBN;
   p.a_rows = A_MN || FEW ? 128 : std::min((p.M + 7) / 8 * 8, 128);
@@ -734,10 +784,8 @@ static int product(const void* A, int64_t lda, const void* B, int64_t ldb, Args 
     p.tile_out = result_map(&mo, p.out, type, 1, p.M, p.N, p.ldo);
   }
   const size_t smem = 1024 + kRingBytes + kEpiWarps * 4096 + 256;
-  if ((r = smem_opt_in((const void*)k_xent_gemm<EPI, A_MN, B_MN, FEW>, smem, "mpq_xent"))) return r;
   const int grid = 2 * std::min(p.mt * p.nt * p.splits, num_sms() / 2);
-  k_xent_gemm<EPI, A_MN, B_MN, FEW><<<grid, kThreads, smem, st>>>(ma, mb, mo, p);
-  return launch_status("mpq_xent product");
+  return launch("mpq_xent product", k_xent_gemm<EPI, A_MN, B_MN, FEW>, grid, kThreads, smem, 0, behind, st, ma, mb, mo, p);
 }
 
 // Width of the piece that starts at column v0.
@@ -792,6 +840,7 @@ MPQ_API int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden,
                                    xent::operand_ok(keep, ldk, keep_cols)),
                 "mpq_xent_forward: keep_cols must be V or a multiple of 256 below it, kept in rows like the operands");
   MPQ_CHECK_ARG((int64_t)((T + 255) / 256) * mpq_xent_tiles(T, V) < (1ll << 31), "mpq_xent_forward: too many tiles");
+  cudaStream_t cs = (cudaStream_t)stream;
   int st = tc::get_encoder();
   if (st) return st;
   xent::Args p{};
@@ -805,18 +854,20 @@ MPQ_API int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden,
   p.keep = reinterpret_cast<uint16_t*>(keep); p.ldk = ldk; p.keep_cols = keep_cols;
   if (T <= xent::kFewScored) {
     p.M = V; p.N = T;
-    st = xent::product<xent::kLse, false, false, true>(weight, ldw, hidden, ldh, p, (cudaStream_t)stream);
+    st = xent::product<xent::kLse, false, false, true>(weight, ldw, hidden, ldh, p, false, cs);
   } else {
     p.M = T; p.N = V;
-    st = xent::product<xent::kLse, false, false>(hidden, ldh, weight, ldw, p, (cudaStream_t)stream);
+    st = xent::product<xent::kLse, false, false>(hidden, ldh, weight, ldw, p, false, cs);
   }
   if (st) return st;
   const int live = T <= xent::kFewScored ? (V + 31) / 32 : p.parts;  // parts that hold columns
-  xent::k_xent_join<<<T, live > 1024 && T <= 512 ? 512 : 128, 0, (cudaStream_t)stream>>>(p.part, p.parts, live, tgt, labels,
-                                                                                         ignore, V, lse, nll);
-  if ((st = launch_status("mpq_xent_forward (join)")) || reduction == 0) return st;
-  xent::k_xent_reduce<<<1, 1024, 0, (cudaStream_t)stream>>>(nll, labels, ignore, T, reduction == 2, loss, count);
-  return launch_status("mpq_xent_forward (reduce)");
+  // threads for a token: kHeld parts each, as far as a CTA goes
+  const int threads = live <= 1024 ? 128 : (live <= 2048 ? 256 : (live <= 4096 ? 512 : 1024));
+  st = tc::launch("mpq_xent_forward (join)", xent::k_xent_join, T, threads, 0, 0, true, cs, (const float2*)p.part, p.parts,
+                  live, (const float*)tgt, labels, ignore, V, lse, nll);
+  if (st || reduction == 0) return st;
+  return tc::launch("mpq_xent_forward (reduce)", xent::k_xent_reduce, 1, 1024, 0, 0, true, cs, (const float*)nll, labels,
+                    ignore, T, (int)(reduction == 2), loss, count);
 }
 
 MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden, int64_t ldh, const void* weight,
@@ -844,11 +895,13 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
   int st = tc::get_encoder();
   if (st) return st;
   const int f16 = dtype == 2;
+  bool behind = false;  // a kernel of this call came before
   if (gstride == 0) {
     gmax = nullptr;
   } else {
     xent::k_xent_gmax<<<1, 1024, 0, cs>>>(gout, gstride, labels, ignore, V, T, count, gmax);
     if ((st = launch_status("mpq_xent_backward (scale)"))) return st;
+    behind = true;
   }
   for (int v0 = 0, w; v0 < V; v0 += w) {
     w = xent::piece_at(v0, V, piece, keep_cols);
@@ -861,9 +914,10 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
     p.gout = gout; p.gstride = gstride; p.count = count; p.gmax = gmax;
     if (v0 < keep_cols) {
       dim3 grid(std::min((keep_cols + 2047) / 2048, 4), std::min(T, 32768));
-      xent::k_xent_kept<<<grid, 256, 0, cs>>>((uint16_t*)keep, ldk, T, keep_cols, (const float2*)part, mpq_xent_tiles(T, V),
-                                              T <= xent::kFewScored ? 5 : 7, tgt, lse, labels, ignore, V, gout, gstride, count, gmax, f16);
-      if ((st = launch_status("mpq_xent_backward (kept)"))) return st;
+      st = tc::launch("mpq_xent_backward (kept)", xent::k_xent_kept, grid, 256, 0, 0, behind, cs, (uint16_t*)keep, ldk, T,
+                      keep_cols, (const float2*)part, mpq_xent_tiles(T, V), T <= xent::kFewScored ? 5 : 7, tgt, lse, labels,
+                      ignore, V, gout, gstride, count, (const float*)gmax, f16);
+      if (st) return st;
       dv = keep;
       ldd = ldk;
     } else {
@@ -871,8 +925,9 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
       p.labels = labels; p.ignore = ignore; p.vocab = V; p.v0 = v0;
       p.lse = lse;
       p.out = d; p.ldo = piece;
-      if ((st = xent::product<xent::kGrad, false, false>(hidden, ldh, W, ldw, p, cs))) return st;
+      if ((st = xent::product<xent::kGrad, false, false>(hidden, ldh, W, ldw, p, behind, cs))) return st;
     }
+    behind = true;
     if (dhidden) {
       p.K = w;
       p.out = dhidden; p.ldo = lddh;
@@ -880,18 +935,22 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
       p.splits = xent::splits_for(T, H, w);  // no more for a narrower last piece
       if (T <= xent::kFewGrads) {
         p.M = H; p.N = T;
-        st = xent::product<xent::kOut, true, false, true>(W, ldw, dv, ldd, p, cs);
+        st = xent::product<xent::kOut, true, false, true>(W, ldw, dv, ldd, p, true, cs);
       } else {
         p.M = T; p.N = H;
-        st = xent::product<xent::kOut, false, true>(dv, ldd, W, ldw, p, cs);
+        st = xent::product<xent::kOut, false, true>(dv, ldd, W, ldw, p, true, cs);
       }
       if (st) return st;
       if (planes) {
         const int64_t n = (int64_t)T * H;
-        const int grid = (int)std::min<int64_t>((n + 255) / 256, 8 * xent::num_sms());
-        xent::k_xent_planes<<<grid, 256, 0, cs>>>(acc, p.splits, T, H, acc + (planes - 1) * n, v0 > 0,
-                                                  v0 + w == V ? (uint16_t*)dhidden : nullptr, lddh, f16);
-        if ((st = launch_status("mpq_xent_backward (planes)"))) return st;
+        float* sum = acc + (planes - 1) * n;
+        uint16_t* out = v0 + w == V ? (uint16_t*)dhidden : nullptr;
+        const bool wide = H % 4 == 0 && lddh % 4 == 0 && (reinterpret_cast<uintptr_t>(acc) & 15) == 0 &&
+                          (reinterpret_cast<uintptr_t>(dhidden) & 7) == 0;
+        const dim3 grid(wide ? (H / 4 + 255) / 256 : (H + 255) / 256, std::min(T, 65535));
+        st = tc::launch("mpq_xent_backward (planes)", wide ? xent::k_xent_planes<4> : xent::k_xent_planes<1>, grid, 256, 0, 0,
+                        true, cs, (const float*)acc, p.splits, T, H, sum, (int)(v0 > 0), out, lddh, f16);
+        if (st) return st;
       }
     }
     if (dweight) {
@@ -899,7 +958,7 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
       p.out = reinterpret_cast<uint16_t*>(dweight) + (int64_t)v0 * lddw; p.ldo = lddw;
       p.acc = nullptr;
       p.splits = 1;
-      if ((st = xent::product<xent::kOut, true, true>(dv, ldd, hidden, ldh, p, cs))) return st;
+      if ((st = xent::product<xent::kOut, true, true>(dv, ldd, hidden, ldh, p, true, cs))) return st;
     }
   }
   return MPQ_OK;
