@@ -488,8 +488,8 @@ int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden, int64_t
 /* dhidden (T x H) and dweight (V x H), either may be NULL, from lse and the upstream gradient gout[t * gstride] of
  * each nll (divided by *count where count is given).  keep, ldk, keep_cols, part and tgt: what mpq_xent_forward left
  * (keep is overwritten; keep_cols = 0: nothing was kept).  The other columns' logits are computed again, `piece` (a
- * multiple of 256) columns at a time.  Workspaces: gmax, one float (with gstride != 0); d, T x piece 16-bit values (unless all columns were
- * kept); acc, mpq_xent_planes(T, V, H, piece, keep_cols) x T x H floats. */
+ * multiple of 256) columns at a time.  Workspaces: gmax, one float (with gstride != 0); d, T x piece 16-bit values
+ * (unless all columns were kept); acc, mpq_xent_planes(T, V, H, piece, keep_cols) x T x H floats. */
 int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                       const int64_t* labels, int64_t ignore, const float* lse, const float* gout, int gstride,
                       const float* count, const float* part, const float* tgt, void* keep, int64_t ldk, int keep_cols,

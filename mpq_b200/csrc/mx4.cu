@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(256) k_mx4_quantize(const T* __restrict__ x, i
     uint32_t mag = h[r].largest();
     mag = max(mag, __shfl_xor_sync(two, mag, 1));
     const uint32_t c = scale_code(mag);
-    const float inv = c == 255 ? 0.f : scale_inverse(c);  // a block that is not finite reads back as NaN whatever it holds
+    const float inv = c == 255 ? 0.f : scale_inverse(c);  // a block that is not finite reads back as NaN anyway
     uint2 word;
     #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -243,19 +243,21 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restric
 // W is read once (17 bytes for 32 weights), and the arithmetic has to keep up with that: a block of a row takes 16
 // conversions of two codes to an f16 pair and 16 f16 products a token.  The products are exact: they are multiples of
 // 1/4 up to 36, and the eight that a half of an accumulator adds stay below 2^11 quarters; a block's four sums are
-// added in FP32 and scaled by 2^(cx + cw - 254) once.  (Decoded by byte permutations for dp4a a block took twice the
-// instructions: 14.1 us at 1 x 14336 x 4096.)
+// added in FP32 and scaled by 2^(cx + cw - 254) once.  1 x 4096 x 14336 takes 9.9 us, 3.2 TB/s (13.0 with a shift and a
+// mask to every conversion; 14.1 with byte permutations and dp4a, twice the instructions).
 // Every CTA quantises x for itself into shared memory (f16 values in four planes of 16 bytes a block, so that a warp's
 // reads are free of conflicts) while its first weights are on their way.  A warp takes kFewRows rows of W and one of
 // `slices` parts of K (so that all warps have work whatever N is), a lane every 32nd block; the next blocks are loaded
-// before the last are used.  (A deeper ring in shared memory was slower, 15.0 us against 13.0: the arithmetic bounds it.)
+// before the last are used.  (With a deeper ring in shared memory it took 15.0 us instead of 13.0: the arithmetic bounds
+// it, not the latency.)
 
 constexpr int kFewRows = 4, kFewThreads = 256, kFewWarps = kFewThreads / 32;
 
 template <class T, int TOK>
 __global__ void __launch_bounds__(kFewThreads, 3)
     k_mx4_few(const T* __restrict__ x, int64_t ldx, int tokens, int N, int K, bool vec, const uint8_t* __restrict__ codes,
-              const uint8_t* __restrict__ scales, const T* __restrict__ bias, T* __restrict__ out, int64_t ldo, int slices) {
+              const uint8_t* __restrict__ scales, const T* __restrict__ bias, T* __restrict__ out, int64_t ldo,
+              int slices) {
   extern __shared__ __align__(16) unsigned char sm[];
   __shared__ float part[2][kFewWarps][kFewRows * TOK];
   const int nb = (K + 31) >> 5, kt = (nb + 3) >> 2;
@@ -395,18 +397,21 @@ __global__ void __launch_bounds__(kFewThreads, 3)
 // Product: y[t, n] = sum_k A[t, k] B[n, k] (+ bias[n]), A and B in the stored form, on the block-scaled tensor cores
 // ------------------------------------------------------------------------------------------------------------------
 //
-// Two kernels.  k_mx4_tile, for few rows of A:
-// One CTA per SM walks 128 x BN output tiles (BN = 64 or 128: narrow tiles spread few
-// tokens' work over more SMs; a narrower one's scales would start at an odd TMEM column, which the MMA refuses).  A k-block is one 128-byte swizzle row per operand row = 256 codes, with
-// two 512-byte scale tiles for each operand.  Warp 0 fills a ring of stages by TMA; warp 1's elected thread copies the
-// stage's scales from shared memory to TMEM (tcgen05.cp, replicated to the four lane quadrants) and issues four MMAs
-// of K = 64; warps 2..5 read the FP32 accumulator, add the bias, round once and store.  Two accumulators let the
-// epilogue overlap the next tile.  Scale columns in TMEM belong to the stage, so they are not rewritten before the
-// MMAs that read them are done.  With at most 128 rows of A only those are loaded (a tile load takes two to three cycles a
-// 128-byte row; what the others' shared memory holds stays in their rows of the accumulator), the ring takes the
-// more stages for it, and a cluster of up to
-// four CTAs may share a tile, each with a part of K: they leave their FP32 sums in shared memory, and each adds the parts
-// of its share of the columns, in order.
+// Two kernels.  k_mx4_tile, for few rows of A: one CTA per SM walks 128 x BN output tiles (BN = 64 or 128: narrow tiles
+// spread few tokens' work over more SMs; a narrower one's scales would start at an odd TMEM column, which is not an
+// address that the MMA takes).  A k-block is one 128-byte swizzle row per operand row = 256 codes, with two 512-byte
+// scale tiles for each operand.  Warp 0 fills a ring of stages by TMA; warp 1's elected thread copies the stage's scales
+// from shared memory to TMEM (tcgen05.cp, replicated to the four lane quadrants) and issues four MMAs of K = 64; warps
+// 2..5 read the FP32 accumulator, add the bias, round once and store.  Two accumulators let the epilogue overlap the
+// next tile.  Scale columns in TMEM belong to the stage, so they are not rewritten before the MMAs that read them are
+// done.
+//
+// With at most 128 rows of A only those are loaded (a tile load takes two to three cycles a 128-byte row; what the
+// others' shared memory holds stays in their rows of the accumulator) and the ring takes the more stages for it.  A
+// cluster of up to four CTAs may share a tile, each with a part of K: they leave their FP32 sums in shared memory, and
+// each adds the parts of its share of the columns, in order.  7 x 14336 x 4096 takes 14 us, of which the tensor cores'
+// steps are 5 and the weights at the memory's rate 5; the rest is the quantisation before it, filling the ring and the
+// sum over the cluster, one after the other.
 
 constexpr int kThreads = 192;
 constexpr int kBM = 128, kMostStages = 16;
@@ -463,14 +468,14 @@ struct GemmArgs {
   int* status;
 };
 
-// kCols<T> columns of the accumulator are 128 bytes of a row.  Columns col.. of a warp's 32 rows from row0 on (`lane`: the
-// thread's row): bias, one rounding, and off as a tile, or row by row where the result's rows are not aligned.
+// kCols<T> columns of the accumulator are 128 bytes of a row.  Columns col.. of a warp's 32 rows from row0 on (`lane`:
+// the thread's row): bias, one rounding, and off as a tile, or row by row where the result's rows are not aligned.
 template <class T>
 constexpr int kCols = 128 / sizeof(T);
 
 template <class T>
-__device__ __forceinline__ void store_rows(const GemmArgs& p, const CUtensorMap* map, unsigned char* buf, int lane, int row0,
-                                           int col, const float* v) {
+__device__ __forceinline__ void store_rows(const GemmArgs& p, const CUtensorMap* map, unsigned char* buf, int lane,
+                                           int row0, int col, const float* v) {
   const int lim = p.N - col;
   if (lim <= 0 || row0 >= p.M) return;  // the same for the warp
   const T* bias = reinterpret_cast<const T*>(p.bias);
@@ -1016,7 +1021,7 @@ static int gemm_tile(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc
   p.nt = (p.N + BN - 1) / BN;
   MPQ_CHECK_ARG((int64_t)p.mt * p.nt <= 0x1fffffff, "mpq_mx4_gemm: too many tiles");
   CUtensorMap o{};
-  p.tile_out = result_map(&o, p.out, type_code<T>(), 1, p.M, p.N, p.ldo);
+  p.tile_out = result_map(&o, p.out, type_code<T>(), 1, p.M, p.N, p.ldo, false);
   p.stages = std::min<int>(kMostStages, kTileRing / (BN * 128 + p.a_rows * 128 + 2 * kScale));
   const size_t smem = 1024 + kTileRing + 4 * 4096 + 512;
   const int grid = parts > 1 ? p.mt * p.nt * parts : std::min(p.mt * p.nt, num_sms());
@@ -1024,7 +1029,8 @@ static int gemm_tile(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc
 }
 
 template <class T>
-static int gemm_pair(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc, GemmArgs p, bool behind, cudaStream_t st) {
+static int gemm_pair(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc, GemmArgs p, bool behind,
+                     cudaStream_t st) {
   CUtensorMap a, b, sa, sb;
   int r = code_map(&a, a_codes, p.M, ldc, 128);
   if (r) return r;
@@ -1035,10 +1041,10 @@ static int gemm_pair(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc
   p.nt = (p.N + kPN - 1) / kPN;
   MPQ_CHECK_ARG((int64_t)p.mt * p.nt <= 0x7fffffff, "mpq_mx4_gemm: too many tiles");
   CUtensorMap o{};
-  p.tile_out = result_map(&o, p.out, type_code<T>(), 1, p.M, p.N, p.ldo);
+  p.tile_out = result_map(&o, p.out, type_code<T>(), 1, p.M, p.N, p.ldo, false);
   const size_t smem = 1024 + kPairStages * (kPairOps + kPairSf) + kPairWarps * 4096 + 256;
-  return launch("mpq_mx4_gemm", k_mx4_pair<T>, 2 * std::min(p.mt * p.nt, num_sms() / 2), kPairThreads, smem, 0, behind, st, a, b,
-                        sa, sb, o, p);
+  return launch("mpq_mx4_gemm", k_mx4_pair<T>, 2 * std::min(p.mt * p.nt, num_sms() / 2), kPairThreads, smem, 0, behind,
+                st, a, b, sa, sb, o, p);
 }
 
 // The kernel with the shortest estimate in cycles, from measured parts: a k-block takes 740 in k_mx4_tile (4 MMAs, 4
@@ -1056,7 +1062,8 @@ static int gemm(const uint8_t* a_codes, const uint8_t* b_codes, const GemmArgs& 
     for (int s : {1, 2, 4}) {
       const int64_t tiles = up(p.M, kBM) * up(p.N, w);
       if (s > 1 && (p.M > kBM || tiles * s > sms || nkb < s)) break;
-      const double t = (double)up(tiles, s > 1 ? tiles : sms) * up(nkb, s) * 740.0 + (s > 1 ? 2000.0 + 1000.0 * s : 0.0) + w;
+      const double join = s > 1 ? 2000.0 + 1000.0 * s : 0.0;
+      const double t = (double)up(tiles, s > 1 ? tiles : sms) * up(nkb, s) * 740.0 + join + w;
       if (t < least) {
         least = t;
         bn = w;
@@ -1110,7 +1117,8 @@ static int linear(const void* x, int dtype, int64_t ldx, int M, int N, int K, co
   uint8_t* x_scales = work + 16 * (int64_t)nb * M;
   const int r = quantize<T>(x, ldx, M, K, work, x_scales, st);
   if (r) return r;
-  return gemm<T>(work, codes, GemmArgs{x_scales, scales, bias, out, ldo, M, N, (nb + 3) / 4, 0, 0, 0, 0, 0, status}, K, true, st);
+  const GemmArgs args{x_scales, scales, bias, out, ldo, M, N, (nb + 3) / 4, 0, 0, 0, 0, 0, status};
+  return gemm<T>(work, codes, args, K, true, st);
 }
 
 }  // namespace mx4

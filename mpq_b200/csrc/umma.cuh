@@ -305,9 +305,13 @@ inline int get_encoder() {
 }
 
 // Map of a result [planes, rows, cols] (leading dimension ld, planes contiguous) for chunk_send: type 0 f32, 1 bf16, 2
-// f16.  False where a tile store cannot take it (rows that do not start on 16 bytes).
-inline bool result_map(CUtensorMap* m, void* p, int type, int64_t planes, int64_t rows, int64_t cols, int64_t ld) {
+// f16.  False where a tile store cannot take it: rows that do not start on 16 bytes, or, unless `pads` (what lies
+// between a row's columns and its leading dimension is the kernel's own), rows that do not end on 16 bytes: a tile
+// store writes zeros up to there.
+inline bool result_map(CUtensorMap* m, void* p, int type, int64_t planes, int64_t rows, int64_t cols, int64_t ld,
+                       bool pads) {
   const int size = type == 0 ? 4 : 2;
+  if (!pads && (cols * size) % 16) return false;
   if ((reinterpret_cast<uintptr_t>(p) & 15) || (ld * size) % 16 || (ld * size * rows) >> 40) return false;
   cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
   cuuint64_t strides[2] = {(cuuint64_t)(ld * size), (cuuint64_t)(ld * size * rows)};

@@ -8,15 +8,17 @@
 // room for them, the first columns' distances below the largest of their 128 columns are kept for the backward pass, in
 // 16 bits (log2 units, steps of 2^-11: exp(l) within 2^-12.5 of itself down to 2^-32 of the largest; a bf16 exponential
 // would have rounded d a second time by 2^-9).  They save a quarter of a training step's products for two bytes an
-// entry.  The backward pass takes the vocabulary in pieces: the kept columns first, then pieces whose
-// logits it computes again, with d in 16 bits as the epilogue's result; it multiplies a piece's d with its rows of W
-// (dH, summed over the pieces in FP32) and with H (dW's rows of the piece).  Every sum runs in a fixed order, so
-// results repeat bit for bit.
+// entry.  The backward pass takes the vocabulary in pieces: the kept columns first, then pieces whose logits it computes
+// again, with d in 16 bits as the epilogue's result; it multiplies a piece's d with its rows of W (dH, summed over the
+// pieces in FP32) and with H (dW's rows of the piece).  Every sum runs in a fixed order, so results repeat bit for bit.
 //
 // d is held as 2^k d / u, with u = max|g| (or g itself where all tokens share it), in units of its largest possible
-// magnitude, and the products take the factor back in FP32: in f16 (k = 15) probabilities down to 2^-39 then stay normal numbers, whatever the mean divides by; bf16 has
-// the exponent range and takes k = 0.  Rounding d to 16 bits costs each of its entries 2^-9 (bf16) or 2^-12 (f16) of
-// itself, no more than the rounding of the gradients to the same type.
+// magnitude, and the products take the factor back in FP32: in f16 (k = 15) probabilities down to 2^-39 then stay normal
+// numbers, whatever the mean divides by; bf16 has the exponent range and takes k = 0.  Rounding d to 16 bits costs each
+// of its entries 2^-9 (bf16) or 2^-12 (f16) of itself, no more than the rounding of the gradients to the same type.
+//
+// At 8192 x 128256 x 4096 the three products run at 1355 to 1415 TFLOP/s, sustained under the card's power limit (a
+// plain library product of these sizes: 1281 to 1500); the step takes 21.5 ms.
 //
 // Few tokens take the narrow side of the products: the weights fill the 256 rows of a tile and the tokens its columns, 16
 // at least.  As rows, T tokens would still cost the tensor cores 256 rows: 1 x 128256 x 4096 is bound by reading W, but
@@ -138,8 +140,9 @@ __device__ __forceinline__ int chunk_of(int kblocks) { return EPI == kLse ? kChu
 
 // 64 16-bit values (32 words) of each of a warp's rows from (row0, col) on, `lim` columns wanted: as a tile, or row by
 // row where the result's rows are not aligned.
-__device__ __forceinline__ void store_half_rows(const Args& p, const CUtensorMap* map, unsigned char* buf, int lane, int row0,
-                                                int col, uint16_t* out, int64_t ld, const uint32_t (&w)[32], int lim) {
+__device__ __forceinline__ void store_half_rows(const Args& p, const CUtensorMap* map, unsigned char* buf, int lane,
+                                                int row0, int col, uint16_t* out, int64_t ld, const uint32_t (&w)[32],
+                                                int lim) {
   if (lim <= 0 || row0 >= p.M) return;  // the same for the warp
   chunk_put(buf, lane, w);
   if (p.tile_out)
@@ -201,7 +204,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // the full operand of a stage comes first: what the MMA reads beyond a short A belongs to this kernel's memory
-  const uint32_t stage = (p.a_rows + p.b_rows) * 128, lead_a = FEW ? 0 : p.b_rows * 128, lead_b = FEW ? p.a_rows * 128 : 0;
+  const uint32_t stage = (p.a_rows + p.b_rows) * 128;
+  const uint32_t lead_a = FEW ? 0 : p.b_rows * 128, lead_b = FEW ? p.a_rows * 128 : 0;
   auto s_b = [&](int s) { return ring + s * stage + lead_b; };
   auto s_a = [&](int s) { return ring + s * stage + lead_a; };
 
@@ -474,7 +478,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int c = c0 + 8 * j + 2 * i;
-                w[i] = __byte_perm(distance_bits(fmaf(x[c], kLog2e, -m2)), distance_bits(fmaf(x[c + 1], kLog2e, -m2)), 0x5410);
+                w[i] = __byte_perm(distance_bits(fmaf(x[c], kLog2e, -m2)),
+                                   distance_bits(fmaf(x[c + 1], kLog2e, -m2)), 0x5410);
               }
               chunk_unit(buf, lane, j, make_uint4(w[0], w[1], w[2], w[3]));
             }
@@ -547,9 +552,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-// d of the kept columns, in place of their distances q below the maximum m of their part of the columns (2^shift): g (exp(l - lse) - [v = y]) =
-// g (2^(m - q - lse) - ..); the label's own entry comes from its logit in FP32.  A row to blockIdx.y, eight columns to a
-// thread and step, so that a row's scalars are read once for the columns of a CTA.
+// d of the kept columns, in place of their distances q below the maximum m of their part of the columns (2^shift of
+// them): g (exp(l - lse) - [v = y]) = g (2^(m - q - lse) - ..); the label's own entry comes from its logit in FP32.  A row
+// to blockIdx.y, eight columns to a thread and step, so that a row's scalars are read once for the columns of a CTA.  It
+// moves memory: 4 bytes an entry (511 x 32003: 12 us, 5.4 TB/s).
 __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int64_t ldk, int T, int cols,
                                                    const float2* __restrict__ part, int parts, int shift,
                                                    const float* __restrict__ tgt, const float* __restrict__ lse,
@@ -620,8 +626,10 @@ __global__ void __launch_bounds__(256) k_xent_planes(const float* __restrict__ p
       for (int i = 0; i < W; ++i) a[i] += v[i];
     }
     if constexpr (W == 4) {
-      if (out) *reinterpret_cast<uint2*>(out + row * ldo + c) = make_uint2(pack16(a[0], a[1], f16), pack16(a[2], a[3], f16));
-      else *reinterpret_cast<float4*>(sum + at) = make_float4(a[0], a[1], a[2], a[3]);
+      if (out)
+        *reinterpret_cast<uint2*>(out + row * ldo + c) = make_uint2(pack16(a[0], a[1], f16), pack16(a[2], a[3], f16));
+      else
+        *reinterpret_cast<float4*>(sum + at) = make_float4(a[0], a[1], a[2], a[3]);
     } else {
       if (out) out[row * ldo + c] = (uint16_t)pack16(a[0], 0.f, f16);
       else sum[at] = a[0];
@@ -776,16 +784,17 @@ static int product(const void* A, int64_t lda, const void* B, int64_t ldb, Args 
   if (FEW) {
     // the threads store: a warp's 32 columns of a token are neighbours
   } else if (EPI == kLse) {
-    MPQ_CHECK_ARG(p.keep_cols == 0 || result_map(&mo, p.keep, type, 1, p.M, p.keep_cols, p.ldk),
+    MPQ_CHECK_ARG(p.keep_cols == 0 || result_map(&mo, p.keep, type, 1, p.M, p.keep_cols, p.ldk, true),
                   "mpq_xent_forward: no tensor map for %d kept columns", p.keep_cols);
   } else if (p.acc) {
-    p.tile_out = result_map(&mo, p.acc, 0, p.splits, p.M, p.N, p.N);
+    p.tile_out = result_map(&mo, p.acc, 0, p.splits, p.M, p.N, p.N, false);
   } else {
-    p.tile_out = result_map(&mo, p.out, type, 1, p.M, p.N, p.ldo);
+    p.tile_out = result_map(&mo, p.out, type, 1, p.M, p.N, p.ldo, EPI == kGrad);  // d's rows are workspace
   }
   const size_t smem = 1024 + kRingBytes + kEpiWarps * 4096 + 256;
   const int grid = 2 * std::min(p.mt * p.nt * p.splits, num_sms() / 2);
-  return launch("mpq_xent product", k_xent_gemm<EPI, A_MN, B_MN, FEW>, grid, kThreads, smem, 0, behind, st, ma, mb, mo, p);
+  return launch("mpq_xent product", k_xent_gemm<EPI, A_MN, B_MN, FEW>, grid, kThreads, smem, 0, behind, st, ma, mb, mo,
+                p);
 }
 
 // Width of the piece that starts at column v0.
@@ -825,7 +834,8 @@ MPQ_API int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden,
   MPQ_CHECK_ARG(reduction >= 0 && reduction <= 2 && (reduction == 0 || (loss && count)),
                 "mpq_xent_forward: reduction must be 0 (none), 1 (sum) or 2 (mean); the last two need loss and count");
   MPQ_CHECK_ARG(dtype == 1 || dtype == 2, "mpq_xent_forward: dtype must be 1 (bf16) or 2 (f16)");
-  MPQ_CHECK_ARG(T >= 0 && V >= 1 && H >= 1 && T <= (1 << 24) && V <= (1 << 30), "mpq_xent_forward: bad shape %d x %d x %d", T, V, H);
+  MPQ_CHECK_ARG(T >= 0 && V >= 1 && H >= 1 && T <= (1 << 24) && V <= (1 << 30),
+                "mpq_xent_forward: bad shape %d x %d x %d", T, V, H);
   if (T == 0 && reduction == 0) return MPQ_OK;
   if (T == 0) {
     xent::k_xent_reduce<<<1, 1024, 0, (cudaStream_t)stream>>>(nullptr, nullptr, ignore, 0, reduction == 2, loss, count);
@@ -876,12 +886,14 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
                               int64_t ldk, int keep_cols, float* gmax, void* d, int piece, float* acc, void* dhidden,
                               int64_t lddh, void* dweight, int64_t lddw, int* status, void* stream) {
   MPQ_CHECK_ARG(dtype == 1 || dtype == 2, "mpq_xent_backward: dtype must be 1 (bf16) or 2 (f16)");
-  MPQ_CHECK_ARG(T >= 0 && V >= 1 && H >= 1 && T <= (1 << 24) && V <= (1 << 30), "mpq_xent_backward: bad shape %d x %d x %d", T, V, H);
+  MPQ_CHECK_ARG(T >= 0 && V >= 1 && H >= 1 && T <= (1 << 24) && V <= (1 << 30),
+                "mpq_xent_backward: bad shape %d x %d x %d", T, V, H);
   MPQ_CHECK_ARG(piece >= 256 && piece % 256 == 0, "mpq_xent_backward: the piece must be a multiple of 256 columns");
   MPQ_CHECK_ARG(keep_cols == 0 || keep_cols == V || (keep_cols > 0 && keep_cols < V && keep_cols % 256 == 0),
                 "mpq_xent_backward: keep_cols must be V or a multiple of 256 below it");
   if (T == 0) return MPQ_OK;
-  MPQ_CHECK_ARG(hidden && weight && labels && lse && gout && (gmax || gstride == 0) && status, "mpq_xent_backward: null pointer");
+  MPQ_CHECK_ARG(hidden && weight && labels && lse && gout && (gmax || gstride == 0) && status,
+                "mpq_xent_backward: null pointer");
   MPQ_CHECK_ARG(xent::operand_ok(hidden, ldh, H) && xent::operand_ok(weight, ldw, H),
                 "mpq_xent_backward: operands must be 16-byte aligned with leading dimensions that are multiples of 8");
   MPQ_CHECK_ARG(keep_cols == 0 || (keep && part && tgt && xent::operand_ok(keep, ldk, keep_cols)),
@@ -948,8 +960,8 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
         const bool wide = H % 4 == 0 && lddh % 4 == 0 && (reinterpret_cast<uintptr_t>(acc) & 15) == 0 &&
                           (reinterpret_cast<uintptr_t>(dhidden) & 7) == 0;
         const dim3 grid(wide ? (H / 4 + 255) / 256 : (H + 255) / 256, std::min(T, 65535));
-        st = tc::launch("mpq_xent_backward (planes)", wide ? xent::k_xent_planes<4> : xent::k_xent_planes<1>, grid, 256, 0, 0,
-                        true, cs, (const float*)acc, p.splits, T, H, sum, (int)(v0 > 0), out, lddh, f16);
+        st = tc::launch("mpq_xent_backward (planes)", wide ? xent::k_xent_planes<4> : xent::k_xent_planes<1>, grid, 256,
+                        0, 0, true, cs, (const float*)acc, p.splits, T, H, sum, (int)(v0 > 0), out, lddh, f16);
         if (st) return st;
       }
     }

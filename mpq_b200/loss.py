@@ -5,7 +5,8 @@
 
 The logits (tokens x vocabulary) are not stored: the forward pass reduces them tile by tile inside the product.  The
 backward pass takes the vocabulary in pieces.  It computes a piece's logits again, except for the first columns, which
-the forward pass keeps in 16 bits where a gradient is wanted and ``keep_bytes`` has room: that saves their product.  With ``keep_bytes=0`` nothing of the logits' size outlives a call.
+the forward pass keeps in 16 bits where a gradient is wanted and ``keep_bytes`` has room: that saves their product.
+With ``keep_bytes=0`` nothing of the logits' size outlives a call.
 """
 from __future__ import annotations
 
@@ -111,13 +112,14 @@ class _VocabCrossEntropy(torch.autograd.Function):
         call_on(dev.index, "mpq_xent_backward", t, v, h, _DTYPES[hidden.dtype], x.data_ptr(), x.stride(0), w.data_ptr(),
                 w.stride(0), labels.data_ptr(), ctx.ignore_index, at, gout.data_ptr(), int(each),
                 at + 4 * t if ctx.mean else None, at + 4 * _part_at(t), at + 4 * (t + 1), ptr(keep),
-                0 if keep is None else keep.shape[1], keep_cols, at_acc + 4 * planes * t * h if each else None, ptr(d), piece,
-                at_acc if planes else None, ptr(dh), h, ptr(dw), h, ops.status_word(dev).data_ptr())
+                0 if keep is None else keep.shape[1], keep_cols, at_acc + 4 * planes * t * h if each else None, ptr(d),
+                piece, at_acc if planes else None, ptr(dh), h, ptr(dw), h, ops.status_word(dev).data_ptr())
         return dh, dw, None, None, None, None, None
 
 
 def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, ignore_index: int = -100,
-                        reduction: str = "mean", piece: Optional[int] = None, keep_bytes: int = KEEP_BYTES) -> torch.Tensor:
+                        reduction: str = "mean", piece: Optional[int] = None,
+                        keep_bytes: int = KEEP_BYTES) -> torch.Tensor:
     """Cross entropy of softmax(hidden @ weight.T) at ``labels``, in float32.
 
     ``hidden`` (..., H) and ``weight`` (V, H): bfloat16 or float16; ``labels`` (...): integers.  Labels equal to

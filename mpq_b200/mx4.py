@@ -112,8 +112,8 @@ def dequantize_mx4(q: Mx4Tensor, dtype: torch.dtype = torch.float32) -> torch.Te
         raise ValueError("mpq_b200 kernels require CUDA tensors (there is no CPU path)")
     rows, cols = q.shape
     out = torch.empty(rows, cols, device=q.device, dtype=dtype)
-    call_on(out.device.index, "mpq_mx4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, out.data_ptr(), code,
-            max(cols, 1))
+    call_on(out.device.index, "mpq_mx4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), rows, cols,
+            out.data_ptr(), code, max(cols, 1))
     return out
 
 

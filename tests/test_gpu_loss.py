@@ -237,6 +237,54 @@ def test_shapes_strides_and_types_of_labels(cuda_dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+@pytest.mark.parametrize("t", [5, 130])
+def test_neighbours_of_narrow_operands_are_not_read(cuda_dev, t, dtype):
+    """Rows that end inside 16 bytes, between NaNs: views of wider matrices, taken as they are."""
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(t, 300, 20, dtype, cuda_dev, 5)
+    ref = formulas(x, w, y)
+    wide = [torch.full((r.shape[0], 32), float("nan"), device=cuda_dev, dtype=dtype) for r in (x, w)]
+    for big, part in zip(wide, (x, w)):
+        big[:, :20] = part
+    x, w = (big[:, :20].requires_grad_() for big in wide)
+    loss = vocab_cross_entropy(x, w, y)
+    within(loss, (ref["nll"] * ref["share"]).sum(), (ref["tol"] * ref["share"]).sum() + 1e-6 * ref["nll"].max())
+    dh, dw = torch.autograd.grad(loss, (x, w))
+    within(dh, ref["dh"], ref["tol_h"])
+    within(dw, ref["dw"], ref["tol_w"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,keep_cols", [(5, 0), (130, 0), (130, 300)])
+def test_gradients_into_wider_rows(cuda_dev, t, keep_cols):
+    """The C entries with leading dimensions beyond the columns: what lies between the rows is left alone."""
+    from mpq_b200 import _lib, ops
+    v, h, ld, dtype = 300, 20, 24, torch.bfloat16
+    x, w, y = inputs(t, v, h, dtype, cuda_dev, 6)
+    ref = formulas(x, w, y)
+    xp, wp = (torch.nn.functional.pad(m, (0, ld - h)) for m in (x, w))
+    f32 = lambda *n: torch.zeros(*n, device=cuda_dev)  # noqa: E731
+    lib, status = _lib.load(), ops.status_word(cuda_dev).data_ptr()
+    tiles = lib.mpq_xent_tiles(t, v)
+    part, tgt, lse, nll, loss, count, gmax = f32(2 * t * tiles), f32(t), f32(t), f32(t), f32(1), f32(1), f32(1)
+    keep = torch.zeros(t, 304, device=cuda_dev, dtype=dtype) if keep_cols else None
+    d = torch.zeros(t, 512, device=cuda_dev, dtype=dtype)
+    acc = f32(max(1, lib.mpq_xent_planes(t, v, h, 512, keep_cols)) * t * h)
+    dh, dw = (torch.full((r, ld), 7.0, device=cuda_dev, dtype=dtype) for r in (t, v))
+    _lib.call("mpq_xent_forward", t, v, h, 1, xp.data_ptr(), ld, wp.data_ptr(), ld, y.data_ptr(), -100, part.data_ptr(),
+              part.numel(), tgt.data_ptr(), lse.data_ptr(), nll.data_ptr(), 2, loss.data_ptr(), count.data_ptr(),
+              _lib.ptr(keep), 304, keep_cols, status)
+    gout = torch.ones(1, device=cuda_dev)
+    _lib.call("mpq_xent_backward", t, v, h, 1, xp.data_ptr(), ld, wp.data_ptr(), ld, y.data_ptr(), -100, lse.data_ptr(),
+              gout.data_ptr(), 0, count.data_ptr(), part.data_ptr(), tgt.data_ptr(), _lib.ptr(keep), 304, keep_cols,
+              gmax.data_ptr(), d.data_ptr(), 512, acc.data_ptr(), dh.data_ptr(), ld, dw.data_ptr(), ld, status)
+    within(dh[:, :h], ref["dh"], ref["tol_h"])
+    within(dw[:, :h], ref["dw"], ref["tol_w"])
+    assert (dh[:, h:] == 7.0).all() and (dw[:, h:] == 7.0).all()
+
+
+@pytest.mark.gpu
 def test_streams_and_repeatability(cuda_dev):
     from mpq_b200.loss import vocab_cross_entropy
     x, w, y = inputs(300, 2000, 128, torch.bfloat16, cuda_dev, 11)

@@ -243,6 +243,27 @@ def test_every_code_at_every_place_of_a_block(cuda_dev, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m,n,k", [(1, 40, 70), (2, 129, 300), (300, 1000, 520)])
+def test_product_of_two_stored_matrices(cuda_dev, m, n, k, dtype):
+    """mpq_mx4_gemm against the same product of the values that the two matrices stand for: both operands are exact, so
+    only the FP32 sums (K 2^-23 of the sum of magnitudes, 2^-22 for sums that truncate) and one rounding are off."""
+    from mpq_b200 import _lib, ops
+    from mpq_b200.mx4 import dequantize_mx4, quantize_mx4
+    g = torch.Generator().manual_seed(m + n + k)
+    a, b = (quantize_mx4(torch.randn(r, k, generator=g).to(cuda_dev)) for r in (m, n))
+    out = torch.full((m, n + 3), 7.0, device=cuda_dev, dtype=dtype)
+    _lib.call("mpq_mx4_gemm", m, n, k, a.codes.data_ptr(), a.scales.data_ptr(), b.codes.data_ptr(), b.scales.data_ptr(),
+              None, out.data_ptr(), {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype], n + 3,
+              ops.status_word(cuda_dev).data_ptr())
+    av, bv = dequantize_mx4(a).double(), dequantize_mx4(b).double()
+    want, size = av @ bv.T, av.abs() @ bv.abs().T
+    room = size * k * 2.0 ** -22 + want.abs() * {torch.float32: 0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    assert ((out[:, :n].double() - want).abs() <= room).all()
+    assert (out[:, n:] == 7.0).all()
+
+
+@pytest.mark.gpu
 def test_empty_and_repeatable(cuda_dev):
     from mpq_b200.mx4 import dequantize_mx4, mx4_linear, quantize_mx4
     w = quantize_mx4(values(64, 96, torch.bfloat16, cuda_dev))
