@@ -473,22 +473,40 @@ struct GemmArgs {
 template <class T>
 constexpr int kCols = 128 / sizeof(T);
 
+// 128 bytes of a row, rounded two at a time.
+template <class T>
+__device__ __forceinline__ void pack_row(const float* v, uint32_t (&w)[32]) {
+  #pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __float_as_uint(v[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+}
+
 template <class T>
 __device__ __forceinline__ void store_rows(const GemmArgs& p, const CUtensorMap* map, unsigned char* buf, int lane,
                                            int row0, int col, const float* v) {
   const int lim = p.N - col;
   if (lim <= 0 || row0 >= p.M) return;  // the same for the warp
-  const T* bias = reinterpret_cast<const T*>(p.bias);
-  alignas(16) T o[kCols<T>];
-  #pragma unroll
-  for (int i = 0; i < kCols<T>; ++i) {
-    float f = v[i];
-    if (bias && i < lim) f += to_f32(bias[col + i]);
-    o[i] = from_f32<T>(f);
-  }
   uint32_t w[32];
-  #pragma unroll
-  for (int i = 0; i < 32; ++i) w[i] = reinterpret_cast<const uint32_t*>(o)[i];
+  if (p.bias) {  // a lane's columns, passed around the warp
+    const T* bias = reinterpret_cast<const T*>(p.bias) + col;
+    float own[kCols<T> / 32], f[kCols<T>];
+    #pragma unroll
+    for (int i = 0; i < kCols<T> / 32; ++i) own[i] = lane + 32 * i < lim ? to_f32(bias[lane + 32 * i]) : 0.f;
+    #pragma unroll
+    for (int i = 0; i < kCols<T>; ++i) f[i] = v[i] + __shfl_sync(0xffffffffu, own[i >> 5], i & 31);
+    pack_row<T>(f, w);
+  } else {
+    pack_row<T>(v, w);
+  }
   chunk_put(buf, lane, w);
   if (p.tile_out)
     chunk_send(buf, lane, map, col, row0, 0);
@@ -737,13 +755,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // k_mx4_pair, for many rows of A: a pair of CTAs computes 256 x 256 tiles (tcgen05 cta_group::2, M = N = 256), each CTA
-// loading 128 rows of A and of B a k-block.  A step costs the tensor cores about 128 cycles an MMA, whatever its N, and
-// 57 a scale copy (measured; the two do not overlap), so N is the full 256: 4 MMAs and 6 copies for 256 columns against
-// 8 and 8 for 384.  TMEM holds one accumulator and the scales of 5 stages (24 columns each: 8 of A's 128 rows, 16 of
-// B's 256, the latter in both CTAs); the epilogue takes the accumulator into registers at once, so that the next tile's
-// MMAs wait for the reading only.
+// loading 128 rows of A and of B a k-block.  An MMA takes 128 cycles whatever its N, so N is the full 256.  What bounds
+// the rate is the thread that issues the MMAs: a step's four take it 200 cycles, their commit 95 and a wait 140, out of
+// 512; so the six scale copies of a step are another warp's, which runs up to a ring ahead (in one warp with them a step
+// took 680 to 760 cycles).  TMEM holds one accumulator and the scales of 5 stages (24 columns each: 8 of A's 128 rows,
+// 16 of B's 256, the latter in both CTAs); the epilogue takes the accumulator into registers at once, so that the next
+// tile's MMAs wait for the reading only.  16384 x 4096 x 14336: 380 us, 5.1 PFLOP/s, and 440 under the power limit that
+// a longer run reaches; 300 without the result's stores (a third of the time's power and 470 MB of writes).
 
-constexpr int kPairWarps = 8, kPairThreads = 64 + 32 * kPairWarps, kPairStages = 5, kPairGroup = 8;
+constexpr int kPairWarps = 8, kPairThreads = 96 + 32 * kPairWarps, kPairStages = 5, kPairGroup = 8;
 constexpr int kPM = 256, kPN = 256;
 constexpr uint32_t kPairOps = 2 * kOperand, kPairSf = 3 * kScale;
 constexpr uint32_t kPairCols = 24;  // TMEM columns of a stage's scales, above the accumulator's 256
@@ -760,7 +780,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   uint64_t* empty = full + kPairStages;
   uint64_t* acc_full = empty + kPairStages;
   uint64_t* acc_empty = acc_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  uint64_t* sf_full = acc_empty + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sf_full + kPairStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto s_a = [&](int s) { return ring + s * kPairOps; };
   auto s_b = [&](int s) { return ring + s * kPairOps + kOperand; };
@@ -779,6 +800,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     for (int s = 0; s < kPairStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&sf_full[s], 1);
     }
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 2 * kPairWarps);
@@ -833,56 +855,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   } else if (warp == 1) {
     if (rank == 0) {
       const bool lead = elect_one();
-      const uint64_t da0 = smem_desc_k_sw128(smem_u32(s_a(0))), ds0 = scale_desc(smem_u32(s_sf(0)));
+      const uint64_t da0 = smem_desc_k_sw128(smem_u32(s_a(0)));
       const uint32_t i0 = idesc_mxf4(kPM, kPN, 0), i2 = idesc_mxf4(kPM, kPN, 2);
-      Ring r(kPairStages), c(kPairStages);
-      auto copy = [&]() {  // the next step's scales, as in k_mx4_tile
-        if (!warp_agrees(mbar_wait_cluster(&full[c.s], c.ph) && !*abort_flag)) return false;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t sf = tmem + kPN + c.s * kPairCols;  // A's 2 x 4 columns, then B's 2 x 8
-        const uint64_t ds = desc_add(ds0, c.s * kPairSf);
-        if (lead) {
-          #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            copy_scales<2>(sf + j * 4, desc_add(ds, j * 512));
-            #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              copy_scales<2>(sf + 8 + j * 8 + i * 4, desc_add(ds, kScale * (1 + i) + j * 512));
-          }
-        }
-        __syncwarp();
-        c.next();
-        return true;
-      };
-      int64_t left = (int64_t)((tiles - pair + pairs - 1) / pairs) * nkb;  // steps
-      bool ok = pair >= tiles || copy();
+      Ring r(kPairStages);
+      bool ok = true;
       uint32_t n = 0;  // tiles
       for (int t = pair; t < tiles && ok; t += pairs, ++n) {
-        for (int kb = 0; kb < nkb && ok; ++kb, r.next()) {
-          const uint32_t sf = tmem + kPN + r.s * kPairCols;
-          const uint64_t da = desc_add(da0, r.s * kPairOps), db = desc_add(da, kOperand);
-          const uint32_t add = kb > 0;
-          if (kb == 0) {
-            if (!warp_agrees(mbar_wait_cluster(acc_empty, (n & 1u) ^ 1u))) {
-              ok = false;
-              break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          }
-          if (lead) {  // scales beyond the matrix are zeros, as are its codes
-            #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              mma_mxf4<2>(tmem, desc_add(da, j * 32), desc_add(db, j * 32), j ? i2 : i0, sf, sf + 8, j ? 1u : add);
-          }
-          __syncwarp();
-          if (--left > 0 && !copy()) {
+        if (!warp_agrees(mbar_wait_cluster(acc_empty, (n & 1u) ^ 1u) && !*abort_flag)) {
+          ok = false;
+          break;
+        }
+        for (int kb = 0; kb < nkb; ++kb, r.next()) {
+          if (!warp_agrees(mbar_wait_fast(&sf_full[r.s], r.ph))) {  // the step's operands and scales are in place
             ok = false;
             break;
           }
-          if (lead) {
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t sf = tmem + kPN + r.s * kPairCols;  // A's 2 x 4 columns, then B's 2 x 8
+          const uint64_t da = desc_add(da0, r.s * kPairOps), db = desc_add(da, kOperand);
+          const uint32_t add = kb > 0;
+          if (lead) {  // scales beyond the matrix are zeros, as are its codes
             #pragma unroll
-            for (int j = 2; j < 4; ++j)
-              mma_mxf4<2>(tmem, desc_add(da, j * 32), desc_add(db, j * 32), j & 1 ? i2 : i0, sf + 4, sf + 16, 1u);
+            for (int j = 0; j < 4; ++j)
+              mma_mxf4<2>(tmem, desc_add(da, j * 32), desc_add(db, j * 32), j & 1 ? i2 : i0, sf + (j >> 1) * 4,
+                          sf + 8 + (j >> 1) * 8, j ? 1u : add);
             commit_pair(&empty[r.s]);
             if (kb == nkb - 1) commit_pair(acc_full);
           }
@@ -892,6 +888,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if (!ok && lead) {
         *abort_flag = 1;
         atomicCAS(p.status, 0, 3);
+      }
+    }
+  } else if (warp == 2 + kPairWarps) {
+    if (rank == 0) {
+      const bool lead = elect_one();
+      const uint64_t ds0 = scale_desc(smem_u32(s_sf(0)));
+      Ring c(kPairStages);
+      const int64_t steps = pair < tiles ? (int64_t)((tiles - pair + pairs - 1) / pairs) * nkb : 0;
+      bool ok = true;
+      for (int64_t i = 0; i < steps; ++i, c.next()) {
+        // a stage is filled again once its MMAs are done, which frees its scale columns in TMEM as well
+        if (!warp_agrees(mbar_wait_cluster(&full[c.s], c.ph) && !*abort_flag)) {
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t sf = tmem + kPN + c.s * kPairCols;
+        const uint64_t ds = desc_add(ds0, c.s * kPairSf);
+        if (lead) {
+          #pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            copy_scales<2>(sf + j * 4, desc_add(ds, j * 512));
+            #pragma unroll
+            for (int h = 0; h < 2; ++h)
+              copy_scales<2>(sf + 8 + j * 8 + h * 4, desc_add(ds, kScale * (1 + h) + j * 512));
+          }
+          asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                           smem_u32(&sf_full[c.s]))
+                       : "memory");
+        }
+        __syncwarp();
+      }
+      if (!ok && lead) {
+        *abort_flag = 1;
+        atomicCAS(p.status, 0, 5);
       }
     }
   } else {
