@@ -400,20 +400,21 @@ __global__ void __launch_bounds__(kFewThreads, 3)
 // Two kernels.  k_mx4_tile, for few rows of A: one CTA per SM walks 128 x BN output tiles (BN = 64 or 128: narrow tiles
 // spread few tokens' work over more SMs; a narrower one's scales would start at an odd TMEM column, which is not an
 // address that the MMA takes).  A k-block is one 128-byte swizzle row per operand row = 256 codes, with two 512-byte
-// scale tiles for each operand.  Warp 0 fills a ring of stages by TMA; warp 1's elected thread copies the stage's scales
-// from shared memory to TMEM (tcgen05.cp, replicated to the four lane quadrants) and issues four MMAs of K = 64; warps
-// 2..5 read the FP32 accumulator, add the bias, round once and store.  Two accumulators let the epilogue overlap the
-// next tile.  Scale columns in TMEM belong to the stage, so they are not rewritten before the MMAs that read them are
-// done.
+// scale tiles for each operand.  Warp 0 fills a ring of stages by TMA; warp 6 copies the stages' scales from shared memory
+// to TMEM (tcgen05.cp, replicated to the four lane quadrants); warp 1's elected thread issues four MMAs of K = 64 a
+// stage; warps 2..5 read the FP32 accumulator, add the bias, round once and store.  Two accumulators let the epilogue
+// overlap the next tile.  Scale columns in TMEM belong to the stage, so they are not rewritten before the MMAs that read
+// them are done.
 //
 // With at most 128 rows of A only those are loaded (a tile load takes two to three cycles a 128-byte row; what the
 // others' shared memory holds stays in their rows of the accumulator) and the ring takes the more stages for it.  A
 // cluster of up to four CTAs may share a tile, each with a part of K: they leave their FP32 sums in shared memory, and
 // each adds the parts of its share of the columns, in order.  7 x 14336 x 4096 takes 14 us, of which the tensor cores'
 // steps are 5 and the weights at the memory's rate 5; the rest is the quantisation before it, filling the ring and the
-// sum over the cluster, one after the other.
+// sum over the cluster, one after the other.  (With the scale copies issued by the MMAs' thread a k-block took 740
+// cycles: 8 x 4096 x 14336 13.4 us instead of 11.8.)
 
-constexpr int kThreads = 192;
+constexpr int kThreads = 224;
 constexpr int kBM = 128, kMostStages = 16;
 constexpr uint32_t kTileRing = 204 * 1024;
 constexpr uint32_t kOperand = 128 * 128, kScale = 1024;
@@ -438,6 +439,16 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
   else
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+// What this thread has issued -> one arrival on a barrier of its CTA.
+template <int CTAS>
+__device__ __forceinline__ void commit_one(uint64_t* bar) {
+  if constexpr (CTAS == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
 }
 template <int CTAS>
 __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
@@ -542,7 +553,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* empty = full + kMostStages;
   uint64_t* acc_full = empty + kMostStages;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* sf_full = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sf_full + kMostStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto s_b = [&](int s) { return ring + s * stage; };
   auto s_a = [&](int s) { return ring + s * stage + kOperandB; };
@@ -558,6 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&sf_full[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
@@ -620,13 +633,55 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     const bool lead = elect_one();
     const uint64_t da0 = smem_desc_k_sw128(smem_u32(s_a(0))), db0 = smem_desc_k_sw128(smem_u32(s_b(0)));
-    const uint64_t ds0 = scale_desc(smem_u32(s_sf(0)));
     const uint32_t i0 = idesc_mxf4(kBM, BN, 0), i2 = idesc_mxf4(kBM, BN, 2);
-    Ring r(p.stages), c(p.stages);
-    // Scales of the next step, put in line behind the MMAs in flight: copied right before their own MMAs they would
-    // hold those up (57 cycles a copy).
-    auto copy = [&]() {
-      if (!warp_agrees(mbar_wait_fast(&full[c.s], c.ph) && !*abort_flag)) return false;
+    Ring r(p.stages);
+    bool ok = true;
+    int n = 0;
+    for (int t = first_tile; t < tiles && ok; t += stride, ++n) {
+      const uint32_t acc = tmem + (n & 1) * BN;
+      if (!warp_agrees(mbar_wait_fast(&acc_empty[n & 1], ((uint32_t)(n >> 1) & 1u) ^ 1u) && !*abort_flag)) {
+        ok = false;
+        break;
+      }
+      const uint32_t part = (uint32_t)((t / p.mt) * BN & 127) >> 5;  // the tile's column in its scale tile
+      for (int kb = kb0; kb < kb1; ++kb, r.next()) {
+        if (!warp_agrees(mbar_wait_fast(&sf_full[r.s], r.ph))) {  // the step's operands and scales are in place
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t sf = tmem + kScaleCols + r.s * kStageCols;  // A's 2 x 4 columns, then B's
+        const uint64_t da = desc_add(da0, r.s * stage), db = desc_add(db0, r.s * stage);
+        const uint32_t add = kb > kb0;
+        if (lead) {  // scales beyond the matrix are zeros, as are its codes
+          #pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_mxf4<1>(acc, desc_add(da, j * 32), desc_add(db, j * 32), j & 1 ? i2 : i0, sf + (j >> 1) * 4,
+                        sf + 8 + (j >> 1) * 4 + part, j ? 1u : add);
+          commit_one<1>(&empty[r.s]);
+        }
+        __syncwarp();
+      }
+      // the accumulator is complete (or, after an abort, the issued MMAs have retired)
+      if (lead) commit_one<1>(&acc_full[n & 1]);
+      __syncwarp();
+    }
+    if (!ok && lead) {
+      *abort_flag = 1;
+      atomicCAS(p.status, 0, 3);
+    }
+  } else if (warp == 6) {
+    const bool lead = elect_one();
+    const uint64_t ds0 = scale_desc(smem_u32(s_sf(0)));
+    Ring c(p.stages);
+    const int64_t steps = first_tile < tiles ? (int64_t)((tiles - first_tile + stride - 1) / stride) * (kb1 - kb0) : 0;
+    bool ok = true;
+    for (int64_t i = 0; i < steps; ++i, c.next()) {
+      // a stage is filled again once its MMAs are done, which frees its scale columns in TMEM as well
+      if (!warp_agrees(mbar_wait_fast(&full[c.s], c.ph) && !*abort_flag)) {
+        ok = false;
+        break;
+      }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t sf = tmem + kScaleCols + c.s * kStageCols;
       const uint64_t ds = desc_add(ds0, c.s * 2 * kScale);
@@ -636,56 +691,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           copy_scales<1>(sf + j * 4, desc_add(ds, j * 512));
           copy_scales<1>(sf + 8 + j * 4, desc_add(ds, kScale + j * 512));
         }
+        commit_one<1>(&sf_full[c.s]);
       }
-      __syncwarp();
-      c.next();
-      return true;
-    };
-    int64_t left = (int64_t)((tiles - first_tile + stride - 1) / stride) * (kb1 - kb0);  // steps
-    bool ok = first_tile >= tiles || copy();
-    int n = 0;
-    for (int t = first_tile; t < tiles && ok; t += stride, ++n) {
-      const uint32_t acc = tmem + (n & 1) * BN;
-      if (!warp_agrees(mbar_wait_fast(&acc_empty[n & 1], ((uint32_t)(n >> 1) & 1u) ^ 1u) && !*abort_flag)) {
-        ok = false;
-        break;
-      }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t part = (uint32_t)((t / p.mt) * BN & 127) >> 5;  // the tile's column in its scale tile
-      for (int kb = kb0; kb < kb1; ++kb, r.next()) {
-        const uint32_t sf = tmem + kScaleCols + r.s * kStageCols;
-        const uint64_t da = desc_add(da0, r.s * stage), db = desc_add(db0, r.s * stage);
-        const uint32_t add = kb > kb0;
-        if (lead) {  // scales beyond the matrix are zeros, as are its codes
-          #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            mma_mxf4<1>(acc, desc_add(da, j * 32), desc_add(db, j * 32), j ? i2 : i0, sf, sf + 8 + part, j ? 1u : add);
-        }
-        __syncwarp();
-        if (--left > 0 && !copy()) {
-          ok = false;
-          break;
-        }
-        if (lead) {
-          #pragma unroll
-          for (int j = 2; j < 4; ++j)
-            mma_mxf4<1>(acc, desc_add(da, j * 32), desc_add(db, j * 32), j & 1 ? i2 : i0, sf + 4, sf + 12 + part, 1u);
-          asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                           smem_u32(&empty[r.s]))
-                       : "memory");
-        }
-        __syncwarp();
-      }
-      // the accumulator is complete (or, after an abort, the issued MMAs have retired)
-      if (lead)
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                         smem_u32(&acc_full[n & 1]))
-                     : "memory");
       __syncwarp();
     }
     if (!ok && lead) {
       *abort_flag = 1;
-      atomicCAS(p.status, 0, 3);
+      atomicCAS(p.status, 0, 5);
     }
   } else {
     const int quad = warp & 3;
@@ -723,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (parts > 1) {
     cluster_sync();  // the parts are complete
     const int quad = warp & 3, row = quad * 32 + lane;  // one row tile
-    if (warp >= 2 && quad * 32 < p.M && !*abort_flag) {
+    if (warp >= 2 && warp < 6 && quad * 32 < p.M && !*abort_flag) {
       // each CTA adds the parts of its share of the columns, in order
       #pragma unroll 1
       for (int c0 = rank * kCols<T>; c0 < BN; c0 += parts * kCols<T>) {
@@ -761,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // took 680 to 760 cycles).  TMEM holds one accumulator and the scales of 5 stages (24 columns each: 8 of A's 128 rows,
 // 16 of B's 256, the latter in both CTAs); the epilogue takes the accumulator into registers at once, so that the next
 // tile's MMAs wait for the reading only.  16384 x 4096 x 14336: 380 us, 5.1 PFLOP/s, and 440 under the power limit that
-// a longer run reaches; 300 without the result's stores (a third of the time's power and 470 MB of writes).
+// a longer run reaches; 300 without the result's stores (470 MB).
 
 constexpr int kPairWarps = 8, kPairThreads = 96 + 32 * kPairWarps, kPairStages = 5, kPairGroup = 8;
 constexpr int kPM = 256, kPN = 256;
@@ -914,9 +926,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             for (int h = 0; h < 2; ++h)
               copy_scales<2>(sf + 8 + j * 8 + h * 4, desc_add(ds, kScale * (1 + h) + j * 512));
           }
-          asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                           smem_u32(&sf_full[c.s]))
-                       : "memory");
+          commit_one<2>(&sf_full[c.s]);
         }
         __syncwarp();
       }
@@ -1078,23 +1088,24 @@ static int gemm_pair(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc
                 st, a, b, sa, sb, o, p);
 }
 
-// The kernel with the shortest estimate in cycles, from measured parts: a k-block takes 740 in k_mx4_tile (4 MMAs, 4
-// scale copies, whatever the tile's width) and 860 in k_mx4_pair, the pair's launch 3000 more; a cluster's sum of two
-// parts of K takes 4000, of four 6000.  (us, 512 x 4096 x 4096: 128 columns 13.7, 64 18.7, pair 17.9; 8 x 14336 x 4096:
-// 128 columns in 4 parts 16.3, 2 parts 18.6, whole 26.4.)
+// The kernel with the shortest estimate in cycles, from measured parts: a k-block takes 680 in k_mx4_tile, whatever the
+// tile's width, and 700 in k_mx4_pair; a round of tiles 1000, the pair's launch 3000 more; a cluster's sum of two parts
+// of K 3500, of four 6200, and more for each of its rows.  (us, 512 x 4096 x 4096: 128 columns 11.9, 64 16.9, pair 13.7;
+// 8 x 14336 x 4096: 128 columns in 4 parts 14.5, 2 parts 16.2, whole 24.0; 128 x 4096 x 4096: 64 columns in 2 parts 9.8,
+// whole 10.2, 128 columns in 4 parts 12.6.)
 template <class T>
 static int gemm(const uint8_t* a_codes, const uint8_t* b_codes, const GemmArgs& p, int K, bool behind, cudaStream_t st) {
   const int64_t ldc = 16 * (int64_t)((K + 31) / 32);
   const int sms = num_sms(), nkb = (p.kt + 1) / 2;
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   int bn = 0, parts = 1;  // 0: pairs
-  double least = (double)up(up(p.M, kPM) * up(p.N, kPN), sms / 2) * (nkb * 860.0 + 1000.0) + 3000.0;
+  double least = (double)up(up(p.M, kPM) * up(p.N, kPN), sms / 2) * (nkb * 700.0 + 1000.0) + 3000.0;
   for (int w : {128, 64})
     for (int s : {1, 2, 4}) {
       const int64_t tiles = up(p.M, kBM) * up(p.N, w);
       if (s > 1 && (p.M > kBM || tiles * s > sms || nkb < s)) break;
-      const double join = s > 1 ? 2000.0 + 1000.0 * s : 0.0;
-      const double t = (double)up(tiles, s > 1 ? tiles : sms) * up(nkb, s) * 740.0 + join + w;
+      const double join = s == 1 ? 0.0 : (s == 2 ? 3500.0 + 12.0 * p.M : 6200.0 + 0.4 * w * p.M);
+      const double t = (double)up(tiles, s > 1 ? tiles : sms) * (up(nkb, s) * 680.0 + 1000.0) + join + w;
       if (t < least) {
         least = t;
         bn = w;
@@ -1131,10 +1142,11 @@ static int few_tokens(const void* x, int64_t ldx, int M, int N, int K, const uin
   return launch_status("mpq_mx4_linear (few tokens)");
 }
 
-// x has to fit in shared memory; a second token's arithmetic costs more than k_mx4_tile's start from 40 M weights on
-// (us, few against tile: 4096 x 4096 7.4 and 10.3, 14336 x 4096 15.1 and 13.8; one token 10.0 and 13.8).
+// x has to fit in shared memory; a second token's arithmetic costs more than k_mx4_tile's start from 30 M weights on
+// (us, few against tile: 4096 x 4096 7.6 and 8.5, 14336 x 4096 15.1 and 11.8; one token 9.9 and 11.8, 4096 x 14336 13.2
+// and 14.1).
 static bool takes_few(int M, int N, int K) {
-  return M <= 2 && M * ((K + 31ll) / 32) * 68 <= 200 * 1024 && (M == 1 || (int64_t)N * K <= 40000000);
+  return M <= 2 && M * ((K + 31ll) / 32) * 68 <= 200 * 1024 && (M == 1 || (int64_t)N * K <= 30000000);
 }
 
 template <class T>
