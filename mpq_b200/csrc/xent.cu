@@ -45,7 +45,7 @@ constexpr uint32_t kRingBytes = 192 * 1024;
 constexpr int kMostStages = 11;  // of 16 KB of one operand and 1 KB of the other
 constexpr int kFewScored = 32, kFewGrads = 128;
 constexpr int kChunk = 8;              // k-blocks that the forward pass accumulates before it adds in FP32
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 enum { kLse = 0, kGrad = 1, kOut = 2 };
 
@@ -670,10 +670,12 @@ __global__ void __launch_bounds__(1024) k_xent_join(const float2* __restrict__ p
   for (int i = threadIdx.x + kHeld * blockDim.x; i < nt; i += blockDim.x) s += row[i].y * exp2f(row[i].x - base);
   s = block_sum(s, red);
   if (threadIdx.x == 0) {
-    const float l = (base + log2f(s)) * 0.69314718055994531f;
+    const float l = log2f(s);
     const int64_t y = labels[t];
-    lse[t] = l;
-    nll[t] = y == ignore ? 0.f : (y >= 0 && y < vocab ? l - tgt[t] : __int_as_float(0x7fc00000));
+    const bool inside = y >= 0 && y < vocab;
+    lse[t] = (base + l) * kLn2;
+    // the label's distance below the maximum first: the logits may be far larger than the score
+    nll[t] = y == ignore ? 0.f : (inside ? (fmaf(-tgt[t], kLog2e, base) + l) * kLn2 : __int_as_float(0x7fc00000));
   }
 }
 

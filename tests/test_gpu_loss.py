@@ -211,6 +211,27 @@ def test_large_logits_and_infinities(cuda_dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 40])
+def test_small_scores_of_large_logits(cuda_dev, t):
+    """Scores of 0.05 from logits of 200, which are exact here.  What may be off: 16 roundings of a sum near 1 (2^-24
+    each), and 2e-6 of the score (exponents near -14 rounded at 2^-21, 2^-22 of the exponentials, 1.3e-8 of log2(e))."""
+    from mpq_b200.loss import vocab_cross_entropy
+    v, h = 1000, 64
+    x = torch.zeros(t, h)
+    x[:, 0] = 1.0
+    w = torch.zeros(v, h)
+    w[:, 0] = 189.0 + torch.arange(v) % 3
+    y = torch.arange(t) * 7 + 5
+    x[torch.arange(t), 1 + torch.arange(t)] = 1.0
+    w[y, 1 + torch.arange(t)] = 200.0 - w[y, 0]
+    logits = x.double() @ w.double().T
+    want = torch.logsumexp(logits, 1) - logits[torch.arange(t), y]
+    nll = vocab_cross_entropy(x.to(cuda_dev, torch.bfloat16), w.to(cuda_dev, torch.bfloat16), y.to(cuda_dev),
+                              reduction="none")
+    within(nll, want, 2.0 ** -20 + 2e-6 * want)
+
+
+@pytest.mark.gpu
 def test_shapes_strides_and_types_of_labels(cuda_dev):
     from mpq_b200.loss import vocab_cross_entropy
     x, w, y = inputs(60, 400, 128, torch.bfloat16, cuda_dev, 9)
