@@ -44,7 +44,10 @@ constexpr int kBM = 256, kBN = 256, kGroup = 16;
 constexpr uint32_t kRingBytes = 192 * 1024;
 constexpr int kMostStages = 11;  // of 16 KB of one operand and 1 KB of the other
 constexpr int kFewScored = 32, kFewGrads = 128;
-constexpr int kChunk = 8;              // k-blocks that the forward pass accumulates before it adds in FP32
+// k-blocks that the forward pass accumulates before it adds in FP32.  Over drawn sizes the scores were off by at most
+// 7e-7 of themselves in bf16 at 8; in f16, whose products have more bits to lose, by 1.1e-6 at 8 and 6e-7 at 4 (time of
+// 2047 x 151936 x 1024: 475 us at 8, 520 at 4, 575 at 2).
+constexpr int kChunkBf16 = 8, kChunkF16 = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 enum { kLse = 0, kGrad = 1, kOut = 2 };
@@ -56,6 +59,7 @@ struct Args {
   int a_rows, b_rows;       // rows of A and of B that a CTA loads
   int tile_n;               // columns of a tile (256, or the tokens' 16 .. 128)
   int stages;               // of the ring, each (a_rows + b_rows) x 128 bytes
+  int chunk;                // kLse: k-blocks to an accumulator
   int f16;                  // 1: f16 operands, 0: bf16
   int* status;
   // kLse, kGrad
@@ -134,10 +138,6 @@ __device__ __forceinline__ void unit_at(int u, const Args& p, int kblocks, int& 
   mb = g * kGroup + r - nb * rows;
 }
 
-// k-blocks to an accumulator
-template <int EPI>
-__device__ __forceinline__ int chunk_of(int kblocks) { return EPI == kLse ? kChunk : kblocks; }
-
 // 64 16-bit values (32 words) of each of a warp's rows from (row0, col) on, `lim` columns wanted: as a tile, or row by
 // row where the result's rows are not aligned.
 __device__ __forceinline__ void store_half_rows(const Args& p, const CUtensorMap* map, unsigned char* buf, int lane,
@@ -186,7 +186,7 @@ __device__ __forceinline__ uint32_t distance_bits(float t) {
 // the accumulator.
 //
 // The tensor core's FP32 accumulator truncates, and a score is a small difference of sums of H products; so the
-// forward pass (kLse) accumulates kChunk k-blocks at a time and adds these to nearest in registers.
+// forward pass (kLse) accumulates p.chunk k-blocks at a time and adds these to nearest in registers.
 //
 // FEW: A is the weights' side and B the tokens', one tile of p.tile_n columns; a thread holds a vocabulary row (kLse) or
 // a column of dH (kOut) for half of the tokens.
@@ -285,7 +285,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint64_t da0 = A_MN ? smem_desc_mn_sw128(smem_u32(s_a(0))) : smem_desc_k_sw128(smem_u32(s_a(0)));
       const uint64_t db0 = B_MN ? smem_desc_mn_sw128(smem_u32(s_b(0))) : smem_desc_k_sw128(smem_u32(s_b(0)));
       constexpr uint32_t kStepA = A_MN ? 2048 : 32, kStepB = B_MN ? 2048 : 32;  // K = 16: 16 lines, or 32 bytes of a line
-      const int chunk = chunk_of<EPI>(kblocks);
+      const int chunk = EPI == kLse ? p.chunk : kblocks;
       Ring r(p.stages);
       bool ok = true;
       int n = 0;  // accumulators handed over
@@ -367,7 +367,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         constexpr int kMost = (EPI == kLse ? kFewScored : kFewGrads) / 2;
         float x[kMost];
         bool good = true;
-        const int chunk = chunk_of<EPI>(kblocks);
+        const int chunk = EPI == kLse ? p.chunk : kblocks;
         for (int kc = k0; kc < k1; kc += chunk) {
           if (!(good = take())) break;
           #pragma unroll
@@ -440,7 +440,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         release();
         bool good = true;
         #pragma unroll 1
-        for (int kc = k0 + kChunk; kc < k1; kc += kChunk) {
+        for (int kc = k0 + p.chunk; kc < k1; kc += p.chunk) {
           if (!(good = take())) break;
           #pragma unroll
           for (int c0 = 0; c0 < 128; c0 += 16) {
@@ -775,6 +775,7 @@ static int product(const void* A, int64_t lda, const void* B, int64_t ldb, Args 
   p.tile_n = FEW ? (p.N + 15) / 16 * 16 : kBN;
   p.a_rows = A_MN || FEW ? 128 : std::min((p.M + 7) / 8 * 8, 128);
   p.b_rows = p.tile_n / 2;
+  p.chunk = p.f16 ? kChunkF16 : kChunkBf16;
   p.stages = std::min<int>(kMostStages, kRingBytes / ((p.a_rows + p.b_rows) * 128));
   int r = operand(&ma, A_MN, A, p.M, p.K, lda, p.a_rows, p.f16);
   if (r) return r;
