@@ -23,8 +23,9 @@
 // Few tokens take the narrow side of the products: the weights fill the 256 rows of a tile and the tokens its columns, 16
 // at least.  As rows, T tokens would still cost the tensor cores 256 rows: 1 x 128256 x 4096 is bound by reading W, but
 // drew the full 1000 W doing so, which lowered the clock to 1.1 GHz and W to 4.1 TB/s.  The limits were measured,
-// sustained, at 128256 x 4096 (us, few against many): scores of 32 tokens 203 and 273, of 48 242 and 273, of 64 283 and
-// 254 (each token's maximum and sum cross the lanes then); dH of 64 tokens 202 and 241, of 128 229 and 261.
+// sustained, at 128256 x 4096 (us, few against many): scores of 32 tokens 172 and 224, of 64 185 and 246, of 96 212 and
+// 223 (a step's three products then gain nothing); dH of 64 tokens 197 and 234, of 128 219 and 238, of 192 249 and 258
+// (but a whole step of 190 tokens 903 and 837).
 //
 // A label equal to `ignore` does not count: nll 0, d 0.  A label outside the vocabulary makes the token's nll and its
 // d NaN; no memory is read for it.
@@ -43,7 +44,7 @@ constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
 constexpr int kBM = 256, kBN = 256, kGroup = 16;
 constexpr uint32_t kRingBytes = 192 * 1024;
 constexpr int kMostStages = 11;  // of 16 KB of one operand and 1 KB of the other
-constexpr int kFewScored = 32, kFewGrads = 128;
+constexpr int kFewScored = 64, kFewGrads = 128;
 // k-blocks that the forward pass accumulates before it adds in FP32.  Over drawn sizes the scores were off by at most
 // 7e-7 of themselves in bf16 at 8; in f16, whose products have more bits to lose, by 1.1e-6 at 8 and 6e-7 at 4 (time of
 // 2047 x 151936 x 1024: 475 us at 8, 520 at 4, 575 at 2).

@@ -96,6 +96,25 @@ def test_gradients(cuda_dev, t, v, h, dtype, piece, keep):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("keep", [1 << 31, 0, 100000])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+@pytest.mark.parametrize("t", [16, 17, 32, 33, 48, 63, 64, 65, 96, 129])
+def test_numbers_of_tokens_between_the_forms(cuda_dev, t, dtype, keep):
+    """Token counts at and around those where the products change sides."""
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(t, 1003, 264, dtype, cuda_dev, t)
+    y[0], y[-1] = 1002, 0
+    x.requires_grad_(), w.requires_grad_()
+    ref = formulas(x.detach(), w.detach(), y)
+    within(vocab_cross_entropy(x, w, y, reduction="none"), ref["nll"], ref["tol"])
+    loss = vocab_cross_entropy(x, w, y, keep_bytes=keep)
+    within(loss, (ref["nll"] * ref["share"]).sum(), (ref["tol"] * ref["share"]).sum() + 1e-6 * ref["nll"].max())
+    dh, dw = torch.autograd.grad(loss, (x, w))
+    within(dh, ref["dh"], ref["tol_h"])
+    within(dw, ref["dw"], ref["tol_w"])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(U), ids=str)
 def test_gradients_against_differences(cuda_dev, dtype):
     """Central differences of the 64-bit loss along a direction: eps = 1e-5 leaves 1e-9 of curvature and rounding, so the
