@@ -58,7 +58,7 @@ def _forward(hidden, weight, labels, ignore_index, reduction, keep_bytes):
     x, w = _operand(hidden), _operand(weight)
     tiles = load().mpq_xent_tiles(t, v)
     each = reduction == "none"
-    out = torch.empty((t,) if each else (), device=dev, dtype=torch.float32)
+    out = torch.empty(t, device=dev, dtype=torch.float32) if each else torch.empty((), device=dev, dtype=torch.float32)
     work = torch.empty(_part_at(t) + 2 * t * tiles, device=dev, dtype=torch.float32)
     at, at_out = work.data_ptr(), out.data_ptr()
     keep_cols = _keep(t, v, keep_bytes) if keep_bytes and t else 0

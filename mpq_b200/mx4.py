@@ -97,8 +97,8 @@ def quantize_mx4(x: torch.Tensor) -> Mx4Tensor:
     code = _dtype_code(x.dtype)
     rows, cols = x.shape
     shape_codes, shape_scales = stored_shapes(rows, cols)
-    codes = torch.empty(shape_codes, device=x.device, dtype=torch.uint8)
-    scales = torch.empty(shape_scales, device=x.device, dtype=torch.uint8)
+    codes = torch.empty(*shape_codes, device=x.device, dtype=torch.uint8)
+    scales = torch.empty(*shape_scales, device=x.device, dtype=torch.uint8)
     call_on(x.device.index, "mpq_mx4_quantize", x.data_ptr(), code, max(x.stride(0), cols), rows, cols, codes.data_ptr(),
             scales.data_ptr())
     return Mx4Tensor._checked(codes, scales, (rows, cols))

@@ -345,6 +345,35 @@ def test_streams_and_repeatability(cuda_dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t", [9, 200])
+def test_step_in_a_cuda_graph(cuda_dev, t):
+    """A captured step on new inputs gives what the same step gives outside, bit for bit."""
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(t, 700, 128, torch.bfloat16, cuda_dev, 12)
+    x.requires_grad_(), w.requires_grad_()
+
+    def step():
+        loss = vocab_cross_entropy(x, w, y, piece=256, keep_bytes=2 * 256 * t)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (13, 14):
+        new = inputs(t, 700, 128, torch.bfloat16, cuda_dev, seed)
+        with torch.no_grad():
+            x.copy_(new[0]), w.copy_(new[1]), y.copy_(new[2])
+        graph.replay()
+        got = [r.clone() for r in held]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.gpu
 def test_empty(cuda_dev):
     from mpq_b200.loss import vocab_cross_entropy
     w = torch.randn(30, 16, device=cuda_dev).to(torch.bfloat16).requires_grad_()
