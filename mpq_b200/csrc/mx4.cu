@@ -1122,8 +1122,6 @@ static int few_tokens(const void* x, int64_t ldx, int M, int N, int K, const uin
                       const void* bias, void* out, int64_t ldo, cudaStream_t st) {
   const int nb = (K + 31) / 32, iters = (nb + 31) / 32, groups = (N + kFewRows - 1) / kFewRows;
   const size_t smem = (size_t)TOK * nb * 68;
-  const int r = smem_opt_in((const void*)k_mx4_few<T, TOK>, smem, "mpq_mx4_linear");
-  if (r) return r;
   const bool vec = aligned16(x) && (ldx * (int64_t)sizeof(T)) % 16 == 0;
   const int ctas = num_sms() * (smem <= 70 * 1024 ? 3 : 1);
   // the parts of K with the fewest steps for the busiest warp; a round's sum counts as half of one
@@ -1137,9 +1135,8 @@ static int few_tokens(const void* x, int64_t ldx, int M, int N, int K, const uin
     }
   }
   const int wide = kFewWarps / slices, grid = std::min((groups + wide - 1) / wide, ctas);
-  k_mx4_few<T, TOK><<<grid, kFewThreads, smem, st>>>((const T*)x, ldx, M, N, K, vec, codes, scales, (const T*)bias,
-                                                     (T*)out, ldo, slices);
-  return launch_status("mpq_mx4_linear (few tokens)");
+  return launch("mpq_mx4_linear (few tokens)", k_mx4_few<T, TOK>, grid, kFewThreads, smem, 0, false, st, (const T*)x, ldx, M,
+                N, K, vec, codes, scales, (const T*)bias, (T*)out, ldo, slices);
 }
 
 // x has to fit in shared memory; a second token's arithmetic costs more than k_mx4_tile's start from 30 M weights on

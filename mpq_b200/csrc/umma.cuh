@@ -333,7 +333,7 @@ template <class... P, class... A>
 static int launch(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int cluster, bool behind,
                   cudaStream_t st, A... args) {
   int r = MPQ_OK;
-  if (smem > 48 * 1024 && (r = smem_opt_in((const void*)kernel, smem, what))) return r;
+  if (smem > 40 * 1024 && (r = smem_opt_in((const void*)kernel, smem, what))) return r;  // 48 KB with the static part
   cudaLaunchAttribute at[2];
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;

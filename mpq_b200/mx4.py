@@ -81,11 +81,13 @@ def _rows_of(x: torch.Tensor, what: str) -> torch.Tensor:
     """x as a matrix of rows with unit column stride (a copy only where the strides ask for one)."""
     if not x.is_cuda:
         raise ValueError("mpq_b200 kernels require CUDA tensors (there is no CPU path)")
-    if x.dim() < 1:
+    dims = x.dim()
+    if dims < 1:
         raise ValueError(f"{what} needs at least one dimension")
-    if x.dim() != 2:
+    if dims != 2:
         x = x.reshape(x.numel() // x.shape[-1] if x.shape[-1] else 0, x.shape[-1])
-    if x.numel() and (x.stride(1) != 1 and x.shape[1] != 1 or x.stride(0) < x.shape[1]):
+    cols, (step, unit) = x.shape[1], x.stride()
+    if (unit != 1 and cols != 1 or step < cols) and x.numel():
         x = x.contiguous()
     return x
 

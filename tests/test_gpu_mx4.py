@@ -218,6 +218,23 @@ def test_scales_at_the_ends_of_their_range_in_a_product(cuda_dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,k", [(1, 32 * nb) for nb in (600, 718, 722, 723, 724)] + [(2, 32 * nb) for nb in (301, 361, 362)])
+def test_rows_around_the_default_limit_of_shared_memory(cuda_dev, m, k):
+    """x takes 68 bytes a block and token of shared memory; 48 KB is where a launch has to ask for more."""
+    x = values(m, k, torch.bfloat16, cuda_dev, 8, 0.4)
+    check_linear(x, values(9, k, torch.bfloat16, cuda_dev, 9, 0.4) * 0.05)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m,n,k", [(8, 4096, 4096), (100, 4096, 4096), (128, 2000, 8192), (64, 4100, 1500), (6, 130, 2050)])
+def test_linear_with_a_bias_and_parts_of_k(cuda_dev, m, n, k, dtype):
+    """Shapes whose K a cluster of two or four shares, tiles of 64 and of 128 columns."""
+    x = values(m, k, dtype, cuda_dev, 10, 0.4)
+    check_linear(x, values(n, k, dtype, cuda_dev, 11, 0.4) * 0.05, values(1, n, dtype, cuda_dev, 12, 0.4)[0])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 2, 3, 130])
 def test_every_code_at_every_place_of_a_block(cuda_dev, m):
     """Products with a single element of x: y is the weight itself, exactly, for each of the 16 codes at each of the 96
