@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kFewThreads, 3)
 // each adds the parts of its share of the columns, in order.  7 x 14336 x 4096 takes 14 us, of which the tensor cores'
 // steps are 5 and the weights at the memory's rate 5; the rest is the quantisation before it, filling the ring and the
 // sum over the cluster, one after the other.  (With the scale copies issued by the MMAs' thread a k-block took 740
-// cycles: 8 x 4096 x 14336 13.4 us instead of 11.8.)
+// cycles: 8 x 4096 x 14336 13.4 us instead of 11.8; with x quantised here, by every CTA, 19.6.)
 
 constexpr int kThreads = 224;
 constexpr int kBM = 128, kMostStages = 16;
