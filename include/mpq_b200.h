@@ -478,7 +478,8 @@ int mpq_xent_tiles(int T, int V);
 int mpq_xent_planes(int T, int V, int H, int piece, int keep_cols);
 /* lse[t] = log sum_v exp(h_t . w_v), nll[t] = lse[t] - h_t . w_y (0 where ignored).
  * reduction: 0 none; 1 loss = sum of nll; 2 loss = that over the number of counted labels (NaN for none); count = that
- * number.  Workspaces: part, T x mpq_xent_tiles(T, V) pairs of floats (part_floats: floats it holds); tgt, T floats.
+ * number.  Workspaces: part, T x mpq_xent_tiles(T, V) pairs of floats (part_floats: floats it holds); tgt, T floats
+ * (a copy of nll afterwards, for mpq_xent_backward).
  * keep_cols != 0 (V, or a multiple of 256 below it): keep receives, for mpq_xent_backward, 16-bit distances of those
  * first columns' logits below their tile's largest (T rows, leading dimension ldk). */
 int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,

@@ -3,8 +3,9 @@
 //   l[t, v] = h_t . w_v,   lse_t = log sum_v exp l[t, v],   nll_t = lse_t - l[t, y_t]
 //   d[t, v] = g_t (exp(l[t, v] - lse_t) - [v = y_t]),   dH = d W,   dW = d^T H
 //
-// The forward product reduces each 128 columns of a token's logits to (max, sum of exp) in its epilogue and picks the
-// label's logit out on the way; a second kernel joins them in order.  The logits are not stored.  Where the caller has
+// The forward product reduces each 128 columns of a token's logits to (max, sum of exp) in its epilogue and takes the
+// label's logit out on the way; a second kernel joins them in order, nll = log1p(sum_{v != y} exp(l_v - l_y)), which
+// keeps its digits where the label is nearly certain, and with it d[t, y] = g expm1(-nll).  The logits are not stored.  Where the caller has
 // room for them, the first columns' distances below the largest of their 128 columns are kept for the backward pass, in
 // 16 bits (log2 units, steps of 2^-11: exp(l) within 2^-12.5 of itself down to 2^-32 of the largest; a bf16 exponential
 // would have rounded d a second time by 2^-9).  They save a quarter of a training step's products for two bytes an
@@ -70,7 +71,7 @@ struct Args {
   int v0;                   // first column's vocabulary index
   float2* part;             // kLse: [tokens, parts] (max in log2 units, sum of exp2) of 128 columns each, 32 if few
   int parts;
-  float* tgt;               // kLse: [M] the label's logit
+  float* tgt;               // kLse: [M] the label's logit; kGrad: its score
   uint16_t* keep;           // kLse: distances of the columns below keep_cols (a multiple of 256, or V), [tokens, ldk]
   int64_t ldk;
   int keep_cols;
@@ -391,12 +392,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             float e[4], m2 = 0.f;  // lane i keeps token j + i's maximum
             #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float v = inside ? x[j + i] : -INFINITY, m = warp_max(v), top = m == -INFINITY ? 0.f : m * kLog2e;
-              e[i] = fmaf(v, kLog2e, -top);
-              if (lane == i) m2 = top;
               const int t = t0 + j + i;
-              const int y = __shfl_sync(0xffffffffu, token_label, j + i);
-              if (y == col && t < p.N) p.tgt[t] = v;
+              const bool own = __shfl_sync(0xffffffffu, token_label, j + i) == col;
+              if (own && t < p.N) p.tgt[t] = x[j + i];
+              const float v = inside && !own ? x[j + i] : -INFINITY, m = warp_max(v);
+              const float top = m == -INFINITY ? 0.f : m * kLog2e;
+              e[i] = fmaf(v, kLog2e, -top);
+              if (lane == i) m2 = m == -INFINITY ? m : top;
               if (col < p.keep_cols && t < p.N) p.keep[t * p.ldk + col] = (uint16_t)(distance_bits(e[i]) & 0xffffu);
               e[i] = ex2(e[i]);
             }
@@ -420,7 +422,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const bool live = row < p.M;
       const int n0 = nb * kBN + half * 128;
       int label = -1;  // the label's column among this thread's 128, if it is one of them
-      float g = 0.f, lse2 = 0.f;
+      float g = 0.f, lse2 = 0.f, own_d = 0.f;
       if constexpr (EPI != kOut) {
         if (live) {
           const int64_t y = p.labels[row];
@@ -430,6 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (y != p.ignore) {
               g = factor_of(inside, p.gout, (int64_t)row * p.gstride, p.count, p.gmax, p.f16);
               lse2 = p.lse[row] * kLog2e;
+              own_d = expm1f(-p.tgt[row]);
             }
           }
         }
@@ -461,7 +464,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (__any_sync(0xffffffffu, label >= 0 && label < 128)) {  // few of the warps' tiles hold a label
           float own = 0.f;
           #pragma unroll
-          for (int i = 0; i < 128; ++i) own = label == i ? x[i] : own;
+          for (int i = 0; i < 128; ++i) {
+            own = label == i ? x[i] : own;
+            x[i] = label == i ? -INFINITY : x[i];
+          }
           if (label >= 0 && label < 128) p.tgt[row] = own;
         }
         float m = x[0];
@@ -493,7 +499,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           sum0 += ex2(fmaf(x[i], kLog2e, -m2));
           sum1 += ex2(fmaf(x[i + 1], kLog2e, -m2));
         }
-        if (live) p.part[(int64_t)row * p.parts + 2 * nb + half] = make_float2(lim > 0 ? m2 : -INFINITY, sum0 + sum1);
+        if (live) p.part[(int64_t)row * p.parts + 2 * nb + half] = make_float2(m == -INFINITY ? m : m2, sum0 + sum1);
       } else {
         if (!take()) break;
         float x[128];
@@ -525,8 +531,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 64; i += 2) {
               float a = x[c0 + i], b = x[c0 + i + 1];
               if constexpr (EPI == kGrad) {
-                a = ex2(fmaf(a, kLog2e, -lse2)) - (label == c0 + i ? 1.f : 0.f);
-                b = ex2(fmaf(b, kLog2e, -lse2)) - (label == c0 + i + 1 ? 1.f : 0.f);
+                a = label == c0 + i ? own_d : ex2(fmaf(a, kLog2e, -lse2));
+                b = label == c0 + i + 1 ? own_d : ex2(fmaf(b, kLog2e, -lse2));
                 a = g == 0.f ? 0.f : g * a;
                 b = g == 0.f ? 0.f : g * b;
               } else {
@@ -554,12 +560,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // d of the kept columns, in place of their distances q below the maximum m of their part of the columns (2^shift of
-// them): g (exp(l - lse) - [v = y]) = g (2^(m - q - lse) - ..); the label's own entry comes from its logit in FP32.  A row
+// them): g (exp(l - lse) - [v = y]) = g (2^(m - q - lse) - ..); the label's own entry comes from its score.  A row
 // to blockIdx.y, eight columns to a thread and step, so that a row's scalars are read once for the columns of a CTA.  It
 // moves memory: 4 bytes an entry (511 x 32003: 12 us, 5.4 TB/s).
 __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int64_t ldk, int T, int cols,
                                                    const float2* __restrict__ part, int parts, int shift,
-                                                   const float* __restrict__ tgt, const float* __restrict__ lse,
+                                                   const float* __restrict__ score, const float* __restrict__ lse,
                                                    const int64_t* __restrict__ labels, int64_t ignore, int vocab,
                                                    const float* __restrict__ gout, int gstride,
                                                    const float* __restrict__ count, const float* __restrict__ gmax,
@@ -573,7 +579,7 @@ __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int
     float g = 0.f, own = 0.f;
     if (y != ignore) {
       g = factor_of(inside, gout, (int64_t)row * gstride, count, gmax, f16);
-      if (inside) own = g * (ex2(fmaf(tgt[row], kLog2e, -lse2)) - 1.f);
+      if (inside) own = g * expm1f(-score[row]);
     }
     const int label = inside && y != ignore ? (int)y : -1;
     #pragma unroll 4
@@ -638,11 +644,11 @@ __global__ void __launch_bounds__(256) k_xent_planes(const float* __restrict__ p
   }
 }
 
-// Joins a token's parts: lse = log2-domain maximum and sum -> natural log; one CTA a token, fixed order.  A thread's
-// first kHeld parts stay in registers between the two passes: all of them up to kHeld parts a thread.
+// Joins a token's parts, which leave the label out, with the label's logit: lse and nll; one CTA a token, fixed order.  A
+// thread's first kHeld parts stay in registers between the two passes: all of them up to kHeld parts a thread.
 constexpr int kHeld = 8;
 __global__ void __launch_bounds__(1024) k_xent_join(const float2* __restrict__ part, int ld, int nt,
-                                                    const float* __restrict__ tgt, const int64_t* __restrict__ labels,
+                                                    float* __restrict__ tgt, const int64_t* __restrict__ labels,
                                                     int64_t ignore, int vocab, float* __restrict__ lse,
                                                     float* __restrict__ nll) {
   __shared__ float red[32];
@@ -671,12 +677,20 @@ __global__ void __launch_bounds__(1024) k_xent_join(const float2* __restrict__ p
   for (int i = threadIdx.x + kHeld * blockDim.x; i < nt; i += blockDim.x) s += row[i].y * exp2f(row[i].x - base);
   s = block_sum(s, red);
   if (threadIdx.x == 0) {
-    const float l = log2f(s);
     const int64_t y = labels[t];
     const bool inside = y >= 0 && y < vocab;
-    lse[t] = (base + l) * kLn2;
-    // the label's distance below the maximum first: the logits may be far larger than the score
-    nll[t] = y == ignore ? 0.f : (inside ? (fmaf(-tgt[t], kLog2e, base) + l) * kLn2 : __int_as_float(0x7fc00000));
+    if (y == ignore || !inside) {  // the parts hold every column
+      lse[t] = (base + log2f(s)) * kLn2;
+      nll[t] = tgt[t] = y == ignore ? 0.f : __int_as_float(0x7fc00000);
+    } else {
+      const float l = tgt[t], own = l * kLog2e, all = fmaxf(top, own);
+      const float e = (all + log2f(s * exp2f(top - all) + exp2f(own - all))) * kLn2;
+      const float d = fmaf(-l, kLog2e, top);  // the others' maximum above the label, log2 units
+      lse[t] = e;
+      // beyond 2^64 the label's share of the sum is none
+      const float n = !isfinite(l) ? e - l : (d < 64.f ? log1pf(s * exp2f(d)) : (d + log2f(s)) * kLn2);
+      nll[t] = tgt[t] = n;
+    }
   }
 }
 
@@ -878,7 +892,7 @@ MPQ_API int mpq_xent_forward(int T, int V, int H, int dtype, const void* hidden,
   // threads for a token: kHeld parts each, as far as a CTA goes
   const int threads = live <= 1024 ? 128 : (live <= 2048 ? 256 : (live <= 4096 ? 512 : 1024));
   st = tc::launch("mpq_xent_forward (join)", xent::k_xent_join, T, threads, 0, 0, true, cs, (const float2*)p.part, p.parts,
-                  live, (const float*)tgt, labels, ignore, V, lse, nll);
+                  live, tgt, labels, ignore, V, lse, nll);
   if (st || reduction == 0) return st;
   return tc::launch("mpq_xent_forward (reduce)", xent::k_xent_reduce, 1, 1024, 0, 0, true, cs, (const float*)nll, labels,
                     ignore, T, (int)(reduction == 2), loss, count);
@@ -900,8 +914,8 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
                 "mpq_xent_backward: null pointer");
   MPQ_CHECK_ARG(xent::operand_ok(hidden, ldh, H) && xent::operand_ok(weight, ldw, H),
                 "mpq_xent_backward: operands must be 16-byte aligned with leading dimensions that are multiples of 8");
-  MPQ_CHECK_ARG(keep_cols == 0 || (keep && part && tgt && xent::operand_ok(keep, ldk, keep_cols)),
-                "mpq_xent_backward: the kept columns need their rows, part and tgt");
+  MPQ_CHECK_ARG(tgt && (keep_cols == 0 || (keep && part && xent::operand_ok(keep, ldk, keep_cols))),
+                "mpq_xent_backward: the gradient needs tgt, the kept columns their rows and part");
   MPQ_CHECK_ARG(keep_cols == V || (d && xent::operand_ok(d, piece, 0)), "mpq_xent_backward: a piece needs its workspace");
   MPQ_CHECK_ARG(!dhidden || lddh >= H, "mpq_xent_backward: lddh < H");
   MPQ_CHECK_ARG(!dweight || lddw >= H, "mpq_xent_backward: lddw < H");
@@ -940,6 +954,7 @@ MPQ_API int mpq_xent_backward(int T, int V, int H, int dtype, const void* hidden
       p.M = T; p.N = w; p.K = H;
       p.labels = labels; p.ignore = ignore; p.vocab = V; p.v0 = v0;
       p.lse = lse;
+      p.tgt = const_cast<float*>(tgt);
       p.out = d; p.ldo = piece;
       if ((st = xent::product<xent::kGrad, false, false>(hidden, ldh, W, ldw, p, behind, cs))) return st;
     }

@@ -51,7 +51,8 @@ def _keep(tokens: int, vocab: int, keep_bytes: int) -> int:
 
 def _forward(hidden, weight, labels, ignore_index, reduction, keep_bytes):
     """(result, work, keep, keep_cols) of a checked call.  ``work`` holds, as floats: lse (T), the count of labels, the
-    labels' logits (T), the scores (T, unless they are the result) and, from 8 bytes on, the tiles' partial sums."""
+    scores for the backward pass (T), the scores (T, unless they are the result) and, from 8 bytes on, the tiles' partial
+    sums."""
     t, h = hidden.shape
     v = weight.shape[0]
     dev = hidden.device

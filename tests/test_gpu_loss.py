@@ -251,6 +251,33 @@ def test_small_scores_of_large_logits(cuda_dev, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("keep", [1 << 31, 0])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+@pytest.mark.parametrize("t", [1, 64, 70])
+def test_nearly_certain_labels(cuda_dev, t, dtype, keep):
+    """Scores of 1e-4 and their gradients, from logits that are exact: token t's are column t of the head, its d is
+    column t of the head's gradient.  The score is off by 5e-6 of itself (exponents near -24 rounded at 2^-20, and some
+    rounding of sums), d by one rounding for itself, one for the gradient and 2^-12.5 for a kept distance."""
+    from mpq_b200.loss import vocab_cross_entropy
+    v, h = 1000, 72
+    g = torch.Generator().manual_seed(t)
+    x = torch.eye(t, h, dtype=torch.float64)
+    w = 3.0 + torch.randint(0, 3, (v, h), generator=g).double()
+    y = torch.randint(0, v, (t,), generator=g)
+    w[y, torch.arange(t)] = 20.0
+    logits = x @ w.T
+    rest = torch.exp(logits - 20.0).scatter(1, y[:, None], 0.0)
+    want = torch.log1p(rest.sum(1))
+    d = (rest / (1 + rest.sum(1, keepdim=True))).scatter(1, y[:, None], -(1 - torch.exp(-want))[:, None])
+    xs, ws = x.to(cuda_dev, dtype), w.to(cuda_dev, dtype).requires_grad_()
+    within(vocab_cross_entropy(xs, ws, y.to(cuda_dev), reduction="none"), want, 5e-6 * want)
+    loss = vocab_cross_entropy(xs, ws, y.to(cuda_dev), reduction="sum", keep_bytes=keep)
+    dw, = torch.autograd.grad(loss, ws)
+    u = U[dtype]
+    within(dw[:, :t].T, d, (2 * u + u * u + 2.0 ** -12.4) * d.abs() + (2.0 ** -24 if dtype == torch.float16 else 0))
+
+
+@pytest.mark.gpu
 def test_shapes_strides_and_types_of_labels(cuda_dev):
     from mpq_b200.loss import vocab_cross_entropy
     x, w, y = inputs(60, 400, 128, torch.bfloat16, cuda_dev, 9)
