@@ -148,8 +148,9 @@ __device__ __forceinline__ void split_f16_store(float x, float s, unsigned short
   *reinterpret_cast<__half*>(lo) = __float2half_rn(y - __half2float(h));
 }
 
-// Deterministic block-wide maximum (valid in warp 0); `red` must hold blockDim.x/32 floats.
-__device__ __forceinline__ float block_max(float v, float* red) {
+// Deterministic block-wide maximum (valid in warp 0); `red` must hold blockDim.x/32 floats.  `least`: no value is below it
+// (it fills the lanes that hold no warp's maximum).
+__device__ __forceinline__ float block_max(float v, float* red, float least = 0.f) {
   #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -157,9 +158,9 @@ __device__ __forceinline__ float block_max(float v, float* red) {
   if (lane == 0) red[wid] = v;
   __syncthreads();
   const int nw = (blockDim.x + 31) >> 5;
-  float t = 0.f;
+  float t = least;
   if (wid == 0) {
-    t = lane < nw ? red[lane] : 0.f;
+    t = lane < nw ? red[lane] : least;
     #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
   }

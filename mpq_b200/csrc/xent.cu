@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(1024) k_xent_join(const float2* __restrict__ p
   #pragma unroll
   for (int j = 0; j < kHeld; ++j) m = fmaxf(m, v[j].x);
   for (int i = threadIdx.x + kHeld * blockDim.x; i < nt; i += blockDim.x) m = fmaxf(m, row[i].x);
-  m = block_max(m, red);
+  m = block_max(m, red, -INFINITY);  // logits may all be negative
   if (threadIdx.x == 0) top_s = m;
   __syncthreads();
   const float top = top_s, base = top == -INFINITY ? 0.f : top;

@@ -277,6 +277,62 @@ def test_nearly_certain_labels(cuda_dev, t, dtype, keep):
     within(dw[:, :t].T, d, (2 * u + u * u + 2.0 ** -12.4) * d.abs() + (2.0 ** -24 if dtype == torch.float16 else 0))
 
 
+def exact_logits(t, base, label, v=1000, h=72):
+    """Operands whose logits are `base` everywhere but `label` at each token's own, exactly (the two parts are small whole
+    numbers); column 1 + i of the head's gradient is token i's d."""
+    x, w = torch.zeros(t, h), torch.zeros(v, h)
+    x[:, 0] = 1.0
+    x[torch.arange(t), 1 + torch.arange(t)] = 1.0
+    y = (torch.arange(t) * 7 + 5) % v
+    w[:, 0] = base
+    w[y, 1 + torch.arange(t)] = label - base
+    return x, w, y
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keep", [1 << 31, 0])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+@pytest.mark.parametrize("base,label", [(-60.0, -50.0), (-60.0, -45.0), (-60.0, -70.0), (-110.0, -100.0), (-112.0, -240.0),
+                                        (-1000.0, -990.0), (-1000.0, -1000.0)])
+@pytest.mark.parametrize("t", [1, 40, 64, 70])
+def test_logits_that_are_all_negative(cuda_dev, t, base, label, dtype, keep):
+    """The softmax does not change when all logits are shifted.  A score is off by 5e-6 of itself (as of nearly certain
+    labels).  A d rests on lse in FP32: 2^-22 |lse| of it for two roundings in log2 and ln units, one rounding for itself
+    and one for the gradient, 2^-12.4 where distances are kept, 1e-5 for the exponentials; in f16 d is a multiple of 2^-24
+    of its unit 2^-15 and a gradient of 2^-24."""
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = exact_logits(t, base, label)
+    logits = x.double() @ w.double().T
+    gap = torch.full((t,), base - label).double()
+    want = torch.log1p(999 * torch.exp(gap))
+    p = torch.exp(logits - label - want[:, None])
+    d = p.scatter(1, y[:, None], torch.expm1(-want)[:, None])
+    lse = label + want
+    xs, ws = x.to(cuda_dev, dtype).requires_grad_(), w.to(cuda_dev, dtype).requires_grad_()
+    within(vocab_cross_entropy(xs, ws, y.to(cuda_dev), reduction="none"), want, 5e-6 * want)
+    loss = vocab_cross_entropy(xs, ws, y.to(cuda_dev), reduction="sum", keep_bytes=keep)
+    dh, dw = torch.autograd.grad(loss, (xs, ws))
+    u, f16 = U[dtype], dtype == torch.float16
+    off = (u + 2.0 ** -12.4 + 1e-5 + 2.0 ** -22 * lse.abs()[:, None]) * d.abs() + (2.0 ** -40 if f16 else 0)
+    within(dw[:, 1:1 + t].T, d, (1 + u) * off + u * d.abs() + (2.0 ** -24 if f16 else 0))
+    ref = d @ w.double()
+    within(dh, ref, off @ w.double().abs() + 1e-5 * (d.abs() @ w.double().abs()) + u * ref.abs() + (2.0 ** -24 if f16 else 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 64, 65])
+def test_one_word_of_any_logit(cuda_dev, t):
+    """A vocabulary of one: every score and gradient is 0, whatever the logit."""
+    from mpq_b200.loss import vocab_cross_entropy
+    y = torch.zeros(t, dtype=torch.int64, device=cuda_dev)
+    for size in (-500.0, -10.0, 0.0, 10.0):
+        x = torch.ones(t, 8, device=cuda_dev, dtype=torch.bfloat16).requires_grad_()
+        w = torch.full((1, 8), size, device=cuda_dev, dtype=torch.bfloat16).requires_grad_()
+        nll = vocab_cross_entropy(x, w, y, reduction="none")
+        dh, dw = torch.autograd.grad(nll.sum(), (x, w))
+        assert not nll.any() and not dh.any() and not dw.any()
+
+
 @pytest.mark.gpu
 def test_shapes_strides_and_types_of_labels(cuda_dev):
     from mpq_b200.loss import vocab_cross_entropy
