@@ -167,11 +167,12 @@ __device__ __forceinline__ float warp_max(float v) {
   return __int_as_float(m ^ ((m >> 31) & 0x7fffffff));
 }
 
-// Kept distances: t = log2 units below the maximum (t <= 0), in steps of 1 / kStep.  The sum with 2^23 rounds to a whole
-// number, whose bits end the mantissa.
+// Kept distances: t = log2 units below the maximum, in steps of 1 / kStep.  The sum with 2^23 rounds to a whole number,
+// whose bits end the mantissa.  The maximum was rounded (2^-24 of itself), so its own t may lie above zero by that much:
+// from logits of 2840 on by more than half a step, which would wrap to the largest distance, hence the bound from below.
 constexpr float kStep = 2048.f;
 __device__ __forceinline__ uint32_t distance_bits(float t) {
-  return __float_as_uint(fminf(fmaf(t, -kStep, 8388608.f), 8388608.f + 65535.f));
+  return __float_as_uint(fminf(fmaxf(fmaf(t, -kStep, 8388608.f), 8388608.f), 8388608.f + 65535.f));
 }
 
 // C[M, N] = A B with an epilogue.  A K-major: [M, K] rows; A_MN: [K, M] rows.  B likewise ([N, K] or [K, N] rows).

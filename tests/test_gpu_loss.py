@@ -334,6 +334,36 @@ def test_one_word_of_any_logit(cuda_dev, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("keep", [1 << 31, 0])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+@pytest.mark.parametrize("base", [3008.0, -3008.0, 12032.0, -12032.0])
+@pytest.mark.parametrize("t", [1, 13, 64, 65, 70])
+def test_gradients_of_large_logits(cuda_dev, t, base, dtype, keep):
+    """Logits in the thousands whose largest is not the label's, exactly known: d of the largest column is what matters.
+    Bounds as for logits that are all negative; a kept distance counts from a maximum in log2 units that is off by another
+    2^-24 of itself, which 2^-22 |lse| still covers."""
+    from mpq_b200.loss import vocab_cross_entropy
+    v = 1000
+    x, w, y = exact_logits(t, base, base)
+    i = torch.arange(t)
+    top = 1.0 + i % 13
+    w[y, 1 + i] = top - 2
+    w[(y + 391) % v, 1 + i] = top
+    logits = x.double() @ w.double().T
+    lse = torch.logsumexp(logits, 1)
+    want = lse - logits[i, y]
+    d = torch.exp(logits - lse[:, None]).scatter(1, y[:, None], torch.expm1(-want)[:, None])
+    xs, ws = x.to(cuda_dev, dtype).requires_grad_(), w.to(cuda_dev, dtype).requires_grad_()
+    loss = vocab_cross_entropy(xs, ws, y.to(cuda_dev), reduction="sum", keep_bytes=keep)
+    dh, dw = torch.autograd.grad(loss, (xs, ws))
+    u, f16 = U[dtype], dtype == torch.float16
+    off = (u + 2.0 ** -12.4 + 1e-5 + 2.0 ** -22 * lse.abs()[:, None]) * d.abs() + (2.0 ** -40 if f16 else 0)
+    within(dw[:, 1:1 + t].T, d, (1 + u) * off + u * d.abs() + (2.0 ** -24 if f16 else 0))
+    ref = d @ w.double()
+    within(dh, ref, off @ w.double().abs() + 1e-5 * (d.abs() @ w.double().abs()) + u * ref.abs() + (2.0 ** -24 if f16 else 0))
+
+
+@pytest.mark.gpu
 def test_shapes_strides_and_types_of_labels(cuda_dev):
     from mpq_b200.loss import vocab_cross_entropy
     x, w, y = inputs(60, 400, 128, torch.bfloat16, cuda_dev, 9)
