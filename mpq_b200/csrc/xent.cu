@@ -7,8 +7,8 @@
 // label's logit out on the way; a second kernel joins them in order, nll = log1p(sum_{v != y} exp(l_v - l_y)), which
 // keeps its digits where the label is nearly certain, and with it d[t, y] = g expm1(-nll).  The logits are not stored.  Where the caller has
 // room for them, the first columns' distances below the largest of their 128 columns are kept for the backward pass, in
-// 16 bits (log2 units, steps of 2^-11: exp(l) within 2^-12.5 of itself down to 2^-32 of the largest; a bf16 exponential
-// would have rounded d a second time by 2^-9).  They save a quarter of a training step's products for two bytes an
+// 16 bits (log2 units, steps of 2^-11: exp(l) within 2^-12.5 of itself down to 2^-32 of the largest, nothing below that; a
+// bf16 exponential would have rounded d a second time by 2^-9).  They save a quarter of a training step's products for two bytes an
 // entry.  The backward pass takes the vocabulary in pieces: the kept columns first, then pieces whose logits it computes
 // again, with d in 16 bits as the epilogue's result; it multiplies a piece's d with its rows of W (dH, summed over the
 // pieces in FP32) and with H (dW's rows of the piece).  Every sum runs in a fixed order, so results repeat bit for bit.
@@ -583,6 +583,8 @@ __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int
       if (inside) own = g * expm1f(-score[row]);
     }
     const int label = inside && y != ignore ? (int)y : -1;
+    // log2 units above lse of a column; beyond the distances' range (2^-32 of the part's largest) there is none
+    auto above = [](float up, uint32_t q) { return up + (q == 0xffffu ? -INFINITY : (float)q * (-1.f / kStep)); };
     #pragma unroll 4
     for (int c0 = (blockIdx.x * 256 + threadIdx.x) * 8; c0 < cols; c0 += gridDim.x * 2048) {
       uint4* at = reinterpret_cast<uint4*>(d + row * ldk + c0);
@@ -591,8 +593,8 @@ __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int
       uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
       #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float a = g * ex2(fmaf((float)(w[i] & 0xffffu), -1.f / kStep, up));
-        float b = g * ex2(fmaf((float)(w[i] >> 16), -1.f / kStep, up));
+        float a = g * ex2(above(up, w[i] & 0xffffu));
+        float b = g * ex2(above(up, w[i] >> 16));
         if (label == c0 + 2 * i) a = own;
         if (label == c0 + 2 * i + 1) b = own;
         w[i] = g == 0.f ? 0u : pack16(a, b, f16);

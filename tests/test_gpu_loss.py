@@ -364,6 +364,33 @@ def test_gradients_of_large_logits(cuda_dev, t, base, dtype, keep):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("keep", [1 << 31, 0])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+@pytest.mark.parametrize("t", [1, 64, 65, 130])
+def test_gradients_beside_masked_words(cuda_dev, t, dtype, keep):
+    """Every third word of the head is masked by its type's lowest value (logits at most -3e4, probability 0 in 64 bits):
+    the loss and the gradients are those of the other words alone, and a masked word's gradient is 0."""
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(t, 900, 72, dtype, cuda_dev, 15)
+    y[0] = 1
+    x[:, 0] = 0.5
+    w[:, 0] = 0
+    masked = torch.arange(900, device=cuda_dev) % 3 == 0
+    y = torch.where((y >= 0) & masked[y], y + 1, y)
+    w[masked] = 0
+    w[masked, 0] = torch.finfo(dtype).min
+    at = torch.cumsum(~masked, 0) - 1
+    ref = formulas(x, w[~masked], torch.where(y >= 0, at[y], y))
+    x.requires_grad_(), w.requires_grad_()
+    loss = vocab_cross_entropy(x, w, y, keep_bytes=keep)
+    within(loss, (ref["nll"] * ref["share"]).sum(), (ref["tol"] * ref["share"]).sum() + 1e-6 * ref["nll"].max())
+    dh, dw = torch.autograd.grad(loss, (x, w))
+    within(dh, ref["dh"], ref["tol_h"])
+    within(dw[~masked], ref["dw"], ref["tol_w"])
+    assert not dw[masked].any()
+
+
+@pytest.mark.gpu
 def test_shapes_strides_and_types_of_labels(cuda_dev):
     from mpq_b200.loss import vocab_cross_entropy
     x, w, y = inputs(60, 400, 128, torch.bfloat16, cuda_dev, 9)
