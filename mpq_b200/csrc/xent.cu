@@ -50,7 +50,7 @@ constexpr int kFewScored = 64, kFewGrads = 128;
 // 7e-7 of themselves in bf16 at 8; in f16, whose products have more bits to lose, by 1.1e-6 at 8 and 6e-7 at 4 (time of
 // 2047 x 151936 x 1024: 475 us at 8, 520 at 4, 575 at 2).
 constexpr int kChunkBf16 = 8, kChunkF16 = 4;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 enum { kLse = 0, kGrad = 1, kOut = 2 };
 
@@ -69,7 +69,7 @@ struct Args {
   int64_t ignore;
   int vocab;                // labels in [0, vocab) count
   int v0;                   // first column's vocabulary index
-  float2* part;             // kLse: [tokens, parts] (max in log2 units, sum of exp2) of 128 columns each, 32 if few
+  float2* part;             // kLse: [tokens, parts] (max, sum of exp(l - max)) of 128 columns each, 32 if few
   int parts;
   float* tgt;               // kLse: [M] the label's logit; kGrad: its score
   uint16_t* keep;           // kLse: distances of the columns below keep_cols (a multiple of 256, or V), [tokens, ldk]
@@ -167,12 +167,12 @@ __device__ __forceinline__ float warp_max(float v) {
   return __int_as_float(m ^ ((m >> 31) & 0x7fffffff));
 }
 
-// Kept distances: t = log2 units below the maximum, in steps of 1 / kStep.  The sum with 2^23 rounds to a whole number,
-// whose bits end the mantissa.  The maximum was rounded (2^-24 of itself), so its own t may lie above zero by that much:
-// from logits of 2840 on by more than half a step, which would wrap to the largest distance, hence the bound from below.
+// Kept distances of t = l - max <= 0, in steps of 1 / kStep log2 units.  The sum with 2^23 rounds to a whole number, whose
+// bits end the mantissa.  Maxima stay in the logits' own units: t is exactly 0 for the maximum itself and never above it
+// (the difference to a maximum rounded in log2 units was, by 2^-24 of it), and no logit is too large for log2 units.
 constexpr float kStep = 2048.f;
 __device__ __forceinline__ uint32_t distance_bits(float t) {
-  return __float_as_uint(fminf(fmaxf(fmaf(t, -kStep, 8388608.f), 8388608.f), 8388608.f + 65535.f));
+  return __float_as_uint(fminf(fmaf(t, -kStep * kLog2e, 8388608.f), 8388608.f + 65535.f));
 }
 
 // C[M, N] = A B with an epilogue.  A K-major: [M, K] rows; A_MN: [K, M] rows.  B likewise ([N, K] or [K, N] rows).
@@ -390,22 +390,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           #pragma unroll
           for (int j = 0; j < kMost; j += 4) {
             if (j >= cw || t0 + j >= p.N) break;
-            float e[4], m2 = 0.f;  // lane i keeps token j + i's maximum
+            float e[4], most = 0.f;  // lane i keeps token j + i's maximum
             #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int t = t0 + j + i;
               const bool own = __shfl_sync(0xffffffffu, token_label, j + i) == col;
               if (own && t < p.N) p.tgt[t] = x[j + i];
               const float v = inside && !own ? x[j + i] : -INFINITY, m = warp_max(v);
-              const float top = m == -INFINITY ? 0.f : m * kLog2e;
-              e[i] = fmaf(v, kLog2e, -top);
-              if (lane == i) m2 = m == -INFINITY ? m : top;
+              e[i] = v - (m == -INFINITY ? 0.f : m);
+              if (lane == i) most = m;
               if (col < p.keep_cols && t < p.N) p.keep[t * p.ldk + col] = (uint16_t)(distance_bits(e[i]) & 0xffffu);
-              e[i] = ex2(e[i]);
+              e[i] = ex2(e[i] * kLog2e);
             }
             const float sum = warp_sum4(e, lane);  // lane i: token j + i
             const int t = t0 + j + lane;
-            if (lane < 4 && t < p.N && first < p.M) p.part[(int64_t)t * p.parts + (first >> 5)] = make_float2(m2, sum);
+            if (lane < 4 && t < p.N && first < p.M) p.part[(int64_t)t * p.parts + (first >> 5)] = make_float2(most, sum);
           }
         } else if (inside) {
           #pragma unroll
@@ -423,7 +422,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const bool live = row < p.M;
       const int n0 = nb * kBN + half * 128;
       int label = -1;  // the label's column among this thread's 128, if it is one of them
-      float g = 0.f, lse2 = 0.f, own_d = 0.f;
+      float g = 0.f, lse = 0.f, own_d = 0.f;
       if constexpr (EPI != kOut) {
         if (live) {
           const int64_t y = p.labels[row];
@@ -432,7 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if constexpr (EPI == kGrad) {
             if (y != p.ignore) {
               g = factor_of(inside, p.gout, (int64_t)row * p.gstride, p.count, p.gmax, p.f16);
-              lse2 = p.lse[row] * kLog2e;
+              lse = p.lse[row];
               own_d = expm1f(-p.tgt[row]);
             }
           }
@@ -474,7 +473,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float m = x[0];
         #pragma unroll
         for (int i = 1; i < 128; ++i) m = fmaxf(m, x[i]);
-        const float m2 = m == -INFINITY ? 0.f : m * kLog2e;
+        const float base = m == -INFINITY ? 0.f : m;
         if (n0 < p.keep_cols && row0 < p.M) {
           #pragma unroll
           for (int c0 = 0; c0 < 128; c0 += 64) {
@@ -486,8 +485,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int c = c0 + 8 * j + 2 * i;
-                w[i] = __byte_perm(distance_bits(fmaf(x[c], kLog2e, -m2)),
-                                   distance_bits(fmaf(x[c + 1], kLog2e, -m2)), 0x5410);
+                w[i] = __byte_perm(distance_bits(x[c] - base), distance_bits(x[c + 1] - base), 0x5410);
               }
               chunk_unit(buf, lane, j, make_uint4(w[0], w[1], w[2], w[3]));
             }
@@ -497,10 +495,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float sum0 = 0.f, sum1 = 0.f;
         #pragma unroll
         for (int i = 0; i < 128; i += 2) {
-          sum0 += ex2(fmaf(x[i], kLog2e, -m2));
-          sum1 += ex2(fmaf(x[i + 1], kLog2e, -m2));
+          sum0 += ex2((x[i] - base) * kLog2e);
+          sum1 += ex2((x[i + 1] - base) * kLog2e);
         }
-        if (live) p.part[(int64_t)row * p.parts + 2 * nb + half] = make_float2(m == -INFINITY ? m : m2, sum0 + sum1);
+        if (live) p.part[(int64_t)row * p.parts + 2 * nb + half] = make_float2(m, sum0 + sum1);
       } else {
         if (!take()) break;
         float x[128];
@@ -532,8 +530,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 64; i += 2) {
               float a = x[c0 + i], b = x[c0 + i + 1];
               if constexpr (EPI == kGrad) {
-                a = label == c0 + i ? own_d : ex2(fmaf(a, kLog2e, -lse2));
-                b = label == c0 + i + 1 ? own_d : ex2(fmaf(b, kLog2e, -lse2));
+                a = label == c0 + i ? own_d : ex2((a - lse) * kLog2e);
+                b = label == c0 + i + 1 ? own_d : ex2((b - lse) * kLog2e);
                 a = g == 0.f ? 0.f : g * a;
                 b = g == 0.f ? 0.f : g * b;
               } else {
@@ -561,7 +559,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // d of the kept columns, in place of their distances q below the maximum m of their part of the columns (2^shift of
-// them): g (exp(l - lse) - [v = y]) = g (2^(m - q - lse) - ..); the label's own entry comes from its score.  A row
+// them): g (exp(l - lse) - [v = y]) = g (exp(m - lse) 2^-q - ..); the label's own entry comes from its score.  A row
 // to blockIdx.y, eight columns to a thread and step, so that a row's scalars are read once for the columns of a CTA.  It
 // moves memory: 4 bytes an entry (511 x 32003: 12 us, 5.4 TB/s).
 __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int64_t ldk, int T, int cols,
@@ -576,7 +574,7 @@ __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int
   for (int row = blockIdx.y; row < T; row += gridDim.y) {
     const int64_t y = labels[row];
     const bool inside = y >= 0 && y < vocab;
-    const float lse2 = lse[row] * kLog2e;
+    const float of_all = lse[row];
     float g = 0.f, own = 0.f;
     if (y != ignore) {
       g = factor_of(inside, gout, (int64_t)row * gstride, count, gmax, f16);
@@ -589,7 +587,7 @@ __global__ void __launch_bounds__(256) k_xent_kept(uint16_t* __restrict__ d, int
     for (int c0 = (blockIdx.x * 256 + threadIdx.x) * 8; c0 < cols; c0 += gridDim.x * 2048) {
       uint4* at = reinterpret_cast<uint4*>(d + row * ldk + c0);
       uint4 raw = __ldcs(at);
-      const float up = part[(int64_t)row * parts + (c0 >> shift)].x - lse2;
+      const float up = (part[(int64_t)row * parts + (c0 >> shift)].x - of_all) * kLog2e;
       uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
       #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -676,22 +674,22 @@ __global__ void __launch_bounds__(1024) k_xent_join(const float2* __restrict__ p
   const float top = top_s, base = top == -INFINITY ? 0.f : top;
   float s = 0.f;
   #pragma unroll
-  for (int j = 0; j < kHeld; ++j) s += v[j].y * exp2f(v[j].x - base);
-  for (int i = threadIdx.x + kHeld * blockDim.x; i < nt; i += blockDim.x) s += row[i].y * exp2f(row[i].x - base);
+  for (int j = 0; j < kHeld; ++j) s += v[j].y * expf(v[j].x - base);
+  for (int i = threadIdx.x + kHeld * blockDim.x; i < nt; i += blockDim.x) s += row[i].y * expf(row[i].x - base);
   s = block_sum(s, red);
   if (threadIdx.x == 0) {
     const int64_t y = labels[t];
     const bool inside = y >= 0 && y < vocab;
     if (y == ignore || !inside) {  // the parts hold every column
-      lse[t] = (base + log2f(s)) * kLn2;
+      lse[t] = base + logf(s);
       nll[t] = tgt[t] = y == ignore ? 0.f : __int_as_float(0x7fc00000);
     } else {
-      const float l = tgt[t], own = l * kLog2e, all = fmaxf(top, own);
-      const float e = (all + log2f(s * exp2f(top - all) + exp2f(own - all))) * kLn2;
-      const float d = fmaf(-l, kLog2e, top);  // the others' maximum above the label, log2 units
+      const float l = tgt[t], all = fmaxf(top, l);
+      const float e = all + logf(s * expf(top - all) + expf(l - all));
+      const float d = top - l;  // the others' maximum above the label
       lse[t] = e;
-      // beyond 2^64 the label's share of the sum is none
-      const float n = !isfinite(l) ? e - l : (d < 64.f ? log1pf(s * exp2f(d)) : (d + log2f(s)) * kLn2);
+      // beyond e^44 the label's share of the sum is none
+      const float n = !isfinite(l) ? e - l : (d < 44.f ? log1pf(s * expf(d)) : d + logf(s));
       nll[t] = tgt[t] = n;
     }
   }

@@ -5,6 +5,8 @@ tensor-core products are held to) = delta_t at most for token t; a score is then
 FP32 exponentials and logarithm.  The logits' gradient d is off by 2 delta_t + 1e-5 of p, and by one rounding u (2^-8
 for bf16, 2^-11 for f16) of itself; a product with it adds 1e-5 of the sum of magnitudes and the output's rounding u.
 """
+import math
+
 import pytest
 import torch
 
@@ -388,6 +390,40 @@ def test_gradients_beside_masked_words(cuda_dev, t, dtype, keep):
     within(dh, ref["dh"], ref["tol_h"])
     within(dw[~masked], ref["dw"], ref["tol_w"])
     assert not dw[masked].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keep", [1 << 31, 0])
+@pytest.mark.parametrize("t", [1, 64, 65, 130])
+def test_logits_of_bfloat16s_lowest_value(cuda_dev, t, keep):
+    """Stretches of words whose logits are -3.39e38, further from 0 than FP32 holds in log2 units: scores and gradients are
+    those of the other words; a masked label scores its distance from them; where all words are masked, none is."""
+    from mpq_b200.loss import vocab_cross_entropy
+    low = torch.finfo(torch.bfloat16).min
+    x, w, y = inputs(t, 1000, 72, torch.bfloat16, cuda_dev, 16)
+    y[0] = 1
+    x[:, 0] = 1
+    w[:, 0] = 0
+    masked = torch.zeros(1000, dtype=torch.bool, device=cuda_dev)
+    masked[200:800] = True
+    y = torch.where((y >= 0) & masked[y], y % 200, y)
+    w[masked] = 0
+    w[masked, 0] = low
+    at = torch.cumsum(~masked, 0) - 1
+    ref = formulas(x, w[~masked], torch.where(y >= 0, at[y], y))
+    x.requires_grad_(), w.requires_grad_()
+    loss = vocab_cross_entropy(x, w, y, keep_bytes=keep)
+    within(loss, (ref["nll"] * ref["share"]).sum(), (ref["tol"] * ref["share"]).sum() + 1e-6 * ref["nll"].max())
+    dh, dw = torch.autograd.grad(loss, (x, w))
+    within(dh, ref["dh"], ref["tol_h"])
+    within(dw[~masked], ref["dw"], ref["tol_w"])
+    assert not dw[masked].any()
+    nll = vocab_cross_entropy(x, w, torch.full_like(y, 500), reduction="none")
+    within(nll, torch.full((t,), -low).double(), -1e-6 * low)
+    alone = torch.zeros_like(w)
+    alone[:, 0] = low
+    nll = vocab_cross_entropy(x, alone, torch.full_like(y, 500), reduction="none", keep_bytes=keep)
+    within(nll, torch.full((t,), math.log(1000)).double(), 1e-5)
 
 
 @pytest.mark.gpu
