@@ -79,7 +79,7 @@ struct Args {
   const float* gout;        // kGrad: upstream gradient, gout[t * gstride]
   int gstride;
   const float* count;       // kGrad: divides g where given (the mean's number of labels)
-  const float* gmax;        // kGrad, kOut: largest |g| of the counted tokens; null: all share g
+  const float* gmax;        // kGrad, kOut: largest finite |g| of the counted tokens; null: all share g
   // kGrad, kOut
   void* out;
   int64_t ldo;
@@ -715,7 +715,8 @@ __global__ void __launch_bounds__(1024) k_xent_reduce(const float* __restrict__ 
   }
 }
 
-// gmax = max |g_t| over the tokens that count, g_t = gout[t gstride] (/ count).  One CTA.
+// gmax = max |g_t| over the tokens that count and whose g_t is finite, g_t = gout[t gstride] (/ count): one that is not
+// spoils its own token's gradient only.  One CTA.
 __global__ void __launch_bounds__(1024) k_xent_gmax(const float* __restrict__ gout, int gstride,
                                                     const int64_t* __restrict__ labels, int64_t ignore, int vocab, int T,
                                                     const float* __restrict__ count, float* __restrict__ gmax) {
@@ -724,7 +725,8 @@ __global__ void __launch_bounds__(1024) k_xent_gmax(const float* __restrict__ go
   float m = 0.f;
   for (int t = threadIdx.x; t < T; t += 1024) {
     const int64_t y = labels[t];
-    if (y != ignore && y >= 0 && y < vocab) m = fmaxf(m, fabsf(gout[(int64_t)t * gstride]));
+    const float g = fabsf(gout[(int64_t)t * gstride]);
+    if (y != ignore && y >= 0 && y < vocab && g < INFINITY) m = fmaxf(m, g);
   }
   m = block_max(m, red);
   if (threadIdx.x == 0) *gmax = count && m > 0.f ? m / *count : m;

@@ -427,6 +427,28 @@ def test_logits_of_bfloat16s_lowest_value(cuda_dev, t, keep):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("keep", [1 << 31, 0])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+@pytest.mark.parametrize("t", [5, 70, 140])
+def test_upstream_gradients_that_are_not_finite(cuda_dev, t, dtype, keep):
+    """One token's upstream gradient is infinite or NaN (a loss scaled too far): its own row of dhidden is not finite, the
+    others are what they are without it; also where all other upstream gradients are 0."""
+    from mpq_b200.loss import vocab_cross_entropy
+    x, w, y = inputs(t, 700, 72, dtype, cuda_dev, 17, ignored=0.0)
+    x.requires_grad_()
+    gout = torch.randn(t, generator=torch.Generator().manual_seed(4)).to(cuda_dev)
+    gout[2] = 0
+    ref = formulas(x.detach(), w, y, gout, "none")
+    others = torch.arange(t, device=cuda_dev) != 2
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        for size in (1.0, 0.0):
+            nll = vocab_cross_entropy(x, w, y, reduction="none", keep_bytes=keep)
+            dh = torch.autograd.grad(nll, x, torch.where(others, size * gout, bad))[0]
+            within(dh[others], size * ref["dh"][others.cpu()], ref["tol_h"][others.cpu()])
+            assert not dh[2].isfinite().any()
+
+
+@pytest.mark.gpu
 def test_shapes_strides_and_types_of_labels(cuda_dev):
     from mpq_b200.loss import vocab_cross_entropy
     x, w, y = inputs(60, 400, 128, torch.bfloat16, cuda_dev, 9)
