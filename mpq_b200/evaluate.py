@@ -9,11 +9,14 @@ and the same from the command line, on a registered synthetic shape or a local c
 
     python -m mpq_b200.evaluate --model tiny_llama --sequences 8 --seqlen 512 --tune 20
 
-The output head's logits are not stored: the loss is ``vocab_cross_entropy`` on the hidden states.
+The output head's logits are not stored: the loss is ``vocab_cross_entropy`` on the hidden states.  Decoders whose logits
+are another function of them than hidden @ head.T (a head with a bias; a soft cap or a scale in the configuration) are
+refused.
 """
 from __future__ import annotations
 
 import argparse
+import copy
 import json
 import math
 from typing import Any, Dict, List, Optional
@@ -35,14 +38,56 @@ def _checked_ids(model, ids: torch.Tensor) -> torch.Tensor:
     return ids.to(dev)
 
 
+# What a decoder's configuration says about its logits beyond the head's product, and the values that leave them alone.
+_ON_LOGITS = {"final_logit_softcapping": (None, 0.0), "logit_scale": (None, 1.0), "logits_scaling": (None, 1.0),
+              "lm_head_multiplier": (None, 1.0)}
+
+
+def _checked_head(model) -> torch.Tensor:
+    """The head's weight, where the decoder's logits are hidden @ head.T as far as its head and configuration tell."""
+    head = model.lm_head
+    if head.bias is not None:
+        raise ValueError("the loss is that of hidden @ head.T: a head with a bias is not supported")
+    config = getattr(model, "config", None)
+    for name, neutral in _ON_LOGITS.items():
+        value = getattr(config, name, None)
+        if value not in neutral:
+            raise ValueError(f"the loss is that of hidden @ head.T: a decoder with {name} = {value} is not supported")
+    return head.weight
+
+
+@torch.no_grad()
+def _check_logits(model, ids: torch.Tensor, out) -> None:
+    """Raise where the decoder's own logits of two tokens of ``ids`` are not hidden @ head.T.  ``out``: what its layers gave
+    for ``ids``; they do not run again (the decoder gets the two tokens' hidden states handed back)."""
+    inner, head = model.model, model.lm_head.weight
+    short = copy.copy(out)
+    short.last_hidden_state = out.last_hidden_state[:1, :2]
+    before = inner.__dict__.get("forward")
+    inner.forward = lambda *args, **kwargs: short
+    try:
+        own = model(ids[:1, :2]).logits.float()
+    finally:
+        if before is None:
+            del inner.forward
+        else:
+            inner.forward = before
+    plain = torch.nn.functional.linear(short.last_hidden_state.to(head.dtype), head).float()
+    if own.shape != plain.shape or bool(((own - plain).abs().amax(-1) > 2.0 ** -8 * plain.abs().amax(-1)).any()):
+        raise ValueError(f"{type(model).__name__}'s logits are not hidden @ head.T: its loss is not supported")
+
+
 @torch.no_grad()
 def token_scores(model, ids: torch.Tensor, batch_size: int = 8) -> torch.Tensor:
     """Negative log-likelihood of every token but the first of each sequence: (sequences, tokens - 1) in float32."""
     ids = _checked_ids(model, ids)
-    head = model.lm_head.weight
+    head = _checked_head(model)
     out: List[torch.Tensor] = []
     for part in ids.split(int(batch_size)):
-        hidden = model.model(part[:, :-1]).last_hidden_state.to(head.dtype)
+        states = model.model(part[:, :-1])
+        if not out:
+            _check_logits(model, part[:, :-1], states)
+        hidden = states.last_hidden_state.to(head.dtype)
         out.append(vocab_cross_entropy(hidden, head, part[:, 1:], reduction="none"))
     ops.check_status(ids.device)
     return torch.cat(out)
@@ -57,7 +102,7 @@ def tune_head(model, ids: torch.Tensor, steps: int = 20, lr: float = 1e-3, batch
     """Train the final norm and the output head on ``ids`` (SGD on the mean loss), with the layers as they are; returns
     the loss of each step.  The layers run forward only, so their linears may be in any format."""
     ids = _checked_ids(model, ids)
-    inner, head = model.model, model.lm_head.weight
+    inner, head = model.model, _checked_head(model)
     params = [p for p in (*inner.norm.parameters(), head)]
     wanted = [p.requires_grad for p in params]
     seen: Dict[str, torch.Tensor] = {}
@@ -70,7 +115,9 @@ def tune_head(model, ids: torch.Tensor, steps: int = 20, lr: float = 1e-3, batch
         for step in range(int(steps)):
             part = parts[step % len(parts)]
             with torch.no_grad():
-                inner(part[:, :-1])
+                states = inner(part[:, :-1])
+            if step == 0:
+                _check_logits(model, part[:, :-1], states)
             loss = vocab_cross_entropy(inner.norm(seen["x"]).to(head.dtype), head, part[:, 1:])
             grads = torch.autograd.grad(loss, params)
             with torch.no_grad():

@@ -95,3 +95,77 @@ def test_refuses_ids_without_a_next_token(cuda_dev, decoder):
     for bad in (torch.zeros(3, 1, dtype=torch.long), torch.zeros(5, dtype=torch.long)):
         with pytest.raises(ValueError, match="two tokens"):
             perplexity(model, bad)
+
+
+def small_decoder(family, **changes):
+    """A random decoder of another family on the CPU in float32, with logits of some size."""
+    transformers = pytest.importorskip("transformers")
+    sizes = dict(vocab_size=120, hidden_size=32, intermediate_size=48, num_hidden_layers=1, num_attention_heads=2,
+                 num_key_value_heads=2, max_position_embeddings=64, initializer_range=0.5, pad_token_id=0, bos_token_id=1,
+                 eos_token_id=2)
+    if family in ("Gemma2", "Llama"):
+        sizes["head_dim"] = 16
+    config = getattr(transformers, family + "Config")(**{**sizes, **changes})
+    torch.manual_seed(0)
+    return getattr(transformers, family + "ForCausalLM")(config).eval()
+
+
+@pytest.mark.parametrize("family,changes,plain", [
+    ("Llama", {}, True), ("Llama", {"tie_word_embeddings": True}, True), ("Qwen3", {"head_dim": 16}, True),
+    ("Gemma2", {"final_logit_softcapping": None}, True), ("Granite", {"logits_scaling": 1.0}, True),
+    ("Gemma2", {}, False), ("Granite", {"logits_scaling": 8.0}, False), ("Cohere", {}, False), ("Phi", {}, False)])
+def test_heads_that_are_more_than_a_product_are_refused(family, changes, plain):
+    """By what the head and the configuration say, and by comparing the decoder's own logits; the layers do not run again and
+    the decoder is left as it was."""
+    from mpq_b200.evaluate import _check_logits, _checked_head
+    model = small_decoder(family, **changes)
+    if family == "Phi":
+        torch.nn.init.normal_(model.lm_head.bias)
+    ids = torch.arange(3, 33).view(2, 15)
+    with torch.no_grad():
+        states, logits = model.model(ids), model(ids).logits
+    calls = []
+    hook = model.model.layers[0].register_forward_hook(lambda *a: calls.append(1))
+    if plain:
+        assert _checked_head(model) is model.lm_head.weight
+        _check_logits(model, ids, states)
+    else:
+        with pytest.raises(ValueError, match="hidden @ head.T"):
+            _checked_head(model)
+        with pytest.raises(ValueError, match="hidden @ head.T"):
+            _check_logits(model, ids, states)
+    hook.remove()
+    assert not calls and "forward" not in model.model.__dict__ and states.last_hidden_state.shape[:2] == (2, 15)
+    with torch.no_grad():
+        assert torch.equal(model(ids).logits, logits)
+
+
+def test_logits_changed_in_a_way_that_nothing_tells():
+    from mpq_b200.evaluate import _check_logits, _checked_head
+    model = small_decoder("Llama")
+    ids = torch.arange(3, 33).view(2, 15)
+    with torch.no_grad():
+        states = model.model(ids)
+    _checked_head(model)
+    hook = model.lm_head.register_forward_hook(lambda mod, args, out: 0.9 * out)
+    with pytest.raises(ValueError, match="hidden @ head.T"):
+        _check_logits(model, ids, states)
+    hook.remove()
+    _check_logits(model, ids, states)
+
+
+@pytest.mark.gpu
+def test_scores_of_another_function_are_refused(cuda_dev):
+    from mpq_b200.evaluate import perplexity, token_scores, tune_head
+    model = small_decoder("Gemma2").to(cuda_dev).to(torch.bfloat16)
+    ids = torch.arange(3, 33).view(2, 15)
+    for call in (perplexity, token_scores, tune_head):
+        with pytest.raises(ValueError, match="final_logit_softcapping"):
+            call(model, ids)
+    plain = small_decoder("Gemma2", final_logit_softcapping=None, hidden_size=256).to(cuda_dev).to(torch.bfloat16)
+    with torch.no_grad():
+        logits = plain(ids[:, :-1].to(cuda_dev)).logits.float()
+    want = torch.nn.functional.cross_entropy(logits.flatten(0, 1), ids[:, 1:].flatten().to(cuda_dev), reduction="none")
+    got = token_scores(plain, ids)
+    # the decoder's own logits are rounded to bfloat16: two of them differ by 2^-8 of the largest at most
+    assert float((got.flatten() - want).abs().max()) <= 2.0 ** -8 * 2 * float(logits.abs().max())
