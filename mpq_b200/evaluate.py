@@ -45,7 +45,10 @@ _ON_LOGITS = {"final_logit_softcapping": (None, 0.0), "logit_scale": (None, 1.0)
 
 def _checked_head(model) -> torch.Tensor:
     """The head's weight, where the decoder's logits are hidden @ head.T as far as its head and configuration tell."""
-    head = model.lm_head
+    head = getattr(model, "lm_head", None)
+    if not isinstance(head, torch.nn.Linear):
+        raise ValueError(f"the loss needs the output head as an nn.Linear named lm_head, got {type(head).__name__} (convert "
+                         "the linears of the decoder's layers, model.model, and leave the head as it is)")
     if head.bias is not None:
         raise ValueError("the loss is that of hidden @ head.T: a head with a bias is not supported")
     config = getattr(model, "config", None)

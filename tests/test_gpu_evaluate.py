@@ -169,3 +169,16 @@ def test_scores_of_another_function_are_refused(cuda_dev):
     got = token_scores(plain, ids)
     # the decoder's own logits are rounded to bfloat16: two of them differ by 2^-8 of the largest at most
     assert float((got.flatten() - want).abs().max()) <= 2.0 ** -8 * 2 * float(logits.abs().max())
+
+
+def test_a_head_that_is_no_linear_layer_is_refused():
+    """As it is after converting a whole decoder instead of its layers."""
+    from mpq_b200.evaluate import _checked_head
+    from mpq_b200.mx4 import Mx4Linear, Mx4Tensor
+    model = small_decoder("Llama")
+    codes, scales = torch.zeros(120, 16, dtype=torch.uint8), torch.zeros(1, 1, 512, dtype=torch.uint8)
+    model.lm_head = Mx4Linear(Mx4Tensor(codes, scales, (120, 32)))
+    with pytest.raises(ValueError, match="nn.Linear named lm_head, got Mx4Linear"):
+        _checked_head(model)
+    with pytest.raises(ValueError, match="nn.Linear named lm_head"):
+        _checked_head(torch.nn.Module())
