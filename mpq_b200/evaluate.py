@@ -101,9 +101,10 @@ def perplexity(model, ids: torch.Tensor, batch_size: int = 8) -> float:
     return math.exp(float(token_scores(model, ids, batch_size).double().mean()))
 
 
-def tune_head(model, ids: torch.Tensor, steps: int = 20, lr: float = 1e-3, batch_size: int = 8) -> List[float]:
+def tune_head(model, ids: torch.Tensor, steps: int = 20, lr: float = 1e-2, batch_size: int = 8) -> List[float]:
     """Train the final norm and the output head on ``ids`` (SGD on the mean loss), with the layers as they are; returns
-    the loss of each step.  The layers run forward only, so their linears may be in any format."""
+    the loss of each step.  The layers run forward only, so their linears may be in any format.  The weights are summed up
+    in float32 while the steps run: a step of 16-bit weights by themselves rounds to nothing for most of them."""
     ids = _checked_ids(model, ids)
     inner, head = model.model, _checked_head(model)
     params = [p for p in (*inner.norm.parameters(), head)]
@@ -114,6 +115,7 @@ def tune_head(model, ids: torch.Tensor, steps: int = 20, lr: float = 1e-3, batch
     try:
         for p in params:
             p.requires_grad_(True)
+        sums = [p.detach().float() for p in params]
         parts = ids.split(int(batch_size))
         for step in range(int(steps)):
             part = parts[step % len(parts)]
@@ -124,8 +126,8 @@ def tune_head(model, ids: torch.Tensor, steps: int = 20, lr: float = 1e-3, batch
             loss = vocab_cross_entropy(inner.norm(seen["x"]).to(head.dtype), head, part[:, 1:])
             grads = torch.autograd.grad(loss, params)
             with torch.no_grad():
-                for p, g in zip(params, grads):
-                    p.add_(g.to(p.dtype), alpha=-float(lr))
+                for p, total, g in zip(params, sums, grads):
+                    p.copy_(total.add_(g, alpha=-float(lr)))
             losses.append(loss.detach())
     finally:
         hook.remove()
@@ -145,7 +147,7 @@ def main(argv: Optional[List[str]] = None) -> Dict[str, Any]:
     ap.add_argument("--batch-size", type=int, default=8)
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--tune", type=int, default=0, help="training steps of the final norm and the head afterwards")
-    ap.add_argument("--lr", type=float, default=1e-3)
+    ap.add_argument("--lr", type=float, default=1e-2, help="step size of --tune")
     a = ap.parse_args(argv)
     dev = torch.device("cuda", torch.cuda.current_device())
     model, name = _load_model(a.model, dev, a.seed)

@@ -182,3 +182,20 @@ def test_a_head_that_is_no_linear_layer_is_refused():
         _checked_head(model)
     with pytest.raises(ValueError, match="nn.Linear named lm_head"):
         _checked_head(torch.nn.Module())
+
+
+@pytest.mark.gpu
+def test_tuning_by_its_default_step_moves_the_weights(cuda_dev, decoder):
+    """The first step's gradient promises lr |g|^2 a step; half of that has to arrive over twenty (the loss is convex in the
+    head, its curvature at this step size takes a few per cent, the rounding of the weights to bfloat16 some more)."""
+    from mpq_b200.evaluate import tune_head
+    from mpq_b200.model import calibration_ids
+    model = decoder()
+    ids = calibration_ids(8, 512, 1000, seed=1).to(cuda_dev)
+    with torch.no_grad():
+        hidden = model.model(ids[:, :-1]).last_hidden_state.float()
+        logits = hidden @ model.lm_head.weight.float().T
+        d = torch.softmax(logits, -1) - torch.nn.functional.one_hot(ids[:, 1:], 1000)
+        g = (d.flatten(0, 1).T @ hidden.flatten(0, 1)) / d.shape[:2].numel()
+    losses = tune_head(model, ids)
+    assert len(losses) == 20 and losses[0] - losses[-1] >= 0.5 * 19 * 1e-2 * float(g.square().sum())
