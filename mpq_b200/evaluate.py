@@ -101,12 +101,26 @@ def perplexity(model, ids: torch.Tensor, batch_size: int = 8) -> float:
     return math.exp(float(token_scores(model, ids, batch_size).double().mean()))
 
 
+def _untied_head(model) -> torch.Tensor:
+    """The head's weight, a copy where it was the input embedding's as well."""
+    head = model.lm_head
+    embedding = model.get_input_embeddings()
+    if embedding is not None and embedding.weight.data_ptr() == head.weight.data_ptr():
+        head.weight = torch.nn.Parameter(head.weight.detach().clone(), requires_grad=head.weight.requires_grad)
+        model.config.tie_word_embeddings = False
+    return head.weight
+
+
 def tune_head(model, ids: torch.Tensor, steps: int = 20, lr: float = 1e-2, batch_size: int = 8) -> List[float]:
     """Train the final norm and the output head on ``ids`` (SGD on the mean loss), with the layers as they are; returns
     the loss of each step.  The layers run forward only, so their linears may be in any format.  The weights are summed up
-    in float32 while the steps run: a step of 16-bit weights by themselves rounds to nothing for most of them."""
+    in float32 while the steps run: a step of 16-bit weights by themselves rounds to nothing for most of them.  A head that
+    is tied to the input embedding gets weights of its own first: training the embedding would change the layers' inputs,
+    and by a part of its gradient only."""
     ids = _checked_ids(model, ids)
-    inner, head = model.model, _checked_head(model)
+    inner = model.model
+    _checked_head(model)
+    head = _untied_head(model)
     params = [p for p in (*inner.norm.parameters(), head)]
     wanted = [p.requires_grad for p in params]
     seen: Dict[str, torch.Tensor] = {}

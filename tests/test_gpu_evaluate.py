@@ -199,3 +199,25 @@ def test_tuning_by_its_default_step_moves_the_weights(cuda_dev, decoder):
         g = (d.flatten(0, 1).T @ hidden.flatten(0, 1)) / d.shape[:2].numel()
     losses = tune_head(model, ids)
     assert len(losses) == 20 and losses[0] - losses[-1] >= 0.5 * 19 * 1e-2 * float(g.square().sum())
+
+
+def test_untying_a_head():
+    from mpq_b200.evaluate import _untied_head
+    tied = small_decoder("Llama", tie_word_embeddings=True)
+    before = tied.lm_head.weight
+    head = _untied_head(tied)
+    assert head is tied.lm_head.weight and head is not before and torch.equal(head, before)
+    assert tied.get_input_embeddings().weight is before and not tied.config.tie_word_embeddings
+    assert _untied_head(tied) is head
+
+
+@pytest.mark.gpu
+def test_tuning_a_tied_head_leaves_the_embedding(cuda_dev):
+    from mpq_b200.evaluate import tune_head
+    model = small_decoder("Llama", tie_word_embeddings=True, hidden_size=64).to(cuda_dev).to(torch.bfloat16)
+    embedding = model.get_input_embeddings().weight
+    assert embedding is model.lm_head.weight
+    before = embedding.detach().clone()
+    losses = tune_head(model, torch.arange(3, 33).view(2, 15), steps=5, lr=0.1)
+    assert losses[-1] < losses[0]
+    assert torch.equal(model.get_input_embeddings().weight, before) and not torch.equal(model.lm_head.weight, before)
