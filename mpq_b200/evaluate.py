@@ -35,7 +35,15 @@ def _checked_ids(model, ids: torch.Tensor) -> torch.Tensor:
     ids = torch.as_tensor(ids, dtype=torch.long)
     if ids.dim() != 2 or ids.shape[1] < 2:
         raise ValueError("ids must be (sequences, tokens) with two tokens at least")
+    _check_range(ids, model.get_input_embeddings().weight.shape[0])
     return ids.to(dev)
+
+
+def _check_range(ids: torch.Tensor, words: int) -> None:
+    """Looking up an id that the embedding does not hold would be a device-side failure, which ends the process's GPU
+    context."""
+    if ids.numel() and not (0 <= int(ids.min()) and int(ids.max()) < words):
+        raise ValueError(f"ids must be in [0, {words}), got {int(ids.min())} to {int(ids.max())}")
 
 
 # What a decoder's configuration says about its logits beyond the head's product, and the values that leave them alone.

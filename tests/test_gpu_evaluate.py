@@ -221,3 +221,24 @@ def test_tuning_a_tied_head_leaves_the_embedding(cuda_dev):
     losses = tune_head(model, torch.arange(3, 33).view(2, 15), steps=5, lr=0.1)
     assert losses[-1] < losses[0]
     assert torch.equal(model.get_input_embeddings().weight, before) and not torch.equal(model.lm_head.weight, before)
+
+
+def test_range_of_ids():
+    from mpq_b200.evaluate import _check_range
+    _check_range(torch.tensor([[0, 119], [3, 4]]), 120)
+    _check_range(torch.zeros(0, 4, dtype=torch.long), 120)
+    for bad in (120, -1, -100, 2 ** 40):
+        with pytest.raises(ValueError, match="ids must be in"):
+            _check_range(torch.tensor([[0, 1], [bad, 2]]), 120)
+
+
+@pytest.mark.gpu
+def test_refuses_ids_outside_the_vocabulary(cuda_dev, decoder):
+    from mpq_b200.evaluate import perplexity, token_scores, tune_head
+    model = decoder()
+    for bad in (1000, -100):
+        for ids in (torch.tensor([[1, 2, bad]]), torch.tensor([[1, bad, 2]], device=cuda_dev)):
+            for call in (perplexity, token_scores, tune_head):
+                with pytest.raises(ValueError, match="ids must be in"):
+                    call(model, ids)
+    assert token_scores(model, torch.tensor([[0, 999]])).shape == (1, 1)
