@@ -8,7 +8,8 @@ next to the solved formats of this package as the round-to-nearest baseline at 4
     y = mx4_linear(x, w4, layer.bias)       # x is quantised within the call, token by token
     convert_linears_mx4(model.model)        # every nn.Linear below, in place
 
-The operators run forward only; tensors must be on the GPU (there is no CPU path).
+The operators run forward only: a backward pass through a linear raises.  Tensors must be on the GPU (there is no CPU
+path).
 """
 from __future__ import annotations
 
@@ -119,9 +120,27 @@ def dequantize_mx4(q: Mx4Tensor, dtype: torch.dtype = torch.float32) -> torch.Te
     return out
 
 
+class _ForwardOnly(torch.autograd.Function):
+    """Ties a result to the inputs whose gradient it does not have: a backward pass that needs it raises, where a detached
+    result would leave their gradients short of its part."""
+
+    @staticmethod
+    def forward(ctx, out, *inputs):
+        ctx.mark_dirty(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("mx4_linear runs forward only: it has no gradients for x or the bias (freeze what lies below the "
+                           "4-bit linears, or run them under torch.no_grad())")
+
+
 def mx4_linear(x: torch.Tensor, weight: Mx4Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = Q(x) W^T + b for x (..., K) and a quantised W (N x K): x is quantised row by row, the products accumulate in
-    FP32, and y (x's dtype) is rounded once."""
+    FP32, and y (x's dtype) is rounded once.  Forward only: a backward pass that needs the gradient of x or of the bias
+    raises."""
+    tied = torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad)
+    given = (x, bias)
     rows = _rows_of(x, "mx4_linear")
     code = _dtype_code(x.dtype)
     n, k = weight.shape
@@ -144,11 +163,13 @@ def mx4_linear(x: torch.Tensor, weight: Mx4Tensor, bias: Optional[torch.Tensor] 
             call_on(x.device.index, "mpq_mx4_linear", rows.data_ptr(), code, max(rows.stride(0), k), m, n, k,
                     weight.codes.data_ptr(), weight.scales.data_ptr(), ptr(bias), ptr(work), out.data_ptr(), n,
                     ops.status_word(x.device).data_ptr())
-    return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
+    if x.dim() != 2:
+        out = out.view(*x.shape[:-1], n)
+    return _ForwardOnly.apply(out, *given) if tied else out
 
 
 class Mx4Linear(torch.nn.Module):
-    """A linear layer with its weight in MX4 (forward only)."""
+    """A linear layer with its weight in MX4 (forward only: see ``mx4_linear``)."""
 
     def __init__(self, weight: Mx4Tensor, bias: Optional[torch.Tensor] = None):
         super().__init__()

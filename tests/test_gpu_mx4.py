@@ -331,6 +331,34 @@ def test_product_in_a_cuda_graph(cuda_dev):
         assert torch.equal(y, mx4_linear(x, w))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 64), (5, 64), (300, 64), (2, 3, 64)])
+def test_a_backward_pass_raises(cuda_dev, shape):
+    """A linear in 4 bits has no gradient: through a skip connection, for x or the bias alone, or below other layers; what
+    lies above it trains, and the forward pass is what it is without gradients."""
+    from mpq_b200.mx4 import Mx4Linear, mx4_linear, quantize_mx4
+    w = quantize_mx4(values(64, 64, torch.float32, cuda_dev, 1, 0.3))
+    x, bias = torch.randn(*shape, device=cuda_dev), torch.randn(64, device=cuda_dev)
+    want = mx4_linear(x, w, bias)
+    assert not want.requires_grad
+    for x_grad, bias_grad in ((True, False), (False, True), (True, True)):
+        xs, bs = x.clone().requires_grad_(x_grad), bias.clone().requires_grad_(bias_grad)
+        with torch.no_grad():
+            assert not mx4_linear(xs, w, bs).requires_grad
+        y = mx4_linear(xs, w, bs)
+        assert y.requires_grad and torch.equal(y, want)
+        y += x  # in place, as a residual stream may do
+        with pytest.raises(RuntimeError, match="forward only"):
+            (xs + y).sum().backward()
+        assert xs.grad is None and bs.grad is None
+    layer = Mx4Linear(w, bias)
+    with pytest.raises(RuntimeError, match="forward only"):
+        layer(x.clone().requires_grad_()).sum().backward()
+    above = torch.nn.Linear(64, 3, device=cuda_dev)
+    above(layer(x)).sum().backward()
+    assert above.weight.grad is not None
+
+
 def test_refusals_without_a_gpu():
     from mpq_b200 import _lib
     from mpq_b200.mx4 import Mx4Tensor, dequantize_mx4, mx4_linear, quantize_mx4
