@@ -245,6 +245,10 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restric
 // 1/4 up to 36, and the eight that a half of an accumulator adds stay below 2^11 quarters; a block's four sums are
 // added in FP32 and scaled by 2^(cx + cw - 254) once.  1 x 4096 x 14336 takes 9.9 us, 3.2 TB/s (13.0 with a shift and a
 // mask to every conversion; 14.1 with byte permutations and dp4a, twice the instructions).
+// The scales apply one after the other, W's first: their product may lie outside FP32 where the result does not (x
+// holding its type's lowest value, and a 0 in W for it).  So that no step overflows by itself, x's f16 values carry 2^-10
+// of its block's scale: a sum is then at most 1.125, times 2^127 at most.  Where x's scale has no room for the 2^10 in
+// return, its values keep as much more, and what overflows is the result.
 // Every CTA quantises x for itself into shared memory (f16 values in four planes of 16 bytes a block, so that a warp's
 // reads are free of conflicts) while its first weights are on their way.  A warp takes kFewRows rows of W and one of
 // `slices` parts of K (so that all warps have work whatever N is), a lane every 32nd block; the next blocks are loaded
@@ -310,9 +314,13 @@ __global__ void __launch_bounds__(kFewThreads, 3)
     for (int j = 0; j < 8; ++j) v[j] = v[j] * inv;
     __half2 h[4];
     decode8(encode8(v), h);
+    const uint32_t kept = c > 244 ? min(c - 244, 10u) : 0;  // the values take 2^(kept - 10) of the scale, a normal number
+    const __half2 part = __half2half2(__ushort_as_half((unsigned short)((kept + 5) << 10)));
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __hmul2(h[j], part);
     if (block < nb) {
       xb[((size_t)t * 4 + (q & 3)) * nb + block] = *reinterpret_cast<const uint4*>(h);
-      if ((q & 3) == 0) xs[t * nb + block] = scale_value(c);
+      if ((q & 3) == 0) xs[t * nb + block] = c == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((c + 10 - kept) << 23);
     }
   }
   __syncthreads();
@@ -362,7 +370,7 @@ __global__ void __launch_bounds__(kFewThreads, 3)
           #pragma unroll
           for (int r = 0; r < kFewRows; ++r) {
             const float2 f = __half22float2(lo[t][r]), g = __half22float2(hi[t][r]);
-            acc[t][r] = fmaf((f.x + f.y) + (g.x + g.y), sw[r] * s, acc[t][r]);
+            acc[t][r] = fmaf(((f.x + f.y) + (g.x + g.y)) * sw[r], s, acc[t][r]);
           }
         }
       }

@@ -218,6 +218,41 @@ def test_scales_at_the_ends_of_their_range_in_a_product(cuda_dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2, 3, 130])
+def test_scales_whose_product_leaves_the_range(cuda_dev, m):
+    """Finite results of scales whose product is beyond FP32: a 0 in the weights where x holds its type's lowest value, sums
+    of a quarter, and weights near the largest value against small inputs."""
+    low = torch.finfo(torch.bfloat16).min
+    x = values(m, 160, torch.float32, cuda_dev, 11, 0.3)
+    x[::2, 5] = low
+    w = 40 * values(50, 160, torch.float32, cuda_dev, 12, 0.3)
+    w[:, 5] = 0
+    check_linear(x, w)
+    check_linear(x.bfloat16(), w.bfloat16())
+    x[:, :32], w[:, :32] = 0, 0
+    x[:, 0], x[:, 1] = 2.0 ** 127, 2.0 ** 124
+    w[:, 1], w[:, 2] = 4.0, 32.0
+    w[:, 32:] = 0
+    check_linear(x, w)  # (1/2 2^125) (1/2 2^3) = 2^126
+    for big, small in ((126, -100), (122, -126), (118, 0), (0, 118), (-100, 126)):
+        a = values(m, 160, torch.float32, cuda_dev, 13, 0.1).clamp(-2, 2) * 2.0 ** small
+        b = values(50, 160, torch.float32, cuda_dev, 14, 0.1).clamp(-2, 2) * 2.0 ** big
+        check_linear(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2])
+def test_results_below_the_normal_range(cuda_dev, m):
+    """Few tokens: block sums are exact down to FP32's smallest number, so a result is off by 2^-149 a block and lane."""
+    from mpq_b200.mx4 import mx4_linear, quantize_mx4
+    a = values(m, 160, torch.float32, cuda_dev, 15, 0.3) * 2.0 ** -70
+    b = values(50, 160, torch.float32, cuda_dev, 16, 0.3) * 2.0 ** -60
+    want = plain_values(*plain_quantize(a)) @ plain_values(*plain_quantize(b)).T
+    err = (mx4_linear(a, quantize_mx4(b)).cpu().double() - want).abs()
+    assert bool((err <= 2.0 ** -149 * 10).all()) and bool(want.abs().min() > 0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m,k", [(1, 32 * nb) for nb in (600, 718, 722, 723, 724)] + [(2, 32 * nb) for nb in (301, 361, 362)])
 def test_rows_around_the_default_limit_of_shared_memory(cuda_dev, m, k):
     """x takes 68 bytes a block and token of shared memory; 48 KB is where a launch has to ask for more."""
