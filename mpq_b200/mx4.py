@@ -13,6 +13,7 @@ path).
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -86,7 +87,7 @@ def _rows_of(x: torch.Tensor, what: str) -> torch.Tensor:
     if dims < 1:
         raise ValueError(f"{what} needs at least one dimension")
     if dims != 2:
-        x = x.reshape(x.numel() // x.shape[-1] if x.shape[-1] else 0, x.shape[-1])
+        x = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
     cols, (step, unit) = x.shape[1], x.stride()
     if (unit != 1 and cols != 1 or step < cols) and x.numel():
         x = x.contiguous()

@@ -332,6 +332,19 @@ def test_empty_and_repeatable(cuda_dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(0,), (4, 0), (2, 3, 0), (2, 0, 0), (0, 3, 0)])
+def test_linear_over_no_columns(cuda_dev, shape):
+    """Sums over nothing, for every token there is: the bias alone, or zeros."""
+    from mpq_b200.mx4 import dequantize_mx4, mx4_linear, quantize_mx4
+    none = quantize_mx4(torch.zeros(5, 0, device=cuda_dev))
+    bias = torch.arange(5.0, device=cuda_dev)
+    x = torch.zeros(shape, device=cuda_dev)
+    assert torch.equal(mx4_linear(x, none), torch.zeros(*shape[:-1], 5, device=cuda_dev))
+    assert torch.equal(mx4_linear(x, none, bias), bias.expand(*shape[:-1], 5))
+    assert dequantize_mx4(quantize_mx4(x)).shape == (math.prod(shape[:-1]), 0)
+
+
+@pytest.mark.gpu
 def test_another_stream_and_layers(cuda_dev):
     """Work queued on a stream of its own, and the module form against the function."""
     from mpq_b200.mx4 import Mx4Linear, convert_linears_mx4, mx4_linear, quantize_mx4
