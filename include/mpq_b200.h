@@ -444,7 +444,9 @@ int mpq_pack_bits(const uint8_t* src, int64_t sp, int64_t so, int n_pack, int n_
  * dtype: 0 float32, 1 bfloat16, 2 float16.  Stored form of a rows x cols matrix, with nb = ceil(cols / 32) blocks a
  * row: codes rows x 16 nb bytes (column 2j in the low half of byte j; sign, two exponent bits, one mantissa bit);
  * scales [ceil(rows / 128)][ceil(nb / 4)][512] bytes, (row, block) at byte (row % 32) 16 + (row % 128 / 32) 4 +
- * block % 4 of its tile.  Both 16-byte aligned.  A block stands for code 2^(scale - 127); scale 255 is NaN. */
+ * block % 4 of its tile.  Both 16-byte aligned.  A block stands for code 2^(scale - 127); scale 255 is NaN.  What pads a
+ * row is 0: the codes of columns beyond cols in its last block, and the scales of blocks beyond nb in their tile (products
+ * read both). */
 
 /* Block scale max(E - 2, 0) with E the biased exponent of the largest magnitude (255 where the block is not finite),
  * elements to nearest even, saturating at 6 scales.  Every byte of codes and scales is written. */

@@ -35,17 +35,39 @@ def _dtype_code(dtype: torch.dtype) -> int:
 def stored_shapes(rows: int, cols: int) -> Tuple[Tuple[int, int], Tuple[int, int, int]]:
     """Shapes of the codes and the scales (uint8) of a rows x cols matrix: two codes to a byte, rows padded to whole
     blocks; scales in tiles of 128 rows x 4 blocks, (row, block) at byte (row % 32) * 16 + (row % 128 // 32) * 4 +
-    block % 4 of its tile (the layout in which the tensor cores take them)."""
+    block % 4 of its tile (the layout in which the tensor cores take them).  Scales of blocks beyond a row's last, up to
+    the tile's four, are 0."""
     blocks = -(-cols // BLOCK)
     return (rows, 16 * blocks), (-(-rows // 128), -(-blocks // 4), 512)
 
 
+def _ends_inside_a_tile(cols: int) -> int:
+    """Blocks of the last scale tile that a row fills, 0 where it fills all four."""
+    return -(-cols // BLOCK) % 4
+
+
+def _clear_padding(scales: torch.Tensor, cols: int) -> None:
+    """Zeros in place of the scales beyond a row's last block.  The tensor cores multiply them with codes of 0, which a scale
+    of 255 would make NaN."""
+    over = _ends_inside_a_tile(cols)
+    if over:
+        scales.view(*scales.shape[:2], 32, 4, 4)[:, -1, :, :, over:] = 0
+
+
 class Mx4Tensor:
-    """A quantised matrix: ``codes`` and ``scales`` in the stored form (see ``stored_shapes``) and its ``shape``."""
+    """A quantised matrix: ``codes`` and ``scales`` in the stored form (see ``stored_shapes``) and its ``shape``.  Scales that
+    end inside a tile are copied, with zeros as their padding whatever it held."""
 
     __slots__ = ("codes", "scales", "shape")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Tuple[int, int]):
+        self._hold(codes, scales, shape)
+        if _ends_inside_a_tile(self.shape[1]):
+            if self.scales is scales:
+                self.scales = scales.clone()
+            _clear_padding(self.scales, self.shape[1])
+
+    def _hold(self, codes, scales, shape) -> None:
         rows, cols = int(shape[0]), int(shape[1])
         want_codes, want_scales = stored_shapes(rows, cols)
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
@@ -72,8 +94,15 @@ class Mx4Tensor:
         q.codes, q.scales, q.shape = codes, scales, shape
         return q
 
+    @classmethod
+    def _padded(cls, codes, scales, shape) -> "Mx4Tensor":
+        """A tensor whose scales are known to be padded by zeros."""
+        q = cls.__new__(cls)
+        q._hold(codes, scales, shape)
+        return q
+
     def to(self, device) -> "Mx4Tensor":
-        return Mx4Tensor(self.codes.to(device), self.scales.to(device), self.shape)
+        return Mx4Tensor._padded(self.codes.to(device), self.scales.to(device), self.shape)
 
     def __repr__(self) -> str:
         return f"Mx4Tensor({self.shape[0]} x {self.shape[1]}, {self.codes.device})"
@@ -185,7 +214,11 @@ class Mx4Linear(torch.nn.Module):
 
     @property
     def mx4_weight(self) -> Mx4Tensor:
-        return Mx4Tensor(self.codes, self.scales, (self.out_features, self.in_features))
+        return Mx4Tensor._padded(self.codes, self.scales, (self.out_features, self.in_features))
+
+    def _load_from_state_dict(self, *args, **kwargs) -> None:
+        super()._load_from_state_dict(*args, **kwargs)
+        _clear_padding(self.scales, self.in_features)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return mx4_linear(x, self.mx4_weight, self.bias)

@@ -344,6 +344,40 @@ def test_linear_over_no_columns(cuda_dev, shape):
     assert dequantize_mx4(quantize_mx4(x)).shape == (math.prod(shape[:-1]), 0)
 
 
+@pytest.mark.parametrize("cols,blocks", [(1, 1), (64, 2), (70, 3), (128, 4), (300, 10)])
+def test_scales_are_padded_by_zeros(cols, blocks):
+    """Whatever a caller's padding held; the caller's tensor and the scales that count stay as they are."""
+    from mpq_b200.mx4 import Mx4Linear, Mx4Tensor, stored_shapes
+    shape_codes, shape_scales = stored_shapes(130, cols)
+    scales = torch.full(shape_scales, 255, dtype=torch.uint8)
+    q = Mx4Tensor(torch.zeros(shape_codes, dtype=torch.uint8), scales, (130, cols))
+    assert bool((scales == 255).all())
+    real = torch.arange(4 * shape_scales[1]).view(1, -1, 1, 1, 4) < blocks
+    want = torch.where(real, 255, 0).expand(2, -1, 32, 4, 4).reshape(shape_scales).to(torch.uint8)
+    assert torch.equal(q.scales, want) and torch.equal(q.to("cpu").scales, want)
+    layer = Mx4Linear(q)
+    layer.load_state_dict({"codes": q.codes, "scales": scales})
+    assert torch.equal(layer.mx4_weight.scales, want) and bool((scales == 255).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2, 3, 300, 2000])
+def test_padding_of_a_callers_scales_does_not_matter(cuda_dev, m):
+    from mpq_b200.mx4 import Mx4Linear, Mx4Tensor, mx4_linear, quantize_mx4
+    for cols in (33, 70, 220):
+        q = quantize_mx4(values(1000, cols, torch.float32, cuda_dev, cols, 0.3))
+        over = -(-cols // 32) % 4
+        scales = q.scales.clone()
+        scales.view(*scales.shape[:2], 32, 4, 4)[:, -1, :, :, over:] = 255
+        x = values(m, cols, torch.float32, cuda_dev, 3, 0.3)
+        want = mx4_linear(x, q)
+        assert bool(want.isfinite().all())
+        assert torch.equal(mx4_linear(x, Mx4Tensor(q.codes, scales, q.shape)), want)
+        layer = Mx4Linear(q)
+        layer.load_state_dict({"codes": q.codes, "scales": scales})
+        assert torch.equal(layer(x), want)
+
+
 @pytest.mark.gpu
 def test_another_stream_and_layers(cuda_dev):
     """Work queued on a stream of its own, and the module form against the function."""
