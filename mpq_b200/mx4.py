@@ -14,7 +14,7 @@ path).
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
@@ -228,15 +228,19 @@ class Mx4Linear(torch.nn.Module):
 
 
 def convert_linears_mx4(module: torch.nn.Module) -> int:
-    """Replace every ``nn.Linear`` below ``module`` by an ``Mx4Linear`` of its weight; returns how many."""
-    done = 0
-    for name, child in module.named_children():
-        if isinstance(child, torch.nn.Linear):
-            setattr(module, name, Mx4Linear.from_linear(child))
-            done += 1
-        else:
-            done += convert_linears_mx4(child)
-    return done
+    """Replace every ``nn.Linear`` below ``module`` by an ``Mx4Linear`` of its weight, at all of its places by the same one
+    where it has several; returns how many there were."""
+    places: Dict[int, List[Tuple[torch.nn.Module, str]]] = {}
+    for parent in module.modules():
+        for name, child in parent._modules.items():
+            if isinstance(child, torch.nn.Linear):
+                places.setdefault(id(child), []).append((parent, name))
+    for at in places.values():
+        parent, name = at[0]
+        layer = Mx4Linear.from_linear(getattr(parent, name))
+        for parent, name in at:
+            setattr(parent, name, layer)
+    return len(places)
 
 
 __all__ = ["Mx4Tensor", "Mx4Linear", "convert_linears_mx4", "dequantize_mx4", "mx4_linear", "quantize_mx4",

@@ -399,6 +399,19 @@ def test_another_stream_and_layers(cuda_dev):
 
 
 @pytest.mark.gpu
+def test_conversion_of_shared_layers(cuda_dev):
+    """A layer with several places, in one module or in two, is converted once and stands at all of them."""
+    from mpq_b200.mx4 import Mx4Linear, convert_linears_mx4
+    shared = torch.nn.Linear(64, 64, device=cuda_dev)
+    net = torch.nn.Sequential(shared, shared, torch.nn.Sequential(shared, torch.nn.Linear(64, 8, device=cuda_dev)))
+    x = torch.randn(3, 64, device=cuda_dev)
+    assert convert_linears_mx4(net) == 2
+    assert isinstance(net[0], Mx4Linear) and net[1] is net[0] and net[2][0] is net[0] and isinstance(net[2][1], Mx4Linear)
+    assert torch.equal(net(x), net[2][1](net[0](net[0](net[0](x)))))
+    assert convert_linears_mx4(net) == 0
+
+
+@pytest.mark.gpu
 def test_product_in_a_cuda_graph(cuda_dev):
     from mpq_b200.mx4 import mx4_linear, quantize_mx4
     w = quantize_mx4(values(300, 512, torch.bfloat16, cuda_dev, 3, 0.3))
