@@ -292,7 +292,8 @@ struct Ring {
 };
 
 // ---- host: tensor maps through the driver entry point (no libcuda link dependency) ----
-static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+// One variable for the library: the inline functions below are one function each, whichever file's copy the linker keeps.
+inline PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
 inline int get_encoder() {
   if (g_encode) return MPQ_OK;

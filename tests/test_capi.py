@@ -47,3 +47,11 @@ def test_invalid_argument_reports_error_without_gpu():
     st = lib.mpq_gemm_f32(7, 1, 1, 1, ctypes.c_float(1.0), None, 1, None, 1, ctypes.c_float(0.0), None, 1, None)
     assert st == 10001
     assert b"null pointer" in lib.mpq_last_error() or b"layout" in lib.mpq_last_error()
+
+
+def test_tensor_map_encoder_is_one_variable():
+    """Several files share the inline functions that set and call the driver's tensor-map encoder: a variable of each file's
+    own would stay null in all but the file whose copy of the functions the linker keeps."""
+    from mpq_b200 import build
+    names = subprocess.run(["nm", "-C", str(build.OUT)], check=True, capture_output=True, text=True).stdout
+    assert len(re.findall(r"mpq::tc::g_encode$", names, flags=re.M)) == 1
