@@ -456,7 +456,8 @@ int mpq_mx4_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols, 
 int mpq_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int rows, int cols, void* out, int dtype,
                        int64_t ldo, void* stream);
 /* out (M x N, dtype) = A B^T + bias: A M x K and B N x K in the stored form, bias N values of dtype or NULL, FP32
- * accumulation on the block-scaled tensor cores, one rounding.  `status`: as mpq_gemm_tc. */
+ * accumulation on the block-scaled tensor cores, one rounding.  `status`: as mpq_gemm_tc, 10 added to
+ * the code. */
 int mpq_mx4_gemm(int M, int N, int K, const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
                  const uint8_t* b_scales, const void* bias, void* out, int dtype, int64_t ldo, int* status,
                  void* stream);
@@ -472,7 +473,7 @@ int mpq_mx4_linear(const void* x, int dtype, int64_t ldx, int M, int N, int K, c
  * No counterpart in the reference (its perplexity scripts call a library's loss on whole logits).  The logits are
  * not stored.  dtype: 1 bfloat16, 2 float16 (hidden, weight and their gradients); operands 16-byte aligned with
  * leading dimensions that are multiples of 8.  Labels equal to `ignore` do not count; labels outside [0, V) give NaN.
- * `status`: as mpq_gemm_tc. */
+ * `status`: as mpq_gemm_tc, 20 added to the code. */
 
 /* Columns of `part` below. */
 int mpq_xent_tiles(int T, int V);

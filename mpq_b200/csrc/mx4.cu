@@ -23,6 +23,8 @@ using namespace tc;
 
 enum { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
+constexpr int kTimedOut = 10;  // added to the code of a wait that ran out: whose it was
+
 // ------------------------------------------------------------------------------------------------------------------
 // Elements
 // ------------------------------------------------------------------------------------------------------------------
@@ -635,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           r.back();
           mbar_wait_fast(&full[r.s], r.ph);
         }
-        atomicCAS(p.status, 0, 2);
+        atomicCAS(p.status, 0, kTimedOut + 2);
       }
     }
   } else if (warp == 1) {
@@ -676,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok && lead) {
       *abort_flag = 1;
-      atomicCAS(p.status, 0, 3);
+      atomicCAS(p.status, 0, kTimedOut + 3);
     }
   } else if (warp == 6) {
     const bool lead = elect_one();
@@ -705,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok && lead) {
       *abort_flag = 1;
-      atomicCAS(p.status, 0, 5);
+      atomicCAS(p.status, 0, kTimedOut + 5);
     }
   } else {
     const int quad = warp & 3;
@@ -714,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int b = n & 1, mb = t % p.mt, nb = t / p.mt;
       const bool ready = !*abort_flag && mbar_wait_fast(&acc_full[b], (uint32_t)(n >> 1) & 1u);
       if (!__all_sync(0xffffffffu, ready) || *abort_flag) {
-        if (!*abort_flag) atomicCAS(p.status, 0, 4);
+        if (!*abort_flag) atomicCAS(p.status, 0, kTimedOut + 4);
         *abort_flag = 1;
         break;
       }
@@ -869,7 +871,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           r.back();
           mbar_wait_cluster(&full[r.s], r.ph);
         }
-        atomicCAS(p.status, 0, 2);
+        atomicCAS(p.status, 0, kTimedOut + 2);
       }
     }
   } else if (warp == 1) {
@@ -907,7 +909,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
       if (!ok && lead) {
         *abort_flag = 1;
-        atomicCAS(p.status, 0, 3);
+        atomicCAS(p.status, 0, kTimedOut + 3);
       }
     }
   } else if (warp == 2 + kPairWarps) {
@@ -940,7 +942,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
       if (!ok && lead) {
         *abort_flag = 1;
-        atomicCAS(p.status, 0, 5);
+        atomicCAS(p.status, 0, kTimedOut + 5);
       }
     }
   } else {
@@ -953,7 +955,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       tile_at(t, mb, nb);
       const bool ready = !*abort_flag && mbar_wait_cluster(acc_full, n & 1u);
       if (!__all_sync(0xffffffffu, ready) || *abort_flag) {
-        if (!*abort_flag) atomicCAS(p.status, 0, 4);
+        if (!*abort_flag) atomicCAS(p.status, 0, kTimedOut + 4);
         *abort_flag = 1;
         break;
       }

@@ -54,6 +54,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 enum { kLse = 0, kGrad = 1, kOut = 2 };
 
+constexpr int kTimedOut = 20;  // added to the code of a wait that ran out: whose it was
+
 struct Args {
   int M, N, K, mt, nt;      // C[M, N] over K; mt x nt tiles
   int splits;               // parts of K; more than one only with `acc`
@@ -278,7 +280,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           r.back();
           mbar_wait_cluster(&full[r.s], r.ph);
         }
-        atomicCAS(p.status, 0, 2);
+        atomicCAS(p.status, 0, kTimedOut + 2);
       }
     }
   } else if (warp == 1) {
@@ -326,7 +328,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if (!ok && lead) {
         *abort_flag = 1;
-        atomicCAS(p.status, 0, 3);
+        atomicCAS(p.status, 0, kTimedOut + 3);
       }
     }
   } else {
@@ -346,7 +348,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     auto take = [&]() {
       const bool ready = !*abort_flag && mbar_wait_cluster(&acc_full[n & 1], (uint32_t)(n >> 1) & 1u);
       if (!__all_sync(0xffffffffu, ready) || *abort_flag) {
-        if (!*abort_flag) atomicCAS(p.status, 0, 4);
+        if (!*abort_flag) atomicCAS(p.status, 0, kTimedOut + 4);
         *abort_flag = 1;
         return false;
       }

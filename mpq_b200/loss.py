@@ -129,7 +129,8 @@ def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torc
     Differentiable once in ``hidden`` and ``weight``, whose gradients come in their own type (for the head's, rows of
     ``hidden`` that do not count must be finite all the same: they meet a zero).  ``keep_bytes`` bounds what the forward
     pass keeps for the backward pass (by default 2 GiB; 0: nothing), ``piece`` the columns of the vocabulary that the
-    backward pass computes again at a time (by default what fits in 1 GiB)."""
+    backward pass computes again at a time (by default what fits in 1 GiB).  Waits inside the kernels are bounded:
+    ``ops.check_status`` raises, once the caller synchronises by it, if one ran out and left a result undefined."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
     if not (hidden.is_cuda and weight.is_cuda and labels.is_cuda):

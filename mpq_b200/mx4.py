@@ -168,7 +168,8 @@ class _ForwardOnly(torch.autograd.Function):
 def mx4_linear(x: torch.Tensor, weight: Mx4Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = Q(x) W^T + b for x (..., K) and a quantised W (N x K): x is quantised row by row, the products accumulate in
     FP32, and y (x's dtype) is rounded once.  Forward only: a backward pass that needs the gradient of x or of the bias
-    raises."""
+    raises.  Waits inside the kernels are bounded: ``ops.check_status`` raises, once the caller synchronises by it, if one
+    ran out and left a result undefined."""
     tied = torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad)
     given = (x, bias)
     rows = _rows_of(x, "mx4_linear")

@@ -115,13 +115,19 @@ def status_word(device: torch.device) -> torch.Tensor:
     return t
 
 
+# Whose wait timed out, by the tens of its code.
+_TIMED_OUT = ("an FP32-faithful product (mpq_gemm_*)", "a 4-bit product (mx4_linear, mpq_mx4_*)",
+              "the vocabulary loss (vocab_cross_entropy, mpq_xent_*)")
+
+
 def check_status(device: torch.device) -> None:
     """Raise if a tensor-core pipeline wait timed out since the last check (host sync)."""
     t = status_word(device)
     v = int(t.item())
     if v:
         t.zero_()
-        raise RuntimeError(f"mpq_gemm_tc: pipeline wait timed out (code {v})")
+        whose = _TIMED_OUT[v // 10] if 0 < v < 10 * len(_TIMED_OUT) else "a tensor-core product"
+        raise RuntimeError(f"{whose}: pipeline wait timed out (code {v}); its results are undefined")
 
 
 def _tma_ok(t: torch.Tensor) -> bool:

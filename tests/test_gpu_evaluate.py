@@ -242,3 +242,15 @@ def test_refuses_ids_outside_the_vocabulary(cuda_dev, decoder):
                 with pytest.raises(ValueError, match="ids must be in"):
                     call(model, ids)
     assert token_scores(model, torch.tensor([[0, 999]])).shape == (1, 1)
+
+
+def test_a_wait_that_ran_out_is_named():
+    """The word that the kernels leave, faked: whose wait it was, once."""
+    from mpq_b200 import ops
+    cpu = torch.device("cpu")
+    word = ops.status_word(cpu)
+    for code, whose in ((3, "FP32-faithful product"), (15, "mx4_linear"), (24, "vocab_cross_entropy"), (99, "tensor-core")):
+        word.fill_(code)
+        with pytest.raises(RuntimeError, match=f"{whose}.*timed out .code {code}.; its results are undefined"):
+            ops.check_status(cpu)
+        ops.check_status(cpu)
