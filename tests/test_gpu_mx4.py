@@ -296,6 +296,33 @@ def test_every_code_at_every_place_of_a_block(cuda_dev, m):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("n,k", [(70, 9000), (1800, 4128), (15001, 1056), (16000, 64)])
+def test_every_code_in_slices_and_rounds(cuda_dev, n, k, m, dtype):
+    """Few tokens, K in slices of several steps and rows in several rounds of a CTA: x has one element in each block, at every
+    place in turn, so that y is a sum of one code of each block, exactly (multiples of 1/8 below 2^16)."""
+    from mpq_b200.mx4 import Mx4Tensor, mx4_linear, stored_shapes
+    nb = -(-k // 32)
+    r, j = torch.arange(n, device=cuda_dev)[:, None], torch.arange(32 * nb, device=cuda_dev)[None]
+    code = ((r * 5 + j * 7 + j // 16 + r * j // 97) % 16) * (j < k)
+    b = torch.arange(nb, device=cuda_dev)[None]
+    c = 125 + (r + 3 * b) % 6
+    scales = torch.zeros(stored_shapes(n, k)[1], dtype=torch.uint8, device=cuda_dev)
+    scales[r // 128, b // 4, (r % 32) * 16 + r % 128 // 32 * 4 + b % 4] = c.to(torch.uint8)
+    pairs = code.view(n, -1, 2)
+    w = Mx4Tensor((pairs[..., 0] + 16 * pairs[..., 1]).to(torch.uint8), scales, (n, k))
+    q = GRID.to(cuda_dev)[code & 7] * torch.where(code >= 8, -1.0, 1.0) * torch.pow(2.0, c.double() - 127).repeat_interleave(32, 1)
+    for place in range(0, 32, m):
+        x = torch.zeros(m, k, device=cuda_dev, dtype=dtype)
+        for t in range(m):
+            at = 32 * torch.arange(nb, device=cuda_dev) + (place + t + 11 * torch.arange(nb, device=cuda_dev)) % 32
+            x[t, at[at < k]] = 1.0
+        want = (x.double() @ q[:, :k].T + 0.0).to(dtype)
+        assert torch.equal(mx4_linear(x, w) + 0.0, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("m,n,k", [(1, 40, 70), (2, 129, 300), (300, 1000, 520)])
 def test_product_of_two_stored_matrices(cuda_dev, m, n, k, dtype):
     """mpq_mx4_gemm against the same product of the values that the two matrices stand for: both operands are exact, so
