@@ -18,7 +18,6 @@ from __future__ import annotations
 import argparse
 import copy
 import json
-import math
 from typing import Any, Dict, List, Optional
 
 import torch
@@ -105,8 +104,8 @@ def token_scores(model, ids: torch.Tensor, batch_size: int = 8) -> torch.Tensor:
 
 
 def perplexity(model, ids: torch.Tensor, batch_size: int = 8) -> float:
-    """exp of the mean score over all scored tokens."""
-    return math.exp(float(token_scores(model, ids, batch_size).double().mean()))
+    """exp of the mean score over all scored tokens (infinity beyond float64)."""
+    return float(token_scores(model, ids, batch_size).double().mean().exp())
 
 
 def _untied_head(model) -> torch.Tensor:

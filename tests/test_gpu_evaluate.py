@@ -254,3 +254,13 @@ def test_a_wait_that_ran_out_is_named():
         with pytest.raises(RuntimeError, match=f"{whose}.*timed out .code {code}.; its results are undefined"):
             ops.check_status(cpu)
         ops.check_status(cpu)
+
+
+def test_perplexities_of_any_score(monkeypatch):
+    from mpq_b200 import evaluate
+    for scores, want in ((torch.tensor([[1.0, 3.0]]), math.exp(2.0)), (torch.tensor([[900.0]]), math.inf),
+                         (torch.tensor([[math.inf]]), math.inf)):
+        monkeypatch.setattr(evaluate, "token_scores", lambda *args: scores)
+        assert evaluate.perplexity(None, None) == pytest.approx(want, rel=1e-12)
+    monkeypatch.setattr(evaluate, "token_scores", lambda *args: torch.tensor([[math.nan, 1.0]]))
+    assert math.isnan(evaluate.perplexity(None, None))
