@@ -264,3 +264,22 @@ def test_perplexities_of_any_score(monkeypatch):
         assert evaluate.perplexity(None, None) == pytest.approx(want, rel=1e-12)
     monkeypatch.setattr(evaluate, "token_scores", lambda *args: torch.tensor([[math.nan, 1.0]]))
     assert math.isnan(evaluate.perplexity(None, None))
+
+
+def test_a_decoder_that_runs_its_layers_itself():
+    """Its hidden states of the two tokens come from other kernels: a difference like theirs is no other function."""
+    transformers = pytest.importorskip("transformers")
+    from mpq_b200.evaluate import _check_logits
+    torch.manual_seed(0)
+    model = transformers.OPTForCausalLM(transformers.OPTConfig(
+        vocab_size=120, hidden_size=32, word_embed_proj_dim=32, ffn_dim=48, num_hidden_layers=1, num_attention_heads=2,
+        max_position_embeddings=64, init_std=0.5)).eval()
+    ids = torch.arange(3, 33).view(2, 15)
+    with torch.no_grad():
+        states = model.model(ids)
+    states.last_hidden_state = states.last_hidden_state * (1 + 2.0 ** -7 * torch.randn(2, 15, 32))
+    _check_logits(model, ids, states)
+    hook = model.lm_head.register_forward_hook(lambda mod, args, out: 0.8 * out)
+    with pytest.raises(ValueError, match="hidden @ head.T"):
+        _check_logits(model, ids, states)
+    hook.remove()
