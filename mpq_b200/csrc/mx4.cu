@@ -74,7 +74,8 @@ __device__ __forceinline__ void decode8(uint32_t codes, __half2 (&h)[4]) {
 }
 // The same with one instruction a pair, each taking its byte out of the word by itself, where the function above adds a
 // shift and a mask.  Only for code that a warp runs together: in code that diverges, ptxas 12.9.86 has lost the
-// operands of this form (seen in reading back and, with the opposite conversion, in quantisation).
+// operands of this form (seen in reading back and, with the opposite conversion, in quantisation; the cause is not known).
+// The use below is checked code by code, at every place of a block, in slices of K and rounds of rows.
 __device__ __forceinline__ void decode8_together(uint32_t codes, __half2 (&h)[4]) {
   uint32_t r[4];
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
@@ -1100,7 +1101,8 @@ static int gemm_pair(const uint8_t* a_codes, const uint8_t* b_codes, int64_t ldc
 
 // The kernel with the shortest estimate in cycles, from measured parts: a k-block takes 680 in k_mx4_tile, whatever the
 // tile's width, and 700 in k_mx4_pair; a round of tiles 1000, the pair's launch 3000 more; a cluster's sum of two parts
-// of K 3500, of four 6200, and more for each of its rows.  (us, 512 x 4096 x 4096: 128 columns 11.9, 64 16.9, pair 13.7;
+// of K 3500, of four 6200, and more for each of its rows.  (Fitted to whole launches: the MMAs' own 512 cycles of a
+// k-block are not reached, see above.  us, 512 x 4096 x 4096: 128 columns 11.9, 64 16.9, pair 13.7;
 // 8 x 14336 x 4096: 128 columns in 4 parts 14.5, 2 parts 16.2, whole 24.0; 128 x 4096 x 4096: 64 columns in 2 parts 9.8,
 // whole 10.2, 128 columns in 4 parts 12.6.)
 template <class T>

@@ -11,7 +11,7 @@ and the same from the command line, on a registered synthetic shape or a local c
 
 The output head's logits are not stored: the loss is ``vocab_cross_entropy`` on the hidden states.  Decoders whose logits
 are another function of them than hidden @ head.T (a head with a bias; a soft cap or a scale in the configuration) are
-refused.
+refused, and so are heads of another type than bfloat16 and float16, which the loss takes.
 """
 from __future__ import annotations
 

@@ -5,8 +5,9 @@
 
 The logits (tokens x vocabulary) are not stored: the forward pass reduces them tile by tile inside the product.  The
 backward pass takes the vocabulary in pieces.  It computes a piece's logits again, except for the first columns, which
-the forward pass keeps in 16 bits where a gradient is wanted and ``keep_bytes`` has room: that saves their product.
-With ``keep_bytes=0`` nothing of the logits' size outlives a call.
+the forward pass keeps in 16 bits where a gradient is wanted and ``keep_bytes`` has room: that saves their product and
+costs digits (probabilities within 2^-12.5 of themselves, and none below 2^-32 of the largest beside them).  With
+``keep_bytes=0`` nothing of the logits' size outlives a call.
 """
 from __future__ import annotations
 
@@ -128,7 +129,8 @@ def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torc
     the vocabulary give NaN.  ``reduction``: "mean" over the labels that count, "sum" or "none" (one score a token).
     Differentiable once in ``hidden`` and ``weight``, whose gradients come in their own type (for the head's, rows of
     ``hidden`` that do not count must be finite all the same: they meet a zero).  ``keep_bytes`` bounds what the forward
-    pass keeps for the backward pass (by default 2 GiB; 0: nothing), ``piece`` the columns of the vocabulary that the
+    pass keeps for the backward pass (by default 2 GiB; 0: nothing; what was kept serves one backward pass, another through
+    the same graph computes it again and may differ in its last digits), ``piece`` the columns of the vocabulary that the
     backward pass computes again at a time (by default what fits in 1 GiB).  Waits inside the kernels are bounded:
     ``ops.check_status`` raises, once the caller synchronises by it, if one ran out and left a result undefined."""
     if reduction not in _REDUCTIONS:
