@@ -107,6 +107,7 @@ def token_scores(model, ids: torch.Tensor, batch_size: int = 8) -> torch.Tensor:
         if not out:
             _check_logits(model, part[:, :-1], states)
         hidden = states.last_hidden_state.to(head.dtype)
+        del states  # its key/value cache
         out.append(vocab_cross_entropy(hidden, head, part[:, 1:], reduction="none"))
     ops.check_status(ids.device)
     return torch.cat(out)
@@ -153,6 +154,7 @@ def tune_head(model, ids: torch.Tensor, steps: int = 20, lr: float = 1e-2, batch
                 states = inner(part[:, :-1])
             if step == 0:
                 _check_logits(model, part[:, :-1], states)
+            del states  # its key/value cache
             loss = vocab_cross_entropy(inner.norm(seen["x"]).to(head.dtype), head, part[:, 1:])
             grads = torch.autograd.grad(loss, params)
             with torch.no_grad():

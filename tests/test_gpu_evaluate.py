@@ -283,3 +283,25 @@ def test_a_decoder_that_runs_its_layers_itself():
     with pytest.raises(ValueError, match="hidden @ head.T"):
         _check_logits(model, ids, states)
     hook.remove()
+
+
+@pytest.mark.gpu
+def test_no_batch_keeps_its_cache(cuda_dev, decoder):
+    """What the layers gave for one batch (its key/value cache with it) is gone when the next one runs."""
+    import weakref
+    from mpq_b200.evaluate import token_scores, tune_head
+    model = decoder()
+    caches, alive = [], []
+
+    def before(mod, args):
+        if "forward" not in mod.__dict__:  # not while the check of the logits hands a batch's states back
+            alive.append(sum(r() is not None for r in caches))
+
+    hooks = [model.model.register_forward_pre_hook(before),
+             model.model.register_forward_hook(lambda mod, args, out: caches.append(weakref.ref(out.past_key_values)))]
+    ids = torch.arange(3, 123, device=cuda_dev).view(6, 20)
+    token_scores(model, ids, batch_size=2)
+    tune_head(model, ids, steps=3, batch_size=2)
+    for h in hooks:
+        h.remove()
+    assert len(alive) == 6 and not any(alive)
